@@ -482,6 +482,45 @@ int omHipMultiHeadAttentionHalf(int nDtype, const uint16_t* pX, const uint16_t* 
                                 const uint16_t* pWout, const float* pBout, void* pOut, int nOutHalf,
                                 int nBatch, int nSeq, int nHeads, int nHeadDim);
 
+/* ===== attention for training (NEW; the reference's autograd nodes keep every probability:
+ * MatMulBackward and SoftmaxBackward of the chain in vit.ixx:163-187) ===== */
+
+/* NEW: O = softmax(fScale Q K^T) V on half-precision data with each row's log-sum-exp kept, the
+ * saved state of omHipAttentionBackwardHalf. nDtype 0 binary16, 1 bfloat16; fp32 accumulate.
+ * Layout: token t of image b has its query heads at pQ + b * nStrideQ + t * nLdQ, head h at
+ * h * nHeadDim of them; pK and pV likewise with nStrideKV, nLdKV and nKVHeads heads, query head
+ * h reading key head h / (nHeads / nKVHeads). A packed projection [nBatch*nSeq, (nHeads +
+ * 2 nKVHeads) * nHeadDim] is three pointers into it with one stride. pOut [nBatch, nSeqQ,
+ * nHeads, nHeadDim] (merged heads) in nDtype, pLse [nBatch, nHeads, nSeqQ] fp32 (natural log).
+ * Masks: pQueryLens and pKeyLens [nBatch] int32 on the device (NULL: nSeqQ, nSeqK for all;
+ * values are taken into 0 .. nSeqQ, nSeqK) bound each image's queries and keys; bCausal lets
+ * query i see keys j <= i + nSeqK - nSeqQ. A query past its length, one that sees no key and one
+ * whose scores are all -inf get O = 0 and lse = -inf. What lies past a length is not read, so
+ * it may hold anything; a NaN or infinity within the lengths may reach every row of its block
+ * of 128 queries or keys, masked by bCausal or not.
+ * P is rounded to nDtype before P V. nHeadDim a multiple of 8 up to 128, nHeads a multiple of
+ * nKVHeads; pointers 16-byte aligned, strides multiples of 8 elements, row strides below 2^23.
+ * Every element of pOut and pLse is written; nSeqK 0 is a sequence without keys. */
+int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                   long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                   const int* pKeyLens, int bCausal, uint16_t* pOut, float* pLse, int nBatch, int nSeqQ,
+                                   int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale);
+/* NEW: the gradients of omHipAttentionTrainForwardHalf at the same arguments: P = exp(fScale Q
+ * K^T - lse) is computed again; delta_i = sum_d dO_id O_id, dV = P^T dO, dS = P (dO V^T - delta),
+ * dQ = fScale dS K, dK = fScale dS^T Q, a key head's dK and dV summed over the query heads that
+ * read it. pOut and pLse as the forward pass left them, pGradOut [nBatch, nSeqQ, nHeads,
+ * nHeadDim] in nDtype. pGradQ, pGradK and pGradV are laid out as pQ, pK and pV are (the same
+ * strides), so a packed projection's gradient is packed; every element of the heads' columns is
+ * written, zeros past the lengths. P and dS are rounded to nDtype as operands (binary16: scaled
+ * by powers of two so that small ones keep their bits), sums are in fp32 in a fixed order:
+ * repeated calls agree bit for bit. Row statistics use the library's per-stream workspace.
+ * Inputs and gradients must not overlap. */
+int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                               long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                               const int* pKeyLens, int bCausal, const uint16_t* pOut, const float* pLse,
+                               const uint16_t* pGradOut, uint16_t* pGradQ, uint16_t* pGradK, uint16_t* pGradV, int nBatch,
+                               int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale);
+
 /* ===== device-resident inference (EngineBridge::inferBatch, EngineBridge.cpp:3525-3772) ===== */
 
 /* NEW: a ResNet-18 classifier (torchvision layout, 3x224x224 input) resident on the device,

@@ -260,6 +260,29 @@ public:
         check(omHipAttentionHalf(nDtype, pQKV, pOut, bOutHalf ? 1 : 0, nBatch, nSeq, nHeads, nHeadDim, fScale),
               "attentionHalf");
     }
+    // Attention for training: softmax(scale Q K^T) V with each row's log-sum-exp kept, on strided rows with shared
+    // key heads, a causal mask and per-image lengths (device, nullable), and its gradients, laid out as Q, K and V are
+    static void attentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV,
+                                          long long nLdQ, long long nStrideQ, long long nLdKV, long long nStrideKV,
+                                          const int* pQueryLens, const int* pKeyLens, bool bCausal, uint16_t* pOut,
+                                          float* pLse, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads,
+                                          int nHeadDim, float fScale) {
+        check(omHipAttentionTrainForwardHalf(nDtype, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens,
+                                             bCausal ? 1 : 0, pOut, pLse, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                                             nHeadDim, fScale),
+              "attentionTrainForwardHalf");
+    }
+    static void attentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV,
+                                      long long nLdQ, long long nStrideQ, long long nLdKV, long long nStrideKV,
+                                      const int* pQueryLens, const int* pKeyLens, bool bCausal, const uint16_t* pOut,
+                                      const float* pLse, const uint16_t* pGradOut, uint16_t* pGradQ, uint16_t* pGradK,
+                                      uint16_t* pGradV, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads,
+                                      int nHeadDim, float fScale) {
+        check(omHipAttentionBackwardHalf(nDtype, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens,
+                                         bCausal ? 1 : 0, pOut, pLse, pGradOut, pGradQ, pGradK, pGradV, nBatch, nSeqQ,
+                                         nSeqK, nHeads, nKVHeads, nHeadDim, fScale),
+              "attentionBackwardHalf");
+    }
     // Linear::forward (linear.ixx:50-58) on half inputs: act(x W + b), W [K,N] ([N,K] when bTransW)
     static void linearHalf(int nDtype, const uint16_t* pInput, const uint16_t* pWeight, bool bTransW,
                            const float* pBias, int nAct, void* pOutput, bool bOutHalf, int nM, int nK, int nN) {

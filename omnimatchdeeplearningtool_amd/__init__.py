@@ -129,6 +129,8 @@ _SIGS = {
     "omHipAttentionHalf": [_i, _vp, _vp, _i, _i, _i, _i, _i, _fl],
     "omHipLinearHalf": [_i, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i],
     "omHipMultiHeadAttentionHalf": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i],
+    "omHipAttentionTrainForwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i, _vp, _vp] + [_i] * 6 + [_fl],
+    "omHipAttentionBackwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i] + [_vp] * 6 + [_i] * 6 + [_fl],
     "omHipConvertF32ToF16": [_vp, _vp, _i],
     "omHipConvertF32ToBF16": [_vp, _vp, _i],
     "omHipConvertF16ToF32": [_vp, _vp, _i],
@@ -553,6 +555,24 @@ class HIPBackend:
         """Fused QKV split + softmax(scale Q K^T) V + head merge (vit.ixx:150-239)."""
         call("omHipAttentionHalf", 1 if bf16 else 0, _ptr(pQKV), _ptr(pOut), 1 if outHalf else 0, nBatch, nSeq, nHeads,
              nHeadDim, fScale)
+
+    @staticmethod
+    def attentionTrainForwardHalf(pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, pOut, pLse,
+                                  nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale, bf16: bool = False) -> None:
+        """softmax(scale Q K^T) V with each row's log-sum-exp kept for attentionBackwardHalf; strided rows, shared key
+        heads, causal mask, per-image lengths (int32 on the device, may be None)."""
+        call("omHipAttentionTrainForwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV,
+             nStrideKV, _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, _ptr(pOut), _ptr(pLse), nBatch, nSeqQ,
+             nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
+
+    @staticmethod
+    def attentionBackwardHalf(pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, pOut, pLse,
+                              pGradOut, pGradQ, pGradK, pGradV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale,
+                              bf16: bool = False) -> None:
+        """dQ, dK, dV of attentionTrainForwardHalf at the same arguments, laid out as Q, K and V are."""
+        call("omHipAttentionBackwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV,
+             nStrideKV, _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, _ptr(pOut), _ptr(pLse), _ptr(pGradOut),
+             _ptr(pGradQ), _ptr(pGradK), _ptr(pGradV), nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
 
     @staticmethod
     def linearHalf(pInput, pWeight, pBias, pOutput, nM, nK, nN, bf16: bool = False, transW: bool = False,

@@ -1,0 +1,680 @@
+// attn_train.hip — attention for training on fp16 / bf16 data: a forward pass
+// that keeps each row's log-sum-exp, and the backward pass that computes the
+// probabilities again from it.
+//
+// The reference trains MultiHeadAttention through autograd nodes of the
+// unfused chain (src/engine/om.engine.vit.ixx:150-239: qkvSplitHeads,
+// tensorBatchedMatmul, tensorSoftmaxLastDim, tensorBatchedMatmul, mergeHeads),
+// which keep the S x S probabilities. With S = scale Q K^T over the keys that
+// a query sees, P = exp(S - lse), lse = log sum exp S:
+//   O  = P V                    dV = P^T dO
+//   dP = dO V^T                 dS = P (dP - delta),  delta_i = sum_d dO_id O_id
+//   dQ = scale dS K             dK = scale dS^T Q
+// A key head's dK and dV are the sums over the query heads that read it. All
+// sums are in fp32 in a fixed order; the products take P and dS rounded to the
+// data's type, as operands of the matrix cores.
+//
+// Query i sees key j where j < the image's key length and, if causal,
+// j <= i + nSeqK - nSeqQ. A query that sees none, or whose scores are all
+// -inf, has O = 0 and lse = -inf and passes no gradient.
+#include "attn_tile.hpp"
+#include "omhip_internal.hpp"
+#include "../../include/omhip.h"
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
+namespace omhip {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTileKeys = 64;    // keys per LDS tile
+constexpr int kBlockQ = 32 * kWaves;
+
+struct AttnTrainParams {
+    const uint16_t *q, *k, *v;
+    long long ldq, sq, ldkv, skv;   // elements between tokens, between images
+    const int *qLens, *kLens;
+    int B, Sq, Sk, H, Hkv, D, causal;
+    float scale;
+    // forward: the context [B, Sq, H, D] and log-sum-exp [B, H, Sq]; backward: their saved values
+    uint16_t* out;
+    float* lse;
+    // backward
+    const uint16_t* gradOut;
+    uint16_t *dq, *dk, *dv;
+    float *lse2, *delta;            // [B, H, SqP]
+    int SqP;                        // Sq rounded up to whole tiles
+    uint32_t heads, blocks;         // grid: heads x blocks workgroups
+};
+
+// ---------------------------------------------------------------- forward
+// A workgroup holds 128 queries of a head, 32 a wave, and walks the keys 64 at
+// a time: S^T = K Q^T (the lane's column is its query), the softmax with a
+// running reference m of the row's maximum, O^T += V^T P^T.
+//  * p = exp2(c s - c m + shift), c = |scale| log2 e (a negative scale flips Q's
+//    signs as it is loaded). m only moves when a tile's maximum exceeds it by
+//    more than 8 / c, so the sums are rescaled a few times a row instead of
+//    every tile; p is at most 2^(8 + shift).
+//  * shift: fp16 keeps 2^-14 .. 2^16 at full precision, so its p is raised by
+//    2^6 (at most 2^14); bf16 needs none.
+//  * the next tile's K and V land in the other pair of buffers meanwhile.
+template <bool BF16, int KD>
+__global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainParams p) {
+    using T = AtTile<KD>;
+    constexpr float kShift = BF16 ? 0.f : 6.f;
+    __shared__ __attribute__((aligned(256))) uint16_t k0[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t v0[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = lane & 31, h = lane >> 5;
+    uint32_t bh, qb;
+    atPlace(blockIdx.x, p.heads, p.blocks, bh, qb);
+    qb = p.blocks - 1 - qb;   // causal: the longest walks first
+    const int b = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);
+    const int kvHead = head / (p.H / p.Hkv);
+    const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
+    const int off = p.Sk - p.Sq;
+    const int q0 = (int)qb * kBlockQ + wave * 32;   // the wave's first query
+    const int query = q0 + l;
+    const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
+    const uint16_t* vBase = p.v + (long long)b * p.skv + (long long)kvHead * p.D;
+
+    // keys seen by the workgroup's and by the wave's queries
+    const int blockLast = min((int)qb * kBlockQ + kBlockQ, nQ) - 1;
+    int kEnd = blockLast >= (int)qb * kBlockQ ? nK : 0;
+    if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
+    int waveEnd = q0 < nQ ? kEnd : 0;
+    if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
+    const int nt = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
+
+    const float c = fmaxf(fabsf(p.scale) * kAtLog2e, FLT_MIN);
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    at_u32x4 qf[T::NS];
+    {
+        const uint16_t* row = p.q + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
+#pragma unroll
+        for (int s = 0; s < T::NS; ++s) {
+            qf[s] = T::direct(row, query < nQ, s, h, p.D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
+        }
+    }
+    typename T::template Copy<kTileKeys, kWaves> copy;
+    const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
+    copy.init(wave, lane, ld2, p.D);
+    auto fetch = [&](int t, uint16_t* kd, uint16_t* vd) {
+        const long long at = (long long)t * kTileKeys * p.ldkv;
+        copy.run(kBase + at, nK - t * kTileKeys, ld2, p.D, kd, wave);
+        copy.run(vBase + at, nK - t * kTileKeys, ld2, p.D, vd, wave);
+    };
+
+    at_f32x16 o[KD];
+#pragma unroll
+    for (int t = 0; t < KD; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+    float m = -INFINITY, sum = 0.f;
+    const float margin = fminf(8.f / c, FLT_MAX);
+
+    auto tile = [&](int t, const uint16_t* kd, const uint16_t* vd) {
+        at_f32x16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+            for (int st = 0; st < T::NS; ++st) s[kb] = atMfma<BF16>(T::natural(kd, 32 * kb, st, l, h), qf[st], s[kb]);
+        }
+        const int key0 = t * kTileKeys;
+        if (key0 + kTileKeys > nK || (p.causal && key0 + kTileKeys - 1 > q0 + off)) {
+            const int seen = (p.causal ? min(nK, query + off + 1) : nK) - key0 - 4 * h;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * kb + 8 * (r / 4) + r % 4 >= seen) s[kb][r] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+        top = fmaxf(top, atOtherHalf(top));
+        if (__any(top > m + margin)) {   // also where m is -inf and the row sees its first key
+            const float next = fmaxf(m, top);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
+            sum *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+            m = next;
+        }
+        const float base = m == -INFINITY ? 0.f : kShift - m * c;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, base));
+                s[kb][r] = e;
+                sum += e;
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const at_u32x4 pf = atPack8<BF16>(s[u / 2], u & 1);
+#pragma unroll
+            for (int dt = 0; dt < KD; ++dt) o[dt] = atMfma<BF16>(T::transposed(vd, 16 * u, dt, lane), pf, o[dt]);
+        }
+    };
+
+    // Copies of tile t + 1 start once every wave is done with tile t - 1, whose
+    // buffers they fill, and are waited for at the top of the next trip.
+    if (nt > 0) fetch(0, k0, v0);
+    for (int t = 0; t < nt; t += 2) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1, k1, v1);
+        if (t * kTileKeys < waveEnd) tile(t, k0, v0);
+        if (t + 1 >= nt) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 2 < nt) fetch(t + 2, k0, v0);
+        if ((t + 1) * kTileKeys < waveEnd) tile(t + 1, k1, v1);
+    }
+
+    if (query >= p.Sq) return;
+    sum += atOtherHalf(sum);
+    const bool empty = !(query < nQ) || sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    if (h == 0)
+        p.lse[((long long)b * p.H + head) * p.Sq + query] = empty ? -INFINITY : m * (c * kAtLn2) + (__logf(sum) - kShift * kAtLn2);
+    uint16_t* row = p.out + (((long long)b * p.Sq + query) * p.H + head) * p.D;
+#pragma unroll
+    for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * dt + 2 * r + 4 * h;
+            const float v[4] = {o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
+            if (d < p.D)
+                *reinterpret_cast<at_u32x2*>(row + d) =
+                    empty ? at_u32x2{0u, 0u} : at_u32x2{atPack2<BF16>(v[0], v[1]), atPack2<BF16>(v[2], v[3])};
+        }
+}
+
+// ---------------------------------------------------------------- backward: row statistics
+// lse2 = lse log2 e and delta = sum_d dO O of every row, [B, H, SqP]. Rows that pass no gradient (past the query
+// length, past Sq, or without a key) get lse2 = +inf, which makes their probabilities 0. A row of a head is read by
+// G lanes, 16 bytes of dO and O each.
+template <bool BF16, int G>
+__global__ __launch_bounds__(256) void attn_train_delta_kernel(AttnTrainParams p) {
+    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / G;   // (b, q, head), head fastest
+    const int c = threadIdx.x % G;
+    if (row >= (long long)p.B * p.SqP * p.H) return;
+    const int head = (int)(row % p.H);
+    const long long bq = row / p.H;
+    const int q = (int)(bq % p.SqP), b = (int)(bq / p.SqP);
+    const bool valid = q < atLength(p.qLens, b, p.Sq);
+    float d = 0.f;
+    if (valid && c * 8 < p.D) {
+        const long long at = (((long long)b * p.Sq + q) * p.H + head) * p.D + c * 8;
+        const at_u32x4 g = *reinterpret_cast<const at_u32x4*>(p.gradOut + at);
+        const at_u32x4 o = *reinterpret_cast<const at_u32x4*>(p.out + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float g0, g1, o0, o1;
+            atUnpack2<BF16>(g[e], g0, g1);
+            atUnpack2<BF16>(o[e], o0, o1);
+            d = __builtin_fmaf(g0, o0, d);
+            d = __builtin_fmaf(g1, o1, d);
+        }
+    }
+#pragma unroll
+    for (int s = G / 2; s > 0; s >>= 1) d += __shfl_xor(d, s, 64);
+    if (c) return;
+    const long long bh = (long long)b * p.H + head;
+    float lse2 = INFINITY;
+    if (valid) {
+        const float lse = p.lse[bh * p.Sq + q];
+        if (lse != -INFINITY) lse2 = lse * kAtLog2e;
+    }
+    p.lse2[bh * p.SqP + q] = lse2;
+    p.delta[bh * p.SqP + q] = lse2 == INFINITY ? 0.f : d;
+}
+
+// dS as halves. bf16 has fp32's range; fp16 loses dS below 2^-14 (a probability of 1 / 4096 times a gradient of
+// 2^-10 is there) and has no value past 65504. A lane's dS all go into one column of the sum (its query's dQ, its
+// key's dK), so the lane scales them by a power of two of its own, which starts where its first non-zero ones come
+// to about 2^9 and is lowered, with the sums so far, whenever they would pass 2^15; it is divided out of the column
+// at the end. Powers of two: no rounding of its own.
+template <bool BF16, int KD>
+struct DsScale {
+    float f = BF16 ? 1.f : 0.f;   // 0: no dS yet
+    // x: |dS| of the lane's column at most, in both half-waves
+    __device__ __forceinline__ void update(float x, at_f32x16 (&acc)[KD]) {
+        if constexpr (BF16) return;
+        if (__any(x * f >= 32768.f || (f == 0.f && x > 0.f))) {
+            if (x * f >= 32768.f || (f == 0.f && x > 0.f)) {
+                // 2^9 / 2^(exponent of x), kept within floats' range; infinities and NaN of x stay what they are
+                const int e = (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 255u) - 127;
+                const float next = __builtin_bit_cast(float, (uint32_t)(min(max(9 - e, -60), 60) + 127) << 23);
+                const float r = f == 0.f ? 0.f : next / f;
+                f = next;
+#pragma unroll
+                for (int t = 0; t < KD; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[t][i] *= r;
+            }
+        }
+    }
+    __device__ __forceinline__ float undo() const { return f == 0.f ? 1.f : 1.f / f; }
+};
+
+// Stores a column of a transposed result: rows 32 dt + 8 (r / 4) + 4 h + r % 4 are the head dimension.
+template <bool BF16, int KD>
+__device__ __forceinline__ void storeColumn(uint16_t* row, const at_f32x16 (&acc)[KD], float f, int h, int D, bool zero) {
+#pragma unroll
+    for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * dt + 2 * r + 4 * h;
+            if (d < D)
+                *reinterpret_cast<at_u32x2*>(row + d) =
+                    zero ? at_u32x2{0u, 0u}
+                         : at_u32x2{atPack2<BF16>(acc[dt][r] * f, acc[dt][r + 1] * f),
+                                    atPack2<BF16>(acc[dt][r + 2] * f, acc[dt][r + 3] * f)};
+        }
+}
+
+// ---------------------------------------------------------------- backward: dQ
+// As the forward pass, a wave holds 32 queries as columns and the workgroup walks the keys: S^T = K Q^T,
+// dP^T = V dO^T, dQ^T += K^T dS^T.
+template <bool BF16, int KD>
+__global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p) {
+    using T = AtTile<KD>;
+    __shared__ __attribute__((aligned(256))) uint16_t k0[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t v0[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = lane & 31, h = lane >> 5;
+    uint32_t bh, qb;
+    atPlace(blockIdx.x, p.heads, p.blocks, bh, qb);
+    qb = p.blocks - 1 - qb;   // causal: the longest walks first
+    const int b = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);
+    const int kvHead = head / (p.H / p.Hkv);
+    const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
+    const int off = p.Sk - p.Sq;
+    const int q0 = (int)qb * kBlockQ + wave * 32;
+    const int query = q0 + l;
+    const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
+    const uint16_t* vBase = p.v + (long long)b * p.skv + (long long)kvHead * p.D;
+
+    const int blockLast = min((int)qb * kBlockQ + kBlockQ, nQ) - 1;
+    int kEnd = blockLast >= (int)qb * kBlockQ ? nK : 0;
+    if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
+    int waveEnd = q0 < nQ ? kEnd : 0;
+    if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
+    const int nt = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
+
+    at_u32x4 qf[T::NS], gf[T::NS];
+    {
+        const uint16_t* row = p.q + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
+        const uint16_t* grow = p.gradOut + (((long long)b * p.Sq + query) * p.H + head) * p.D;
+#pragma unroll
+        for (int s = 0; s < T::NS; ++s) {
+            qf[s] = T::direct(row, query < nQ, s, h, p.D);
+            gf[s] = T::direct(grow, query < nQ, s, h, p.D);
+        }
+    }
+    const long long at = (long long)bh * p.SqP + min(query, p.SqP - 1);
+    const float lse2 = p.lse2[at], delta = p.delta[at];   // rows past the query length hold +inf and 0
+    const float c = p.scale * kAtLog2e;
+    typename T::template Copy<kTileKeys, kWaves> copy;
+    const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
+    copy.init(wave, lane, ld2, p.D);
+    auto fetch = [&](int t, uint16_t* kd, uint16_t* vd) {
+        const long long o = (long long)t * kTileKeys * p.ldkv;
+        copy.run(kBase + o, nK - t * kTileKeys, ld2, p.D, kd, wave);
+        copy.run(vBase + o, nK - t * kTileKeys, ld2, p.D, vd, wave);
+    };
+    at_f32x16 dq[KD];
+#pragma unroll
+    for (int t = 0; t < KD; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
+    DsScale<BF16, KD> scale;
+
+    auto tile = [&](int t, const uint16_t* kd, const uint16_t* vd) {
+        const int key0 = t * kTileKeys;
+        const bool edge = key0 + kTileKeys > nK || (p.causal && key0 + kTileKeys - 1 > q0 + off);
+        const int seen = (p.causal ? min(nK, query + off + 1) : nK) - key0 - 4 * h;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            at_f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int st = 0; st < T::NS; ++st) {
+                s = atMfma<BF16>(T::natural(kd, 32 * kb, st, l, h), qf[st], s);
+                dp = atMfma<BF16>(T::natural(vd, 32 * kb, st, l, h), gf[st], dp);
+            }
+            float most = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse2));
+                if (edge && 32 * kb + 8 * (r / 4) + r % 4 >= seen) e = 0.f;
+                s[r] = e * (dp[r] - delta);
+                if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
+            }
+            if constexpr (!BF16) {
+                scale.update(fmaxf(most, atOtherHalf(most)), dq);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= scale.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const at_u32x4 df = atPack8<BF16>(s, u);
+#pragma unroll
+                for (int dt = 0; dt < KD; ++dt)
+                    dq[dt] = atMfma<BF16>(T::transposed(kd, 32 * kb + 16 * u, dt, lane), df, dq[dt]);
+            }
+        }
+    };
+    if (nt > 0) fetch(0, k0, v0);
+    for (int t = 0; t < nt; t += 2) {   // as in the forward pass
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1, k1, v1);
+        if (t * kTileKeys < waveEnd) tile(t, k0, v0);
+        if (t + 1 >= nt) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 2 < nt) fetch(t + 2, k0, v0);
+        if ((t + 1) * kTileKeys < waveEnd) tile(t + 1, k1, v1);
+    }
+    if (query >= p.Sq) return;
+    uint16_t* row = p.dq + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
+    storeColumn<BF16, KD>(row, dq, p.scale * scale.undo(), h, p.D, lse2 == INFINITY);
+}
+
+// ---------------------------------------------------------------- backward: dK and dV
+// A wave holds 32 keys as columns (a workgroup 128) and the workgroup walks the queries of every head that reads them,
+// 64 at a time: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS. fp16 takes P raised by 2^15 (it is at most 1).
+template <bool BF16, int KD>
+__global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(AttnTrainParams p) {
+    using T = AtTile<KD>;
+    constexpr float kRaise = BF16 ? 0.f : 15.f, kLower = BF16 ? 1.f : 1.f / 32768.f;
+    __shared__ __attribute__((aligned(256))) uint16_t q0[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t g0[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) float s0[2 * kTileKeys];   // lse2, delta
+    __shared__ __attribute__((aligned(256))) uint16_t q1[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) uint16_t g1[kTileKeys * T::RS];
+    __shared__ __attribute__((aligned(256))) float s1[2 * kTileKeys];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = lane & 31, h = lane >> 5;
+    uint32_t bh, block;
+    atPlace(blockIdx.x, p.heads, p.blocks, bh, block);   // causal: the first keys have the longest walks
+    const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv);
+    const int group = p.H / p.Hkv;
+    const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
+    const int off = p.Sk - p.Sq;
+    const int key0 = (int)block * kBlockQ + wave * 32;
+    const int key = key0 + l;
+
+    // query tiles that see a key of the workgroup: t0 .. t1 of each head of the group
+    const int t0 = p.causal ? max(0, (int)block * kBlockQ - off) / kTileKeys : 0;
+    const int t1 = (int)block * kBlockQ < nK ? (nQ + kTileKeys - 1) / kTileKeys : 0;
+    const int per = max(0, t1 - t0), total = per * group;
+
+    at_u32x4 kf[T::NS], vf[T::NS];
+    {
+        const long long at = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
+#pragma unroll
+        for (int s = 0; s < T::NS; ++s) {
+            kf[s] = T::direct(p.k + at, key < nK, s, h, p.D);
+            vf[s] = T::direct(p.v + at, key < nK, s, h, p.D);
+        }
+    }
+    const float c = p.scale * kAtLog2e;
+    typename T::template Copy<kTileKeys, kWaves> copyQ, copyG;
+    const uint32_t ldq2 = (uint32_t)p.ldq * 2u, ldg2 = (uint32_t)(p.H * p.D) * 2u;
+    copyQ.init(wave, lane, ldq2, p.D);
+    copyG.init(wave, lane, ldg2, p.D);
+    auto fetch = [&](int i, uint16_t* qd, uint16_t* gd, float* sd) {
+        const int head = kvHead * group + i / per, t = t0 + i % per;
+        const long long first = (long long)t * kTileKeys;
+        copyQ.run(p.q + (long long)b * p.sq + first * p.ldq + (long long)head * p.D, nQ - t * kTileKeys, ldq2, p.D, qd, wave);
+        copyG.run(p.gradOut + (((long long)b * p.Sq + first) * p.H + head) * p.D, nQ - t * kTileKeys, ldg2, p.D, gd, wave);
+        if (wave < 2) {   // rows past the query length hold +inf and 0
+            const float* from = (wave == 0 ? p.lse2 : p.delta) + ((long long)b * p.H + head) * p.SqP + first;
+            atCopy4(atView(from, kTileKeys * 4), sd + wave * kTileKeys, lane * 4);
+        }
+    };
+    at_f32x16 dk[KD], dv[KD];
+#pragma unroll
+    for (int t = 0; t < KD; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
+    DsScale<BF16, KD> scale;
+
+    auto tile = [&](int i, const uint16_t* qd, const uint16_t* gd, const float* sd) {
+        const int first = (t0 + i % per) * kTileKeys;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            const int qs = first + 32 * qb;
+            if (p.causal && qs + 31 + off < key0) continue;   // none of these queries sees the wave's keys
+            at_f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int st = 0; st < T::NS; ++st) {
+                s = atMfma<BF16>(T::natural(qd, 32 * qb, st, l, h), kf[st], s);
+                dp = atMfma<BF16>(T::natural(gd, 32 * qb, st, l, h), vf[st], dp);
+            }
+            const bool edge = p.causal && qs + off < key0 + 31;
+            const int firstSeen = key - off - qs - 4 * h;   // rows from here on see the lane's key
+            float most = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const at_f32x4 lse2 = *reinterpret_cast<const at_f32x4*>(sd + 32 * qb + 8 * j + 4 * h);
+                const at_f32x4 delta = *reinterpret_cast<const at_f32x4*>(sd + kTileKeys + 32 * qb + 8 * j + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * j + e;
+                    float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, kRaise - lse2[e]));
+                    if (edge && 8 * j + e < firstSeen) w = 0.f;
+                    s[r] = w;
+                    dp[r] = w * (dp[r] - delta[e]);
+                    if constexpr (!BF16) most = fmaxf(most, fabsf(dp[r]));
+                }
+            }
+            if constexpr (!BF16) {
+                scale.update(fmaxf(most, atOtherHalf(most)), dk);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] *= scale.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const at_u32x4 pf = atPack8<BF16>(s, u), df = atPack8<BF16>(dp, u);
+#pragma unroll
+                for (int dt = 0; dt < KD; ++dt) {
+                    dv[dt] = atMfma<BF16>(T::transposed(gd, 32 * qb + 16 * u, dt, lane), pf, dv[dt]);
+                    dk[dt] = atMfma<BF16>(T::transposed(qd, 32 * qb + 16 * u, dt, lane), df, dk[dt]);
+                }
+            }
+        }
+    };
+    if (total > 0) fetch(0, q0, g0, s0);
+    for (int i = 0; i < total; i += 2) {   // as in the forward pass
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (i + 1 < total) fetch(i + 1, q1, g1, s1);
+        if (key0 < nK) tile(i, q0, g0, s0);
+        if (i + 1 >= total) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (i + 2 < total) fetch(i + 2, q0, g0, s0);
+        if (key0 < nK) tile(i + 1, q1, g1, s1);
+    }
+    if (key >= p.Sk) return;
+    const long long at = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
+    storeColumn<BF16, KD>(p.dk + at, dk, p.scale * kLower * scale.undo(), h, p.D, key >= nK);
+    storeColumn<BF16, KD>(p.dv + at, dv, kLower, h, p.D, key >= nK);
+}
+
+// ---------------------------------------------------------------- checks and launches
+template <bool BF16, int KD>
+int launchForward(AttnTrainParams& p) {
+    p.heads = (uint32_t)(p.B * p.H);
+    p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
+    hipLaunchKernelGGL((attn_train_forward_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+template <bool BF16, int G>
+int launchDelta(const AttnTrainParams& p, long long rows) {
+    hipLaunchKernelGGL((attn_train_delta_kernel<BF16, G>), dim3((unsigned)((rows * G + 255) / 256)), dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+template <bool BF16, int KD>
+int launchBackward(AttnTrainParams& p) {
+    if (p.Sq > 0) {
+        const long long rows = (long long)p.B * p.SqP * p.H;
+        const int rc = KD == 4 || KD == 3 ? launchDelta<BF16, 16>(p, rows) : KD == 2 ? launchDelta<BF16, 8>(p, rows)
+                                                                                     : launchDelta<BF16, 4>(p, rows);
+        if (rc) return rc;
+        p.heads = (uint32_t)(p.B * p.H);
+        p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
+        hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
+        OMHIP_CHECK_LAUNCH();
+    }
+    if (p.Sk > 0) {
+        p.heads = (uint32_t)(p.B * p.Hkv);
+        p.blocks = (uint32_t)((p.Sk + kBlockQ - 1) / kBlockQ);
+        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
+        OMHIP_CHECK_LAUNCH();
+    }
+    return 0;
+}
+
+template <bool BF16>
+int forward(AttnTrainParams& p) {
+    switch ((p.D + 31) / 32) {
+        case 1: return launchForward<BF16, 1>(p);
+        case 2: return launchForward<BF16, 2>(p);
+        case 3: return launchForward<BF16, 3>(p);
+        default: return launchForward<BF16, 4>(p);
+    }
+}
+
+template <bool BF16>
+int backward(AttnTrainParams& p) {
+    switch ((p.D + 31) / 32) {
+        case 1: return launchBackward<BF16, 1>(p);
+        case 2: return launchBackward<BF16, 2>(p);
+        case 3: return launchBackward<BF16, 3>(p);
+        default: return launchBackward<BF16, 4>(p);
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What both directions ask of their sizes; 0, 1 (nothing to do) or -1.
+int checkSizes(const char* name, int nDtype, long long nLdQ, long long nStrideQ, long long nLdKV, long long nStrideKV,
+               int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale) {
+    if (nDtype != 0 && nDtype != 1) return fail("%s: dtype must be 0 (fp16) or 1 (bf16)", name);
+    if (nBatch < 0 || nSeqQ < 0 || nSeqK < 0) return fail("%s: negative size", name);
+    if (nHeads < 1 || nKVHeads < 1 || nHeads % nKVHeads != 0)
+        return fail("%s: %d query heads are not a multiple of %d key heads", name, nHeads, nKVHeads);
+    if (nHeadDim < 8 || nHeadDim > 128 || nHeadDim % 8 != 0)
+        return fail("%s: head dimension %d (supported: multiples of 8 up to 128)", name, nHeadDim);
+    if (!std::isfinite(fScale)) return fail("%s: scale must be finite", name);
+    if (nLdQ < (long long)nHeads * nHeadDim || nLdKV < (long long)nKVHeads * nHeadDim)
+        return fail("%s: a row stride is below the heads' width", name);
+    if (nLdQ >= kAtMaxLd || nLdKV >= kAtMaxLd) return fail("%s: a row stride reaches 2^23 elements", name);
+    if ((nLdQ | nStrideQ | nLdKV | nStrideKV) & 7) return fail("%s: strides must be multiples of 8 elements", name);
+    if (nStrideQ < 0 || nStrideKV < 0) return fail("%s: negative stride", name);
+    // grid and row counters
+    if (nSeqQ > (1 << 30) || nSeqK > (1 << 30)) return fail("%s: a sequence exceeds 2^30 tokens", name);
+    if ((long long)nBatch * nHeads * ((std::max(nSeqQ, nSeqK) + 63LL) / 64) > 0x3fffffffLL)
+        return fail("%s: too many (image, head, token) triples", name);
+    return nBatch == 0 ? 1 : 0;
+}
+
+}  // namespace
+
+}  // namespace omhip
+
+using namespace omhip;
+
+extern "C" {
+
+int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                   long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                   const int* pKeyLens, int bCausal, uint16_t* pOut, float* pLse, int nBatch, int nSeqQ,
+                                   int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale) {
+    const char* name = "omHipAttentionTrainForwardHalf";
+    clearError();
+    const int rc = checkSizes(name, nDtype, nLdQ, nStrideQ, nLdKV, nStrideKV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                              nHeadDim, fScale);
+    if (rc < 0) return -1;
+    if (rc || nSeqQ == 0) return 0;
+    if (!pQ || !pOut || !pLse || (nSeqK > 0 && (!pK || !pV))) return fail("%s: null pointer", name);
+    if (!aligned16(pQ) || !aligned16(pK) || !aligned16(pV) || !aligned16(pOut))
+        return fail("%s: data must be 16-byte aligned", name);
+    AttnTrainParams p{};
+    p.q = pQ; p.k = pK; p.v = pV;
+    p.ldq = nLdQ; p.sq = nStrideQ; p.ldkv = nLdKV; p.skv = nStrideKV;
+    p.qLens = pQueryLens; p.kLens = pKeyLens;
+    p.B = nBatch; p.Sq = nSeqQ; p.Sk = nSeqK; p.H = nHeads; p.Hkv = nKVHeads; p.D = nHeadDim;
+    p.causal = bCausal != 0;
+    p.scale = fScale;
+    p.out = pOut; p.lse = pLse;
+    return nDtype == 1 ? forward<true>(p) : forward<false>(p);
+}
+
+int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                               long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                               const int* pKeyLens, int bCausal, const uint16_t* pOut, const float* pLse,
+                               const uint16_t* pGradOut, uint16_t* pGradQ, uint16_t* pGradK, uint16_t* pGradV, int nBatch,
+                               int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale) {
+    const char* name = "omHipAttentionBackwardHalf";
+    clearError();
+    const int rc = checkSizes(name, nDtype, nLdQ, nStrideQ, nLdKV, nStrideKV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                              nHeadDim, fScale);
+    if (rc < 0) return -1;
+    if (rc || (nSeqQ == 0 && nSeqK == 0)) return 0;
+    if ((nSeqQ > 0 && (!pQ || !pOut || !pLse || !pGradOut || !pGradQ)) || (nSeqK > 0 && (!pK || !pV || !pGradK || !pGradV)))
+        return fail("%s: null pointer", name);
+    for (const void* x : {(const void*)pQ, (const void*)pK, (const void*)pV, (const void*)pOut, (const void*)pGradOut,
+                          (const void*)pGradQ, (const void*)pGradK, (const void*)pGradV})
+        if (!aligned16(x)) return fail("%s: data must be 16-byte aligned", name);
+    AttnTrainParams p{};
+    p.q = pQ; p.k = pK; p.v = pV;
+    p.ldq = nLdQ; p.sq = nStrideQ; p.ldkv = nLdKV; p.skv = nStrideKV;
+    p.qLens = pQueryLens; p.kLens = pKeyLens;
+    p.B = nBatch; p.Sq = nSeqQ; p.Sk = nSeqK; p.H = nHeads; p.Hkv = nKVHeads; p.D = nHeadDim;
+    p.causal = bCausal != 0;
+    p.scale = fScale;
+    p.out = const_cast<uint16_t*>(pOut); p.lse = const_cast<float*>(pLse);
+    p.gradOut = pGradOut;
+    p.dq = pGradQ; p.dk = pGradK; p.dv = pGradV;
+    p.SqP = (nSeqQ + kTileKeys - 1) / kTileKeys * kTileKeys;
+    const size_t rows = (size_t)nBatch * nHeads * p.SqP;
+    if (rows) {
+        p.lse2 = static_cast<float*>(workspace(rows * 2 * sizeof(float), kWsOperand));
+        if (!p.lse2) return -1;   // workspace() recorded the cause
+        p.delta = p.lse2 + rows;
+    }
+    return nDtype == 1 ? backward<true>(p) : backward<false>(p);
+}
+
+}  // extern "C"
