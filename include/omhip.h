@@ -521,6 +521,46 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
                                const uint16_t* pGradOut, uint16_t* pGradQ, uint16_t* pGradK, uint16_t* pGradV, int nBatch,
                                int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale);
 
+/* ===== dropout (omCudaDropout, cuda_kernels.cu:2266-2337, keeps a float mask; here the mask is a
+ * function of the generator's state and is never stored) ===== */
+
+/* NEW: pOut [nRows, nCols] = keep ? (pX + pBias[column]) * s : 0, + pResidual, in fp32, rounded
+ * once to the type. nDtype 0 binary16, 1 bfloat16, 2 fp32 (pX, pResidual, pOut); pBias [nCols]
+ * fp32 and pResidual may be NULL; pOut may be pX or pResidual.
+ * Bits: Philox4x32-10 with key (seed low, seed high) and counter (group, nStream, step low, step
+ * high), group = row * ceil(nCols / 8) + column / 8; column j of a group takes half j % 2 (low
+ * first) of word j / 2. keep: the 16 bits are at least T = round(65536 fProb); s = 65536 / (65536
+ * - T) (0 where T is 65536). pRng: {seed, step}, two 64-bit words on the device, read when the
+ * kernel runs, so a captured graph draws anew once they are changed; nStream tells the dropouts
+ * of one step apart. fProb within 0 .. 1; at most 2^31 - 1 groups. */
+int omHipDropout(int nDtype, const void* pX, const float* pBias, const void* pResidual, void* pOut, int nRows, int nCols,
+                 float fProb, const uint64_t* pRng, int nStream);
+/* NEW: the gradient of omHipDropout with the same fProb, state and nStream: pGradX = keep ?
+ * pGradOut * s : 0 in nDtype (the residual's gradient is pGradOut itself) and, where it is not
+ * NULL, pGradBias [nCols] fp32 = the sums of the unrounded pGradX over the rows, in a fixed order.
+ * pGradX may be pGradOut. */
+int omHipDropoutBackward(int nDtype, const void* pGradOut, void* pGradX, float* pGradBias, int nRows, int nCols, float fProb,
+                         const uint64_t* pRng, int nStream);
+
+/* ===== group norm, channels last (omCudaGroupNorm, cuda_kernels.cu:3205-3490, is NCHW and runs
+ * the activation apart) ===== */
+
+/* NEW: pY = act((x - mean) / sqrt(var + fEps) * pGamma + pBeta) on x [nBatch, nPixels, nChannels]
+ * (tokens), mean and biased variance over the pixels and the nChannels / nGroups channels of a
+ * group. nDtype 0 binary16, 1 bfloat16, 2 fp32 (pX, pY); statistics and pGamma, pBeta [nChannels]
+ * (NULL: 1, 0) fp32. nAct 0 none, 1 ReLU, 2 SiLU (z / (1 + exp(-z))). pMean and pInvStd [nBatch,
+ * nGroups] (may be NULL) receive mean and 1 / sqrt(var + fEps) for the backward pass. Statistics
+ * hold for means far above the spread; they are added in a fixed order. pY may be pX. nBatch at
+ * most 65535. */
+int omHipGroupNormNhwc(int nDtype, const void* pX, const float* pGamma, const float* pBeta, void* pY, float* pMean,
+                       float* pInvStd, int nBatch, int nPixels, int nChannels, int nGroups, float fEps, int nAct);
+/* NEW: the gradients of omHipGroupNormNhwc from pX and its saved pMean and pInvStd: pGradX in
+ * nDtype, pGradGamma and pGradBeta [nChannels] fp32 (each may be NULL). nAct 1 takes its gate from
+ * the saved output pY (> 0), which the other activations do not read (NULL). pGradX may be pGradY. */
+int omHipGroupNormNhwcBackward(int nDtype, const void* pGradY, const void* pX, const void* pY, const float* pMean,
+                               const float* pInvStd, const float* pGamma, const float* pBeta, void* pGradX, float* pGradGamma,
+                               float* pGradBeta, int nBatch, int nPixels, int nChannels, int nGroups, int nAct);
+
 /* ===== device-resident inference (EngineBridge::inferBatch, EngineBridge.cpp:3525-3772) ===== */
 
 /* NEW: a ResNet-18 classifier (torchvision layout, 3x224x224 input) resident on the device,

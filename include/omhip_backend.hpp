@@ -283,6 +283,32 @@ public:
                                          nSeqK, nHeads, nKVHeads, nHeadDim, fScale),
               "attentionBackwardHalf");
     }
+    // Dropout with a mask that is a function of the generator's state (pRng, device: seed, step), nStream and the place:
+    // keep ? (x + bias) * s : 0, + residual (both nullable); nDtype 0 fp16, 1 bf16, 2 fp32
+    static void dropout(int nDtype, const void* pX, const float* pBias, const void* pResidual, void* pOut, int nRows,
+                        int nCols, float fProb, const uint64_t* pRng, int nStream) {
+        check(omHipDropout(nDtype, pX, pBias, pResidual, pOut, nRows, nCols, fProb, pRng, nStream), "dropout");
+    }
+    static void dropoutBackward(int nDtype, const void* pGradOut, void* pGradX, float* pGradBias, int nRows, int nCols,
+                                float fProb, const uint64_t* pRng, int nStream) {
+        check(omHipDropoutBackward(nDtype, pGradOut, pGradX, pGradBias, nRows, nCols, fProb, pRng, nStream),
+              "dropoutBackward");
+    }
+    // Group norm of [batch, pixels, channels] with an activation (0 none, 1 ReLU, 2 SiLU), and its gradients
+    static void groupNormNhwc(int nDtype, const void* pX, const float* pGamma, const float* pBeta, void* pY, float* pMean,
+                              float* pInvStd, int nBatch, int nPixels, int nChannels, int nGroups, float fEps, int nAct) {
+        check(omHipGroupNormNhwc(nDtype, pX, pGamma, pBeta, pY, pMean, pInvStd, nBatch, nPixels, nChannels, nGroups, fEps,
+                                 nAct),
+              "groupNormNhwc");
+    }
+    static void groupNormNhwcBackward(int nDtype, const void* pGradY, const void* pX, const void* pY, const float* pMean,
+                                      const float* pInvStd, const float* pGamma, const float* pBeta, void* pGradX,
+                                      float* pGradGamma, float* pGradBeta, int nBatch, int nPixels, int nChannels,
+                                      int nGroups, int nAct) {
+        check(omHipGroupNormNhwcBackward(nDtype, pGradY, pX, pY, pMean, pInvStd, pGamma, pBeta, pGradX, pGradGamma,
+                                         pGradBeta, nBatch, nPixels, nChannels, nGroups, nAct),
+              "groupNormNhwcBackward");
+    }
     // Linear::forward (linear.ixx:50-58) on half inputs: act(x W + b), W [K,N] ([N,K] when bTransW)
     static void linearHalf(int nDtype, const uint16_t* pInput, const uint16_t* pWeight, bool bTransW,
                            const float* pBias, int nAct, void* pOutput, bool bOutHalf, int nM, int nK, int nN) {

@@ -131,6 +131,10 @@ _SIGS = {
     "omHipMultiHeadAttentionHalf": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i],
     "omHipAttentionTrainForwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i, _vp, _vp] + [_i] * 6 + [_fl],
     "omHipAttentionBackwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i] + [_vp] * 6 + [_i] * 6 + [_fl],
+    "omHipDropout": [_i, _vp, _vp, _vp, _vp, _i, _i, _fl, _vp, _i],
+    "omHipDropoutBackward": [_i, _vp, _vp, _vp, _i, _i, _fl, _vp, _i],
+    "omHipGroupNormNhwc": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _fl, _i],
+    "omHipGroupNormNhwcBackward": [_i] + [_vp] * 10 + [_i] * 5,
     "omHipConvertF32ToF16": [_vp, _vp, _i],
     "omHipConvertF32ToBF16": [_vp, _vp, _i],
     "omHipConvertF16ToF32": [_vp, _vp, _i],
@@ -573,6 +577,35 @@ class HIPBackend:
         call("omHipAttentionBackwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV,
              nStrideKV, _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, _ptr(pOut), _ptr(pLse), _ptr(pGradOut),
              _ptr(pGradQ), _ptr(pGradK), _ptr(pGradV), nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
+
+    @staticmethod
+    def dropout(pX, pBias, pResidual, pOut, nRows, nCols, fProb, pRng, nStream, nDtype: int = 2) -> None:
+        """keep ? (x + bias) * s : 0, + residual; the mask is a function of pRng (device: seed, step), nStream and the
+        place (bias and residual may be None). nDtype 0 fp16, 1 bf16, 2 fp32."""
+        call("omHipDropout", nDtype, _ptr(pX), _ptr(pBias), _ptr(pResidual), _ptr(pOut), nRows, nCols, fProb, _ptr(pRng),
+             nStream)
+
+    @staticmethod
+    def dropoutBackward(pGradOut, pGradX, pGradBias, nRows, nCols, fProb, pRng, nStream, nDtype: int = 2) -> None:
+        """dropout's gradient with the same bits; pGradBias (fp32 column sums) may be None."""
+        call("omHipDropoutBackward", nDtype, _ptr(pGradOut), _ptr(pGradX), _ptr(pGradBias), nRows, nCols, fProb,
+             _ptr(pRng), nStream)
+
+    @staticmethod
+    def groupNormNhwc(pX, pGamma, pBeta, pY, pMean, pInvStd, nBatch, nPixels, nChannels, nGroups, fEps, nAct,
+                      nDtype: int = 2) -> None:
+        """act(group norm) of [batch, pixels, channels]; nAct 0 none, 1 ReLU, 2 SiLU. Gamma, beta and the saved
+        statistics may be None."""
+        call("omHipGroupNormNhwc", nDtype, _ptr(pX), _ptr(pGamma), _ptr(pBeta), _ptr(pY), _ptr(pMean), _ptr(pInvStd),
+             nBatch, nPixels, nChannels, nGroups, fEps, nAct)
+
+    @staticmethod
+    def groupNormNhwcBackward(pGradY, pX, pY, pMean, pInvStd, pGamma, pBeta, pGradX, pGradGamma, pGradBeta, nBatch, nPixels,
+                              nChannels, nGroups, nAct, nDtype: int = 2) -> None:
+        """groupNormNhwc's gradients from the saved statistics; pY (the saved output) is read for ReLU only."""
+        call("omHipGroupNormNhwcBackward", nDtype, _ptr(pGradY), _ptr(pX), _ptr(pY), _ptr(pMean), _ptr(pInvStd),
+             _ptr(pGamma), _ptr(pBeta), _ptr(pGradX), _ptr(pGradGamma), _ptr(pGradBeta), nBatch, nPixels, nChannels,
+             nGroups, nAct)
 
     @staticmethod
     def linearHalf(pInput, pWeight, pBias, pOutput, nM, nK, nN, bf16: bool = False, transW: bool = False,

@@ -28,7 +28,8 @@ DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 COMMON = ["-O3", "-std=c++20", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
 
 SOURCES = ["runtime.cpp", "eltwise.hip", "gemm_f32.hip", "conv.hip", "conv_stem.hip", "conv_wgrad.hip", "gemm_half.hip", "gemm_half_heads.hip", "train.hip",
-           "pool.hip", "attention.hip", "attention_f32.hip", "attn_train.hip", "infer.hip", "loss.hip", "mha.hip", "heads.hip"]
+           "pool.hip", "attention.hip", "attention_f32.hip", "attn_train.hip", "infer.hip", "loss.hip", "mha.hip", "heads.hip",
+           "dropout.hip", "group_norm.hip"]
 # conv tiles keep at most 128 accumulators per lane: forcing the VGPR form of
 # the MFMA operands stops the register allocator from copying every
 # accumulator between AGPRs and VGPRs on each trip of the mainloop (and, in

@@ -1,0 +1,473 @@
+// group_norm.hip — group normalisation with an activation on channels-last
+// data [image, pixel, channel] (the layout of transformer tokens), forward and
+// backward.
+//
+// The reference normalises groups of an NCHW tensor and runs the activation as
+// its own pass (omCudaGroupNorm, cuda_kernels.cu:3205-3490). Over the pixels
+// and the C / G channels of group g of image n:
+//   xhat = (x - mean) inv, inv = 1 / sqrt(var + eps); z = xhat gamma + beta; y = act(z)
+//   backward, dz = dy act'(z): dbeta = sum dz, dgamma = sum dz xhat over images and pixels,
+//   dx = inv (gamma dz - mean_g(gamma dz) - xhat mean_g(gamma dz xhat))
+//
+// Both directions are bound by memory: one pass that leaves per-channel sums of
+// a chunk of an image's pixels, one small launch that joins them, one pass that
+// writes the result. A thread holds 8 neighbouring channels of a row (16 bytes
+// of halves), so every access is a stretch of whole rows.
+//
+// Variance: a thread adds x - k and (x - k)^2 with k its own first value of the
+// channel, turns them into (count, mean, sum of squared differences from the
+// mean), and those are joined pairwise, M = Ma + Mb + (mb - ma)^2 na nb / n
+// (T. F. Chan, G. H. Golub, R. J. LeVeque, "Updating formulae and a pairwise
+// algorithm for computing sample variances", 1979): a mean far above the
+// spread costs no digits. The order is fixed; nothing is added atomically.
+#include "omhip_internal.hpp"
+#include "vec_io.hpp"
+#include "../../include/omhip.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace omhip {
+
+namespace {
+
+struct GroupNormParams {
+    const void *x, *y, *gradY;
+    void* out;                      // y or dx
+    const float *gamma, *beta;      // null: 1, 0
+    float *mean, *inv;              // [N, G]
+    float2* partial;                // [N, chunks, C]: forward (mean, M), backward (sum dz, sum dz xhat)
+    float2* means;                  // backward, [N, G]: the group means of gamma dz and gamma dz xhat
+    float *gradGamma, *gradBeta;    // or null
+    int N, P, C, G, per;            // per: channels of a group
+    int chunks, rowsPerChunk;
+    float eps;
+};
+
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2 };
+
+// (count, mean, sum of squared differences) of a and b together.
+struct Moments {
+    float n, mean, m2;
+};
+__device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
+    const float n = a.n + b.n;
+    if (b.n == 0.f) return a;
+    const float d = b.mean - a.mean, f = b.n / n;
+    return {n, __builtin_fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+}
+
+// Rows of a chunk.
+__device__ __forceinline__ int chunkRows(const GroupNormParams& p, int chunk) {
+    return min(p.P - chunk * p.rowsPerChunk, p.rowsPerChunk);
+}
+
+// Where a thread of a pass works: 8 channels from c on (n of them exist), rows tr, tr + TR, ... of its chunk.
+template <int TC>
+struct Place {
+    static constexpr int TR = 256 / TC;
+    int c, n, tr, first, rows, image, chunk;
+    long long base;   // element of the image's first row
+    __device__ __forceinline__ explicit Place(const GroupNormParams& p) {
+        c = ((int)blockIdx.x * TC + (int)threadIdx.x % TC) * 8;
+        n = min(8, p.C - c);
+        tr = threadIdx.x / TC;
+        chunk = blockIdx.y;
+        image = blockIdx.z;
+        first = chunk * p.rowsPerChunk;
+        rows = chunkRows(p, chunk);
+        base = (long long)image * p.P * p.C;
+    }
+    __device__ __forceinline__ long long at(const GroupNormParams& p, int r) const {
+        return base + (long long)(first + r) * p.C + c;
+    }
+};
+
+// What a thread needs of its channels.
+struct Channels {
+    float mean[8], inv[8], gamma[8], beta[8];
+    __device__ __forceinline__ void load(const GroupNormParams& p, int image, int c, int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = i < n;
+            const int g = in ? (c + i) / p.per : 0;
+            mean[i] = p.mean[(long long)image * p.G + g];
+            inv[i] = p.inv[(long long)image * p.G + g];
+            gamma[i] = in && p.gamma ? p.gamma[c + i] : 1.f;
+            beta[i] = in && p.beta ? p.beta[c + i] : 0.f;
+        }
+    }
+};
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == kActRelu) return z > 0.f ? z : 0.f;
+    if constexpr (ACT == kActSilu) return z * sigmoid(z);
+    return z;
+}
+
+// dz of dy. ReLU's gate is the saved output, so no rounding of z decides it.
+template <int ACT>
+__device__ __forceinline__ float gradient(float dy, float z, float y) {
+    if constexpr (ACT == kActRelu) return y > 0.f ? dy : 0.f;
+    if constexpr (ACT == kActSilu) {
+        const float s = sigmoid(z);
+        return dy * s * __builtin_fmaf(z, 1.f - s, 1.f);
+    }
+    return dy;
+}
+
+// ---------------------------------------------------------------- forward
+template <int DT, int TC>
+__global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams p) {
+    using W = Place<TC>;
+    __shared__ float2 part[8][256];
+    const W w(p);
+    float shift[8], s[8], q[8];
+    float count = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) shift[i] = s[i] = q[i] = 0.f;
+    if (w.n > 0) {
+        if (w.tr < w.rows) Vec8<DT>::load(p.x, w.at(p, w.tr), w.n, shift);
+        for (int r = w.tr; r < w.rows; r += W::TR) {
+            float x[8];
+            Vec8<DT>::load(p.x, w.at(p, r), w.n, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = x[i] - shift[i];
+                s[i] += d;
+                q[i] = __builtin_fmaf(d, d, q[i]);
+            }
+            count += 1.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float m = count > 0.f ? s[i] / count : 0.f;
+        part[i][threadIdx.x] = {shift[i] + m, fmaxf(__builtin_fmaf(-m, s[i], q[i]), 0.f)};
+    }
+    // row threads tr and tr + half together, half = TR / 2 .. 1; thread tr then stands for rows tr, tr + half, ...
+#pragma unroll
+    for (int half = W::TR / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (w.tr < half) {
+            auto rowsOf = [&](int tr) { return (float)(tr < w.rows ? (w.rows - tr + 2 * half - 1) / (2 * half) : 0); };
+            const float na = rowsOf(w.tr), nb = rowsOf(w.tr + half);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 a = part[i][threadIdx.x], b = part[i][threadIdx.x + half * TC];
+                const Moments j = join({na, a.x, a.y}, {nb, b.x, b.y});
+                part[i][threadIdx.x] = {j.mean, j.m2};
+            }
+        }
+    }
+    if (w.tr == 0 && w.n > 0) {
+        float2* to = p.partial + ((long long)w.image * p.chunks + w.chunk) * p.C + w.c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < w.n) to[i] = part[i][threadIdx.x];
+    }
+}
+
+// One wave per (image, group).
+__global__ __launch_bounds__(64) void group_norm_join_kernel(GroupNormParams p) {
+    const int g = blockIdx.x, image = blockIdx.y, lane = threadIdx.x;
+    const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
+    Moments t{0.f, 0.f, 0.f};
+    for (long long e = lane; e < (long long)p.chunks * p.per; e += 64) {
+        const int chunk = (int)(e / p.per), c = (int)(e - (long long)chunk * p.per);
+        const float2 v = from[(long long)chunk * p.C + c];
+        t = join(t, {(float)chunkRows(p, chunk), v.x, v.y});
+    }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+        t = join(t, {__shfl_down(t.n, s, 64), __shfl_down(t.mean, s, 64), __shfl_down(t.m2, s, 64)});
+    if (lane == 0) {
+        p.mean[(long long)image * p.G + g] = t.mean;
+        p.inv[(long long)image * p.G + g] = 1.f / sqrtf(t.m2 / t.n + p.eps);
+    }
+}
+
+template <int DT, int TC, int ACT>
+__global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p) {
+    using W = Place<TC>;
+    const W w(p);
+    if (w.n <= 0) return;
+    Channels ch;
+    ch.load(p, w.image, w.c, w.n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ch.inv[i] *= ch.gamma[i];
+    for (int r = w.tr; r < w.rows; r += W::TR) {
+        float x[8];
+        Vec8<DT>::load(p.x, w.at(p, r), w.n, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = activate<ACT>(__builtin_fmaf(x[i] - ch.mean[i], ch.inv[i], ch.beta[i]));
+        Vec8<DT>::store(p.out, w.at(p, r), w.n, x);
+    }
+}
+
+// ---------------------------------------------------------------- backward
+// xhat and dz of 8 channels of a row
+template <int DT, int ACT>
+__device__ __forceinline__ void loadRow(const GroupNormParams& p, const Channels& ch, long long at, int n, float (&xhat)[8],
+                                        float (&dz)[8]) {
+    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    Vec8<DT>::load(p.x, at, n, xhat);
+    Vec8<DT>::load(p.gradY, at, n, dz);
+    if constexpr (ACT == kActRelu) Vec8<DT>::load(p.y, at, n, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        xhat[i] = (xhat[i] - ch.mean[i]) * ch.inv[i];
+        dz[i] = gradient<ACT>(dz[i], __builtin_fmaf(xhat[i], ch.gamma[i], ch.beta[i]), y[i]);
+    }
+}
+
+template <int DT, int TC, int ACT>
+__global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p) {
+    using W = Place<TC>;
+    __shared__ float2 part[8][256];
+    const W w(p);
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+    if (w.n > 0) {
+        Channels ch;
+        ch.load(p, w.image, w.c, w.n);
+        for (int r = w.tr; r < w.rows; r += W::TR) {
+            float xhat[8], dz[8];
+            loadRow<DT, ACT>(p, ch, w.at(p, r), w.n, xhat, dz);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] += dz[i];
+                b[i] = __builtin_fmaf(dz[i], xhat[i], b[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[i][threadIdx.x] = {a[i], b[i]};
+#pragma unroll
+    for (int half = W::TR / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (w.tr < half)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 u = part[i][threadIdx.x], v = part[i][threadIdx.x + half * TC];
+                part[i][threadIdx.x] = {u.x + v.x, u.y + v.y};
+            }
+    }
+    if (w.tr == 0 && w.n > 0) {
+        float2* to = p.partial + ((long long)w.image * p.chunks + w.chunk) * p.C + w.c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < w.n) to[i] = part[i][threadIdx.x];
+    }
+}
+
+// Workgroups 0 .. N * G - 1: a group's means of gamma dz and gamma dz xhat. The others: dgamma and dbeta of 32
+// channels, eight interleaved runs over images and chunks a channel.
+__global__ __launch_bounds__(256) void group_norm_join_backward_kernel(GroupNormParams p) {
+    __shared__ float2 part[256];
+    const int t = threadIdx.x;
+    float2 s{0.f, 0.f};
+    const long long groups = (long long)p.N * p.G;
+    if (blockIdx.x < groups) {
+        const int image = (int)(blockIdx.x / p.G), g = (int)(blockIdx.x % p.G);
+        const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
+        for (long long e = t; e < (long long)p.chunks * p.per; e += 256) {
+            const int chunk = (int)(e / p.per), c = (int)(e - (long long)chunk * p.per);
+            const float2 v = from[(long long)chunk * p.C + c];
+            const float gamma = p.gamma ? p.gamma[g * p.per + c] : 1.f;
+            s.x = __builtin_fmaf(gamma, v.x, s.x);
+            s.y = __builtin_fmaf(gamma, v.y, s.y);
+        }
+        part[t] = s;
+#pragma unroll
+        for (int half = 128; half > 0; half /= 2) {
+            __syncthreads();
+            if (t < half) part[t] = {part[t].x + part[t + half].x, part[t].y + part[t + half].y};
+        }
+        if (t == 0) {
+            const float f = 1.f / ((float)p.P * (float)p.per);
+            p.means[blockIdx.x] = {part[0].x * f, part[0].y * f};
+        }
+        return;
+    }
+    const int c = (int)(blockIdx.x - groups) * 32 + (t & 31);
+    if (c < p.C)
+        for (long long e = t >> 5; e < (long long)p.N * p.chunks; e += 8) {
+            const float2 v = p.partial[e * p.C + c];
+            s.x += v.x;
+            s.y += v.y;
+        }
+    part[t] = s;
+    __syncthreads();
+    if (t < 32 && c < p.C) {
+        s = {0.f, 0.f};
+        for (int i = 0; i < 8; ++i) s = {s.x + part[t + 32 * i].x, s.y + part[t + 32 * i].y};
+        if (p.gradBeta) p.gradBeta[c] = s.x;
+        if (p.gradGamma) p.gradGamma[c] = s.y;
+    }
+}
+
+template <int DT, int TC, int ACT>
+__global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParams p) {
+    using W = Place<TC>;
+    const W w(p);
+    if (w.n <= 0) return;
+    Channels ch;
+    ch.load(p, w.image, w.c, w.n);
+    float2 m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] = p.means[(long long)w.image * p.G + (i < w.n ? (w.c + i) / p.per : 0)];
+    for (int r = w.tr; r < w.rows; r += W::TR) {
+        float xhat[8], dz[8];
+        loadRow<DT, ACT>(p, ch, w.at(p, r), w.n, xhat, dz);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            dz[i] = ch.inv[i] * (__builtin_fmaf(dz[i], ch.gamma[i], -m[i].x) - xhat[i] * m[i].y);
+        Vec8<DT>::store(p.out, w.at(p, r), w.n, dz);
+    }
+}
+
+// ---------------------------------------------------------------- launches
+template <int DT, int TC, int ACT>
+int launchForward(const GroupNormParams& p) {
+    const dim3 grid((p.C + 8 * TC - 1) / (8 * TC), p.chunks, p.N);
+    hipLaunchKernelGGL((group_norm_moments_kernel<DT, TC>), grid, dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    hipLaunchKernelGGL(group_norm_join_kernel, dim3(p.G, p.N), dim3(64), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    hipLaunchKernelGGL((group_norm_apply_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+template <int DT, int TC, int ACT>
+int launchBackward(const GroupNormParams& p) {
+    const dim3 grid((p.C + 8 * TC - 1) / (8 * TC), p.chunks, p.N);
+    hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    const int channels = p.gradGamma || p.gradBeta ? (p.C + 31) / 32 : 0;
+    hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(p.N * p.G + channels), dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    hipLaunchKernelGGL((group_norm_gradient_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+template <int DT, int TC>
+int byAct(const GroupNormParams& p, int act, bool backward) {
+    if (backward)
+        return act == kActNone ? launchBackward<DT, TC, kActNone>(p)
+             : act == kActRelu ? launchBackward<DT, TC, kActRelu>(p)
+                               : launchBackward<DT, TC, kActSilu>(p);
+    return act == kActNone ? launchForward<DT, TC, kActNone>(p)
+         : act == kActRelu ? launchForward<DT, TC, kActRelu>(p)
+                           : launchForward<DT, TC, kActSilu>(p);
+}
+
+template <int DT>
+int byWidth(const GroupNormParams& p, int tc, int act, bool backward) {
+    return tc == 64 ? byAct<DT, 64>(p, act, backward) : tc == 32 ? byAct<DT, 32>(p, act, backward)
+                                                                 : byAct<DT, 8>(p, act, backward);
+}
+
+size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+
+// Checks, chunks and workspace that both directions share; 0, 1 (nothing to do) or -1.
+int groupNormParams(const char* name, int nDtype, int nBatch, int nPixels, int nChannels, int nGroups, int nAct, float* pMean,
+                    float* pInvStd, GroupNormParams& p, int& tc) {
+    if (nDtype < 0 || nDtype > 2) return fail("%s: dtype must be 0 (fp16), 1 (bf16) or 2 (fp32)", name);
+    if (nAct < kActNone || nAct > kActSilu) return fail("%s: activation must be 0 (none), 1 (ReLU) or 2 (SiLU)", name);
+    if (nBatch < 0 || nPixels < 0 || nChannels < 0) return fail("%s: negative size", name);
+    if (nGroups < 1 || nChannels % nGroups != 0)
+        return fail("%s: %d channels do not form %d groups", name, nChannels, nGroups);
+    if (nBatch == 0 || nPixels == 0 || nChannels == 0) return 1;
+    if (nBatch > 65535) return fail("%s: more than 65535 images", name);
+    if ((long long)nBatch * nGroups > 0x3fffffffLL) return fail("%s: too many (image, group) pairs", name);
+    p.N = nBatch; p.P = nPixels; p.C = nChannels; p.G = nGroups; p.per = nChannels / nGroups;
+    // channels a workgroup takes: 512 (1 KB of a row of halves), less where the row has less
+    const int vecs = (int)((nChannels + 7LL) / 8);
+    tc = vecs > 32 ? 64 : vecs > 8 ? 32 : 8;
+    const int tiles = (vecs + tc - 1) / tc;
+    // chunks of pixels: eight workgroups a CU, and four rows a thread at least
+    const int most = (int)((nPixels + 4LL * (256 / tc) - 1) / (4 * (256 / tc)));
+    int chunks = (int)std::clamp<long long>((8LL * cuCount() + (long long)tiles * nBatch - 1) / ((long long)tiles * nBatch), 1,
+                                            std::min(most, 65535));
+    p.rowsPerChunk = (nPixels + chunks - 1) / chunks;
+    p.chunks = (nPixels + p.rowsPerChunk - 1) / p.rowsPerChunk;
+    const size_t groups = (size_t)nBatch * nGroups;
+    const size_t bPartial = up256((size_t)nBatch * p.chunks * nChannels * sizeof(float2));
+    char* ws = static_cast<char*>(workspace(bPartial + up256(groups * sizeof(float2)) * 2, kWsOperand));
+    if (!ws) return -1;   // workspace() recorded the cause
+    p.partial = reinterpret_cast<float2*>(ws);
+    p.means = reinterpret_cast<float2*>(ws + bPartial);
+    float* own = reinterpret_cast<float*>(ws + bPartial + up256(groups * sizeof(float2)));
+    p.mean = pMean ? pMean : own;
+    p.inv = pInvStd ? pInvStd : own + groups;
+    return 0;
+}
+
+bool elementAligned(const void* p, int nDtype) { return (reinterpret_cast<uintptr_t>(p) & (nDtype == 2 ? 3u : 1u)) == 0; }
+
+}  // namespace
+
+}  // namespace omhip
+
+using namespace omhip;
+
+extern "C" {
+
+int omHipGroupNormNhwc(int nDtype, const void* pX, const float* pGamma, const float* pBeta, void* pY, float* pMean,
+                       float* pInvStd, int nBatch, int nPixels, int nChannels, int nGroups, float fEps, int nAct) {
+    const char* name = "omHipGroupNormNhwc";
+    clearError();
+    if (!(fEps >= 0.f)) return fail("%s: eps must not be negative", name);
+    for (const void* x : {(const void*)pGamma, (const void*)pBeta, (const void*)pMean, (const void*)pInvStd})
+        if (!elementAligned(x, 2)) return fail("%s: a pointer is not aligned to its elements", name);
+    if (nDtype >= 0 && nDtype <= 2 && (!elementAligned(pX, nDtype) || !elementAligned(pY, nDtype)))
+        return fail("%s: a pointer is not aligned to its elements", name);
+    if (nBatch > 0 && nPixels > 0 && nChannels > 0 && (!pX || !pY)) return fail("%s: null pointer", name);
+    GroupNormParams p{};
+    int tc = 0;
+    const int rc = groupNormParams(name, nDtype, nBatch, nPixels, nChannels, nGroups, nAct, pMean, pInvStd, p, tc);
+    if (rc) return rc < 0 ? -1 : 0;
+    p.x = pX; p.out = pY; p.gamma = pGamma; p.beta = pBeta; p.eps = fEps;
+    return nDtype == 0 ? byWidth<0>(p, tc, nAct, false) : nDtype == 1 ? byWidth<1>(p, tc, nAct, false)
+                                                                     : byWidth<2>(p, tc, nAct, false);
+}
+
+int omHipGroupNormNhwcBackward(int nDtype, const void* pGradY, const void* pX, const void* pY, const float* pMean,
+                               const float* pInvStd, const float* pGamma, const float* pBeta, void* pGradX, float* pGradGamma,
+                               float* pGradBeta, int nBatch, int nPixels, int nChannels, int nGroups, int nAct) {
+    const char* name = "omHipGroupNormNhwcBackward";
+    clearError();
+    for (const void* x : {(const void*)pGamma, (const void*)pBeta, (const void*)pMean, (const void*)pInvStd,
+                          (const void*)pGradGamma, (const void*)pGradBeta})
+        if (!elementAligned(x, 2)) return fail("%s: a pointer is not aligned to its elements", name);
+    if (nDtype >= 0 && nDtype <= 2)
+        for (const void* x : {pGradY, pX, pY, (const void*)pGradX})
+            if (!elementAligned(x, nDtype)) return fail("%s: a pointer is not aligned to its elements", name);
+    if (nBatch > 0 && nPixels > 0 && nChannels > 0) {
+        if (!pGradY || !pX || !pMean || !pInvStd || !pGradX) return fail("%s: null pointer", name);
+        if (nAct == kActRelu && !pY) return fail("%s: ReLU needs the saved output", name);
+    }
+    GroupNormParams p{};
+    int tc = 0;
+    const int rc = groupNormParams(name, nDtype, nBatch, nPixels, nChannels, nGroups, nAct, const_cast<float*>(pMean),
+                                   const_cast<float*>(pInvStd), p, tc);
+    if (rc < 0) return -1;
+    if (rc) {   // nothing to sum
+        for (float* g : {pGradGamma, pGradBeta})
+            if (g && nChannels > 0 && byteFill(g, 0, (size_t)nChannels * sizeof(float))) return -1;
+        return 0;
+    }
+    p.x = pX; p.y = pY; p.gradY = pGradY; p.out = pGradX; p.gamma = pGamma; p.beta = pBeta;
+    p.gradGamma = pGradGamma; p.gradBeta = pGradBeta;
+    return nDtype == 0 ? byWidth<0>(p, tc, nAct, true) : nDtype == 1 ? byWidth<1>(p, tc, nAct, true)
+                                                                    : byWidth<2>(p, tc, nAct, true);
+}
+
+}  // extern "C"
