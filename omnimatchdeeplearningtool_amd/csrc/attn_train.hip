@@ -48,6 +48,8 @@ struct AttnTrainParams {
     uint16_t *dq, *dk, *dv;
     float *lse2, *delta;            // [B, H, SqP]
     int SqP;                        // Sq rounded up to whole tiles
+    int parts;                      // dK, dV: workgroups that share a block of keys
+    float *dkPart, *dvPart;         // parts > 1: [B, Hkv, parts, blocks * kBlockQ, D]
     uint32_t heads, blocks;         // grid: heads x blocks workgroups
 };
 
@@ -290,6 +292,19 @@ __device__ __forceinline__ void storeColumn(uint16_t* row, const at_f32x16 (&acc
         }
 }
 
+template <int KD>
+__device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc)[KD], float f, int h, int D) {
+#pragma unroll
+    for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * dt + 2 * r + 4 * h;
+            if (d < D)
+                *reinterpret_cast<at_f32x4*>(row + d) =
+                    at_f32x4{acc[dt][r] * f, acc[dt][r + 1] * f, acc[dt][r + 2] * f, acc[dt][r + 3] * f};
+        }
+}
+
 // ---------------------------------------------------------------- backward: dQ
 // As the forward pass, a wave holds 32 queries as columns and the workgroup walks the keys: S^T = K Q^T,
 // dP^T = V dO^T, dQ^T += K^T dS^T.
@@ -405,6 +420,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
 // ---------------------------------------------------------------- backward: dK and dV
 // A wave holds 32 keys as columns (a workgroup 128) and the workgroup walks the queries of every head that reads them,
 // 64 at a time: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS. fp16 takes P raised by 2^15 (it is at most 1).
+// Where the blocks of keys are few for the card, `parts` workgroups take a share of a block's walk each and leave fp32
+// sums, which attn_train_dkv_join_kernel adds in order.
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(AttnTrainParams p) {
     using T = AtTile<KD>;
@@ -418,7 +435,9 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(At
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, block;
-    atPlace(blockIdx.x, p.heads, p.blocks, bh, block);   // causal: the first keys have the longest walks
+    atPlace(blockIdx.x, p.heads, p.blocks * p.parts, bh, block);   // causal: the first keys have the longest walks
+    const int part = (int)(block % (uint32_t)p.parts);
+    block /= (uint32_t)p.parts;
     const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv);
     const int group = p.H / p.Hkv;
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
@@ -430,6 +449,7 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(At
     const int t0 = p.causal ? max(0, (int)block * kBlockQ - off) / kTileKeys : 0;
     const int t1 = (int)block * kBlockQ < nK ? (nQ + kTileKeys - 1) / kTileKeys : 0;
     const int per = max(0, t1 - t0), total = per * group;
+    const int begin = (int)((long long)total * part / p.parts), end = (int)((long long)total * (part + 1) / p.parts);
 
     at_u32x4 kf[T::NS], vf[T::NS];
     {
@@ -509,22 +529,53 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(At
             }
         }
     };
-    if (total > 0) fetch(0, q0, g0, s0);
-    for (int i = 0; i < total; i += 2) {   // as in the forward pass
+    if (end > begin) fetch(begin, q0, g0, s0);
+    for (int i = begin; i < end; i += 2) {   // as in the forward pass
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (i + 1 < total) fetch(i + 1, q1, g1, s1);
+        if (i + 1 < end) fetch(i + 1, q1, g1, s1);
         if (key0 < nK) tile(i, q0, g0, s0);
-        if (i + 1 >= total) break;
+        if (i + 1 >= end) break;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (i + 2 < total) fetch(i + 2, q0, g0, s0);
+        if (i + 2 < end) fetch(i + 2, q0, g0, s0);
         if (key0 < nK) tile(i + 1, q1, g1, s1);
+    }
+    if (p.parts > 1) {
+        const long long row = ((long long)bh * p.parts + part) * ((long long)p.blocks * kBlockQ) + key;
+        storeColumnF32<KD>(p.dkPart + row * p.D, dk, p.scale * kLower * scale.undo(), h, p.D);
+        storeColumnF32<KD>(p.dvPart + row * p.D, dv, kLower, h, p.D);
+        return;
     }
     if (key >= p.Sk) return;
     const long long at = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
     storeColumn<BF16, KD>(p.dk + at, dk, p.scale * kLower * scale.undo(), h, p.D, key >= nK);
     storeColumn<BF16, KD>(p.dv + at, dv, kLower, h, p.D, key >= nK);
+}
+
+// The parts' sums of dK (blockIdx.y 0) or dV (1), eight values of a key a thread.
+template <bool BF16>
+__global__ __launch_bounds__(256) void attn_train_dkv_join_kernel(AttnTrainParams p) {
+    const int chunks = p.D / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;   // (b, key, kvHead, chunk)
+    if (i >= (long long)p.B * p.Sk * p.Hkv * chunks) return;
+    const int c = (int)(i % chunks);
+    const long long bkh = i / chunks;
+    const int kvHead = (int)(bkh % p.Hkv);
+    const int key = (int)(bkh / p.Hkv % p.Sk), b = (int)(bkh / p.Hkv / p.Sk);
+    const long long keys = (long long)p.blocks * kBlockQ;
+    const float* from = (blockIdx.y ? p.dvPart : p.dkPart) +
+                        (((long long)b * p.Hkv + kvHead) * p.parts * keys + key) * p.D + c * 8;
+    at_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int part = 0; part < p.parts; ++part)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            s[e] += *reinterpret_cast<const at_f32x4*>(from + (long long)part * keys * p.D + 4 * e);
+    at_u32x4 v = {atPack2<BF16>(s[0][0], s[0][1]), atPack2<BF16>(s[0][2], s[0][3]), atPack2<BF16>(s[1][0], s[1][1]),
+                  atPack2<BF16>(s[1][2], s[1][3])};
+    if (key >= atLength(p.kLens, b, p.Sk)) v = at_u32x4{0u, 0u, 0u, 0u};
+    uint16_t* to = (blockIdx.y ? p.dv : p.dk) + (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
+    *reinterpret_cast<at_u32x4*>(to + c * 8) = v;
 }
 
 // ---------------------------------------------------------------- checks and launches
@@ -559,8 +610,14 @@ int launchBackward(AttnTrainParams& p) {
     if (p.Sk > 0) {
         p.heads = (uint32_t)(p.B * p.Hkv);
         p.blocks = (uint32_t)((p.Sk + kBlockQ - 1) / kBlockQ);
-        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
+        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD>), dim3(p.heads * p.blocks * p.parts), dim3(256), 0, stream(), p);
         OMHIP_CHECK_LAUNCH();
+        if (p.parts > 1) {
+            const long long n = (long long)p.B * p.Sk * p.Hkv * (p.D / 8);
+            hipLaunchKernelGGL((attn_train_dkv_join_kernel<BF16>), dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0,
+                               stream(), p);
+            OMHIP_CHECK_LAUNCH();
+        }
     }
     return 0;
 }
@@ -583,6 +640,13 @@ int backward(AttnTrainParams& p) {
         case 3: return launchBackward<BF16, 3>(p);
         default: return launchBackward<BF16, 4>(p);
     }
+}
+
+// Workgroups that share a block of keys' walk of `tiles` query tiles: as many as give every CU four workgroups (a causal
+// mask makes walks of all lengths, which four even out), of four tiles at least.
+int dkvParts(long long keyBlocks, int tiles) {
+    if (keyBlocks == 0 || tiles == 0) return 1;
+    return (int)std::clamp<long long>((4LL * cuCount() + keyBlocks - 1) / keyBlocks, 1, std::max(1, tiles / 4));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -669,10 +733,15 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
     p.dq = pGradQ; p.dk = pGradK; p.dv = pGradV;
     p.SqP = (nSeqQ + kTileKeys - 1) / kTileKeys * kTileKeys;
     const size_t rows = (size_t)nBatch * nHeads * p.SqP;
+    const size_t keyBlocks = (size_t)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1) / kBlockQ);
+    p.parts = dkvParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads));
+    const size_t sums = p.parts > 1 ? keyBlocks * p.parts * kBlockQ * nHeadDim : 0;
     if (rows) {
-        p.lse2 = static_cast<float*>(workspace(rows * 2 * sizeof(float), kWsOperand));
+        p.lse2 = static_cast<float*>(workspace((rows + sums) * 2 * sizeof(float), kWsOperand));
         if (!p.lse2) return -1;   // workspace() recorded the cause
         p.delta = p.lse2 + rows;
+        p.dkPart = p.delta + rows;
+        p.dvPart = p.dkPart + sums;
     }
     return nDtype == 1 ? backward<true>(p) : backward<false>(p);
 }
