@@ -163,12 +163,18 @@ struct AtTile {
     }
 };
 
-// Blocks of one (image, key head) run on one XCD (consecutive block ids go to
-// the 8 XCDs in turn), so its keys and values, or queries, stay in one L2:
-// id -> (head, block) with `heads` heads of `blocks` blocks each.
-__device__ __forceinline__ void atPlace(uint32_t id, uint32_t heads, uint32_t blocks, uint32_t& head, uint32_t& block) {
+// Workgroup id -> (head, block) of `heads` heads with `blocks` blocks each. Consecutive ids go to the 8 XCDs in turn;
+// both orders keep a head's blocks on one XCD where they can, so that what they share stays in one L2.
+//  * blocks of equal length: the blocks of 8 heads at a time;
+//  * a causal mask (byLength): all heads' first blocks, which the callers make the longest, then their second ones.
+//    Head after head, the last heads' long blocks would start late and run alone.
+__device__ __forceinline__ void atPlace(uint32_t id, uint32_t heads, uint32_t blocks, bool byLength, uint32_t& head,
+                                        uint32_t& block) {
     const uint32_t whole = heads / 8 * 8 * blocks;   // ids of the whole groups of 8 heads
-    if (id < whole) {
+    if (byLength) {
+        head = id % heads;
+        block = id / heads;
+    } else if (id < whole) {
         const uint32_t xcd = id & 7, i = id >> 3;
         head = i / blocks * 8 + xcd;
         block = i % blocks;

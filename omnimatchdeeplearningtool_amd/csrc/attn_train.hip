@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, qb;
-    atPlace(blockIdx.x, p.heads, p.blocks, bh, qb);
+    atPlace(blockIdx.x, p.heads, p.blocks, p.causal, bh, qb);
     qb = p.blocks - 1 - qb;   // causal: the longest walks first
     const int b = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);
     const int kvHead = head / (p.H / p.Hkv);
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, qb;
-    atPlace(blockIdx.x, p.heads, p.blocks, bh, qb);
+    atPlace(blockIdx.x, p.heads, p.blocks, p.causal, bh, qb);
     qb = p.blocks - 1 - qb;   // causal: the longest walks first
     const int b = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);
     const int kvHead = head / (p.H / p.Hkv);
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(At
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, block;
-    atPlace(blockIdx.x, p.heads, p.blocks * p.parts, bh, block);   // causal: the first keys have the longest walks
+    atPlace(blockIdx.x, p.heads, p.blocks * p.parts, p.causal, bh, block);   // causal: the first keys have the longest walks
     const int part = (int)(block % (uint32_t)p.parts);
     block /= (uint32_t)p.parts;
     const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv);
