@@ -96,8 +96,45 @@ __device__ __forceinline__ void atCopy4(__amdgpu_buffer_rsrc_t r, float* dst, ui
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (AtLdsPtr)dst, 4, voff, 0, 0, 0);
 }
 
-// The other half-wave's value of the same column.
-__device__ __forceinline__ float atOtherHalf(float v) { return __shfl_xor(v, 32, 64); }
+// Order of a stretch of straight code, a kind of instruction at a time (__builtin_amdgcn_sched_group_barrier). Left
+// alone, the scheduler reads each fragment right before the MFMA that takes it and the wave waits out every read.
+template <int N>
+__device__ __forceinline__ void atMfmas() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
+template <int N>
+__device__ __forceinline__ void atReads() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
+template <int N>
+__device__ __forceinline__ void atValu() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
+template <int N>
+__device__ __forceinline__ void atTrans() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x400, N, 0); }
+// N MFMAs that take `reads` LDS reads, READS a MFMA: `ahead` of them first, then one MFMA and READS reads in turn.
+template <int N, int READS, int AHEAD>
+__device__ __forceinline__ void atPipeline() {
+    atReads<AHEAD * READS>();
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        atMfmas<1>();
+        atReads<READS>();
+    }
+    atMfmas<AHEAD>();
+}
+
+// The two half-waves' values of a column (lanes l and l + 32), in the same order in both.
+__device__ __forceinline__ void atBothHalves(float v, float& lower, float& upper) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    lower = __builtin_bit_cast(float, (uint32_t)r[0]);
+    upper = __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+__device__ __forceinline__ float atMaxHalves(float v) {
+    float a, b;
+    atBothHalves(v, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float atSumHalves(float v) {
+    float a, b;
+    atBothHalves(v, a, b);
+    return a + b;
+}
 
 // KD: 32-column blocks of the padded head dimension.
 template <int KD>

@@ -132,6 +132,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
 #pragma unroll
             for (int st = 0; st < T::NS; ++st) s[kb] = atMfma<BF16>(T::natural(kd, 32 * kb, st, l, h), qf[st], s[kb]);
         }
+        atPipeline<2 * T::NS, 1, 4>();
         const int key0 = t * kTileKeys;
         if (key0 + kTileKeys > nK || (p.causal && key0 + kTileKeys - 1 > q0 + off)) {
             const int seen = (p.causal ? min(nK, query + off + 1) : nK) - key0 - 4 * h;
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-        top = fmaxf(top, atOtherHalf(top));
+        top = atMaxHalves(top);
         if (__any(top > m + margin)) {   // also where m is -inf and the row sees its first key
             const float next = fmaxf(m, top);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
@@ -159,19 +160,33 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
         }
         const float base = m == -INFINITY ? 0.f : kShift - m * c;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int u = 0; u < 4; ++u) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, base));
-                s[kb][r] = e;
+            for (int r = 8 * (u & 1); r < 8 * (u & 1) + 8; ++r) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][r], c, base));
+                s[u / 2][r] = e;
                 sum += e;
             }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
             const at_u32x4 pf = atPack8<BF16>(s[u / 2], u & 1);
 #pragma unroll
             for (int dt = 0; dt < KD; ++dt) o[dt] = atMfma<BF16>(T::transposed(vd, 16 * u, dt, lane), pf, o[dt]);
         }
+        // the weights of step u + 1 are computed, and its fragments read, under the MFMAs of step u
+        atReads<2 * KD>();
+        atValu<20>();
+        atTrans<8>();
+        atValu<20>();
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int dt = 0; dt < KD; ++dt) {
+                atMfmas<1>();
+                if (u < 3) {
+                    atReads<2>();
+                    atTrans<8 / KD>();
+                    atValu<20 / KD>();
+                }
+            }
     };
 
     // Copies of tile t + 1 start once every wave is done with tile t - 1, whose
@@ -190,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     }
 
     if (query >= p.Sq) return;
-    sum += atOtherHalf(sum);
+    sum = atSumHalves(sum);
     const bool empty = !(query < nQ) || sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
     if (h == 0)
@@ -387,7 +402,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
                 if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
             }
             if constexpr (!BF16) {
-                scale.update(fmaxf(most, atOtherHalf(most)), dq);
+                scale.update(atMaxHalves(most), dq);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= scale.f;
             }
@@ -514,7 +529,7 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(At
                 }
             }
             if constexpr (!BF16) {
-                scale.update(fmaxf(most, atOtherHalf(most)), dk);
+                scale.update(atMaxHalves(most), dk);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= scale.f;
             }
