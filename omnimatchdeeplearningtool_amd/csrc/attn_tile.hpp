@@ -136,6 +136,10 @@ __device__ __forceinline__ float atSumHalves(float v) {
     return a + b;
 }
 
+__device__ __forceinline__ at_u32x2 atReadTransposed(const char* at) {
+    return __builtin_bit_cast(at_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_i16x4*)at));
+}
+
 // KD: 32-column blocks of the padded head dimension.
 template <int KD>
 struct AtTile {
@@ -174,24 +178,39 @@ struct AtTile {
         }
     };
 
-    // ---- LDS -> fragments
-    static __device__ __forceinline__ at_u32x4 natural(const uint16_t* tile, int row0, int s, int l, int h) {
-        const int c = (2 * s + h) ^ swizzle(l);
-        return *reinterpret_cast<const at_u32x4*>(tile + (row0 + l) * RS + c * 8);
-    }
-    static __device__ __forceinline__ at_u32x4 transposed(const uint16_t* tile, int row0, int t, int lane) {
-        const int a = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
-        const int c = 4 * t + 2 * g + ((a & 3) >> 1);
-        at_u32x2 p[2];
+    // ---- LDS -> fragments. The lane's byte offsets in a tile, made once: the compiler would make them again before
+    // every read.
+    struct Lane {
+        uint32_t nat[NS], tr[KD][2];
+        __device__ __forceinline__ explicit Lane(int lane) {
+            const int l = lane & 31, h = lane >> 5, a = lane & 15, g = (lane >> 4) & 1;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int r = 8 * j + 4 * h + (a >> 2);
-            const uint16_t* at = tile + (row0 + r) * RS + (c ^ swizzle(r)) * 8 + 4 * (a & 1);
-            p[j] = __builtin_bit_cast(
-                at_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_i16x4*)at));
+            for (int s = 0; s < NS; ++s) {
+                nat[s] = (uint32_t)(l * RS + ((2 * s + h) ^ swizzle(l)) * 8) * 2u;
+                asm volatile("" : "+v"(nat[s]));
+            }
+#pragma unroll
+            for (int t = 0; t < KD; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int r = 8 * j + 4 * h + (a >> 2), c = 4 * t + 2 * g + ((a & 3) >> 1);
+                    tr[t][j] = (uint32_t)(r * RS + (c ^ swizzle(r)) * 8 + 4 * (a & 1)) * 2u;
+                    asm volatile("" : "+v"(tr[t][j]));
+                }
         }
-        return at_u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
-    }
+        // rows row0 .. row0 + 31 (a multiple of 32), columns 16 s ...
+        __device__ __forceinline__ at_u32x4 natural(const uint16_t* tile, int row0, int s) const {
+            return *reinterpret_cast<const at_u32x4*>(reinterpret_cast<const char*>(tile) + nat[s] + row0 * RS * 2);
+        }
+        // columns 32 t ... of rows row0 .. row0 + 15 (a multiple of 16)
+        __device__ __forceinline__ at_u32x4 transposed(const uint16_t* tile, int row0, int t) const {
+            at_u32x2 p[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                p[j] = atReadTransposed(reinterpret_cast<const char*>(tile) + tr[t][j] + row0 * RS * 2);
+            return at_u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
+        }
+    };
 
     // ---- memory -> fragment: row `row` of `rows` (row0: its address' start), columns 16 s + 8 h ...
     static __device__ __forceinline__ at_u32x4 direct(const uint16_t* rowPtr, bool valid, int s, int h, int D) {

@@ -46,7 +46,7 @@ struct AttnTrainParams {
     // backward
     const uint16_t* gradOut;
     uint16_t *dq, *dk, *dv;
-    float *lse2, *delta;            // [B, H, SqP]
+    float* stats;                   // [B, H, SqP / 32]: shift of 32 rows, then their delta
     int SqP;                        // Sq rounded up to whole tiles
     int parts;                      // dK, dV: workgroups that share a block of keys
     float *dkPart, *dvPart;         // parts > 1: [B, Hkv, parts, blocks * kBlockQ, D]
@@ -106,6 +106,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
             for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
         }
     }
+    const typename T::Lane at(lane);
     typename T::template Copy<kTileKeys, kWaves> copy;
     const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
     copy.init(wave, lane, ld2, p.D);
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-            for (int st = 0; st < T::NS; ++st) s[kb] = atMfma<BF16>(T::natural(kd, 32 * kb, st, l, h), qf[st], s[kb]);
+            for (int st = 0; st < T::NS; ++st) s[kb] = atMfma<BF16>(at.natural(kd, 32 * kb, st), qf[st], s[kb]);
         }
         atPipeline<2 * T::NS, 1, 4>();
         const int key0 = t * kTileKeys;
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
             }
             const at_u32x4 pf = atPack8<BF16>(s[u / 2], u & 1);
 #pragma unroll
-            for (int dt = 0; dt < KD; ++dt) o[dt] = atMfma<BF16>(T::transposed(vd, 16 * u, dt, lane), pf, o[dt]);
+            for (int dt = 0; dt < KD; ++dt) o[dt] = atMfma<BF16>(at.transposed(vd, 16 * u, dt), pf, o[dt]);
         }
         // the weights of step u + 1 are computed, and its fragments read, under the MFMAs of step u
         atReads<2 * KD>();
@@ -189,20 +190,22 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
             }
     };
 
-    // Copies of tile t + 1 start once every wave is done with tile t - 1, whose
-    // buffers they fill, and are waited for at the top of the next trip.
+    // Copies of tile t + 1 start once every wave is done with tile t - 1, whose buffers they fill, and are waited for at
+    // the top of the next trip. Whole pairs of trips, then what is left: a way out of the middle would cost every trip
+    // copies of the sums.
+    auto trip = [&](int t, const uint16_t* kd, const uint16_t* vd, uint16_t* kNext, uint16_t* vNext) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1, kNext, vNext);
+        if (t * kTileKeys < waveEnd) tile(t, kd, vd);
+    };
     if (nt > 0) fetch(0, k0, v0);
-    for (int t = 0; t < nt; t += 2) {
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1, k1, v1);
-        if (t * kTileKeys < waveEnd) tile(t, k0, v0);
-        if (t + 1 >= nt) break;
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (t + 2 < nt) fetch(t + 2, k0, v0);
-        if ((t + 1) * kTileKeys < waveEnd) tile(t + 1, k1, v1);
+    int t = 0;
+    for (; t + 1 < nt; t += 2) {
+        trip(t, k0, v0, k1, v1);
+        trip(t + 1, k1, v1, k0, v0);
     }
+    if (t < nt) trip(t, k0, v0, k1, v1);
 
     if (query >= p.Sq) return;
     sum = atSumHalves(sum);
@@ -224,9 +227,13 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
 }
 
 // ---------------------------------------------------------------- backward: row statistics
-// lse2 = lse log2 e and delta = sum_d dO O of every row, [B, H, SqP]. Rows that pass no gradient (past the query
-// length, past Sq, or without a key) get lse2 = +inf, which makes their probabilities 0. A row of a head is read by
+// shift = -lse log2 e and delta = sum_d dO O of every row, 32 rows at a time. Rows that pass no gradient (past the query
+// length, past Sq, or without a key) get shift = -inf, which makes their probabilities 0. A row of a head is read by
 // G lanes, 16 bytes of dO and O each.
+// P of the dK / dV kernel is taken raised by 2^15 in fp16 (it is at most 1, and loses bits below 2^-14): part of shift.
+template <bool BF16>
+constexpr float kRaise = BF16 ? 0.f : 15.f;
+
 template <bool BF16, int G>
 __global__ __launch_bounds__(256) void attn_train_delta_kernel(AttnTrainParams p) {
     const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / G;   // (b, q, head), head fastest
@@ -254,13 +261,14 @@ __global__ __launch_bounds__(256) void attn_train_delta_kernel(AttnTrainParams p
     for (int s = G / 2; s > 0; s >>= 1) d += __shfl_xor(d, s, 64);
     if (c) return;
     const long long bh = (long long)b * p.H + head;
-    float lse2 = INFINITY;
+    float shift = -INFINITY;
     if (valid) {
         const float lse = p.lse[bh * p.Sq + q];
-        if (lse != -INFINITY) lse2 = lse * kAtLog2e;
+        if (lse != -INFINITY) shift = kRaise<BF16> - lse * kAtLog2e;
     }
-    p.lse2[bh * p.SqP + q] = lse2;
-    p.delta[bh * p.SqP + q] = lse2 == INFINITY ? 0.f : d;
+    float* to = p.stats + 2 * (bh * p.SqP + (q & ~31)) + (q & 31);
+    to[0] = shift;
+    to[32] = shift == -INFINITY ? 0.f : d;
 }
 
 // dS as halves. bf16 has fp32's range; fp16 loses dS below 2^-14 (a probability of 1 / 4096 times a gradient of
@@ -361,9 +369,11 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
             gf[s] = T::direct(grow, query < nQ, s, h, p.D);
         }
     }
-    const long long at = (long long)bh * p.SqP + min(query, p.SqP - 1);
-    const float lse2 = p.lse2[at], delta = p.delta[at];   // rows past the query length hold +inf and 0
+    // rows past the query length hold -inf and 0
+    const float* stats = p.stats + 2 * ((long long)bh * p.SqP + min(q0, p.SqP - 32)) + l;
+    const float shift = stats[0] - kRaise<BF16>, delta = stats[32];
     const float c = p.scale * kAtLog2e;
+    const typename T::Lane at(lane);
     typename T::template Copy<kTileKeys, kWaves> copy;
     const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
     copy.init(wave, lane, ld2, p.D);
@@ -390,13 +400,13 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
             for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
             for (int st = 0; st < T::NS; ++st) {
-                s = atMfma<BF16>(T::natural(kd, 32 * kb, st, l, h), qf[st], s);
-                dp = atMfma<BF16>(T::natural(vd, 32 * kb, st, l, h), gf[st], dp);
+                s = atMfma<BF16>(at.natural(kd, 32 * kb, st), qf[st], s);
+                dp = atMfma<BF16>(at.natural(vd, 32 * kb, st), gf[st], dp);
             }
             float most = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse2));
+                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, shift));
                 if (edge && 32 * kb + 8 * (r / 4) + r % 4 >= seen) e = 0.f;
                 s[r] = e * (dp[r] - delta);
                 if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
@@ -411,161 +421,233 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
                 const at_u32x4 df = atPack8<BF16>(s, u);
 #pragma unroll
                 for (int dt = 0; dt < KD; ++dt)
-                    dq[dt] = atMfma<BF16>(T::transposed(kd, 32 * kb + 16 * u, dt, lane), df, dq[dt]);
+                    dq[dt] = atMfma<BF16>(at.transposed(kd, 32 * kb + 16 * u, dt), df, dq[dt]);
             }
         }
     };
+    auto trip = [&](int t, const uint16_t* kd, const uint16_t* vd, uint16_t* kNext, uint16_t* vNext) {   // as in the forward pass
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1, kNext, vNext);
+        if (t * kTileKeys < waveEnd) tile(t, kd, vd);
+    };
     if (nt > 0) fetch(0, k0, v0);
-    for (int t = 0; t < nt; t += 2) {   // as in the forward pass
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1, k1, v1);
-        if (t * kTileKeys < waveEnd) tile(t, k0, v0);
-        if (t + 1 >= nt) break;
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (t + 2 < nt) fetch(t + 2, k0, v0);
-        if ((t + 1) * kTileKeys < waveEnd) tile(t + 1, k1, v1);
+    int t = 0;
+    for (; t + 1 < nt; t += 2) {
+        trip(t, k0, v0, k1, v1);
+        trip(t + 1, k1, v1, k0, v0);
     }
+    if (t < nt) trip(t, k0, v0, k1, v1);
     if (query >= p.Sq) return;
     uint16_t* row = p.dq + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
-    storeColumn<BF16, KD>(row, dq, p.scale * scale.undo(), h, p.D, lse2 == INFINITY);
+    storeColumn<BF16, KD>(row, dq, p.scale * scale.undo(), h, p.D, shift == -INFINITY);
 }
 
 // ---------------------------------------------------------------- backward: dK and dV
-// A wave holds 32 keys as columns (a workgroup 128) and the workgroup walks the queries of every head that reads them,
-// 64 at a time: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS. fp16 takes P raised by 2^15 (it is at most 1).
+// A workgroup holds 128 keys of a key head and walks the queries of every head that reads them, 32 at a time. Four
+// pairs of waves hold 32 keys each, as columns; of a pair (both waves are on one SIMD),
+//  * the first computes S = Q K^T, P and dV^T += dO^T P, and leaves P (fp32, in its registers' order) in LDS;
+//  * the second, one tile behind, computes dP = dO V^T, dS from that P, and dK^T += Q^T dS.
+// One wave doing both needs 128 + 64 registers for its sums and K, V fragments at a head dimension of 128, so only one
+// fits a SIMD and every LDS read and exponential of it is waited out: 465 us at 2 x 4096 x 16 heads on 4 of 128,
+// causal, against (measured below) two waves that fill each other's gaps. Q and dO tiles are in three buffers: the
+// next one's copy, the first waves' and the second waves'.
 // Where the blocks of keys are few for the card, `parts` workgroups take a share of a block's walk each and leave fp32
 // sums, which attn_train_dkv_join_kernel adds in order.
-template <bool BF16, int KD>
-__global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_train_dkv_kernel(AttnTrainParams p) {
+constexpr int kTileQ = 32;
+
+// LDS of the kernel. Each buffer is an array of its own, so that the compiler sees that a copy into one does not touch
+// the others and lets reads of them go ahead of it.
+struct DkvBuffers {
+    uint16_t *q[3], *g[3];
+    float* stats[3];     // shift, delta
+    float* weights;      // P by tile parity and pair
+};
+
+// A wave's work in attn_train_dkv_kernel.
+template <bool BF16, int KD, bool SECOND>
+__device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffers& lds, int wave, int lane) {
     using T = AtTile<KD>;
-    constexpr float kRaise = BF16 ? 0.f : 15.f, kLower = BF16 ? 1.f : 1.f / 32768.f;
-    __shared__ __attribute__((aligned(256))) uint16_t q0[kTileKeys * T::RS];
-    __shared__ __attribute__((aligned(256))) uint16_t g0[kTileKeys * T::RS];
-    __shared__ __attribute__((aligned(256))) float s0[2 * kTileKeys];   // lse2, delta
-    __shared__ __attribute__((aligned(256))) uint16_t q1[kTileKeys * T::RS];
-    __shared__ __attribute__((aligned(256))) uint16_t g1[kTileKeys * T::RS];
-    __shared__ __attribute__((aligned(256))) float s1[2 * kTileKeys];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l = lane & 31, h = lane >> 5;
+    constexpr float kLower = BF16 ? 1.f : 1.f / 32768.f;   // takes kRaise out
+    const int l = lane & 31, h = lane >> 5, pair = wave & 3;
     uint32_t bh, block;
-    atPlace(blockIdx.x, p.heads, p.blocks * p.parts, p.causal, bh, block);   // causal: the first keys have the longest walks
+    atPlace(blockIdx.x, p.heads, p.blocks * p.parts, p.causal, bh, block);   // causal: the first keys' walks are longest
     const int part = (int)(block % (uint32_t)p.parts);
     block /= (uint32_t)p.parts;
     const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv);
     const int group = p.H / p.Hkv;
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
     const int off = p.Sk - p.Sq;
-    const int key0 = (int)block * kBlockQ + wave * 32;
+    const int key0 = (int)block * kBlockQ + pair * 32;
     const int key = key0 + l;
 
-    // query tiles that see a key of the workgroup: t0 .. t1 of each head of the group
-    const int t0 = p.causal ? max(0, (int)block * kBlockQ - off) / kTileKeys : 0;
-    const int t1 = (int)block * kBlockQ < nK ? (nQ + kTileKeys - 1) / kTileKeys : 0;
+    // query tiles that see a key of the workgroup: t0 .. t1 of each head of the group; this part's share of them
+    const int t0 = p.causal ? max(0, (int)block * kBlockQ - off) / kTileQ : 0;
+    const int t1 = (int)block * kBlockQ < nK ? (nQ + kTileQ - 1) / kTileQ : 0;
     const int per = max(0, t1 - t0), total = per * group;
-    const int begin = (int)((long long)total * part / p.parts), end = (int)((long long)total * (part + 1) / p.parts);
+    const int begin = (int)((long long)total * part / p.parts), n = (int)((long long)total * (part + 1) / p.parts) - begin;
 
-    at_u32x4 kf[T::NS], vf[T::NS];
+    const typename T::Lane at(lane);
+    const long long place = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
+    at_u32x4 own[T::NS];   // K, or V
     {
-        const long long at = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
+        const uint16_t* row = (SECOND ? p.v : p.k) + place;
 #pragma unroll
-        for (int s = 0; s < T::NS; ++s) {
-            kf[s] = T::direct(p.k + at, key < nK, s, h, p.D);
-            vf[s] = T::direct(p.v + at, key < nK, s, h, p.D);
-        }
+        for (int s = 0; s < T::NS; ++s) own[s] = T::direct(row, key < nK, s, h, p.D);
     }
     const float c = p.scale * kAtLog2e;
-    typename T::template Copy<kTileKeys, kWaves> copyQ, copyG;
+    constexpr int kCopyWaves = T::CH * kTileQ / 64 < 8 ? T::CH * kTileQ / 64 : 8;   // a head dimension of 32 has 2 instructions
+    typename T::template Copy<kTileQ, kCopyWaves> copyQ, copyG;
     const uint32_t ldq2 = (uint32_t)p.ldq * 2u, ldg2 = (uint32_t)(p.H * p.D) * 2u;
     copyQ.init(wave, lane, ldq2, p.D);
     copyG.init(wave, lane, ldg2, p.D);
-    auto fetch = [&](int i, uint16_t* qd, uint16_t* gd, float* sd) {
-        const int head = kvHead * group + i / per, t = t0 + i % per;
-        const long long first = (long long)t * kTileKeys;
-        copyQ.run(p.q + (long long)b * p.sq + first * p.ldq + (long long)head * p.D, nQ - t * kTileKeys, ldq2, p.D, qd, wave);
-        copyG.run(p.gradOut + (((long long)b * p.Sq + first) * p.H + head) * p.D, nQ - t * kTileKeys, ldg2, p.D, gd, wave);
-        if (wave < 2) {   // rows past the query length hold +inf and 0
-            const float* from = (wave == 0 ? p.lse2 : p.delta) + ((long long)b * p.H + head) * p.SqP + first;
-            atCopy4(atView(from, kTileKeys * 4), sd + wave * kTileKeys, lane * 4);
+    int fetchHead = per > 0 ? kvHead * group + begin / per : 0, fetchT = per > 0 ? t0 + begin % per : 0;
+    auto fetch = [&](uint16_t* qd, uint16_t* gd, float* sd) {   // the next tile of the walk
+        const long long first = (long long)fetchT * kTileQ;
+        const int rows = nQ - fetchT * kTileQ;
+        if (wave < kCopyWaves) {
+            copyQ.run(p.q + (long long)b * p.sq + first * p.ldq + (long long)fetchHead * p.D, rows, ldq2, p.D, qd, wave);
+            copyG.run(p.gradOut + (((long long)b * p.Sq + first) * p.H + fetchHead) * p.D, rows, ldg2, p.D, gd, wave);
+        }
+        if (wave == 7)   // rows past the query length hold -inf and 0
+            atCopy4(atView(p.stats + 2 * (((long long)b * p.H + fetchHead) * p.SqP + first), 2 * kTileQ * 4), sd, lane * 4);
+        if (++fetchT == t1) {
+            fetchT = t0;
+            ++fetchHead;
         }
     };
-    at_f32x16 dk[KD], dv[KD];
+    at_f32x16 acc[KD];
 #pragma unroll
     for (int t = 0; t < KD; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
+        for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     DsScale<BF16, KD> scale;
 
-    auto tile = [&](int i, const uint16_t* qd, const uint16_t* gd, const float* sd) {
-        const int first = (t0 + i % per) * kTileKeys;
+    // nat: the tile whose product with the wave's own fragments makes S or dP; tr: the one that the sums take
+    auto work = [&](int first, const uint16_t* nat, const uint16_t* tr, const float* sd, float* wd) {
+        at_f32x16 s;
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-            const int qs = first + 32 * qb;
-            if (p.causal && qs + 31 + off < key0) continue;   // none of these queries sees the wave's keys
-            at_f32x16 s, dp;
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+        for (int st = 0; st < T::NS; ++st) s = atMfma<BF16>(at.natural(nat, 0, st), own[st], s);
+        atPipeline<T::NS, 1, T::NS < 4 ? T::NS : 4>();
+        if constexpr (!SECOND) {
 #pragma unroll
-            for (int st = 0; st < T::NS; ++st) {
-                s = atMfma<BF16>(T::natural(qd, 32 * qb, st, l, h), kf[st], s);
-                dp = atMfma<BF16>(T::natural(gd, 32 * qb, st, l, h), vf[st], dp);
+            for (int j = 0; j < 4; ++j) {
+                const at_f32x4 shift = *reinterpret_cast<const at_f32x4*>(sd + 8 * j + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, shift[e]));
             }
-            const bool edge = p.causal && qs + off < key0 + 31;
-            const int firstSeen = key - off - qs - 4 * h;   // rows from here on see the lane's key
+            if (p.causal && first + off < key0 + 31) {
+                const int firstSeen = key - off - first - 4 * h;   // rows from here on see the lane's key
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (8 * (r / 4) + r % 4 < firstSeen) s[r] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<at_f32x4*>(wd + j * 256 + lane * 4) =
+                    at_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+        } else {
             float most = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const at_f32x4 lse2 = *reinterpret_cast<const at_f32x4*>(sd + 32 * qb + 8 * j + 4 * h);
-                const at_f32x4 delta = *reinterpret_cast<const at_f32x4*>(sd + kTileKeys + 32 * qb + 8 * j + 4 * h);
+                const at_f32x4 w = *reinterpret_cast<const at_f32x4*>(wd + j * 256 + lane * 4);
+                const at_f32x4 delta = *reinterpret_cast<const at_f32x4*>(sd + kTileQ + 8 * j + 4 * h);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * j + e;
-                    float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, kRaise - lse2[e]));
-                    if (edge && 8 * j + e < firstSeen) w = 0.f;
-                    s[r] = w;
-                    dp[r] = w * (dp[r] - delta[e]);
-                    if constexpr (!BF16) most = fmaxf(most, fabsf(dp[r]));
+                    s[4 * j + e] = w[e] * (s[4 * j + e] - delta[e]);
+                    if constexpr (!BF16) most = fmaxf(most, fabsf(s[4 * j + e]));
                 }
             }
             if constexpr (!BF16) {
-                scale.update(atMaxHalves(most), dk);
+                scale.update(atMaxHalves(most), acc);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] *= scale.f;
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const at_u32x4 pf = atPack8<BF16>(s, u), df = atPack8<BF16>(dp, u);
-#pragma unroll
-                for (int dt = 0; dt < KD; ++dt) {
-                    dv[dt] = atMfma<BF16>(T::transposed(gd, 32 * qb + 16 * u, dt, lane), pf, dv[dt]);
-                    dk[dt] = atMfma<BF16>(T::transposed(qd, 32 * qb + 16 * u, dt, lane), df, dk[dt]);
-                }
+                for (int r = 0; r < 16; ++r) s[r] *= scale.f;
             }
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const at_u32x4 f = atPack8<BF16>(s, u);
+#pragma unroll
+            for (int dt = 0; dt < KD; ++dt) acc[dt] = atMfma<BF16>(at.transposed(tr, 16 * u, dt), f, acc[dt]);
+        }
+        if constexpr (SECOND && BF16) {   // one stretch of code with the product above
+            atReads<8>();   // weights, delta
+            atValu<20>();
+        }
+        atPipeline<2 * KD, 2, KD < 3 ? KD : 3>();
     };
-    if (end > begin) fetch(begin, q0, g0, s0);
-    for (int i = begin; i < end; i += 2) {   // as in the forward pass
+
+    // Trip i: the first waves take tile i from the buffers i % 3, the second ones tile i - 1 from those before, and tile
+    // i + 1 is copied into those after. Every wave makes trips 0 .. n, and so the same number of barriers. A tile whose
+    // queries see none of the wave's keys (the first few of a causal walk) has weights 0; leaving it out would cost
+    // every trip copies of the sums.
+    int t = per > 0 ? t0 + begin % per : 0;   // the wave's next tile
+    auto meet = [&](int i, auto bufTag) {
+        constexpr int NEXT = (decltype(bufTag)::value + 1) % 3;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (i + 1 < end) fetch(i + 1, q1, g1, s1);
-        if (key0 < nK) tile(i, q0, g0, s0);
-        if (i + 1 >= end) break;
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (i + 2 < end) fetch(i + 2, q0, g0, s0);
-        if (key0 < nK) tile(i + 1, q1, g1, s1);
+        if (i + 1 < n) fetch(lds.q[NEXT], lds.g[NEXT], lds.stats[NEXT]);
+    };
+    auto trip = [&](int i, auto bufTag) {
+        constexpr int BUF = decltype(bufTag)::value, MINE = SECOND ? (BUF + 2) % 3 : BUF;
+        meet(i, bufTag);
+        float* wd = lds.weights + (((SECOND ? ~i : i) & 1) * 4 + pair) * (kTileQ * 32);
+        if constexpr (SECOND)
+            work(t * kTileQ, lds.g[MINE], lds.q[MINE], lds.stats[MINE], wd);
+        else
+            work(t * kTileQ, lds.q[MINE], lds.g[MINE], lds.stats[MINE], wd);
+        if (++t == t1) t = t0;
+    };
+    if (n > 0) {
+        fetch(lds.q[0], lds.g[0], lds.stats[0]);
+        if constexpr (SECOND) meet(0, std::integral_constant<int, 0>{});
+        // whole rounds of the three buffers, then what is left: a way out of the middle of a round would cost every
+        // trip copies of the sums
+        using F = std::integral_constant<int, SECOND ? 1 : 0>;
+        using S = std::integral_constant<int, SECOND ? 2 : 1>;
+        using L = std::integral_constant<int, SECOND ? 0 : 2>;
+        int i = SECOND ? 1 : 0;
+        const int last = SECOND ? n : n - 1;
+        for (; i + 2 <= last; i += 3) {
+            trip(i, F{});
+            trip(i + 1, S{});
+            trip(i + 2, L{});
+        }
+        if (i <= last) trip(i, F{});
+        if (i + 1 <= last) trip(i + 1, S{});
+        if constexpr (!SECOND) __syncthreads();   // the second waves' last trip begins; nothing is copied any more
     }
+    const float f = SECOND ? p.scale * kLower * scale.undo() : kLower;
     if (p.parts > 1) {
         const long long row = ((long long)bh * p.parts + part) * ((long long)p.blocks * kBlockQ) + key;
-        storeColumnF32<KD>(p.dkPart + row * p.D, dk, p.scale * kLower * scale.undo(), h, p.D);
-        storeColumnF32<KD>(p.dvPart + row * p.D, dv, kLower, h, p.D);
-        return;
+        storeColumnF32<KD>((SECOND ? p.dkPart : p.dvPart) + row * p.D, acc, f, h, p.D);
+    } else if (key < p.Sk) {
+        storeColumn<BF16, KD>((SECOND ? p.dk : p.dv) + place, acc, f, h, p.D, key >= nK);
     }
-    if (key >= p.Sk) return;
-    const long long at = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
-    storeColumn<BF16, KD>(p.dk + at, dk, p.scale * kLower * scale.undo(), h, p.D, key >= nK);
-    storeColumn<BF16, KD>(p.dv + at, dv, kLower, h, p.D, key >= nK);
+}
+
+template <bool BF16, int KD>
+__global__ __launch_bounds__(512, 2) void attn_train_dkv_kernel(AttnTrainParams p) {
+    constexpr int N = kTileQ * AtTile<KD>::RS;
+    __shared__ __attribute__((aligned(256))) uint16_t q0[N];
+    __shared__ __attribute__((aligned(256))) uint16_t q1[N];
+    __shared__ __attribute__((aligned(256))) uint16_t q2[N];
+    __shared__ __attribute__((aligned(256))) uint16_t g0[N];
+    __shared__ __attribute__((aligned(256))) uint16_t g1[N];
+    __shared__ __attribute__((aligned(256))) uint16_t g2[N];
+    __shared__ __attribute__((aligned(256))) float s0[2 * kTileQ];
+    __shared__ __attribute__((aligned(256))) float s1[2 * kTileQ];
+    __shared__ __attribute__((aligned(256))) float s2[2 * kTileQ];
+    __shared__ __attribute__((aligned(16))) float weights[2 * 4 * kTileQ * 32];   // behind the tiles: their offsets fit a read's 16 bits
+    const DkvBuffers lds{{q0, q1, q2}, {g0, g1, g2}, {s0, s1, s2}, weights};
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave < 4)
+        dkvWalk<BF16, KD, false>(p, lds, wave, lane);
+    else
+        dkvWalk<BF16, KD, true>(p, lds, wave, lane);
 }
 
 // The parts' sums of dK (blockIdx.y 0) or dV (1), eight values of a key a thread.
@@ -625,7 +707,7 @@ int launchBackward(AttnTrainParams& p) {
     if (p.Sk > 0) {
         p.heads = (uint32_t)(p.B * p.Hkv);
         p.blocks = (uint32_t)((p.Sk + kBlockQ - 1) / kBlockQ);
-        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD>), dim3(p.heads * p.blocks * p.parts), dim3(256), 0, stream(), p);
+        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD>), dim3(p.heads * p.blocks * p.parts), dim3(512), 0, stream(), p);
         OMHIP_CHECK_LAUNCH();
         if (p.parts > 1) {
             const long long n = (long long)p.B * p.Sk * p.Hkv * (p.D / 8);
@@ -752,10 +834,9 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
     p.parts = dkvParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads));
     const size_t sums = p.parts > 1 ? keyBlocks * p.parts * kBlockQ * nHeadDim : 0;
     if (rows) {
-        p.lse2 = static_cast<float*>(workspace((rows + sums) * 2 * sizeof(float), kWsOperand));
-        if (!p.lse2) return -1;   // workspace() recorded the cause
-        p.delta = p.lse2 + rows;
-        p.dkPart = p.delta + rows;
+        p.stats = static_cast<float*>(workspace((rows + sums) * 2 * sizeof(float), kWsOperand));
+        if (!p.stats) return -1;   // workspace() recorded the cause
+        p.dkPart = p.stats + 2 * rows;
         p.dvPart = p.dkPart + sums;
     }
     return nDtype == 1 ? backward<true>(p) : backward<false>(p);
