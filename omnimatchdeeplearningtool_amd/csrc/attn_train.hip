@@ -226,50 +226,11 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
         }
 }
 
-// ---------------------------------------------------------------- backward: row statistics
-// shift = -lse log2 e and delta = sum_d dO O of every row, 32 rows at a time. Rows that pass no gradient (past the query
-// length, past Sq, or without a key) get shift = -inf, which makes their probabilities 0. A row of a head is read by
-// G lanes, 16 bytes of dO and O each.
-// P of the dK / dV kernel is taken raised by 2^15 in fp16 (it is at most 1, and loses bits below 2^-14): part of shift.
+// ---------------------------------------------------------------- backward
+// P of the dK / dV kernel is taken raised by 2^15 in fp16 (it is at most 1, and loses bits below 2^-14): part of the
+// row statistics' shift.
 template <bool BF16>
 constexpr float kRaise = BF16 ? 0.f : 15.f;
-
-template <bool BF16, int G>
-__global__ __launch_bounds__(256) void attn_train_delta_kernel(AttnTrainParams p) {
-    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / G;   // (b, q, head), head fastest
-    const int c = threadIdx.x % G;
-    if (row >= (long long)p.B * p.SqP * p.H) return;
-    const int head = (int)(row % p.H);
-    const long long bq = row / p.H;
-    const int q = (int)(bq % p.SqP), b = (int)(bq / p.SqP);
-    const bool valid = q < atLength(p.qLens, b, p.Sq);
-    float d = 0.f;
-    if (valid && c * 8 < p.D) {
-        const long long at = (((long long)b * p.Sq + q) * p.H + head) * p.D + c * 8;
-        const at_u32x4 g = *reinterpret_cast<const at_u32x4*>(p.gradOut + at);
-        const at_u32x4 o = *reinterpret_cast<const at_u32x4*>(p.out + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float g0, g1, o0, o1;
-            atUnpack2<BF16>(g[e], g0, g1);
-            atUnpack2<BF16>(o[e], o0, o1);
-            d = __builtin_fmaf(g0, o0, d);
-            d = __builtin_fmaf(g1, o1, d);
-        }
-    }
-#pragma unroll
-    for (int s = G / 2; s > 0; s >>= 1) d += __shfl_xor(d, s, 64);
-    if (c) return;
-    const long long bh = (long long)b * p.H + head;
-    float shift = -INFINITY;
-    if (valid) {
-        const float lse = p.lse[bh * p.Sq + q];
-        if (lse != -INFINITY) shift = kRaise<BF16> - lse * kAtLog2e;
-    }
-    float* to = p.stats + 2 * (bh * p.SqP + (q & ~31)) + (q & 31);
-    to[0] = shift;
-    to[32] = shift == -INFINITY ? 0.f : d;
-}
 
 // dS as halves. bf16 has fp32's range; fp16 loses dS below 2^-14 (a probability of 1 / 4096 times a gradient of
 // 2^-10 is there) and has no value past 65504. A lane's dS all go into one column of the sum (its query's dQ, its
@@ -330,7 +291,9 @@ __device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc
 
 // ---------------------------------------------------------------- backward: dQ
 // As the forward pass, a wave holds 32 queries as columns and the workgroup walks the keys: S^T = K Q^T,
-// dP^T = V dO^T, dQ^T += K^T dS^T.
+// dP^T = V dO^T, dQ^T += K^T dS^T. It also makes and leaves the rows' statistics, shift = -lse log2 e and delta =
+// sum_d dO O, for the dK / dV kernel that follows; rows that pass no gradient (past the query length, past Sq, or
+// without a key) get shift = -inf, which makes their probabilities 0.
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p) {
     using T = AtTile<KD>;
@@ -369,9 +332,33 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
             gf[s] = T::direct(grow, query < nQ, s, h, p.D);
         }
     }
-    // rows past the query length hold -inf and 0
-    const float* stats = p.stats + 2 * ((long long)bh * p.SqP + min(q0, p.SqP - 32)) + l;
-    const float shift = stats[0] - kRaise<BF16>, delta = stats[32];
+    float shift = -INFINITY, delta = 0.f;
+    {
+        const uint16_t* orow = p.out + (((long long)b * p.Sq + query) * p.H + head) * p.D;
+#pragma unroll
+        for (int s = 0; s < T::NS; ++s) {
+            const at_u32x4 o = T::direct(orow, query < nQ, s, h, p.D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float g0, g1, o0, o1;
+                atUnpack2<BF16>(gf[s][e], g0, g1);
+                atUnpack2<BF16>(o[e], o0, o1);
+                delta = __builtin_fmaf(g0, o0, delta);
+                delta = __builtin_fmaf(g1, o1, delta);
+            }
+        }
+        delta = atSumHalves(delta);
+        const float lse = query < nQ ? p.lse[(long long)bh * p.Sq + query] : -INFINITY;
+        if (lse == -INFINITY)
+            delta = 0.f;
+        else
+            shift = -lse * kAtLog2e;
+        if (h == 0 && query < p.SqP) {
+            float* to = p.stats + 2 * ((long long)bh * p.SqP + q0) + l;
+            to[0] = shift + kRaise<BF16>;
+            to[32] = delta;
+        }
+    }
     const float c = p.scale * kAtLog2e;
     const typename T::Lane at(lane);
     typename T::template Copy<kTileKeys, kWaves> copy;
@@ -389,9 +376,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
         for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
     DsScale<BF16, KD> scale;
 
-    auto tile = [&](int t, const uint16_t* kd, const uint16_t* vd) {
-        const int key0 = t * kTileKeys;
-        const bool edge = key0 + kTileKeys > nK || (p.causal && key0 + kTileKeys - 1 > q0 + off);
+    auto tile = [&](auto edgeTag, int key0, const uint16_t* kd, const uint16_t* vd) {
+        constexpr bool EDGE = decltype(edgeTag)::value;   // some query does not see some of the keys
         const int seen = (p.causal ? min(nK, query + off + 1) : nK) - key0 - 4 * h;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -403,11 +389,12 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
                 s = atMfma<BF16>(at.natural(kd, 32 * kb, st), qf[st], s);
                 dp = atMfma<BF16>(at.natural(vd, 32 * kb, st), gf[st], dp);
             }
+            atPipeline<2 * T::NS, 1, 4>();
             float most = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, shift));
-                if (edge && 32 * kb + 8 * (r / 4) + r % 4 >= seen) e = 0.f;
+                if (EDGE && 32 * kb + 8 * (r / 4) + r % 4 >= seen) e = 0.f;
                 s[r] = e * (dp[r] - delta);
                 if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
             }
@@ -420,16 +407,24 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
             for (int u = 0; u < 2; ++u) {
                 const at_u32x4 df = atPack8<BF16>(s, u);
 #pragma unroll
-                for (int dt = 0; dt < KD; ++dt)
-                    dq[dt] = atMfma<BF16>(at.transposed(kd, 32 * kb + 16 * u, dt), df, dq[dt]);
+                for (int dt = 0; dt < KD; ++dt) dq[dt] = atMfma<BF16>(at.transposed(kd, 32 * kb + 16 * u, dt), df, dq[dt]);
             }
+            atPipeline<2 * KD, 2, KD < 3 ? KD : 3>();
         }
+    };
+    auto step = [&](int t, const uint16_t* kd, const uint16_t* vd) {
+        const int key0 = t * kTileKeys;
+        if (key0 >= waveEnd) return;
+        if (key0 + kTileKeys > nK || (p.causal && key0 + kTileKeys - 1 > q0 + off))
+            tile(std::true_type{}, key0, kd, vd);
+        else
+            tile(std::false_type{}, key0, kd, vd);
     };
     auto trip = [&](int t, const uint16_t* kd, const uint16_t* vd, uint16_t* kNext, uint16_t* vNext) {   // as in the forward pass
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (t + 1 < nt) fetch(t + 1, kNext, vNext);
-        if (t * kTileKeys < waveEnd) tile(t, kd, vd);
+        step(t, kd, vd);
     };
     if (nt > 0) fetch(0, k0, v0);
     int t = 0;
@@ -685,20 +680,9 @@ int launchForward(AttnTrainParams& p) {
     return 0;
 }
 
-template <bool BF16, int G>
-int launchDelta(const AttnTrainParams& p, long long rows) {
-    hipLaunchKernelGGL((attn_train_delta_kernel<BF16, G>), dim3((unsigned)((rows * G + 255) / 256)), dim3(256), 0, stream(), p);
-    OMHIP_CHECK_LAUNCH();
-    return 0;
-}
-
 template <bool BF16, int KD>
 int launchBackward(AttnTrainParams& p) {
     if (p.Sq > 0) {
-        const long long rows = (long long)p.B * p.SqP * p.H;
-        const int rc = KD == 4 || KD == 3 ? launchDelta<BF16, 16>(p, rows) : KD == 2 ? launchDelta<BF16, 8>(p, rows)
-                                                                                     : launchDelta<BF16, 4>(p, rows);
-        if (rc) return rc;
         p.heads = (uint32_t)(p.B * p.H);
         p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
         hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
