@@ -129,21 +129,24 @@ __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
     }
 }
 
-// gradBias[c] = the chunks' partial sums, eight interleaved runs of them a column, then those in order.
-__global__ __launch_bounds__(256) void dropout_bias_sum_kernel(const float* partials, float* gradBias, int chunks, int cols) {
-    __shared__ float part[8][33];
+// gradBias[c] = the chunks' partial sums: 32 interleaved runs of them a column, then those pairwise. (8 runs took 20 us
+// for 512 chunks of 1024 columns: loads waited out one by one.)
+__global__ __launch_bounds__(1024) void dropout_bias_sum_kernel(const float* partials, float* gradBias, int chunks, int cols) {
+    __shared__ float part[32][33];
     const int tc = threadIdx.x & 31, tr = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + tc;
     float s = 0.f;
-    if (c < cols)
-        for (int i = tr; i < chunks; i += 8) s += partials[(long long)i * cols + c];
-    part[tr][tc] = s;
-    __syncthreads();
-    if (tr == 0 && c < cols) {
-        s = 0.f;
-        for (int i = 0; i < 8; ++i) s += part[i][tc];
-        gradBias[c] = s;
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = tr; i < chunks; i += 32) s += partials[(long long)i * cols + c];
     }
+    part[tr][tc] = s;
+#pragma unroll
+    for (int half = 16; half > 0; half /= 2) {
+        __syncthreads();
+        if (tr < half) part[tr][tc] += part[tr + half][tc];
+    }
+    if (tr == 0 && c < cols) gradBias[c] = part[0][tc];
 }
 
 template <int DT>
@@ -177,7 +180,7 @@ int backwardWithBias(DropoutParams& p, float* pGradBias) {
                  : tc == 16 ? launchDropoutBias<DT, 16>(p, chunks)
                             : launchDropoutBias<DT, 4>(p, chunks);
     if (rc) return rc;
-    hipLaunchKernelGGL(dropout_bias_sum_kernel, dim3((p.cols + 31) / 32), dim3(256), 0, stream(), p.partials, pGradBias,
+    hipLaunchKernelGGL(dropout_bias_sum_kernel, dim3((p.cols + 31) / 32), dim3(1024), 0, stream(), p.partials, pGradBias,
                        chunks, p.cols);
     OMHIP_CHECK_LAUNCH();
     return 0;

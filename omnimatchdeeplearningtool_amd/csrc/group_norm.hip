@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace omhip {
 
@@ -83,6 +84,15 @@ struct Place {
     }
 };
 
+// Calls f(rows, r) for the thread's rows r, r + TR, ..., four at a time, so that as many loads are under way, then the
+// rest one by one. (The loads of a row after a store could not be moved before it: the output may be the input.)
+template <class W, class F>
+__device__ __forceinline__ void forRows(const W& w, F&& f) {
+    int r = w.tr;
+    for (; r + 3 * W::TR < w.rows; r += 4 * W::TR) f(std::integral_constant<int, 4>{}, r);
+    for (; r < w.rows; r += W::TR) f(std::integral_constant<int, 1>{}, r);
+}
+
 // What a thread needs of its channels.
 struct Channels {
     float mean[8], inv[8], gamma[8], beta[8];
@@ -99,7 +109,7 @@ struct Channels {
     }
 };
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
@@ -131,17 +141,21 @@ __global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams
     for (int i = 0; i < 8; ++i) shift[i] = s[i] = q[i] = 0.f;
     if (w.n > 0) {
         if (w.tr < w.rows) Vec8<DT>::load(p.x, w.at(p, w.tr), w.n, shift);
-        for (int r = w.tr; r < w.rows; r += W::TR) {
-            float x[8];
-            Vec8<DT>::load(p.x, w.at(p, r), w.n, x);
+        forRows<W>(w, [&](auto rowsTag, int r) {
+            constexpr int ROWS = decltype(rowsTag)::value;
+            float x[ROWS][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = x[i] - shift[i];
-                s[i] += d;
-                q[i] = __builtin_fmaf(d, d, q[i]);
-            }
-            count += 1.f;
-        }
+            for (int k = 0; k < ROWS; ++k) Vec8<DT>::load(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float d = x[k][i] - shift[i];
+                    s[i] += d;
+                    q[i] = __builtin_fmaf(d, d, q[i]);
+                }
+            count += (float)ROWS;
+        });
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -199,30 +213,39 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p
     ch.load(p, w.image, w.c, w.n);
 #pragma unroll
     for (int i = 0; i < 8; ++i) ch.inv[i] *= ch.gamma[i];
-    for (int r = w.tr; r < w.rows; r += W::TR) {
-        float x[8];
-        Vec8<DT>::load(p.x, w.at(p, r), w.n, x);
+    forRows<W>(w, [&](auto rowsTag, int r) {
+        constexpr int ROWS = decltype(rowsTag)::value;
+        float x[ROWS][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = activate<ACT>(__builtin_fmaf(x[i] - ch.mean[i], ch.inv[i], ch.beta[i]));
-        Vec8<DT>::store(p.out, w.at(p, r), w.n, x);
-    }
+        for (int k = 0; k < ROWS; ++k) Vec8<DT>::load(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[k][i] = activate<ACT>(__builtin_fmaf(x[k][i] - ch.mean[i], ch.inv[i], ch.beta[i]));
+            Vec8<DT>::store(p.out, w.at(p, r + k * W::TR), w.n, x[k]);
+        }
+    });
 }
 
 // ---------------------------------------------------------------- backward
 // xhat and dz of 8 channels of a row
 template <int DT, int ACT>
-__device__ __forceinline__ void loadRow(const GroupNormParams& p, const Channels& ch, long long at, int n, float (&xhat)[8],
-                                        float (&dz)[8]) {
-    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    Vec8<DT>::load(p.x, at, n, xhat);
-    Vec8<DT>::load(p.gradY, at, n, dz);
-    if constexpr (ACT == kActRelu) Vec8<DT>::load(p.y, at, n, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        xhat[i] = (xhat[i] - ch.mean[i]) * ch.inv[i];
-        dz[i] = gradient<ACT>(dz[i], __builtin_fmaf(xhat[i], ch.gamma[i], ch.beta[i]), y[i]);
+struct Row {
+    float xhat[8], dz[8], y[ACT == kActRelu ? 8 : 1];
+    __device__ __forceinline__ void load(const GroupNormParams& p, long long at, int n) {
+        Vec8<DT>::load(p.x, at, n, xhat);
+        Vec8<DT>::load(p.gradY, at, n, dz);
+        if constexpr (ACT == kActRelu) Vec8<DT>::load(p.y, at, n, y);
     }
-}
+    __device__ __forceinline__ void work(const Channels& ch) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            xhat[i] = (xhat[i] - ch.mean[i]) * ch.inv[i];
+            dz[i] = gradient<ACT>(dz[i], __builtin_fmaf(xhat[i], ch.gamma[i], ch.beta[i]), y[ACT == kActRelu ? i : 0]);
+        }
+    }
+};
 
 template <int DT, int TC, int ACT>
 __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p) {
@@ -235,15 +258,21 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
     if (w.n > 0) {
         Channels ch;
         ch.load(p, w.image, w.c, w.n);
-        for (int r = w.tr; r < w.rows; r += W::TR) {
-            float xhat[8], dz[8];
-            loadRow<DT, ACT>(p, ch, w.at(p, r), w.n, xhat, dz);
+        forRows<W>(w, [&](auto rowsTag, int r) {
+            constexpr int ROWS = decltype(rowsTag)::value;
+            Row<DT, ACT> row[ROWS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                a[i] += dz[i];
-                b[i] = __builtin_fmaf(dz[i], xhat[i], b[i]);
+            for (int k = 0; k < ROWS; ++k) row[k].load(p, w.at(p, r + k * W::TR), w.n);
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                row[k].work(ch);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a[i] += row[k].dz[i];
+                    b[i] = __builtin_fmaf(row[k].dz[i], row[k].xhat[i], b[i]);
+                }
             }
-        }
+        });
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[i][threadIdx.x] = {a[i], b[i]};
@@ -266,46 +295,51 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
 }
 
 // Workgroups 0 .. N * G - 1: a group's means of gamma dz and gamma dz xhat. The others: dgamma and dbeta of 32
-// channels, eight interleaved runs over images and chunks a channel.
-__global__ __launch_bounds__(256) void group_norm_join_backward_kernel(GroupNormParams p) {
-    __shared__ float2 part[256];
+// channels, 32 interleaved runs over images and chunks a channel (with 8, the loads' latency took 58 us at 32 x 28 x 28
+// x 512, now under 5).
+__global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p) {
+    __shared__ float2 part[1024];
     const int t = threadIdx.x;
     float2 s{0.f, 0.f};
     const long long groups = (long long)p.N * p.G;
-    if (blockIdx.x < groups) {
+    const bool group = blockIdx.x < groups;
+    const int c = group ? 0 : (int)(blockIdx.x - groups) * 32 + (t & 31);
+    if (group) {
         const int image = (int)(blockIdx.x / p.G), g = (int)(blockIdx.x % p.G);
         const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
-        for (long long e = t; e < (long long)p.chunks * p.per; e += 256) {
-            const int chunk = (int)(e / p.per), c = (int)(e - (long long)chunk * p.per);
-            const float2 v = from[(long long)chunk * p.C + c];
-            const float gamma = p.gamma ? p.gamma[g * p.per + c] : 1.f;
+#pragma unroll 4
+        for (long long e = t; e < (long long)p.chunks * p.per; e += 1024) {
+            const int chunk = (int)(e / p.per), k = (int)(e - (long long)chunk * p.per);
+            const float2 v = from[(long long)chunk * p.C + k];
+            const float gamma = p.gamma ? p.gamma[g * p.per + k] : 1.f;
             s.x = __builtin_fmaf(gamma, v.x, s.x);
             s.y = __builtin_fmaf(gamma, v.y, s.y);
         }
-        part[t] = s;
-#pragma unroll
-        for (int half = 128; half > 0; half /= 2) {
-            __syncthreads();
-            if (t < half) part[t] = {part[t].x + part[t + half].x, part[t].y + part[t + half].y};
-        }
-        if (t == 0) {
-            const float f = 1.f / ((float)p.P * (float)p.per);
-            p.means[blockIdx.x] = {part[0].x * f, part[0].y * f};
-        }
-        return;
-    }
-    const int c = (int)(blockIdx.x - groups) * 32 + (t & 31);
-    if (c < p.C)
-        for (long long e = t >> 5; e < (long long)p.N * p.chunks; e += 8) {
+    } else if (c < p.C) {
+#pragma unroll 8
+        for (long long e = t >> 5; e < (long long)p.N * p.chunks; e += 32) {
             const float2 v = p.partial[e * p.C + c];
             s.x += v.x;
             s.y += v.y;
         }
+    }
     part[t] = s;
-    __syncthreads();
-    if (t < 32 && c < p.C) {
-        s = {0.f, 0.f};
-        for (int i = 0; i < 8; ++i) s = {s.x + part[t + 32 * i].x, s.y + part[t + 32 * i].y};
+#pragma unroll
+    for (int half = 512; half >= 32; half /= 2) {   // down to 32 sums: a channel each, or a group's
+        __syncthreads();
+        if (t < half) part[t] = {part[t].x + part[t + half].x, part[t].y + part[t + half].y};
+    }
+    if (t >= 32) return;
+    s = part[t];
+    if (group) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) {
+            s.x += __shfl_down(s.x, d, 64);
+            s.y += __shfl_down(s.y, d, 64);
+        }
+        const float f = 1.f / ((float)p.P * (float)p.per);
+        if (t == 0) p.means[blockIdx.x] = {s.x * f, s.y * f};
+    } else if (c < p.C) {
         if (p.gradBeta) p.gradBeta[c] = s.x;
         if (p.gradGamma) p.gradGamma[c] = s.y;
     }
@@ -321,14 +355,20 @@ __global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParam
     float2 m[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) m[i] = p.means[(long long)w.image * p.G + (i < w.n ? (w.c + i) / p.per : 0)];
-    for (int r = w.tr; r < w.rows; r += W::TR) {
-        float xhat[8], dz[8];
-        loadRow<DT, ACT>(p, ch, w.at(p, r), w.n, xhat, dz);
+    forRows<W>(w, [&](auto rowsTag, int r) {
+        constexpr int ROWS = decltype(rowsTag)::value;
+        Row<DT, ACT> row[ROWS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            dz[i] = ch.inv[i] * (__builtin_fmaf(dz[i], ch.gamma[i], -m[i].x) - xhat[i] * m[i].y);
-        Vec8<DT>::store(p.out, w.at(p, r), w.n, dz);
-    }
+        for (int k = 0; k < ROWS; ++k) row[k].load(p, w.at(p, r + k * W::TR), w.n);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            row[k].work(ch);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                row[k].dz[i] = ch.inv[i] * (__builtin_fmaf(row[k].dz[i], ch.gamma[i], -m[i].x) - row[k].xhat[i] * m[i].y);
+            Vec8<DT>::store(p.out, w.at(p, r + k * W::TR), w.n, row[k].dz);
+        }
+    });
 }
 
 // ---------------------------------------------------------------- launches
@@ -350,7 +390,7 @@ int launchBackward(const GroupNormParams& p) {
     hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     const int channels = p.gradGamma || p.gradBeta ? (p.C + 31) / 32 : 0;
-    hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(p.N * p.G + channels), dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(p.N * p.G + channels), dim3(1024), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     hipLaunchKernelGGL((group_norm_gradient_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
