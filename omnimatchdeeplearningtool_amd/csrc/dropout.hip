@@ -67,7 +67,7 @@ __device__ __forceinline__ Bits philox(uint32_t group, uint32_t stream, uint64_t
 
 // One group of 8 columns a thread: out = keep ? (x + bias) scale : 0, + residual. The backward pass is the same
 // without bias and residual.
-template <int DT>
+template <int DT, bool EVEN>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutParams p) {
     const uint32_t g = blockIdx.x * 256u + threadIdx.x;
     if (g >= p.groups) return;
@@ -75,24 +75,24 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutParams p) {
     const int n = min(8, p.cols - (int)c);
     const long long at = (long long)r * p.cols + c;
     float x[8], res[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    Vec8<DT>::load(p.x, at, n, x);
-    if (p.residual) Vec8<DT>::load(p.residual, at, n, res);
+    Vec8<DT>::template load<EVEN>(p.x, at, n, x);
+    if (p.residual) Vec8<DT>::template load<EVEN>(p.residual, at, n, res);
     if (p.bias) {
         float b[8];
-        Vec8<2>::load(p.bias, c, n, b);
+        Vec8<2>::load<EVEN>(p.bias, c, n, b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] += b[i];
     }
     const Bits bits = philox(g, p.stream, p.rng[0], p.rng[1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = bits.keep(i, p.threshold) ? __builtin_fmaf(x[i], p.scale, res[i]) : res[i];
-    Vec8<DT>::store(p.out, at, n, x);
+    Vec8<DT>::template store<EVEN>(p.out, at, n, x);
 }
 
 // Backward with the bias gradient: a workgroup takes TC groups of columns and a chunk of rows, 256 / TC rows at a
 // time, and adds each column's kept gradients (unrounded) in row order; the threads of a column group are added in
 // order at the end and leave one row of partial sums a chunk.
-template <int DT, int TC>
+template <int DT, int TC, bool EVEN>
 __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
     constexpr int TR = 256 / TC;
     __shared__ float part[TR][TC * 8 + 1];
@@ -107,14 +107,14 @@ __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
         for (int r = (int)first + tr; r < last; r += TR) {
             const long long at = (long long)r * p.cols + c;
             float x[8];
-            Vec8<DT>::load(p.x, at, n, x);
+            Vec8<DT>::template load<EVEN>(p.x, at, n, x);
             const Bits bits = philox((uint32_t)r * p.perRow.d + cg, p.stream, seed, step);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 x[i] = bits.keep(i, p.threshold) ? x[i] * p.scale : 0.f;
                 sum[i] += x[i];
             }
-            Vec8<DT>::store(p.out, at, n, x);
+            Vec8<DT>::template store<EVEN>(p.out, at, n, x);
         }
     }
 #pragma unroll
@@ -151,14 +151,22 @@ __global__ __launch_bounds__(1024) void dropout_bias_sum_kernel(const float* par
 
 template <int DT>
 int launchDropout(const DropoutParams& p) {
-    hipLaunchKernelGGL((dropout_kernel<DT>), dim3((p.groups + 255u) / 256u), dim3(256), 0, stream(), p);
+    const dim3 grid((p.groups + 255u) / 256u);
+    if (p.cols % 8 == 0)
+        hipLaunchKernelGGL((dropout_kernel<DT, true>), grid, dim3(256), 0, stream(), p);
+    else
+        hipLaunchKernelGGL((dropout_kernel<DT, false>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }
 
 template <int DT, int TC>
 int launchDropoutBias(const DropoutParams& p, int chunks) {
-    hipLaunchKernelGGL((dropout_bias_kernel<DT, TC>), dim3((p.perRow.d + TC - 1) / TC, chunks), dim3(256), 0, stream(), p);
+    const dim3 grid((p.perRow.d + TC - 1) / TC, chunks);
+    if (p.cols % 8 == 0)
+        hipLaunchKernelGGL((dropout_bias_kernel<DT, TC, true>), grid, dim3(256), 0, stream(), p);
+    else
+        hipLaunchKernelGGL((dropout_bias_kernel<DT, TC, false>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }

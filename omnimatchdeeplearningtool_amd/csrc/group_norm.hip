@@ -20,6 +20,7 @@
 // (T. F. Chan, G. H. Golub, R. J. LeVeque, "Updating formulae and a pairwise
 // algorithm for computing sample variances", 1979): a mean far above the
 // spread costs no digits. The order is fixed; nothing is added atomically.
+#include "fastdiv.hpp"
 #include "omhip_internal.hpp"
 #include "vec_io.hpp"
 #include "../../include/omhip.h"
@@ -41,6 +42,7 @@ struct GroupNormParams {
     float2* means;                  // backward, [N, G]: the group means of gamma dz and gamma dz xhat
     float *gradGamma, *gradBeta;    // or null
     int N, P, C, G, per;            // per: channels of a group
+    FastDiv byPer;
     int chunks, rowsPerChunk;
     float eps;
 };
@@ -94,17 +96,32 @@ __device__ __forceinline__ void forRows(const W& w, F&& f) {
 }
 
 // What a thread needs of its channels.
+template <bool EVEN>
 struct Channels {
     float mean[8], inv[8], gamma[8], beta[8];
     __device__ __forceinline__ void load(const GroupNormParams& p, int image, int c, int n) {
+        const int g0 = c / p.per, g1 = (c + n - 1) / p.per;   // the first and the last channel's group
+        const float *m = p.mean + (long long)image * p.G, *v = p.inv + (long long)image * p.G;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool in = i < n;
-            const int g = in ? (c + i) / p.per : 0;
-            mean[i] = p.mean[(long long)image * p.G + g];
-            inv[i] = p.inv[(long long)image * p.G + g];
-            gamma[i] = in && p.gamma ? p.gamma[c + i] : 1.f;
-            beta[i] = in && p.beta ? p.beta[c + i] : 0.f;
+            gamma[i] = 1.f;
+            beta[i] = 0.f;
+        }
+        if (p.gamma) Vec8<2>::load<EVEN>(p.gamma, c, n, gamma);
+        if (p.beta) Vec8<2>::load<EVEN>(p.beta, c, n, beta);
+        if (g0 == g1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                mean[i] = m[g0];
+                inv[i] = v[g0];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int g = i < n ? (c + i) / p.per : g0;
+                mean[i] = m[g];
+                inv[i] = v[g];
+            }
         }
     }
 };
@@ -130,7 +147,7 @@ __device__ __forceinline__ float gradient(float dy, float z, float y) {
 }
 
 // ---------------------------------------------------------------- forward
-template <int DT, int TC>
+template <int DT, int TC, bool EVEN>
 __global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams p) {
     using W = Place<TC>;
     __shared__ float2 part[8][256];
@@ -140,12 +157,12 @@ __global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams
 #pragma unroll
     for (int i = 0; i < 8; ++i) shift[i] = s[i] = q[i] = 0.f;
     if (w.n > 0) {
-        if (w.tr < w.rows) Vec8<DT>::load(p.x, w.at(p, w.tr), w.n, shift);
+        if (w.tr < w.rows) Vec8<DT>::template load<EVEN>(p.x, w.at(p, w.tr), w.n, shift);
         forRows<W>(w, [&](auto rowsTag, int r) {
             constexpr int ROWS = decltype(rowsTag)::value;
             float x[ROWS][8];
 #pragma unroll
-            for (int k = 0; k < ROWS; ++k) Vec8<DT>::load(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
+            for (int k = 0; k < ROWS; ++k) Vec8<DT>::template load<EVEN>(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
 #pragma unroll
             for (int k = 0; k < ROWS; ++k)
 #pragma unroll
@@ -189,11 +206,13 @@ __global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams
 __global__ __launch_bounds__(64) void group_norm_join_kernel(GroupNormParams p) {
     const int g = blockIdx.x, image = blockIdx.y, lane = threadIdx.x;
     const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
+    const uint32_t n = (uint32_t)p.chunks * (uint32_t)p.per;
     Moments t{0.f, 0.f, 0.f};
-    for (long long e = lane; e < (long long)p.chunks * p.per; e += 64) {
-        const int chunk = (int)(e / p.per), c = (int)(e - (long long)chunk * p.per);
+#pragma unroll 4
+    for (uint32_t e = lane; e < n; e += 64) {
+        const uint32_t chunk = p.byPer.div(e), c = e - chunk * (uint32_t)p.per;
         const float2 v = from[(long long)chunk * p.C + c];
-        t = join(t, {(float)chunkRows(p, chunk), v.x, v.y});
+        t = join(t, {(float)chunkRows(p, (int)chunk), v.x, v.y});
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1)
@@ -204,12 +223,12 @@ __global__ __launch_bounds__(64) void group_norm_join_kernel(GroupNormParams p) 
     }
 }
 
-template <int DT, int TC, int ACT>
+template <int DT, int TC, int ACT, bool EVEN>
 __global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p) {
     using W = Place<TC>;
     const W w(p);
     if (w.n <= 0) return;
-    Channels ch;
+    Channels<EVEN> ch;
     ch.load(p, w.image, w.c, w.n);
 #pragma unroll
     for (int i = 0; i < 8; ++i) ch.inv[i] *= ch.gamma[i];
@@ -217,28 +236,28 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p
         constexpr int ROWS = decltype(rowsTag)::value;
         float x[ROWS][8];
 #pragma unroll
-        for (int k = 0; k < ROWS; ++k) Vec8<DT>::load(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
+        for (int k = 0; k < ROWS; ++k) Vec8<DT>::template load<EVEN>(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 x[k][i] = activate<ACT>(__builtin_fmaf(x[k][i] - ch.mean[i], ch.inv[i], ch.beta[i]));
-            Vec8<DT>::store(p.out, w.at(p, r + k * W::TR), w.n, x[k]);
+            Vec8<DT>::template store<EVEN>(p.out, w.at(p, r + k * W::TR), w.n, x[k]);
         }
     });
 }
 
 // ---------------------------------------------------------------- backward
 // xhat and dz of 8 channels of a row
-template <int DT, int ACT>
+template <int DT, int ACT, bool EVEN>
 struct Row {
     float xhat[8], dz[8], y[ACT == kActRelu ? 8 : 1];
     __device__ __forceinline__ void load(const GroupNormParams& p, long long at, int n) {
-        Vec8<DT>::load(p.x, at, n, xhat);
-        Vec8<DT>::load(p.gradY, at, n, dz);
-        if constexpr (ACT == kActRelu) Vec8<DT>::load(p.y, at, n, y);
+        Vec8<DT>::template load<EVEN>(p.x, at, n, xhat);
+        Vec8<DT>::template load<EVEN>(p.gradY, at, n, dz);
+        if constexpr (ACT == kActRelu) Vec8<DT>::template load<EVEN>(p.y, at, n, y);
     }
-    __device__ __forceinline__ void work(const Channels& ch) {
+    __device__ __forceinline__ void work(const Channels<EVEN>& ch) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             xhat[i] = (xhat[i] - ch.mean[i]) * ch.inv[i];
@@ -247,7 +266,7 @@ struct Row {
     }
 };
 
-template <int DT, int TC, int ACT>
+template <int DT, int TC, int ACT, bool EVEN>
 __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p) {
     using W = Place<TC>;
     __shared__ float2 part[8][256];
@@ -256,11 +275,11 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
     if (w.n > 0) {
-        Channels ch;
+        Channels<EVEN> ch;
         ch.load(p, w.image, w.c, w.n);
         forRows<W>(w, [&](auto rowsTag, int r) {
             constexpr int ROWS = decltype(rowsTag)::value;
-            Row<DT, ACT> row[ROWS];
+            Row<DT, ACT, EVEN> row[ROWS];
 #pragma unroll
             for (int k = 0; k < ROWS; ++k) row[k].load(p, w.at(p, r + k * W::TR), w.n);
 #pragma unroll
@@ -294,28 +313,39 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
     }
 }
 
-// Workgroups 0 .. N * G - 1: a group's means of gamma dz and gamma dz xhat. The others: dgamma and dbeta of 32
-// channels, 32 interleaved runs over images and chunks a channel (with 8, the loads' latency took 58 us at 32 x 28 x 28
-// x 512, now under 5).
+// The first workgroups: the means of gamma dz and gamma dz xhat of 16 groups, a wave each. The others: dgamma and dbeta
+// of 32 channels, 32 interleaved runs over images and chunks a channel (with 8 runs, the loads' latency took 58 us at
+// 32 x 28 x 28 x 512).
 __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p) {
     __shared__ float2 part[1024];
     const int t = threadIdx.x;
     float2 s{0.f, 0.f};
-    const long long groups = (long long)p.N * p.G;
-    const bool group = blockIdx.x < groups;
-    const int c = group ? 0 : (int)(blockIdx.x - groups) * 32 + (t & 31);
-    if (group) {
-        const int image = (int)(blockIdx.x / p.G), g = (int)(blockIdx.x % p.G);
+    const uint32_t groups = (uint32_t)(p.N * p.G), groupBlocks = (groups + 15u) / 16u;
+    if (blockIdx.x < groupBlocks) {
+        const uint32_t id = blockIdx.x * 16u + (uint32_t)(t >> 6), lane = (uint32_t)t & 63u;
+        if (id >= groups) return;
+        const uint32_t image = id / (uint32_t)p.G, g = id - image * (uint32_t)p.G;
         const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
+        const uint32_t n = (uint32_t)p.chunks * (uint32_t)p.per;
 #pragma unroll 4
-        for (long long e = t; e < (long long)p.chunks * p.per; e += 1024) {
-            const int chunk = (int)(e / p.per), k = (int)(e - (long long)chunk * p.per);
+        for (uint32_t e = lane; e < n; e += 64) {
+            const uint32_t chunk = p.byPer.div(e), k = e - chunk * (uint32_t)p.per;
             const float2 v = from[(long long)chunk * p.C + k];
             const float gamma = p.gamma ? p.gamma[g * p.per + k] : 1.f;
             s.x = __builtin_fmaf(gamma, v.x, s.x);
             s.y = __builtin_fmaf(gamma, v.y, s.y);
         }
-    } else if (c < p.C) {
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) {
+            s.x += __shfl_down(s.x, d, 64);
+            s.y += __shfl_down(s.y, d, 64);
+        }
+        const float f = 1.f / ((float)p.P * (float)p.per);
+        if (lane == 0) p.means[id] = {s.x * f, s.y * f};
+        return;
+    }
+    const int c = (int)(blockIdx.x - groupBlocks) * 32 + (t & 31);
+    if (c < p.C) {
 #pragma unroll 8
         for (long long e = t >> 5; e < (long long)p.N * p.chunks; e += 32) {
             const float2 v = p.partial[e * p.C + c];
@@ -325,39 +355,29 @@ __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNor
     }
     part[t] = s;
 #pragma unroll
-    for (int half = 512; half >= 32; half /= 2) {   // down to 32 sums: a channel each, or a group's
+    for (int half = 512; half >= 32; half /= 2) {   // down to a sum a channel
         __syncthreads();
         if (t < half) part[t] = {part[t].x + part[t + half].x, part[t].y + part[t + half].y};
     }
-    if (t >= 32) return;
-    s = part[t];
-    if (group) {
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            s.x += __shfl_down(s.x, d, 64);
-            s.y += __shfl_down(s.y, d, 64);
-        }
-        const float f = 1.f / ((float)p.P * (float)p.per);
-        if (t == 0) p.means[blockIdx.x] = {s.x * f, s.y * f};
-    } else if (c < p.C) {
-        if (p.gradBeta) p.gradBeta[c] = s.x;
-        if (p.gradGamma) p.gradGamma[c] = s.y;
+    if (t < 32 && c < p.C) {
+        if (p.gradBeta) p.gradBeta[c] = part[t].x;
+        if (p.gradGamma) p.gradGamma[c] = part[t].y;
     }
 }
 
-template <int DT, int TC, int ACT>
+template <int DT, int TC, int ACT, bool EVEN>
 __global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParams p) {
     using W = Place<TC>;
     const W w(p);
     if (w.n <= 0) return;
-    Channels ch;
+    Channels<EVEN> ch;
     ch.load(p, w.image, w.c, w.n);
     float2 m[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) m[i] = p.means[(long long)w.image * p.G + (i < w.n ? (w.c + i) / p.per : 0)];
     forRows<W>(w, [&](auto rowsTag, int r) {
         constexpr int ROWS = decltype(rowsTag)::value;
-        Row<DT, ACT> row[ROWS];
+        Row<DT, ACT, EVEN> row[ROWS];
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) row[k].load(p, w.at(p, r + k * W::TR), w.n);
 #pragma unroll
@@ -366,52 +386,57 @@ __global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParam
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 row[k].dz[i] = ch.inv[i] * (__builtin_fmaf(row[k].dz[i], ch.gamma[i], -m[i].x) - row[k].xhat[i] * m[i].y);
-            Vec8<DT>::store(p.out, w.at(p, r + k * W::TR), w.n, row[k].dz);
+            Vec8<DT>::template store<EVEN>(p.out, w.at(p, r + k * W::TR), w.n, row[k].dz);
         }
     });
 }
 
 // ---------------------------------------------------------------- launches
-template <int DT, int TC, int ACT>
+template <int DT, int TC, int ACT, bool EVEN>
 int launchForward(const GroupNormParams& p) {
     const dim3 grid((p.C + 8 * TC - 1) / (8 * TC), p.chunks, p.N);
-    hipLaunchKernelGGL((group_norm_moments_kernel<DT, TC>), grid, dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL((group_norm_moments_kernel<DT, TC, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     hipLaunchKernelGGL(group_norm_join_kernel, dim3(p.G, p.N), dim3(64), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
-    hipLaunchKernelGGL((group_norm_apply_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL((group_norm_apply_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }
 
-template <int DT, int TC, int ACT>
+template <int DT, int TC, int ACT, bool EVEN>
 int launchBackward(const GroupNormParams& p) {
     const dim3 grid((p.C + 8 * TC - 1) / (8 * TC), p.chunks, p.N);
-    hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     const int channels = p.gradGamma || p.gradBeta ? (p.C + 31) / 32 : 0;
-    hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(p.N * p.G + channels), dim3(1024), 0, stream(), p);
+    hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3((p.N * p.G + 15) / 16 + channels), dim3(1024), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
-    hipLaunchKernelGGL((group_norm_gradient_kernel<DT, TC, ACT>), grid, dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL((group_norm_gradient_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     return 0;
+}
+
+template <int DT, int TC, bool EVEN>
+int byAct(const GroupNormParams& p, int act, bool backward) {
+    if (backward)
+        return act == kActNone ? launchBackward<DT, TC, kActNone, EVEN>(p)
+             : act == kActRelu ? launchBackward<DT, TC, kActRelu, EVEN>(p)
+                               : launchBackward<DT, TC, kActSilu, EVEN>(p);
+    return act == kActNone ? launchForward<DT, TC, kActNone, EVEN>(p)
+         : act == kActRelu ? launchForward<DT, TC, kActRelu, EVEN>(p)
+                           : launchForward<DT, TC, kActSilu, EVEN>(p);
 }
 
 template <int DT, int TC>
-int byAct(const GroupNormParams& p, int act, bool backward) {
-    if (backward)
-        return act == kActNone ? launchBackward<DT, TC, kActNone>(p)
-             : act == kActRelu ? launchBackward<DT, TC, kActRelu>(p)
-                               : launchBackward<DT, TC, kActSilu>(p);
-    return act == kActNone ? launchForward<DT, TC, kActNone>(p)
-         : act == kActRelu ? launchForward<DT, TC, kActRelu>(p)
-                           : launchForward<DT, TC, kActSilu>(p);
+int byRows(const GroupNormParams& p, int act, bool backward) {
+    return p.C % 8 == 0 ? byAct<DT, TC, true>(p, act, backward) : byAct<DT, TC, false>(p, act, backward);
 }
 
 template <int DT>
 int byWidth(const GroupNormParams& p, int tc, int act, bool backward) {
-    return tc == 64 ? byAct<DT, 64>(p, act, backward) : tc == 32 ? byAct<DT, 32>(p, act, backward)
-                                                                 : byAct<DT, 8>(p, act, backward);
+    return tc == 64 ? byRows<DT, 64>(p, act, backward) : tc == 32 ? byRows<DT, 32>(p, act, backward)
+                                                                  : byRows<DT, 8>(p, act, backward);
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -426,8 +451,10 @@ int groupNormParams(const char* name, int nDtype, int nBatch, int nPixels, int n
         return fail("%s: %d channels do not form %d groups", name, nChannels, nGroups);
     if (nBatch == 0 || nPixels == 0 || nChannels == 0) return 1;
     if (nBatch > 65535) return fail("%s: more than 65535 images", name);
+    if (nChannels > (1 << 18)) return fail("%s: more than 2^18 channels", name);
     if ((long long)nBatch * nGroups > 0x3fffffffLL) return fail("%s: too many (image, group) pairs", name);
     p.N = nBatch; p.P = nPixels; p.C = nChannels; p.G = nGroups; p.per = nChannels / nGroups;
+    p.byPer = FastDiv::make((uint32_t)p.per);
     // channels a workgroup takes: 512 (1 KB of a row of halves), less where the row has less
     const int vecs = (int)((nChannels + 7LL) / 8);
     tc = vecs > 32 ? 64 : vecs > 8 ? 32 : 8;
@@ -435,7 +462,7 @@ int groupNormParams(const char* name, int nDtype, int nBatch, int nPixels, int n
     // chunks of pixels: eight workgroups a CU, and four rows a thread at least
     const int most = (int)((nPixels + 4LL * (256 / tc) - 1) / (4 * (256 / tc)));
     int chunks = (int)std::clamp<long long>((8LL * cuCount() + (long long)tiles * nBatch - 1) / ((long long)tiles * nBatch), 1,
-                                            std::min(most, 65535));
+                                            std::min(most, 4096));   // chunks x channels stay below 2^31
     p.rowsPerChunk = (nPixels + chunks - 1) / chunks;
     p.chunks = (nPixels + p.rowsPerChunk - 1) / p.rowsPerChunk;
     const size_t groups = (size_t)nBatch * nGroups;

@@ -25,30 +25,59 @@ struct Vec8 {
         if constexpr (DT == 1) return __builtin_bit_cast(uint16_t, (__bf16)v);
         if constexpr (DT == 2) return v;
     }
-    // n: values of the group (1 .. 8); the others read as 0 and are not written
+    typedef uint32_t Word4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
+
+    static __device__ __forceinline__ void loadWhole(const Elem* p, float (&v)[8]) {
+        if constexpr (DT == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const Float4 f = *reinterpret_cast<const Float4*>(p + 4 * k);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * k + i] = f[i];
+            }
+        } else {
+            const Word4 w = *reinterpret_cast<const Word4*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = toFloat((uint16_t)w[i]);
+                v[2 * i + 1] = toFloat((uint16_t)(w[i] >> 16));
+            }
+        }
+    }
+    static __device__ __forceinline__ void storeWhole(Elem* p, const float (&v)[8]) {
+        if constexpr (DT == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                *reinterpret_cast<Float4*>(p + 4 * k) = Float4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+        } else {
+            Word4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)fromFloat(v[2 * i]) | (uint32_t)fromFloat(v[2 * i + 1]) << 16;
+            *reinterpret_cast<Word4*>(p) = w;
+        }
+    }
+    // n: values of the group (1 .. 8); the others read as 0 and are not written. EVEN: rows are whole groups (n is 8),
+    // known when the kernel is compiled: with the choice left to each access the compiler splits the wide ones.
+    template <bool EVEN>
     static __device__ __forceinline__ void load(const void* base, long long at, int n, float (&v)[8]) {
         const Elem* p = static_cast<const Elem*>(base) + at;
-        Elem e[8];
-        if (n == 8) {
-            __builtin_memcpy(e, p, sizeof(e));
+        if (EVEN || n == 8) {
+            loadWhole(p, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : Elem(0);
+            for (int i = 0; i < 8; ++i) v[i] = i < n ? toFloat(p[i]) : 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = toFloat(e[i]);
     }
+    template <bool EVEN>
     static __device__ __forceinline__ void store(void* base, long long at, int n, const float (&v)[8]) {
         Elem* p = static_cast<Elem*>(base) + at;
-        Elem e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = fromFloat(v[i]);
-        if (n == 8) {
-            __builtin_memcpy(p, e, sizeof(e));
+        if (EVEN || n == 8) {
+            storeWhole(p, v);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i < n) p[i] = e[i];
+                if (i < n) p[i] = fromFloat(v[i]);
         }
     }
 };
