@@ -104,18 +104,26 @@ __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
     const long long first = (long long)blockIdx.y * p.rowsPerChunk;
     const int last = (int)min((long long)p.rows, first + p.rowsPerChunk);
     if (n > 0) {
-        for (int r = (int)first + tr; r < last; r += TR) {
-            const long long at = (long long)r * p.cols + c;
-            float x[8];
-            Vec8<DT>::template load<EVEN>(p.x, at, n, x);
-            const Bits bits = philox((uint32_t)r * p.perRow.d + cg, p.stream, seed, step);
+        // four rows at a time, so that as many loads are under way
+        auto rows = [&](auto rowsTag, int r) {
+            constexpr int ROWS = decltype(rowsTag)::value;
+            float x[ROWS][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = bits.keep(i, p.threshold) ? x[i] * p.scale : 0.f;
-                sum[i] += x[i];
+            for (int k = 0; k < ROWS; ++k) Vec8<DT>::template load<EVEN>(p.x, (long long)(r + k * TR) * p.cols + c, n, x[k]);
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                const Bits bits = philox((uint32_t)(r + k * TR) * p.perRow.d + cg, p.stream, seed, step);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[k][i] = bits.keep(i, p.threshold) ? x[k][i] * p.scale : 0.f;
+                    sum[i] += x[k][i];
+                }
+                Vec8<DT>::template store<EVEN>(p.out, (long long)(r + k * TR) * p.cols + c, n, x[k]);
             }
-            Vec8<DT>::template store<EVEN>(p.out, at, n, x);
-        }
+        };
+        int r = (int)first + tr;
+        for (; r < last - 3 * TR; r += 4 * TR) rows(std::integral_constant<int, 4>{}, r);
+        for (; r < last; r += TR) rows(std::integral_constant<int, 1>{}, r);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[tr][tc * 8 + i] = sum[i];
