@@ -48,10 +48,44 @@ struct AttnTrainParams {
     uint16_t *dq, *dk, *dv;
     float* stats;                   // [B, H, SqP / 32]: shift of 32 rows, then their delta
     int SqP;                        // Sq rounded up to whole tiles
-    int parts;                      // dK, dV: workgroups that share a block of keys
-    float *dkPart, *dvPart;         // parts > 1: [B, Hkv, parts, blocks * kBlockQ, D]
+    // workgroups that share a block's walk, and their fp32 results where there are several
+    int keyParts;                   // forward, dQ: of a block of queries
+    float *rowPart, *lsePart;       // [B, Sq, H, keyParts, D] contexts or dQ, [B, H, Sq, keyParts] log-sum-exps
+    int parts;                      // dK, dV: of a block of keys
+    float *dkPart, *dvPart;         // [B, Hkv, parts, blocks * kBlockQ, D]
     uint32_t heads, blocks;         // grid: heads x blocks workgroups
 };
+
+// Stores a column of a transposed result: rows 32 dt + 8 (r / 4) + 4 h + r % 4 are the head dimension.
+template <bool BF16, int KD>
+__device__ __forceinline__ void storeColumn(uint16_t* row, const at_f32x16 (&acc)[KD], float f, int h, int D, bool zero) {
+#pragma unroll
+    for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * dt + 2 * r + 4 * h;
+            if (d < D)
+                *reinterpret_cast<at_u32x2*>(row + d) =
+                    zero ? at_u32x2{0u, 0u}
+                         : at_u32x2{atPack2<BF16>(acc[dt][r] * f, acc[dt][r + 1] * f),
+                                    atPack2<BF16>(acc[dt][r + 2] * f, acc[dt][r + 3] * f)};
+        }
+}
+
+template <int KD>
+__device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc)[KD], float f, int h, int D,
+                                               bool zero) {
+#pragma unroll
+    for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * dt + 2 * r + 4 * h;
+            if (d < D)
+                *reinterpret_cast<at_f32x4*>(row + d) =
+                    zero ? at_f32x4{0.f, 0.f, 0.f, 0.f}
+                         : at_f32x4{acc[dt][r] * f, acc[dt][r + 1] * f, acc[dt][r + 2] * f, acc[dt][r + 3] * f};
+        }
+}
 
 // ---------------------------------------------------------------- forward
 // A workgroup holds 128 queries of a head, 32 a wave, and walks the keys 64 at
@@ -75,8 +109,9 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, qb;
-    atPlace(blockIdx.x, p.heads, p.blocks, p.causal, bh, qb);
-    qb = p.blocks - 1 - qb;   // causal: the longest walks first
+    atPlace(blockIdx.x, p.heads, p.blocks * p.keyParts, p.causal, bh, qb);
+    const int part = (int)(qb % (uint32_t)p.keyParts);
+    qb = p.blocks - 1 - qb / (uint32_t)p.keyParts;   // causal: the longest walks first
     const int b = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);
     const int kvHead = head / (p.H / p.Hkv);
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
@@ -92,7 +127,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
     int waveEnd = q0 < nQ ? kEnd : 0;
     if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
-    const int nt = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
+    const int tiles = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
+    const int tBegin = (int)((long long)tiles * part / p.keyParts), nt = (int)((long long)tiles * (part + 1) / p.keyParts);
 
     const float c = fmaxf(fabsf(p.scale) * kAtLog2e, FLT_MIN);
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
@@ -199,8 +235,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
         if (t + 1 < nt) fetch(t + 1, kNext, vNext);
         if (t * kTileKeys < waveEnd) tile(t, kd, vd);
     };
-    if (nt > 0) fetch(0, k0, v0);
-    int t = 0;
+    if (nt > tBegin) fetch(tBegin, k0, v0);
+    int t = tBegin;
     for (; t + 1 < nt; t += 2) {
         trip(t, k0, v0, k1, v1);
         trip(t + 1, k1, v1, k0, v0);
@@ -211,19 +247,48 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     sum = atSumHalves(sum);
     const bool empty = !(query < nQ) || sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
-    if (h == 0)
-        p.lse[((long long)b * p.H + head) * p.Sq + query] = empty ? -INFINITY : m * (c * kAtLn2) + (__logf(sum) - kShift * kAtLn2);
-    uint16_t* row = p.out + (((long long)b * p.Sq + query) * p.H + head) * p.D;
+    const float lse = empty ? -INFINITY : m * (c * kAtLn2) + (__logf(sum) - kShift * kAtLn2);
+    const long long row = ((long long)b * p.Sq + query) * p.H + head;
+    const long long stat = ((long long)b * p.H + head) * p.Sq + query;
+    if (p.keyParts > 1) {
+        if (h == 0) p.lsePart[stat * p.keyParts + part] = lse;
+        storeColumnF32<KD>(p.rowPart + (row * p.keyParts + part) * p.D, o, inv, h, p.D, empty);
+    } else {
+        if (h == 0) p.lse[stat] = lse;
+        storeColumn<BF16, KD>(p.out + row * p.D, o, inv, h, p.D, empty);
+    }
+}
+
+// The parts' contexts, each the mean of its keys: out = sum_i exp(lse_i - lse) out_i, eight values of a row a thread.
+template <bool BF16>
+__global__ __launch_bounds__(256) void attn_train_join_kernel(AttnTrainParams p) {
+    const int chunks = p.D / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;   // (b, q, head, chunk)
+    if (i >= (long long)p.B * p.Sq * p.H * chunks) return;
+    const int c = (int)(i % chunks);
+    const long long row = i / chunks;
+    const int head = (int)(row % p.H);
+    const long long bq = row / p.H;
+    const int q = (int)(bq % p.Sq), b = (int)(bq / p.Sq);
+    const long long stat = ((long long)b * p.H + head) * p.Sq + q;
+    const float* lse = p.lsePart + stat * p.keyParts;
+    const float* from = p.rowPart + row * p.keyParts * p.D + c * 8;
+    float top = -INFINITY;
+    for (int k = 0; k < p.keyParts; ++k) top = fmaxf(top, lse[k]);
+    const bool empty = top == -INFINITY;
+    float total = 0.f;
+    at_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int k = 0; k < p.keyParts; ++k) {
+        const float w = __expf(lse[k] - (empty ? 0.f : top));
+        total += w;
 #pragma unroll
-    for (int dt = 0; dt < KD; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * dt + 2 * r + 4 * h;
-            const float v[4] = {o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
-            if (d < p.D)
-                *reinterpret_cast<at_u32x2*>(row + d) =
-                    empty ? at_u32x2{0u, 0u} : at_u32x2{atPack2<BF16>(v[0], v[1]), atPack2<BF16>(v[2], v[3])};
-        }
+        for (int e = 0; e < 2; ++e) s[e] += w * *reinterpret_cast<const at_f32x4*>(from + (long long)k * p.D + 4 * e);
+    }
+    const float inv = empty ? 0.f : 1.f / total;
+    if (c == 0) p.lse[stat] = empty ? -INFINITY : top + __logf(total);
+    *reinterpret_cast<at_u32x4*>(p.out + row * p.D + c * 8) =
+        at_u32x4{atPack2<BF16>(s[0][0] * inv, s[0][1] * inv), atPack2<BF16>(s[0][2] * inv, s[0][3] * inv),
+                 atPack2<BF16>(s[1][0] * inv, s[1][1] * inv), atPack2<BF16>(s[1][2] * inv, s[1][3] * inv)};
 }
 
 // ---------------------------------------------------------------- backward
@@ -260,35 +325,6 @@ struct DsScale {
     __device__ __forceinline__ float undo() const { return f == 0.f ? 1.f : 1.f / f; }
 };
 
-// Stores a column of a transposed result: rows 32 dt + 8 (r / 4) + 4 h + r % 4 are the head dimension.
-template <bool BF16, int KD>
-__device__ __forceinline__ void storeColumn(uint16_t* row, const at_f32x16 (&acc)[KD], float f, int h, int D, bool zero) {
-#pragma unroll
-    for (int dt = 0; dt < KD; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * dt + 2 * r + 4 * h;
-            if (d < D)
-                *reinterpret_cast<at_u32x2*>(row + d) =
-                    zero ? at_u32x2{0u, 0u}
-                         : at_u32x2{atPack2<BF16>(acc[dt][r] * f, acc[dt][r + 1] * f),
-                                    atPack2<BF16>(acc[dt][r + 2] * f, acc[dt][r + 3] * f)};
-        }
-}
-
-template <int KD>
-__device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc)[KD], float f, int h, int D) {
-#pragma unroll
-    for (int dt = 0; dt < KD; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * dt + 2 * r + 4 * h;
-            if (d < D)
-                *reinterpret_cast<at_f32x4*>(row + d) =
-                    at_f32x4{acc[dt][r] * f, acc[dt][r + 1] * f, acc[dt][r + 2] * f, acc[dt][r + 3] * f};
-        }
-}
-
 // ---------------------------------------------------------------- backward: dQ
 // As the forward pass, a wave holds 32 queries as columns and the workgroup walks the keys: S^T = K Q^T,
 // dP^T = V dO^T, dQ^T += K^T dS^T. It also makes and leaves the rows' statistics, shift = -lse log2 e and delta =
@@ -304,8 +340,9 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, qb;
-    atPlace(blockIdx.x, p.heads, p.blocks, p.causal, bh, qb);
-    qb = p.blocks - 1 - qb;   // causal: the longest walks first
+    atPlace(blockIdx.x, p.heads, p.blocks * p.keyParts, p.causal, bh, qb);
+    const int part = (int)(qb % (uint32_t)p.keyParts);
+    qb = p.blocks - 1 - qb / (uint32_t)p.keyParts;   // causal: the longest walks first
     const int b = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);
     const int kvHead = head / (p.H / p.Hkv);
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
@@ -320,7 +357,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
     if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
     int waveEnd = q0 < nQ ? kEnd : 0;
     if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
-    const int nt = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
+    const int tiles = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
+    const int tBegin = (int)((long long)tiles * part / p.keyParts), nt = (int)((long long)tiles * (part + 1) / p.keyParts);
 
     at_u32x4 qf[T::NS], gf[T::NS];
     {
@@ -353,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
             delta = 0.f;
         else
             shift = -lse * kAtLog2e;
-        if (h == 0 && query < p.SqP) {
+        if (h == 0 && part == 0 && query < p.SqP) {
             float* to = p.stats + 2 * ((long long)bh * p.SqP + q0) + l;
             to[0] = shift + kRaise<BF16>;
             to[32] = delta;
@@ -381,6 +419,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
         const int seen = (p.causal ? min(nK, query + off + 1) : nK) - key0 - 4 * h;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
+            if (EDGE && kb == 1 && key0 + 32 >= waveEnd) break;   // the wave's queries see none of these
             at_f32x16 s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
@@ -426,16 +465,43 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
         if (t + 1 < nt) fetch(t + 1, kNext, vNext);
         step(t, kd, vd);
     };
-    if (nt > 0) fetch(0, k0, v0);
-    int t = 0;
+    if (nt > tBegin) fetch(tBegin, k0, v0);
+    int t = tBegin;
     for (; t + 1 < nt; t += 2) {
         trip(t, k0, v0, k1, v1);
         trip(t + 1, k1, v1, k0, v0);
     }
     if (t < nt) trip(t, k0, v0, k1, v1);
     if (query >= p.Sq) return;
-    uint16_t* row = p.dq + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
-    storeColumn<BF16, KD>(row, dq, p.scale * scale.undo(), h, p.D, shift == -INFINITY);
+    const float f = p.scale * scale.undo();
+    const bool none = shift == -INFINITY;
+    if (p.keyParts > 1)
+        storeColumnF32<KD>(p.rowPart + ((((long long)b * p.Sq + query) * p.H + head) * p.keyParts + part) * p.D, dq, f, h, p.D,
+                           none);
+    else
+        storeColumn<BF16, KD>(p.dq + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D, dq, f, h, p.D,
+                              none);
+}
+
+// The parts' sums of dQ, eight values of a row a thread.
+template <bool BF16>
+__global__ __launch_bounds__(256) void attn_train_dq_join_kernel(AttnTrainParams p) {
+    const int chunks = p.D / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;   // (b, q, head, chunk)
+    if (i >= (long long)p.B * p.Sq * p.H * chunks) return;
+    const int c = (int)(i % chunks);
+    const long long row = i / chunks;
+    const int head = (int)(row % p.H);
+    const long long bq = row / p.H;
+    const int q = (int)(bq % p.Sq), b = (int)(bq / p.Sq);
+    const float* from = p.rowPart + row * p.keyParts * p.D + c * 8;
+    at_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int k = 0; k < p.keyParts; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s[e] += *reinterpret_cast<const at_f32x4*>(from + (long long)k * p.D + 4 * e);
+    *reinterpret_cast<at_u32x4*>(p.dq + (long long)b * p.sq + (long long)q * p.ldq + (long long)head * p.D + c * 8) =
+        at_u32x4{atPack2<BF16>(s[0][0], s[0][1]), atPack2<BF16>(s[0][2], s[0][3]), atPack2<BF16>(s[1][0], s[1][1]),
+                 atPack2<BF16>(s[1][2], s[1][3])};
 }
 
 // ---------------------------------------------------------------- backward: dK and dV
@@ -606,6 +672,16 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
         using L = std::integral_constant<int, SECOND ? 0 : 2>;
         int i = SECOND ? 1 : 0;
         const int last = SECOND ? n : n - 1;
+        if (key0 >= nK) {   // a pair without keys copies and meets the others
+            for (; i + 2 <= last; i += 3) {
+                meet(i, F{});
+                meet(i + 1, S{});
+                meet(i + 2, L{});
+            }
+            if (i <= last) meet(i, F{});
+            if (i + 1 <= last) meet(i + 1, S{});
+            i = last + 1;
+        }
         for (; i + 2 <= last; i += 3) {
             trip(i, F{});
             trip(i + 1, S{});
@@ -618,7 +694,7 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
     const float f = SECOND ? p.scale * kLower * scale.undo() : kLower;
     if (p.parts > 1) {
         const long long row = ((long long)bh * p.parts + part) * ((long long)p.blocks * kBlockQ) + key;
-        storeColumnF32<KD>((SECOND ? p.dkPart : p.dvPart) + row * p.D, acc, f, h, p.D);
+        storeColumnF32<KD>((SECOND ? p.dkPart : p.dvPart) + row * p.D, acc, f, h, p.D, false);
     } else if (key < p.Sk) {
         storeColumn<BF16, KD>((SECOND ? p.dk : p.dv) + place, acc, f, h, p.D, key >= nK);
     }
@@ -675,8 +751,13 @@ template <bool BF16, int KD>
 int launchForward(AttnTrainParams& p) {
     p.heads = (uint32_t)(p.B * p.H);
     p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
-    hipLaunchKernelGGL((attn_train_forward_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL((attn_train_forward_kernel<BF16, KD>), dim3(p.heads * p.blocks * p.keyParts), dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
+    if (p.keyParts > 1) {
+        const long long n = (long long)p.B * p.Sq * p.H * (p.D / 8);
+        hipLaunchKernelGGL((attn_train_join_kernel<BF16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream(), p);
+        OMHIP_CHECK_LAUNCH();
+    }
     return 0;
 }
 
@@ -685,8 +766,13 @@ int launchBackward(AttnTrainParams& p) {
     if (p.Sq > 0) {
         p.heads = (uint32_t)(p.B * p.H);
         p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
-        hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD>), dim3(p.heads * p.blocks), dim3(256), 0, stream(), p);
+        hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD>), dim3(p.heads * p.blocks * p.keyParts), dim3(256), 0, stream(), p);
         OMHIP_CHECK_LAUNCH();
+        if (p.keyParts > 1) {
+            const long long n = (long long)p.B * p.Sq * p.H * (p.D / 8);
+            hipLaunchKernelGGL((attn_train_dq_join_kernel<BF16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream(), p);
+            OMHIP_CHECK_LAUNCH();
+        }
     }
     if (p.Sk > 0) {
         p.heads = (uint32_t)(p.B * p.Hkv);
@@ -723,11 +809,11 @@ int backward(AttnTrainParams& p) {
     }
 }
 
-// Workgroups that share a block of keys' walk of `tiles` query tiles: as many as give every CU four workgroups (a causal
-// mask makes walks of all lengths, which four even out), of four tiles at least.
-int dkvParts(long long keyBlocks, int tiles) {
-    if (keyBlocks == 0 || tiles == 0) return 1;
-    return (int)std::clamp<long long>((4LL * cuCount() + keyBlocks - 1) / keyBlocks, 1, std::max(1, tiles / 4));
+// Workgroups that share a block's walk of `tiles` 64-row tiles: as many as give every CU `perCu` workgroups, of four
+// tiles at least. The dK / dV walk asks for four, forward and dQ for two: their parts cost more (a row's result each).
+int walkParts(long long blocks, int tiles, int perCu) {
+    if (blocks == 0 || tiles == 0) return 1;
+    return (int)std::clamp<long long>(((long long)perCu * cuCount() + blocks - 1) / blocks, 1, std::max(1, tiles / 4));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -783,6 +869,13 @@ int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_
     p.causal = bCausal != 0;
     p.scale = fScale;
     p.out = pOut; p.lse = pLse;
+    p.keyParts = walkParts((long long)nBatch * nHeads * ((nSeqQ + kBlockQ - 1) / kBlockQ), (nSeqK + kTileKeys - 1) / kTileKeys, 2);
+    if (p.keyParts > 1) {
+        const size_t rows = (size_t)nBatch * nHeads * nSeqQ * p.keyParts;
+        p.rowPart = static_cast<float*>(workspace(rows * (nHeadDim + 1) * sizeof(float), kWsOperand));
+        if (!p.rowPart) return -1;   // workspace() recorded the cause
+        p.lsePart = p.rowPart + rows * nHeadDim;
+    }
     return nDtype == 1 ? forward<true>(p) : forward<false>(p);
 }
 
@@ -815,13 +908,17 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
     p.SqP = (nSeqQ + kTileKeys - 1) / kTileKeys * kTileKeys;
     const size_t rows = (size_t)nBatch * nHeads * p.SqP;
     const size_t keyBlocks = (size_t)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1) / kBlockQ);
-    p.parts = dkvParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads));
+    p.parts = walkParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads), 4);
+    const long long queryBlocks = (long long)nBatch * nHeads * ((nSeqQ + kBlockQ - 1) / kBlockQ);
+    p.keyParts = walkParts(queryBlocks, (nSeqK + kTileKeys - 1) / kTileKeys, 2);
+    const size_t rowSums = p.keyParts > 1 ? (size_t)nBatch * nHeads * nSeqQ * p.keyParts * nHeadDim : 0;
     const size_t sums = p.parts > 1 ? keyBlocks * p.parts * kBlockQ * nHeadDim : 0;
     if (rows) {
-        p.stats = static_cast<float*>(workspace((rows + sums) * 2 * sizeof(float), kWsOperand));
+        p.stats = static_cast<float*>(workspace(((rows + sums) * 2 + rowSums) * sizeof(float), kWsOperand));
         if (!p.stats) return -1;   // workspace() recorded the cause
         p.dkPart = p.stats + 2 * rows;
         p.dvPart = p.dkPart + sums;
+        p.rowPart = p.dvPart + sums;
     }
     return nDtype == 1 ? backward<true>(p) : backward<false>(p);
 }

@@ -193,6 +193,16 @@ def test_shared_heads_packed_and_padded_rows(hip, H, Hkv):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Sq,Sk,H,Hkv,D", [(1, 4000, 2, 1, 64), (5, 1500, 4, 4, 128), (1500, 5, 3, 1, 64), (700, 700, 4, 1, 96),
+                                           (300, 1030, 2, 2, 40)], ids=str)
+def test_walks_shared_by_workgroups(hip, Sq, Sk, H, Hkv, D, causal):
+    """Few blocks and long walks: parts of a walk without a visible key, and images of other lengths, among them."""
+    run(hip, 3, Sq, Sk, H, Hkv, D, bf16=D > 64, causal=causal, klens=[Sk, 0, Sk // 3], qlens=[Sq, Sq, (Sq + 1) // 2],
+        seed=Sq + D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
 def test_lengths_per_image(hip, causal, bf16):
     """Images without queries or keys, with one, with all, and lengths outside their range."""
