@@ -56,20 +56,30 @@ struct AttnTrainParams {
     uint32_t heads, blocks;         // grid: heads x blocks workgroups
 };
 
-// Stores a column of a transposed result: rows 32 dt + 8 (r / 4) + 4 h + r % 4 are the head dimension.
+// Stores a wave's 32 rows of a transposed result (the lane's column is row l; its registers hold head dimensions 32 dt +
+// 8 (r / 4) + 4 h + r % 4) times f, or zeros, as halves. Rows are turned around in `stage`, 32 rows of the wave's own in
+// LDS, and leave as whole chunks of 16 bytes, 64 / CH rows an instruction: stored from the registers, every instruction
+// would touch 32 rows for 16 bytes each. rows: how many of the 32 exist.
 template <bool BF16, int KD>
-__device__ __forceinline__ void storeColumn(uint16_t* row, const at_f32x16 (&acc)[KD], float f, int h, int D, bool zero) {
+__device__ __forceinline__ void storeRows(uint16_t* to, long long ld, int rows, const at_f32x16 (&acc)[KD], float f, bool zero,
+                                          uint16_t* stage, int lane, int D) {
+    using T = AtTile<KD>;
+    const int l = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int dt = 0; dt < KD; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * dt + 2 * r + 4 * h;
-            if (d < D)
-                *reinterpret_cast<at_u32x2*>(row + d) =
-                    zero ? at_u32x2{0u, 0u}
-                         : at_u32x2{atPack2<BF16>(acc[dt][r] * f, acc[dt][r + 1] * f),
-                                    atPack2<BF16>(acc[dt][r + 2] * f, acc[dt][r + 3] * f)};
-        }
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<at_u32x2*>(stage + l * T::RS + ((4 * dt + r / 4) ^ T::swizzle(l)) * 8 + 4 * h) =
+                zero ? at_u32x2{0u, 0u}
+                     : at_u32x2{atPack2<BF16>(acc[dt][r] * f, acc[dt][r + 1] * f),
+                                atPack2<BF16>(acc[dt][r + 2] * f, acc[dt][r + 3] * f)};
+    __builtin_amdgcn_wave_barrier();   // the wave's own LDS operations complete in order
+#pragma unroll
+    for (int i = 0; i < T::CH / 2; ++i) {
+        const int id = i * 64 + lane, row = id / T::CH, c = id % T::CH;
+        const at_u32x4 v = *reinterpret_cast<const at_u32x4*>(stage + row * T::RS + (c ^ T::swizzle(row)) * 8);
+        if (row < rows && c * 8 < D) *reinterpret_cast<at_u32x4*>(to + (long long)row * ld + c * 8) = v;
+    }
 }
 
 template <int KD>
@@ -243,7 +253,6 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     }
     if (t < nt) trip(t, k0, v0, k1, v1);
 
-    if (query >= p.Sq) return;
     sum = atSumHalves(sum);
     const bool empty = !(query < nQ) || sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
@@ -251,11 +260,14 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     const long long row = ((long long)b * p.Sq + query) * p.H + head;
     const long long stat = ((long long)b * p.H + head) * p.Sq + query;
     if (p.keyParts > 1) {
+        if (query >= p.Sq) return;
         if (h == 0) p.lsePart[stat * p.keyParts + part] = lse;
         storeColumnF32<KD>(p.rowPart + (row * p.keyParts + part) * p.D, o, inv, h, p.D, empty);
     } else {
-        if (h == 0) p.lse[stat] = lse;
-        storeColumn<BF16, KD>(p.out + row * p.D, o, inv, h, p.D, empty);
+        if (h == 0 && query < p.Sq) p.lse[stat] = lse;
+        __syncthreads();   // every wave is done with the tiles
+        storeRows<BF16, KD>(p.out + (((long long)b * p.Sq + q0) * p.H + head) * p.D, (long long)p.H * p.D, p.Sq - q0, o, inv,
+                            empty, (wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RS, lane, p.D);
     }
 }
 
@@ -472,15 +484,17 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
         trip(t + 1, k1, v1, k0, v0);
     }
     if (t < nt) trip(t, k0, v0, k1, v1);
-    if (query >= p.Sq) return;
     const float f = p.scale * scale.undo();
     const bool none = shift == -INFINITY;
-    if (p.keyParts > 1)
-        storeColumnF32<KD>(p.rowPart + ((((long long)b * p.Sq + query) * p.H + head) * p.keyParts + part) * p.D, dq, f, h, p.D,
-                           none);
-    else
-        storeColumn<BF16, KD>(p.dq + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D, dq, f, h, p.D,
-                              none);
+    if (p.keyParts > 1) {
+        if (query < p.Sq)
+            storeColumnF32<KD>(p.rowPart + ((((long long)b * p.Sq + query) * p.H + head) * p.keyParts + part) * p.D, dq, f, h,
+                               p.D, none);
+    } else {
+        __syncthreads();   // every wave is done with the tiles
+        storeRows<BF16, KD>(p.dq + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D, p.ldq, p.Sq - q0, dq, f,
+                            none, (wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RS, lane, p.D);
+    }
 }
 
 // The parts' sums of dQ, eight values of a row a thread.
@@ -695,8 +709,13 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
     if (p.parts > 1) {
         const long long row = ((long long)bh * p.parts + part) * ((long long)p.blocks * kBlockQ) + key;
         storeColumnF32<KD>((SECOND ? p.dkPart : p.dvPart) + row * p.D, acc, f, h, p.D, false);
-    } else if (key < p.Sk) {
-        storeColumn<BF16, KD>((SECOND ? p.dk : p.dv) + place, acc, f, h, p.D, key >= nK);
+    } else {
+        __syncthreads();   // every wave is done with the tiles and the weights
+        constexpr int kStage = 32 * T::RS;
+        uint16_t* stage = reinterpret_cast<uint16_t*>(lds.weights) + (KD <= 2 ? wave : pair) * kStage;
+        if (KD > 2 && SECOND) stage = pair == 0 ? lds.q[0] : pair == 1 ? lds.q[1] : pair == 2 ? lds.q[2] : lds.g[0];
+        const long long first = (long long)b * p.skv + (long long)key0 * p.ldkv + (long long)kvHead * p.D;
+        storeRows<BF16, KD>((SECOND ? p.dk : p.dv) + first, p.ldkv, p.Sk - key0, acc, f, key >= nK, stage, lane, p.D);
     }
 }
 
