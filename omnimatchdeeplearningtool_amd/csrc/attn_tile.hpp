@@ -212,7 +212,19 @@ struct AtTile {
         }
     };
 
-    // ---- memory -> fragment: row `row` of `rows` (row0: its address' start), columns 16 s + 8 h ...
+    // ---- memory -> fragments of a wave's 32 rows, through 32 rows of LDS of its own: whole rows an instruction. Loaded
+    // straight into the fragments' lanes, every instruction would touch 32 rows for 32 bytes each. start() and, once the
+    // wave's copies have landed, take().
+    static __device__ __forceinline__ void start(const uint16_t* row0, int rows, long long ld, int D, uint16_t* stage, int lane) {
+        Copy<32, 1> c;
+        c.init(0, lane, (uint32_t)ld * 2u, D);
+        c.run(row0, rows, (uint32_t)ld * 2u, D, stage, 0);
+    }
+    static __device__ __forceinline__ void take(const Lane& at, const uint16_t* stage, at_u32x4 (&f)[NS]) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) f[s] = at.natural(stage, 0, s);
+    }
+    // The same straight from memory, of row `rowPtr` ...: columns 16 s + 8 h ...
     static __device__ __forceinline__ at_u32x4 direct(const uint16_t* rowPtr, bool valid, int s, int h, int D) {
         const int c = 16 * s + 8 * h;
         return valid && c < D ? *reinterpret_cast<const at_u32x4*>(rowPtr + c) : at_u32x4{0u, 0u, 0u, 0u};

@@ -142,16 +142,6 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
 
     const float c = fmaxf(fabsf(p.scale) * kAtLog2e, FLT_MIN);
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    at_u32x4 qf[T::NS];
-    {
-        const uint16_t* row = p.q + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
-#pragma unroll
-        for (int s = 0; s < T::NS; ++s) {
-            qf[s] = T::direct(row, query < nQ, s, h, p.D);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
-        }
-    }
     const typename T::Lane at(lane);
     typename T::template Copy<kTileKeys, kWaves> copy;
     const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
@@ -161,6 +151,18 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
         copy.run(kBase + at, nK - t * kTileKeys, ld2, p.D, kd, wave);
         copy.run(vBase + at, nK - t * kTileKeys, ld2, p.D, vd, wave);
     };
+
+    // the wave's queries through its part of the second pair of buffers, which tile 1 is copied to after the first barrier
+    uint16_t* stage = (wave < 2 ? k1 : v1) + (wave & 1) * 32 * T::RS;
+    T::start(p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D, nQ - q0, p.ldq, p.D, stage, lane);
+    if (nt > tBegin) fetch(tBegin, k0, v0);
+    __builtin_amdgcn_s_waitcnt(0);
+    at_u32x4 qf[T::NS];
+    T::take(at, stage, qf);
+#pragma unroll
+    for (int s = 0; s < T::NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
 
     at_f32x16 o[KD];
 #pragma unroll
@@ -245,7 +247,6 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
         if (t + 1 < nt) fetch(t + 1, kNext, vNext);
         if (t * kTileKeys < waveEnd) tile(t, kd, vd);
     };
-    if (nt > tBegin) fetch(tBegin, k0, v0);
     int t = tBegin;
     for (; t + 1 < nt; t += 2) {
         trip(t, k0, v0, k1, v1);
@@ -372,43 +373,6 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
     const int tiles = kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0;
     const int tBegin = (int)((long long)tiles * part / p.keyParts), nt = (int)((long long)tiles * (part + 1) / p.keyParts);
 
-    at_u32x4 qf[T::NS], gf[T::NS];
-    {
-        const uint16_t* row = p.q + (long long)b * p.sq + (long long)query * p.ldq + (long long)head * p.D;
-        const uint16_t* grow = p.gradOut + (((long long)b * p.Sq + query) * p.H + head) * p.D;
-#pragma unroll
-        for (int s = 0; s < T::NS; ++s) {
-            qf[s] = T::direct(row, query < nQ, s, h, p.D);
-            gf[s] = T::direct(grow, query < nQ, s, h, p.D);
-        }
-    }
-    float shift = -INFINITY, delta = 0.f;
-    {
-        const uint16_t* orow = p.out + (((long long)b * p.Sq + query) * p.H + head) * p.D;
-#pragma unroll
-        for (int s = 0; s < T::NS; ++s) {
-            const at_u32x4 o = T::direct(orow, query < nQ, s, h, p.D);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float g0, g1, o0, o1;
-                atUnpack2<BF16>(gf[s][e], g0, g1);
-                atUnpack2<BF16>(o[e], o0, o1);
-                delta = __builtin_fmaf(g0, o0, delta);
-                delta = __builtin_fmaf(g1, o1, delta);
-            }
-        }
-        delta = atSumHalves(delta);
-        const float lse = query < nQ ? p.lse[(long long)bh * p.Sq + query] : -INFINITY;
-        if (lse == -INFINITY)
-            delta = 0.f;
-        else
-            shift = -lse * kAtLog2e;
-        if (h == 0 && part == 0 && query < p.SqP) {
-            float* to = p.stats + 2 * ((long long)bh * p.SqP + q0) + l;
-            to[0] = shift + kRaise<BF16>;
-            to[32] = delta;
-        }
-    }
     const float c = p.scale * kAtLog2e;
     const typename T::Lane at(lane);
     typename T::template Copy<kTileKeys, kWaves> copy;
@@ -419,6 +383,76 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
         copy.run(kBase + o, nK - t * kTileKeys, ld2, p.D, kd, wave);
         copy.run(vBase + o, nK - t * kTileKeys, ld2, p.D, vd, wave);
     };
+    // Q and dO of the wave's queries, and delta. Head dimensions up to 64: by whole rows, Q through its part of the second
+    // pair of buffers, which tile 1 is copied to after the first barrier, dO through rows of its own; larger ones straight
+    // into fragments (LDS for dO would leave one workgroup a CU, and the chunks of dO and O for delta spill).
+    constexpr bool kStaged = KD <= 2;
+    __shared__ __attribute__((aligned(256))) uint16_t gStage[kStaged ? kBlockQ * T::RS : 8];
+    __shared__ float rowDelta[kWaves][32];
+    const uint16_t* qRows = p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D;
+    const uint16_t* gRows = p.gradOut + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
+    const uint16_t* oRows = p.out + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
+    const long long ldo = (long long)p.H * p.D;
+    const float lse = query < nQ ? p.lse[(long long)bh * p.Sq + query] : -INFINITY;
+    auto dot = [&](const at_u32x4& x, const at_u32x4& y, float d) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x0, x1, y0, y1;
+            atUnpack2<BF16>(x[e], x0, x1);
+            atUnpack2<BF16>(y[e], y0, y1);
+            d = __builtin_fmaf(x0, y0, d);
+            d = __builtin_fmaf(x1, y1, d);
+        }
+        return d;
+    };
+    at_u32x4 qf[T::NS], gf[T::NS];
+    float delta = 0.f;
+    if constexpr (kStaged) {
+        uint16_t *qStage = (wave < 2 ? k1 : v1) + (wave & 1) * 32 * T::RS, *dStage = gStage + wave * 32 * T::RS;
+        T::start(qRows, nQ - q0, p.ldq, p.D, qStage, lane);
+        T::start(gRows, nQ - q0, ldo, p.D, dStage, lane);
+        if (nt > tBegin) fetch(tBegin, k0, v0);
+        constexpr int N = T::CH / 2;   // instructions of 64 / CH rows, a whole chunk a lane
+        at_u32x4 g[N], o[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = (i * 64 + lane) / T::CH, d = (i * 64 + lane) % T::CH * 8;
+            const bool in = q0 + row < nQ && d < p.D;
+            g[i] = in ? *reinterpret_cast<const at_u32x4*>(gRows + row * ldo + d) : at_u32x4{0u, 0u, 0u, 0u};
+            o[i] = in ? *reinterpret_cast<const at_u32x4*>(oRows + row * ldo + d) : at_u32x4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float d = dot(g[i], o[i], 0.f);
+#pragma unroll
+            for (int s = T::CH / 2; s > 0; s >>= 1) d += __shfl_xor(d, s, 64);
+            if (lane % T::CH == 0) rowDelta[wave][(i * 64 + lane) / T::CH] = d;
+        }
+        __builtin_amdgcn_wave_barrier();   // the wave's own LDS operations complete in order
+        delta = rowDelta[wave][l];
+        __builtin_amdgcn_s_waitcnt(0);
+        T::take(at, qStage, qf);
+        T::take(at, dStage, gf);
+    } else {
+        if (nt > tBegin) fetch(tBegin, k0, v0);
+#pragma unroll
+        for (int s = 0; s < T::NS; ++s) {
+            qf[s] = T::direct(qRows + l * p.ldq, query < nQ, s, h, p.D);
+            gf[s] = T::direct(gRows + l * ldo, query < nQ, s, h, p.D);
+            delta = dot(gf[s], T::direct(oRows + l * ldo, query < nQ, s, h, p.D), delta);
+        }
+        delta = atSumHalves(delta);
+    }
+    float shift = -INFINITY;
+    if (lse == -INFINITY)
+        delta = 0.f;
+    else
+        shift = -lse * kAtLog2e;
+    if (h == 0 && part == 0 && query < p.SqP) {
+        float* to = p.stats + 2 * ((long long)bh * p.SqP + q0) + l;
+        to[0] = shift + kRaise<BF16>;
+        to[32] = delta;
+    }
     at_f32x16 dq[KD];
 #pragma unroll
     for (int t = 0; t < KD; ++t)
@@ -477,7 +511,6 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
         if (t + 1 < nt) fetch(t + 1, kNext, vNext);
         step(t, kd, vd);
     };
-    if (nt > tBegin) fetch(tBegin, k0, v0);
     int t = tBegin;
     for (; t + 1 < nt; t += 2) {
         trip(t, k0, v0, k1, v1);
@@ -563,13 +596,12 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
     const int begin = (int)((long long)total * part / p.parts), n = (int)((long long)total * (part + 1) / p.parts) - begin;
 
     const typename T::Lane at(lane);
-    const long long place = (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
-    at_u32x4 own[T::NS];   // K, or V
-    {
-        const uint16_t* row = (SECOND ? p.v : p.k) + place;
-#pragma unroll
-        for (int s = 0; s < T::NS; ++s) own[s] = T::direct(row, key < nK, s, h, p.D);
-    }
+    // K or V of the wave's keys through LDS that nothing is copied to, and no weights go to, before the first barrier
+    constexpr int kStage = 32 * T::RS;
+    uint16_t* stage = reinterpret_cast<uint16_t*>(lds.weights) + (KD <= 2 ? wave : pair) * kStage;
+    if (KD > 2 && SECOND) stage = pair == 0 ? lds.q[1] : pair == 1 ? lds.q[2] : pair == 2 ? lds.g[1] : lds.g[2];
+    const long long first = (long long)b * p.skv + (long long)key0 * p.ldkv + (long long)kvHead * p.D;
+    T::start((SECOND ? p.v : p.k) + first, nK - key0, p.ldkv, p.D, stage, lane);
     const float c = p.scale * kAtLog2e;
     constexpr int kCopyWaves = T::CH * kTileQ / 64 < 8 ? T::CH * kTileQ / 64 : 8;   // a head dimension of 32 has 2 instructions
     typename T::template Copy<kTileQ, kCopyWaves> copyQ, copyG;
@@ -597,6 +629,11 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     DsScale<BF16, KD> scale;
+
+    if (n > 0) fetch(lds.q[0], lds.g[0], lds.stats[0]);
+    __builtin_amdgcn_s_waitcnt(0);
+    at_u32x4 own[T::NS];   // K, or V
+    T::take(at, stage, own);
 
     // nat: the tile whose product with the wave's own fragments makes S or dP; tr: the one that the sums take
     auto work = [&](int first, const uint16_t* nat, const uint16_t* tr, const float* sd, float* wd) {
@@ -677,7 +714,6 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
         if (++t == t1) t = t0;
     };
     if (n > 0) {
-        fetch(lds.q[0], lds.g[0], lds.stats[0]);
         if constexpr (SECOND) meet(0, std::integral_constant<int, 0>{});
         // whole rounds of the three buffers, then what is left: a way out of the middle of a round would cost every
         // trip copies of the sums
@@ -711,10 +747,6 @@ __device__ __forceinline__ void dkvWalk(const AttnTrainParams& p, const DkvBuffe
         storeColumnF32<KD>((SECOND ? p.dkPart : p.dvPart) + row * p.D, acc, f, h, p.D, false);
     } else {
         __syncthreads();   // every wave is done with the tiles and the weights
-        constexpr int kStage = 32 * T::RS;
-        uint16_t* stage = reinterpret_cast<uint16_t*>(lds.weights) + (KD <= 2 ? wave : pair) * kStage;
-        if (KD > 2 && SECOND) stage = pair == 0 ? lds.q[0] : pair == 1 ? lds.q[1] : pair == 2 ? lds.q[2] : lds.g[0];
-        const long long first = (long long)b * p.skv + (long long)key0 * p.ldkv + (long long)kvHead * p.D;
         storeRows<BF16, KD>((SECOND ? p.dk : p.dv) + first, p.ldkv, p.Sk - key0, acc, f, key >= nK, stage, lane, p.D);
     }
 }
