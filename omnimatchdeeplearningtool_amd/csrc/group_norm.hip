@@ -44,6 +44,8 @@ struct GroupNormParams {
     int N, P, C, G, per;            // per: channels of a group
     FastDiv byPer;
     int chunks, rowsPerChunk;
+    int width;                      // channels of a workgroup: 8 TC, or as many whole groups as those hold (small)
+    int small;                      // an image's rows and whole groups in a workgroup
     float eps;
 };
 
@@ -72,8 +74,8 @@ struct Place {
     int c, n, tr, first, rows, image, chunk;
     long long base;   // element of the image's first row
     __device__ __forceinline__ explicit Place(const GroupNormParams& p) {
-        c = ((int)blockIdx.x * TC + (int)threadIdx.x % TC) * 8;
-        n = min(8, p.C - c);
+        c = (int)blockIdx.x * p.width + (int)threadIdx.x % TC * 8;
+        n = min(8, min(p.C, ((int)blockIdx.x + 1) * p.width) - c);
         tr = threadIdx.x / TC;
         chunk = blockIdx.y;
         image = blockIdx.z;
@@ -99,9 +101,9 @@ __device__ __forceinline__ void forRows(const W& w, F&& f) {
 template <bool EVEN>
 struct Channels {
     float mean[8], inv[8], gamma[8], beta[8];
-    __device__ __forceinline__ void load(const GroupNormParams& p, int image, int c, int n) {
+    // m, v: the image's groups' means and inverse deviations
+    __device__ __forceinline__ void load(const GroupNormParams& p, int c, int n, const float* m, const float* v) {
         const int g0 = c / p.per, g1 = (c + n - 1) / p.per;   // the first and the last channel's group
-        const float *m = p.mean + (long long)image * p.G, *v = p.inv + (long long)image * p.G;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             gamma[i] = 1.f;
@@ -147,11 +149,11 @@ __device__ __forceinline__ float gradient(float dy, float z, float y) {
 }
 
 // ---------------------------------------------------------------- forward
+// (mean, sum of squared differences) of the workgroup's channels over its chunk of rows: part[i][tc] for channel i of
+// column group tc (its first TC entries, once the workgroup has met).
 template <int DT, int TC, bool EVEN>
-__global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams p) {
+__device__ __forceinline__ void chunkMoments(const GroupNormParams& p, const Place<TC>& w, float2 (&part)[8][256]) {
     using W = Place<TC>;
-    __shared__ float2 part[8][256];
-    const W w(p);
     float shift[8], s[8], q[8];
     float count = 0.f;
 #pragma unroll
@@ -194,12 +196,24 @@ __global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams
             }
         }
     }
+}
+
+template <int TC>
+__device__ __forceinline__ void leavePart(const GroupNormParams& p, const Place<TC>& w, const float2 (&part)[8][256]) {
     if (w.tr == 0 && w.n > 0) {
         float2* to = p.partial + ((long long)w.image * p.chunks + w.chunk) * p.C + w.c;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < w.n) to[i] = part[i][threadIdx.x];
     }
+}
+
+template <int DT, int TC, bool EVEN>
+__global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams p) {
+    __shared__ float2 part[8][256];
+    const Place<TC> w(p);
+    chunkMoments<DT, TC, EVEN>(p, w, part);
+    leavePart(p, w, part);
 }
 
 // One wave per (image, group).
@@ -223,13 +237,10 @@ __global__ __launch_bounds__(64) void group_norm_join_kernel(GroupNormParams p) 
     }
 }
 
+// y of the workgroup's rows
 template <int DT, int TC, int ACT, bool EVEN>
-__global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p) {
+__device__ __forceinline__ void applyRows(const GroupNormParams& p, const Place<TC>& w, Channels<EVEN>& ch) {
     using W = Place<TC>;
-    const W w(p);
-    if (w.n <= 0) return;
-    Channels<EVEN> ch;
-    ch.load(p, w.image, w.c, w.n);
 #pragma unroll
     for (int i = 0; i < 8; ++i) ch.inv[i] *= ch.gamma[i];
     forRows<W>(w, [&](auto rowsTag, int r) {
@@ -245,6 +256,49 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p
             Vec8<DT>::template store<EVEN>(p.out, w.at(p, r + k * W::TR), w.n, x[k]);
         }
     });
+}
+
+template <int DT, int TC, int ACT, bool EVEN>
+__global__ __launch_bounds__(256) void group_norm_apply_kernel(GroupNormParams p) {
+    const Place<TC> w(p);
+    if (w.n <= 0) return;
+    Channels<EVEN> ch;
+    ch.load(p, w.c, w.n, p.mean + (long long)w.image * p.G, p.inv + (long long)w.image * p.G);
+    applyRows<DT, TC, ACT, EVEN>(p, w, ch);
+}
+
+// An image of few pixels in one launch: a workgroup has all rows of its channels, and its channels are whole groups.
+// Per-group values by the group's number within the workgroup; p.mean and p.inv receive them too.
+template <int DT, int TC, int ACT, bool EVEN>
+__global__ __launch_bounds__(256) void group_norm_small_kernel(GroupNormParams p) {
+    __shared__ float2 part[8][256];
+    __shared__ float mean[TC * 8], inv[TC * 8];
+    const Place<TC> w(p);
+    chunkMoments<DT, TC, EVEN>(p, w, part);
+    __syncthreads();
+    const int c0 = (int)blockIdx.x * p.width, g0 = c0 / p.per, groups = min(p.C - c0, p.width) / p.per;
+    const int lane = threadIdx.x & 63;
+    for (int g = (int)threadIdx.x >> 6; g < groups; g += 4) {   // a wave a group
+        Moments t{0.f, 0.f, 0.f};
+        for (int k = lane; k < p.per; k += 64) {
+            const int c = g * p.per + k;
+            const float2 v = part[c & 7][c >> 3];
+            t = join(t, {(float)p.P, v.x, v.y});
+        }
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1)
+            t = join(t, {__shfl_down(t.n, s, 64), __shfl_down(t.mean, s, 64), __shfl_down(t.m2, s, 64)});
+        if (lane == 0) {
+            const float v = 1.f / sqrtf(t.m2 / t.n + p.eps);
+            mean[g] = p.mean[(long long)w.image * p.G + g0 + g] = t.mean;
+            inv[g] = p.inv[(long long)w.image * p.G + g0 + g] = v;
+        }
+    }
+    __syncthreads();
+    if (w.n <= 0) return;
+    Channels<EVEN> ch;
+    ch.load(p, w.c, w.n, mean - g0, inv - g0);
+    applyRows<DT, TC, ACT, EVEN>(p, w, ch);
 }
 
 // ---------------------------------------------------------------- backward
@@ -266,17 +320,16 @@ struct Row {
     }
 };
 
+// (sum of dz, sum of dz xhat) of the workgroup's channels over its chunk of rows, as chunkMoments leaves its values
 template <int DT, int TC, int ACT, bool EVEN>
-__global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p) {
+__device__ __forceinline__ void chunkSums(const GroupNormParams& p, const Place<TC>& w, float2 (&part)[8][256]) {
     using W = Place<TC>;
-    __shared__ float2 part[8][256];
-    const W w(p);
     float a[8], b[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
     if (w.n > 0) {
         Channels<EVEN> ch;
-        ch.load(p, w.image, w.c, w.n);
+        ch.load(p, w.c, w.n, p.mean + (long long)w.image * p.G, p.inv + (long long)w.image * p.G);
         forRows<W>(w, [&](auto rowsTag, int r) {
             constexpr int ROWS = decltype(rowsTag)::value;
             Row<DT, ACT, EVEN> row[ROWS];
@@ -305,22 +358,24 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
                 part[i][threadIdx.x] = {u.x + v.x, u.y + v.y};
             }
     }
-    if (w.tr == 0 && w.n > 0) {
-        float2* to = p.partial + ((long long)w.image * p.chunks + w.chunk) * p.C + w.c;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < w.n) to[i] = part[i][threadIdx.x];
-    }
+}
+
+template <int DT, int TC, int ACT, bool EVEN>
+__global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p) {
+    __shared__ float2 part[8][256];
+    const Place<TC> w(p);
+    chunkSums<DT, TC, ACT, EVEN>(p, w, part);
+    leavePart(p, w, part);
 }
 
 // The first workgroups: the means of gamma dz and gamma dz xhat of 16 groups, a wave each. The others: dgamma and dbeta
 // of 32 channels, 32 interleaved runs over images and chunks a channel (with 8 runs, the loads' latency took 58 us at
 // 32 x 28 x 28 x 512).
-__global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p) {
+__global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p, uint32_t groupBlocks) {
     __shared__ float2 part[1024];
     const int t = threadIdx.x;
     float2 s{0.f, 0.f};
-    const uint32_t groups = (uint32_t)(p.N * p.G), groupBlocks = (groups + 15u) / 16u;
+    const uint32_t groups = (uint32_t)(p.N * p.G);
     if (blockIdx.x < groupBlocks) {
         const uint32_t id = blockIdx.x * 16u + (uint32_t)(t >> 6), lane = (uint32_t)t & 63u;
         if (id >= groups) return;
@@ -365,16 +420,15 @@ __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNor
     }
 }
 
+// dx of the workgroup's rows; means: those of the image's groups
 template <int DT, int TC, int ACT, bool EVEN>
-__global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParams p) {
+__device__ __forceinline__ void gradientRows(const GroupNormParams& p, const Place<TC>& w, const float2* means) {
     using W = Place<TC>;
-    const W w(p);
-    if (w.n <= 0) return;
     Channels<EVEN> ch;
-    ch.load(p, w.image, w.c, w.n);
+    ch.load(p, w.c, w.n, p.mean + (long long)w.image * p.G, p.inv + (long long)w.image * p.G);
     float2 m[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = p.means[(long long)w.image * p.G + (i < w.n ? (w.c + i) / p.per : 0)];
+    for (int i = 0; i < 8; ++i) m[i] = means[(i < w.n ? w.c + i : w.c) / p.per];
     forRows<W>(w, [&](auto rowsTag, int r) {
         constexpr int ROWS = decltype(rowsTag)::value;
         Row<DT, ACT, EVEN> row[ROWS];
@@ -391,10 +445,63 @@ __global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParam
     });
 }
 
+template <int DT, int TC, int ACT, bool EVEN>
+__global__ __launch_bounds__(256) void group_norm_gradient_kernel(GroupNormParams p) {
+    const Place<TC> w(p);
+    if (w.n > 0) gradientRows<DT, TC, ACT, EVEN>(p, w, p.means + (long long)w.image * p.G);
+}
+
+// As group_norm_small_kernel. dgamma and dbeta of one image are its sums; of several, the sums are left for the join.
+template <int DT, int TC, int ACT, bool EVEN>
+__global__ __launch_bounds__(256) void group_norm_small_backward_kernel(GroupNormParams p) {
+    __shared__ float2 part[8][256];
+    __shared__ float2 means[TC * 8];
+    const Place<TC> w(p);
+    chunkSums<DT, TC, ACT, EVEN>(p, w, part);
+    if (p.N > 1) {
+        leavePart(p, w, part);
+    } else if (w.tr == 0 && w.n > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < w.n) {
+                const float2 v = part[i][threadIdx.x];
+                if (p.gradBeta) p.gradBeta[w.c + i] = v.x;
+                if (p.gradGamma) p.gradGamma[w.c + i] = v.y;
+            }
+    }
+    __syncthreads();
+    const int c0 = (int)blockIdx.x * p.width, g0 = c0 / p.per, groups = min(p.C - c0, p.width) / p.per;
+    const int lane = threadIdx.x & 63;
+    for (int g = (int)threadIdx.x >> 6; g < groups; g += 4) {   // a wave a group
+        float2 s{0.f, 0.f};
+        for (int k = lane; k < p.per; k += 64) {
+            const int c = g * p.per + k;
+            const float2 v = part[c & 7][c >> 3];
+            const float gamma = p.gamma ? p.gamma[c0 + c] : 1.f;
+            s.x = __builtin_fmaf(gamma, v.x, s.x);
+            s.y = __builtin_fmaf(gamma, v.y, s.y);
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) {
+            s.x += __shfl_down(s.x, d, 64);
+            s.y += __shfl_down(s.y, d, 64);
+        }
+        const float f = 1.f / ((float)p.P * (float)p.per);
+        if (lane == 0) means[g] = {s.x * f, s.y * f};
+    }
+    __syncthreads();
+    if (w.n > 0) gradientRows<DT, TC, ACT, EVEN>(p, w, means - g0);
+}
+
 // ---------------------------------------------------------------- launches
 template <int DT, int TC, int ACT, bool EVEN>
 int launchForward(const GroupNormParams& p) {
-    const dim3 grid((p.C + 8 * TC - 1) / (8 * TC), p.chunks, p.N);
+    const dim3 grid((p.C + p.width - 1) / p.width, p.chunks, p.N);
+    if (p.small) {
+        hipLaunchKernelGGL((group_norm_small_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
+        OMHIP_CHECK_LAUNCH();
+        return 0;
+    }
     hipLaunchKernelGGL((group_norm_moments_kernel<DT, TC, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     hipLaunchKernelGGL(group_norm_join_kernel, dim3(p.G, p.N), dim3(64), 0, stream(), p);
@@ -406,12 +513,20 @@ int launchForward(const GroupNormParams& p) {
 
 template <int DT, int TC, int ACT, bool EVEN>
 int launchBackward(const GroupNormParams& p) {
-    const dim3 grid((p.C + 8 * TC - 1) / (8 * TC), p.chunks, p.N);
-    hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
+    const dim3 grid((p.C + p.width - 1) / p.width, p.chunks, p.N);
+    const int groupBlocks = p.small ? 0 : (p.N * p.G + 15) / 16;
+    const int channelBlocks = (p.gradGamma || p.gradBeta) && !(p.small && p.N == 1) ? (p.C + 31) / 32 : 0;
+    if (p.small)
+        hipLaunchKernelGGL((group_norm_small_backward_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
+    else
+        hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
-    const int channels = p.gradGamma || p.gradBeta ? (p.C + 31) / 32 : 0;
-    hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3((p.N * p.G + 15) / 16 + channels), dim3(1024), 0, stream(), p);
-    OMHIP_CHECK_LAUNCH();
+    if (groupBlocks + channelBlocks > 0) {
+        hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(groupBlocks + channelBlocks), dim3(1024), 0, stream(), p,
+                           (uint32_t)groupBlocks);
+        OMHIP_CHECK_LAUNCH();
+    }
+    if (p.small) return 0;
     hipLaunchKernelGGL((group_norm_gradient_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     return 0;
@@ -430,7 +545,7 @@ int byAct(const GroupNormParams& p, int act, bool backward) {
 
 template <int DT, int TC>
 int byRows(const GroupNormParams& p, int act, bool backward) {
-    return p.C % 8 == 0 ? byAct<DT, TC, true>(p, act, backward) : byAct<DT, TC, false>(p, act, backward);
+    return p.C % 8 == 0 && p.width % 8 == 0 ? byAct<DT, TC, true>(p, act, backward) : byAct<DT, TC, false>(p, act, backward);
 }
 
 template <int DT>
@@ -464,6 +579,22 @@ int groupNormParams(const char* name, int nDtype, int nBatch, int nPixels, int n
     const int most = (int)((nPixels + 4LL * (256 / tc) - 1) / (4 * (256 / tc)));
     int chunks = (int)std::clamp<long long>((2LL * cuCount() + (long long)tiles * nBatch - 1) / ((long long)tiles * nBatch), 1,
                                             std::min(most, 4096));   // chunks x channels stay below 2^31
+    p.width = 8 * tc;
+    // Images of few pixels take one launch of workgroups that hold whole groups and all rows, where those are short walks
+    // (8 rows a thread, 2 where the workgroups are fewer than the CUs) and not so many that narrow rows cost more than
+    // launches. One launch against three, bf16 SiLU, forward and backward: 64 x 196 x 512 13.3 / 19.9 against 17.7 / 23.0
+    // us, 2 x 64 x 1024 7.4 / 8.9 against 10.8 / 12.4; beyond the rule 8 x 256 x 320 (48 workgroups, 8 rows) 18.6 / 29.1
+    // against 12.0 / 13.9, 64 x 49 x 2048 (2048 workgroups) 17.9 / 24.8 against 17.6 / 21.9.
+    const int smallTc = p.per <= 64 ? 8 : p.per <= 256 ? 32 : 64;
+    const int wholeGroups = std::max(1, 8 * smallTc / p.per) * p.per;
+    const long long smallBlocks = (long long)nBatch * ((nChannels + wholeGroups - 1) / wholeGroups);
+    const int mostRows = (smallBlocks < cuCount() ? 2 : 8) * (256 / smallTc);
+    p.small = p.per <= 512 && nPixels <= mostRows && smallBlocks <= 4LL * cuCount();
+    if (p.small) {
+        tc = smallTc;
+        chunks = 1;
+        p.width = wholeGroups;
+    }
     p.rowsPerChunk = (nPixels + chunks - 1) / chunks;
     p.chunks = (nPixels + p.rowsPerChunk - 1) / p.rowsPerChunk;
     const size_t groups = (size_t)nBatch * nGroups;
