@@ -108,6 +108,12 @@ __device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc
 //  * shift: fp16 keeps 2^-14 .. 2^16 at full precision, so its p is raised by
 //    2^6 (at most 2^14); bf16 needs none.
 //  * the next tile's K and V land in the other pair of buffers meanwhile.
+// 32 x 32 x 16 MFMAs with 32 queries a wave: an LDS fragment feeds 32 columns, half of what 16 x 16 tiles would read.
+// Measured: 2 images x 4096 tokens, 16 query heads on 4 of 128, causal, bf16: 140 us (0.98 PFLOP/s of the visible pairs;
+// a large library product reaches 1.27 here), matrix cores busy 56 % of CU cycles at 1.96 GHz, no bank conflicts: bound by
+// the two waves of a SIMD that share its issue between MFMAs (1024 cycles a tile) and exponentials (1050). ViT-B/16 b64
+// (197 tokens, 768 heads of 64, fp16): 21.7 us, 3.6 TB/s over its compulsory bytes; four tiles a walk, so its start
+// and end (copies in, results out) are half of it.
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainParams p) {
     using T = AtTile<KD>;
@@ -343,6 +349,9 @@ struct DsScale {
 // dP^T = V dO^T, dQ^T += K^T dS^T. It also makes and leaves the rows' statistics, shift = -lse log2 e and delta =
 // sum_d dO O, for the dK / dV kernel that follows; rows that pass no gradient (past the query length, past Sq, or
 // without a key) get shift = -inf, which makes their probabilities 0.
+// dQ and dK / dV are two kernels that each compute S and dP, 7 products where one pass would need 5: sums of a row's dQ
+// over workgroups would have to be added atomically, in an order that changes, or written whole for every block of keys.
+// Measured (sizes as for the forward pass): 212 us (0.97 PFLOP/s), matrix cores busy 53 %; ViT-B/16 b64 36 us.
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p) {
     using T = AtTile<KD>;
@@ -557,9 +566,9 @@ __global__ __launch_bounds__(256) void attn_train_dq_join_kernel(AttnTrainParams
 //  * the first computes S = Q K^T, P and dV^T += dO^T P, and leaves P (fp32, in its registers' order) in LDS;
 //  * the second, one tile behind, computes dP = dO V^T, dS from that P, and dK^T += Q^T dS.
 // One wave doing both needs 128 + 64 registers for its sums and K, V fragments at a head dimension of 128, so only one
-// fits a SIMD and every LDS read and exponential of it is waited out: 465 us at 2 x 4096 x 16 heads on 4 of 128,
-// causal, against (measured below) two waves that fill each other's gaps. Q and dO tiles are in three buffers: the
-// next one's copy, the first waves' and the second waves'.
+// fits a SIMD and every LDS read and exponential of it is waited out: 465-489 us at 2 x 4096 x 16 heads on 4 of 128,
+// causal, against 296-319 us (0.93 PFLOP/s, matrix cores busy 48 %) for two waves that fill each other's gaps. ViT-B/16
+// b64: 40 us. Q and dO tiles are in three buffers: the next one's copy, the first waves' and the second waves'.
 // Where the blocks of keys are few for the card, `parts` workgroups take a share of a block's walk each and leave fp32
 // sums, which attn_train_dkv_join_kernel adds in order.
 constexpr int kTileQ = 32;
@@ -861,7 +870,9 @@ int backward(AttnTrainParams& p) {
 }
 
 // Workgroups that share a block's walk of `tiles` 64-row tiles: as many as give every CU `perCu` workgroups, of four
-// tiles at least. The dK / dV walk asks for four, forward and dQ for two: their parts cost more (a row's result each).
+// tiles at least. Two of them, the long walk of one block and the short one of another, make a causal grid even; dK / dV
+// of head dimensions up to 64 hold two workgroups a CU at once and ask for four. (Parts cost fp32 sums of every row: 2 x
+// 4096 x 16 heads on 4 of 128 backward 499 us with two a CU, 516 with four, about 730 unshared.)
 int walkParts(long long blocks, int tiles, int perCu) {
     if (blocks == 0 || tiles == 0) return 1;
     return (int)std::clamp<long long>(((long long)perCu * cuCount() + blocks - 1) / blocks, 1, std::max(1, tiles / 4));
@@ -959,7 +970,7 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
     p.SqP = (nSeqQ + kTileKeys - 1) / kTileKeys * kTileKeys;
     const size_t rows = (size_t)nBatch * nHeads * p.SqP;
     const size_t keyBlocks = (size_t)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1) / kBlockQ);
-    p.parts = walkParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads), 4);
+    p.parts = walkParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads), nHeadDim <= 64 ? 4 : 2);
     const long long queryBlocks = (long long)nBatch * nHeads * ((nSeqQ + kBlockQ - 1) / kBlockQ);
     p.keyParts = walkParts(queryBlocks, (nSeqK + kTileKeys - 1) / kTileKeys, 2);
     const size_t rowSums = p.keyParts > 1 ? (size_t)nBatch * nHeads * nSeqQ * p.keyParts * nHeadDim : 0;
