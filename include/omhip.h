@@ -514,7 +514,8 @@ int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_
  * written, zeros past the lengths. P and dS are rounded to nDtype as operands (binary16: scaled
  * by powers of two so that small ones keep their bits), sums are in fp32 in a fixed order:
  * repeated calls agree bit for bit. Row statistics use the library's per-stream workspace.
- * Inputs and gradients must not overlap. */
+ * Inputs and gradients must not overlap, nor two images' gradients: an image stride that the
+ * forward pass takes for inputs shared by images (0) is refused here. */
 int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
                                long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
                                const int* pKeyLens, int bCausal, const uint16_t* pOut, const float* pLse,
@@ -532,7 +533,7 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
  * first) of word j / 2. keep: the 16 bits are at least T = round(65536 fProb); s = 65536 / (65536
  * - T) (0 where T is 65536). pRng: {seed, step}, two 64-bit words on the device, read when the
  * kernel runs, so a captured graph draws anew once they are changed; nStream tells the dropouts
- * of one step apart. fProb within 0 .. 1; at most 2^31 - 1 groups. */
+ * of one step apart. fProb within 0 .. 1; at most 2^31 - 2^16 groups. */
 int omHipDropout(int nDtype, const void* pX, const float* pBias, const void* pResidual, void* pOut, int nRows, int nCols,
                  float fProb, const uint64_t* pRng, int nStream);
 /* NEW: the gradient of omHipDropout with the same fProb, state and nStream: pGradX = keep ?
@@ -551,7 +552,7 @@ int omHipDropoutBackward(int nDtype, const void* pGradOut, void* pGradX, float* 
  * (NULL: 1, 0) fp32. nAct 0 none, 1 ReLU, 2 SiLU (z / (1 + exp(-z))). pMean and pInvStd [nBatch,
  * nGroups] (may be NULL) receive mean and 1 / sqrt(var + fEps) for the backward pass. Statistics
  * hold for means far above the spread; they are added in a fixed order. pY may be pX. nBatch at
- * most 65535, nChannels at most 2^18. */
+ * most 65535, nPixels at most 2^30, nChannels at most 2^18. */
 int omHipGroupNormNhwc(int nDtype, const void* pX, const float* pGamma, const float* pBeta, void* pY, float* pMean,
                        float* pInvStd, int nBatch, int nPixels, int nChannels, int nGroups, float fEps, int nAct);
 /* NEW: the gradients of omHipGroupNormNhwc from pX and its saved pMean and pInvStd: pGradX in

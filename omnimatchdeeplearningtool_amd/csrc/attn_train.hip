@@ -294,17 +294,17 @@ __global__ __launch_bounds__(256) void attn_train_join_kernel(AttnTrainParams p)
     const float* from = p.rowPart + row * p.keyParts * p.D + c * 8;
     float top = -INFINITY;
     for (int k = 0; k < p.keyParts; ++k) top = fmaxf(top, lse[k]);
-    const bool empty = top == -INFINITY;
+    const float from0 = top == -INFINITY ? 0.f : top;
     float total = 0.f;
     at_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int k = 0; k < p.keyParts; ++k) {
-        const float w = __expf(lse[k] - (empty ? 0.f : top));
+        const float w = __expf(lse[k] - from0);
         total += w;
 #pragma unroll
         for (int e = 0; e < 2; ++e) s[e] += w * *reinterpret_cast<const at_f32x4*>(from + (long long)k * p.D + 4 * e);
     }
-    const float inv = empty ? 0.f : 1.f / total;
-    if (c == 0) p.lse[stat] = empty ? -INFINITY : top + __logf(total);
+    const float inv = total == 0.f ? 0.f : 1.f / total;   // 0: no part has a key
+    if (c == 0) p.lse[stat] = total == 0.f ? -INFINITY : from0 + __logf(total);
     *reinterpret_cast<at_u32x4*>(p.out + row * p.D + c * 8) =
         at_u32x4{atPack2<BF16>(s[0][0] * inv, s[0][1] * inv), atPack2<BF16>(s[0][2] * inv, s[0][3] * inv),
                  atPack2<BF16>(s[1][0] * inv, s[1][1] * inv), atPack2<BF16>(s[1][2] * inv, s[1][3] * inv)};
@@ -878,6 +878,14 @@ int walkParts(long long blocks, int tiles, int perCu) {
     return (int)std::clamp<long long>(((long long)perCu * cuCount() + blocks - 1) / blocks, 1, std::max(1, tiles / 4));
 }
 
+// Whether the images' rows of `width` elements lie apart, image after image or token after token (gradients are written
+// there).
+bool imagesApart(int nBatch, int nSeq, long long nLd, long long nStride, long long nWidth) {
+    return nBatch <= 1 || nSeq == 0 || nStride >= (nSeq - 1) * nLd + nWidth ||
+           (nStride >= nWidth && nLd >= (nBatch - 1) * nStride + nWidth);
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // What both directions ask of their sizes; 0, 1 (nothing to do) or -1.
@@ -923,6 +931,8 @@ int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_
     if (!pQ || !pOut || !pLse || (nSeqK > 0 && (!pK || !pV))) return fail("%s: null pointer", name);
     if (!aligned16(pQ) || !aligned16(pK) || !aligned16(pV) || !aligned16(pOut))
         return fail("%s: data must be 16-byte aligned", name);
+    if (!aligned4(pLse) || !aligned4(pQueryLens) || !aligned4(pKeyLens))
+        return fail("%s: a pointer is not aligned to its elements", name);
     AttnTrainParams p{};
     p.q = pQ; p.k = pK; p.v = pV;
     p.ldq = nLdQ; p.sq = nStrideQ; p.ldkv = nLdKV; p.skv = nStrideKV;
@@ -957,6 +967,11 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
     for (const void* x : {(const void*)pQ, (const void*)pK, (const void*)pV, (const void*)pOut, (const void*)pGradOut,
                           (const void*)pGradQ, (const void*)pGradK, (const void*)pGradV})
         if (!aligned16(x)) return fail("%s: data must be 16-byte aligned", name);
+    if (!aligned4(pLse) || !aligned4(pQueryLens) || !aligned4(pKeyLens))
+        return fail("%s: a pointer is not aligned to its elements", name);
+    if (!imagesApart(nBatch, nSeqQ, nLdQ, nStrideQ, (long long)nHeads * nHeadDim) ||
+        !imagesApart(nBatch, nSeqK, nLdKV, nStrideKV, (long long)nKVHeads * nHeadDim))
+        return fail("%s: the images' gradients would overlap at these strides", name);
     AttnTrainParams p{};
     p.q = pQ; p.k = pK; p.v = pV;
     p.ldq = nLdQ; p.sq = nStrideQ; p.ldkv = nLdKV; p.skv = nStrideKV;

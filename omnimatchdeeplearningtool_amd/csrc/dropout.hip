@@ -210,7 +210,8 @@ int dropoutParams(const char* name, int nDtype, int nRows, int nCols, float fPro
     if (!(fProb >= 0.f && fProb <= 1.f)) return fail("%s: probability %g is not within 0 .. 1", name, (double)fProb);
     if (nRows == 0 || nCols == 0) return 1;
     const long long groups = (long long)nRows * ((nCols + 7LL) / 8);
-    if (groups > 0x7fffffffLL) return fail("%s: %d rows of %d columns exceed 2^31 groups of 8", name, nRows, nCols);
+    // row counters run up to four rows a thread past the last one
+    if (groups > 0x7fff0000LL) return fail("%s: %d rows of %d columns exceed 2^31 - 2^16 groups of 8", name, nRows, nCols);
     if (!pRng || (reinterpret_cast<uintptr_t>(pRng) & 7u)) return fail("%s: the generator's state must be 8-byte aligned", name);
     p.rng = static_cast<const uint64_t*>(pRng);
     p.stream = (uint32_t)nStream;

@@ -566,6 +566,7 @@ int groupNormParams(const char* name, int nDtype, int nBatch, int nPixels, int n
         return fail("%s: %d channels do not form %d groups", name, nChannels, nGroups);
     if (nBatch == 0 || nPixels == 0 || nChannels == 0) return 1;
     if (nBatch > 65535) return fail("%s: more than 65535 images", name);
+    if (nPixels > (1 << 30)) return fail("%s: more than 2^30 pixels", name);
     if (nChannels > (1 << 18)) return fail("%s: more than 2^18 channels", name);
     if ((long long)nBatch * nGroups > 0x3fffffffLL) return fail("%s: too many (image, group) pairs", name);
     p.N = nBatch; p.P = nPixels; p.C = nChannels; p.G = nGroups; p.per = nChannels / nGroups;

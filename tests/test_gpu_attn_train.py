@@ -385,6 +385,55 @@ def test_empty_sequences(hip):
     H.attentionBackwardHalf(*[None] * 3, 64, 0, 64, 0, None, None, False, *[None] * 6, 0, 5, 5, 1, 1, 64, 1.0)
 
 
+@pytest.mark.gpu
+def test_tokens_of_all_images_in_turn(hip):
+    """Rows in the order token, image: the image stride is the heads' width, the row stride all images'."""
+    B, S, H, D = 3, 70, 2, 64
+    w = H * D
+    c = Case(hip, B, S, S, H, H, D, seed=17)
+    c.forward()
+    c.backward()
+    turned = [to_dev(hip, np.ascontiguousarray(bits(t, False).transpose(1, 0, 2))) for t in c.store]
+    out, lse = empty_dev(hip, (B, S, H, D), np.uint16), empty_dev(hip, (B, H, S))
+    grads = [empty_dev(hip, (S, B, w), np.uint16) for _ in range(3)]
+    args = [*[t.ptr for t in turned], B * w, w, B * w, w, None, None, False]
+    hip.HIPBackend.attentionTrainForwardHalf(*args, out, lse, *c.dims, c.scale)
+    hip.HIPBackend.attentionBackwardHalf(*args, out, lse, c.dgrad, *grads, *c.dims, c.scale)
+    want = c.results()
+    assert np.array_equal(out.numpy(), want[0]) and np.array_equal(lse.numpy(), want[1])
+    for g, x in zip(grads, want[2:]):
+        assert np.array_equal(g.numpy().transpose(1, 0, 2), x)
+
+
+@pytest.mark.gpu
+def test_keys_shared_by_images(hip):
+    """An image stride of 0: the forward pass reads one set of keys for every image."""
+    c = Case(hip, 3, 20, 90, 2, 2, 64, seed=18)
+    for i in (1, 2):
+        c.store[i][1:] = c.store[i][:1]
+        c.dev[i].upload(bits(c.store[i], False))
+    c.forward()
+    out, lse = empty_dev(hip, (3, 20, 2, 64), np.uint16), empty_dev(hip, (3, 2, 20))
+    args = c.args()
+    args[6] = 0
+    hip.HIPBackend.attentionTrainForwardHalf(*args, out, lse, *c.dims, c.scale)
+    assert np.array_equal(out.numpy(), c.dout.numpy()) and np.array_equal(lse.numpy(), c.dlse.numpy())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sk", [100, 2000])
+def test_nan_reaches_its_rows(hip, Sk):
+    """A NaN query makes its own row NaN, context and log-sum-exp, and no other head's; one workgroup a row's keys or
+    several."""
+    c = Case(hip, 1, 40, Sk, 2, 2, 64, seed=19)
+    c.store[0][0, 7, :64] = np.nan
+    c.dev[0].upload(bits(c.store[0], False))
+    c.forward()
+    out, lse = value(c.dout.numpy(), False), c.dlse.numpy()
+    assert np.isnan(out[0, 7, 0]).all() and np.isnan(lse[0, 0, 7])
+    assert np.isnan(lse).sum() == 1 and np.isnan(out).sum() == 64
+
+
 # ---------------------------------------------------------------- refusals: checked before anything touches a device
 GOOD = dict(dtype=0, ldq=128, sq=1280, ldkv=64, skv=640, batch=1, seq_q=10, seq_k=10, heads=2, kv=1, dim=64, scale=0.125,
             ptr=4096, q=4096)
@@ -404,3 +453,22 @@ def test_refusals(bad):
     for name, middle in (("omHipAttentionTrainForwardHalf", [p, p]), ("omHipAttentionBackwardHalf", [p] * 6)):
         with pytest.raises(om.OmHipError, match=name):
             om.call(name, *front, *middle, *back)
+
+
+@pytest.mark.parametrize("sq,skv", [(0, 640), (1280, 0), (1272, 640), (1280, 56)], ids=str)
+def test_overlapping_gradients_are_refused(sq, skv):
+    """Two images of 10 tokens, 2 heads of 64 on one: rows of 128 and 64 elements."""
+    import omnimatchdeeplearningtool_amd as om
+    args = [0, 4096, 4096, 4096, 128, sq, 64, skv, None, None, 0, *[4096] * 6, 2, 10, 10, 2, 1, 64, 0.125]
+    with pytest.raises(om.OmHipError, match="overlap"):
+        om.call("omHipAttentionBackwardHalf", *args)
+
+
+@pytest.mark.parametrize("place", [8, 9])
+def test_misaligned_lengths_are_refused(place):
+    import omnimatchdeeplearningtool_amd as om
+    args = [0, 4096, 4096, 4096, 128, 1280, 64, 640, None, None, 0]
+    args[place] = 4098
+    for name, n in (("omHipAttentionTrainForwardHalf", 2), ("omHipAttentionBackwardHalf", 6)):
+        with pytest.raises(om.OmHipError, match="aligned"):
+            om.call(name, *args, *[4096] * n, 1, 10, 10, 2, 1, 64, 0.125)

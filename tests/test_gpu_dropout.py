@@ -231,7 +231,7 @@ def test_no_rows(hip):
 
 GOOD = dict(dt=2, x=4096, out=4096, rows=4, cols=8, p=0.5, rng=4096)
 BAD = [dict(dt=3), dict(dt=-1), dict(x=None), dict(out=None), dict(rng=None), dict(rng=4100), dict(rows=-1), dict(cols=-1),
-       dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(x=4098), dict(dt=0, x=4097), dict(rows=2 ** 30, cols=100)]
+       dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(x=4098), dict(dt=0, x=4097), dict(rows=2 ** 30, cols=100), dict(rows=2 ** 31 - 1, cols=1)]
 
 
 @pytest.mark.parametrize("bad", BAD, ids=str)

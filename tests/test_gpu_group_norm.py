@@ -261,7 +261,7 @@ def test_nothing_to_do(hip):
 
 GOOD = dict(dt=2, x=4096, y=4096, st=4096, n=1, p=4, c=8, g=2, eps=1e-5, a=0)
 BAD = [dict(dt=3), dict(dt=-1), dict(x=None), dict(a=3), dict(a=-1), dict(g=0), dict(g=3), dict(n=-1), dict(p=-1), dict(c=-8),
-       dict(n=65536), dict(c=2 ** 18 + 2), dict(x=4098), dict(dt=0, x=4097), dict(st=4098)]
+       dict(n=65536), dict(c=2 ** 18 + 2), dict(p=2 ** 30 + 1), dict(x=4098), dict(dt=0, x=4097), dict(st=4098)]
 
 
 @pytest.mark.parametrize("bad", BAD, ids=str)
