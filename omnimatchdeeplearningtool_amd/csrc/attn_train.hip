@@ -869,13 +869,14 @@ int backward(AttnTrainParams& p) {
     }
 }
 
-// Workgroups that share a block's walk of `tiles` 64-row tiles: as many as give every CU `perCu` workgroups, of four
-// tiles at least. Two of them, the long walk of one block and the short one of another, make a causal grid even; dK / dV
+// Workgroups that share a block's walk of `tiles` 64-row tiles: as many as give every CU `perCu` workgroups and no more
+// (one workgroup past that starts a second round: 1 x 2048 x 5 heads of 128 causal backward 75.3 us, rounded up 89.4), of
+// four tiles at least. Two of them, the long walk of one block and the short one of another, make a causal grid even; dK / dV
 // of head dimensions up to 64 hold two workgroups a CU at once and ask for four. (Parts cost fp32 sums of every row: 2 x
 // 4096 x 16 heads on 4 of 128 backward 499 us with two a CU, 516 with four, about 730 unshared.)
 int walkParts(long long blocks, int tiles, int perCu) {
     if (blocks == 0 || tiles == 0) return 1;
-    return (int)std::clamp<long long>(((long long)perCu * cuCount() + blocks - 1) / blocks, 1, std::max(1, tiles / 4));
+    return (int)std::clamp<long long>((long long)perCu * cuCount() / blocks, 1, std::max(1, tiles / 4));
 }
 
 // Whether the images' rows of `width` elements lie apart, image after image or token after token (gradients are written
