@@ -103,7 +103,7 @@ struct Channels {
     float mean[8], inv[8], gamma[8], beta[8];
     // m, v: the image's groups' means and inverse deviations
     __device__ __forceinline__ void load(const GroupNormParams& p, int c, int n, const float* m, const float* v) {
-        const int g0 = c / p.per, g1 = (c + n - 1) / p.per;   // the first and the last channel's group
+        const int g0 = (int)p.byPer.div((uint32_t)c), g1 = (int)p.byPer.div((uint32_t)(c + n - 1));   // the first and the last channel's group
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             gamma[i] = 1.f;
@@ -120,7 +120,7 @@ struct Channels {
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int g = i < n ? (c + i) / p.per : g0;
+                const int g = i < n ? (int)p.byPer.div((uint32_t)(c + i)) : g0;
                 mean[i] = m[g];
                 inv[i] = v[g];
             }
@@ -428,7 +428,7 @@ __device__ __forceinline__ void gradientRows(const GroupNormParams& p, const Pla
     ch.load(p, w.c, w.n, p.mean + (long long)w.image * p.G, p.inv + (long long)w.image * p.G);
     float2 m[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = means[(i < w.n ? w.c + i : w.c) / p.per];
+    for (int i = 0; i < 8; ++i) m[i] = means[p.byPer.div((uint32_t)(i < w.n ? w.c + i : w.c))];
     forRows<W>(w, [&](auto rowsTag, int r) {
         constexpr int ROWS = decltype(rowsTag)::value;
         Row<DT, ACT, EVEN> row[ROWS];
