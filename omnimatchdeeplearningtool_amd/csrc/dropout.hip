@@ -39,6 +39,7 @@ struct DropoutParams {
     FastDiv perRow;          // groups of 8 columns in a row
     uint32_t groups;
     int rowsPerChunk;
+    bool streaming;          // streaming stores
 };
 
 // Ten rounds of Philox4x32 on counter c with key k.
@@ -86,7 +87,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutParams p) {
     const Bits bits = philox(g, p.stream, p.rng[0], p.rng[1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = bits.keep(i, p.threshold) ? __builtin_fmaf(x[i], p.scale, res[i]) : res[i];
-    Vec8<DT>::template store<EVEN>(p.out, at, n, x);
+    forStores(p.streaming, [&](auto streamTag) {
+        Vec8<DT>::template store<EVEN, decltype(streamTag)::value>(p.out, at, n, x);
+    });
 }
 
 // Backward with the bias gradient: a workgroup takes TC groups of columns and a chunk of rows, 256 / TC rows at a
@@ -105,7 +108,7 @@ __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
     const int last = (int)min((long long)p.rows, first + p.rowsPerChunk);
     if (n > 0) {
         // four rows at a time, so that as many loads are under way
-        auto rows = [&](auto rowsTag, int r) {
+        auto rows = [&](auto rowsTag, auto streamTag, int r) {
             constexpr int ROWS = decltype(rowsTag)::value;
             float x[ROWS][8];
 #pragma unroll
@@ -118,12 +121,15 @@ __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
                     x[k][i] = bits.keep(i, p.threshold) ? x[k][i] * p.scale : 0.f;
                     sum[i] += x[k][i];
                 }
-                Vec8<DT>::template store<EVEN>(p.out, (long long)(r + k * TR) * p.cols + c, n, x[k]);
+                Vec8<DT>::template store<EVEN, decltype(streamTag)::value>(p.out, (long long)(r + k * TR) * p.cols + c, n,
+                                                                           x[k]);
             }
         };
-        int r = (int)first + tr;
-        for (; r < last - 3 * TR; r += 4 * TR) rows(std::integral_constant<int, 4>{}, r);
-        for (; r < last; r += TR) rows(std::integral_constant<int, 1>{}, r);
+        forStores(p.streaming, [&](auto stream) {
+            int r = (int)first + tr;
+            for (; r < last - 3 * TR; r += 4 * TR) rows(std::integral_constant<int, 4>{}, stream, r);
+            for (; r < last; r += TR) rows(std::integral_constant<int, 1>{}, stream, r);
+        });
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[tr][tc * 8 + i] = sum[i];
@@ -221,6 +227,7 @@ int dropoutParams(const char* name, int nDtype, int nRows, int nCols, float fPro
     p.cols = nCols;
     p.perRow = FastDiv::make((uint32_t)((nCols + 7LL) / 8));
     p.groups = (uint32_t)groups;
+    p.streaming = (long long)nRows * nCols * (nDtype == 2 ? 4 : 2) >= kStreamBytes;
     return 0;
 }
 

@@ -44,6 +44,7 @@ struct GroupNormParams {
     int N, P, C, G, per;            // per: channels of a group
     FastDiv byPer;
     int chunks, rowsPerChunk;
+    bool stream;                    // streaming stores
     int width;                      // channels of a workgroup: 8 TC, or as many whole groups as those hold (small)
     int small;                      // an image's rows and whole groups in a workgroup
     float eps;
@@ -243,18 +244,20 @@ __device__ __forceinline__ void applyRows(const GroupNormParams& p, const Place<
     using W = Place<TC>;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ch.inv[i] *= ch.gamma[i];
-    forRows<W>(w, [&](auto rowsTag, int r) {
-        constexpr int ROWS = decltype(rowsTag)::value;
-        float x[ROWS][8];
+    forStores(p.stream, [&](auto streamTag) {
+        forRows<W>(w, [&](auto rowsTag, int r) {
+            constexpr int ROWS = decltype(rowsTag)::value;
+            float x[ROWS][8];
 #pragma unroll
-        for (int k = 0; k < ROWS; ++k) Vec8<DT>::template load<EVEN>(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
+            for (int k = 0; k < ROWS; ++k) Vec8<DT>::template load<EVEN>(p.x, w.at(p, r + k * W::TR), w.n, x[k]);
 #pragma unroll
-        for (int k = 0; k < ROWS; ++k) {
+            for (int k = 0; k < ROWS; ++k) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[k][i] = activate<ACT>(__builtin_fmaf(x[k][i] - ch.mean[i], ch.inv[i], ch.beta[i]));
-            Vec8<DT>::template store<EVEN>(p.out, w.at(p, r + k * W::TR), w.n, x[k]);
-        }
+                for (int i = 0; i < 8; ++i)
+                    x[k][i] = activate<ACT>(__builtin_fmaf(x[k][i] - ch.mean[i], ch.inv[i], ch.beta[i]));
+                Vec8<DT>::template store<EVEN, decltype(streamTag)::value>(p.out, w.at(p, r + k * W::TR), w.n, x[k]);
+            }
+        });
     });
 }
 
@@ -429,19 +432,21 @@ __device__ __forceinline__ void gradientRows(const GroupNormParams& p, const Pla
     float2 m[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) m[i] = means[p.byPer.div((uint32_t)(i < w.n ? w.c + i : w.c))];
-    forRows<W>(w, [&](auto rowsTag, int r) {
-        constexpr int ROWS = decltype(rowsTag)::value;
-        Row<DT, ACT, EVEN> row[ROWS];
+    forStores(p.stream, [&](auto streamTag) {
+        forRows<W>(w, [&](auto rowsTag, int r) {
+            constexpr int ROWS = decltype(rowsTag)::value;
+            Row<DT, ACT, EVEN> row[ROWS];
 #pragma unroll
-        for (int k = 0; k < ROWS; ++k) row[k].load(p, w.at(p, r + k * W::TR), w.n);
+            for (int k = 0; k < ROWS; ++k) row[k].load(p, w.at(p, r + k * W::TR), w.n);
 #pragma unroll
-        for (int k = 0; k < ROWS; ++k) {
-            row[k].work(ch);
+            for (int k = 0; k < ROWS; ++k) {
+                row[k].work(ch);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                row[k].dz[i] = ch.inv[i] * (__builtin_fmaf(row[k].dz[i], ch.gamma[i], -m[i].x) - row[k].xhat[i] * m[i].y);
-            Vec8<DT>::template store<EVEN>(p.out, w.at(p, r + k * W::TR), w.n, row[k].dz);
-        }
+                for (int i = 0; i < 8; ++i)
+                    row[k].dz[i] = ch.inv[i] * (__builtin_fmaf(row[k].dz[i], ch.gamma[i], -m[i].x) - row[k].xhat[i] * m[i].y);
+                Vec8<DT>::template store<EVEN, decltype(streamTag)::value>(p.out, w.at(p, r + k * W::TR), w.n, row[k].dz);
+            }
+        });
     });
 }
 
@@ -581,6 +586,7 @@ int groupNormParams(const char* name, int nDtype, int nBatch, int nPixels, int n
     int chunks = (int)std::clamp<long long>((2LL * cuCount() + (long long)tiles * nBatch - 1) / ((long long)tiles * nBatch), 1,
                                             std::min(most, 4096));   // chunks x channels stay below 2^31
     p.width = 8 * tc;
+    p.stream = (long long)nBatch * nPixels * nChannels * (nDtype == 2 ? 4 : 2) >= kStreamBytes;
     // Images of few pixels take one launch of workgroups that hold whole groups and all rows, where those are short walks
     // (8 rows a thread, 2 where the workgroups are fewer than the CUs) and not so many that narrow rows cost more than
     // launches. One launch against three, bf16 SiLU, forward and backward: 64 x 196 x 512 13.3 / 19.9 against 17.7 / 23.0

@@ -185,6 +185,23 @@ def test_long_batch(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [512, 509], ids=str)
+def test_large_output(hip, cols):
+    """Over 24 MB (streaming stores): every value is kept and doubled or dropped, the mask as on the host, forward and
+    backward."""
+    rows = 13001
+    x = O.randn((rows, cols), 6, 1.0)
+    dx, out, gx, gb = to_dev(hip, x), empty_dev(hip, x.shape), empty_dev(hip, x.shape), empty_dev(hip, (cols,))
+    rng = state(hip, 12, 34)
+    hip.HIPBackend.dropout(dx, None, None, out, rows, cols, 0.5, rng, 2)
+    hip.HIPBackend.dropoutBackward(dx, gx, gb, rows, cols, 0.5, rng, 2)
+    y = out.numpy()
+    assert np.all((y == 0) | (y == 2 * x)) and np.array_equal(gx.numpy(), y)
+    assert np.array_equal(y[:20] != 0, mask(20, cols, 0.5, 12, 34, 2))
+    assert np.all(np.abs(gb.numpy() - y.sum(0, dtype=np.float64)) <= 1.01 * (rows + 2) * U * np.abs(y).sum(0, dtype=np.float64))
+
+
+@pytest.mark.gpu
 def test_replayed_graph_draws_from_the_state(hip, streams):
     """A graph of forward and backward replays with the state of the moment: fresh masks after it changes, the same
     before; eager work of another size runs between the replays."""

@@ -148,6 +148,13 @@ def test_addresses_off_the_vector(hip, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [128, 125], ids=str)
+def test_large_output(hip, C):
+    """Over 24 MB: streaming stores."""
+    run(hip, 2, 26000, C, 1, dt=2, a=2)
+
+
+@pytest.mark.gpu
 def test_mean_far_above_the_spread(hip):
     """A mean of 1000 spreads: sums of squares alone would leave nothing of the variance."""
     run(hip, 2, 3000, 32, 4, dt=2, mean=1000.0, std=1.0)
