@@ -551,8 +551,9 @@ int omHipDropoutBackward(int nDtype, const void* pGradOut, void* pGradX, float* 
  * group. nDtype 0 binary16, 1 bfloat16, 2 fp32 (pX, pY); statistics and pGamma, pBeta [nChannels]
  * (NULL: 1, 0) fp32. nAct 0 none, 1 ReLU, 2 SiLU (z / (1 + exp(-z))). pMean and pInvStd [nBatch,
  * nGroups] (may be NULL) receive mean and 1 / sqrt(var + fEps) for the backward pass. Statistics
- * hold for means far above the spread; they are added in a fixed order. pY may be pX. nBatch at
- * most 65535, nPixels at most 2^30, nChannels at most 2^18. */
+ * hold for means far above the spread, up to the largest fp32; the sum of a group's squared
+ * differences from its mean has to stay within fp32. They are added in a fixed order. pY may be
+ * pX. nBatch at most 65535, nPixels at most 2^30, nChannels at most 2^18. */
 int omHipGroupNormNhwc(int nDtype, const void* pX, const float* pGamma, const float* pBeta, void* pY, float* pMean,
                        float* pInvStd, int nBatch, int nPixels, int nChannels, int nGroups, float fEps, int nAct);
 /* NEW: the gradients of omHipGroupNormNhwc from pX and its saved pMean and pInvStd: pGradX in

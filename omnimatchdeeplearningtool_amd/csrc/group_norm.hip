@@ -52,7 +52,8 @@ struct GroupNormParams {
 
 enum { kActNone = 0, kActRelu = 1, kActSilu = 2 };
 
-// (count, mean, sum of squared differences) of a and b together.
+// (count, mean, sum of squared differences) of a and b together. An empty a (count and mean 0) makes d the whole of b's
+// mean, whose square may pass fp32's range: the count is multiplied in first.
 struct Moments {
     float n, mean, m2;
 };
@@ -60,7 +61,7 @@ __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
     const float n = a.n + b.n;
     if (b.n == 0.f) return a;
     const float d = b.mean - a.mean, f = b.n / n;
-    return {n, __builtin_fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+    return {n, __builtin_fmaf(d, f, a.mean), a.m2 + b.m2 + d * (a.n * f) * d};
 }
 
 // Rows of a chunk.
@@ -180,7 +181,8 @@ __device__ __forceinline__ void chunkMoments(const GroupNormParams& p, const Pla
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float m = count > 0.f ? s[i] / count : 0.f;
-        part[i][threadIdx.x] = {shift[i] + m, fmaxf(__builtin_fmaf(-m, s[i], q[i]), 0.f)};
+        const float m2 = __builtin_fmaf(-m, s[i], q[i]);
+        part[i][threadIdx.x] = {shift[i] + m, m2 < 0.f ? 0.f : m2};   // NaN, of infinite data, stays
     }
     // row threads tr and tr + half together, half = TR / 2 .. 1; thread tr then stands for rows tr, tr + half, ...
 #pragma unroll

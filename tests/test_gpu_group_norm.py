@@ -291,3 +291,93 @@ def test_more_refusals():
         om.call("omHipGroupNormNhwcBackward", 2, 4096, 4096, None, 4096, 4096, None, None, 4096, None, None, 1, 4, 8, 2, 1)
     with pytest.raises(om.OmHipError, match="null"):
         om.call("omHipGroupNormNhwcBackward", 2, 4096, 4096, None, None, 4096, None, None, 4096, None, None, 1, 4, 8, 2, 0)
+
+
+def far_case(hip, size, dt, spread):
+    """A mean of 1e20: its square has no fp32 value."""
+    c = Case(hip, *size, dt=dt, seed=7)
+    c.x = store(np.float32(1e20) + O.randn(c.x.shape, 7, 1.0) * np.float32(spread), dt)
+    c.dx.upload(c.x)
+    c.forward()
+    c.backward()
+    return c
+
+
+FAR = [(3, 20, 64, 8), (1, 20, 60, 4), (2, 300, 12, 4), (1, 400, 64, 1)]   # one launch, one launch of one image, three launches
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [1, 2], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", FAR, ids=str)
+def test_constant_image_far_from_zero(hip, size, dt):
+    """1e20 everywhere: mean is the value itself, inv 1 / sqrt(eps), xhat 0, so y is beta, dgamma 0 and dbeta the sums."""
+    c = far_case(hip, size, dt, 0.0)
+    N, P, C, G = size
+    y, mean, inv, gx, ggamma, gbeta = c.results()
+    assert np.all(mean == value(c.x, dt)[0, 0, 0]) and np.allclose(inv, EPS ** -0.5, rtol=4 * U, atol=0)
+    assert np.array_equal(value(y, dt).reshape(N, P, C), np.broadcast_to(value(store(c.beta, dt), dt), (N, P, C)))
+    g = value(c.g, dt).astype(np.float64)
+    assert np.all(ggamma == 0)
+    assert np.all(np.abs(gbeta - g.sum((0, 1))) <= 1.01 * (N * P + 8) * U * np.abs(g).sum((0, 1)))
+    d = (g * c.gamma).reshape(N, P, G, C // G)
+    avg = lambda t: t.mean((1, 3), keepdims=True)  # noqa: E731
+    want = EPS ** -0.5 * (d - avg(d))
+    lim = EPS ** -0.5 * ((P * C // G + 8) * U * avg(np.abs(d)) + 8 * U * (np.abs(d) + np.abs(avg(d)))) + HALF_STEP[dt] * np.abs(want)
+    assert np.all(np.abs(value(gx, dt).reshape(want.shape) - want) <= 1.01 * lim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [1, 2], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", FAR[:3], ids=str)
+def test_spread_far_from_zero(hip, size, dt):
+    """1e20 +- 3e17. At most 16 joins lie between a value and its group (5 of row threads, one or two of a lane's entries,
+    6 of lanes, chunks): each rounds the mean, u |mean|, on top of the sums' (n + 4) u. A mean that is off by e moves a
+    join's squared difference by 2 e |mb - ma|; over 16 of them, by Cauchy-Schwarz, 2 sqrt(16) e / std of the variance and
+    e^2 / var, half of which is inv's."""
+    c = far_case(hip, size, dt, 3e17)
+    N, P, C, G = size
+    per, n, joins = C // G, P * C // G, 16
+    x = value(c.x, dt).astype(np.float64).reshape(N, P, G, per)
+    y, mean, inv, gx, ggamma, gbeta = c.results()
+    avg = lambda t: t.mean((1, 3), keepdims=True)  # noqa: E731
+    mu = avg(x)
+    sd = np.sqrt(avg((x - mu) ** 2))
+    em = (n + 4) * U * 2 * np.abs(x - mu).max((1, 3), keepdims=True) + (joins + 2) * U * np.abs(mu)
+    mean, inv = (t.astype(np.float64).reshape(N, 1, G, 1) for t in (mean, inv))
+    ev = (n + 8) * U + joins ** 0.5 * em / sd + (em / sd) ** 2
+    assert ev.max() < 2.0 ** -8
+    assert np.all(np.abs(mean - mu) <= em)
+    assert np.all(np.abs(inv * sd - 1) <= ev)
+    gamma, beta = (t.astype(np.float64).reshape(G, per) for t in (c.gamma, c.beta))
+    xhat = (x - mu) / sd
+    want = xhat * gamma + beta
+    lim = np.abs(gamma) * (em / sd + np.abs(xhat) * (ev + 3 * U)) + 3 * U * (np.abs(want) + np.abs(beta)) + HALF_STEP[dt] * np.abs(want)
+    assert np.all(np.abs(value(y, dt).reshape(want.shape) - want) <= 1.01 * lim)
+    # from the saved statistics: x - mean is exact (neighbours of each other) but for a rounding of the result
+    xhat = (x - mean) * inv
+    g = value(c.g, dt).astype(np.float64).reshape(x.shape)
+    d = g * gamma
+    want = inv * (d - avg(d) - xhat * avg(d * xhat))
+    e2 = (n + 10) * U * avg(np.abs(d * xhat))
+    lim = inv * ((n + 8) * U * avg(np.abs(d)) + np.abs(xhat) * e2 + 5 * U * (np.abs(d) + np.abs(avg(d)) + np.abs(xhat * avg(d * xhat))))
+    lim += (HALF_STEP[dt] + 2 * U) * np.abs(want) + 2.0 ** -126   # its size is 1e-18: no subnormals
+    assert np.all(np.abs(value(gx, dt).reshape(want.shape) - want) <= 1.01 * lim)
+    for got, t in ((ggamma, g * xhat), (gbeta, g)):
+        assert np.all(np.abs(got - t.sum((0, 1)).reshape(-1)) <= 1.01 * (N * P + 12) * U * np.abs(t).sum((0, 1)).reshape(-1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(1, 1, 8, 8), (2, 1, 16, 16), (1, 300, 8, 8)], ids=str)
+def test_infinity_is_no_constant(hip, size):
+    """Groups that one thread's rows make up: an infinity leaves no deviation, so inv and the group's values are NaN."""
+    c = Case(hip, *size)
+    N, P, C, G = size
+    c.x[0, P - 1, 3] = np.inf
+    c.x[0, 0, 5] = -np.inf
+    c.dx.upload(c.x)
+    c.forward()
+    y, inv = c.y.numpy().reshape(N, P, C), c.inv.numpy()
+    bad = np.zeros((N, C), bool)
+    bad[0, [3, 5]] = True
+    assert np.array_equal(np.isnan(inv), bad)
+    assert np.array_equal(np.isnan(y), np.broadcast_to(bad[:, None], y.shape))
