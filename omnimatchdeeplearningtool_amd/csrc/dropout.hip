@@ -144,11 +144,12 @@ __global__ __launch_bounds__(256) void dropout_bias_kernel(DropoutParams p) {
 }
 
 // gradBias[c] = the chunks' partial sums: 32 interleaved runs of them a column, then those pairwise. (8 runs took 20 us
-// for 512 chunks of 1024 columns: loads waited out one by one.)
-__global__ __launch_bounds__(1024) void dropout_bias_sum_kernel(const float* partials, float* gradBias, int chunks, int cols) {
+// for 512 chunks of 1024 columns: loads waited out one by one.) Workgroups count through both dimensions of the grid: 2^22
+// of them, 2^27 columns, are 2^32 threads, and a grid keeps 32 bits of its threads in a dimension.
+__global__ __launch_bounds__(1024) void dropout_bias_sum_kernel(const float* partials, float* gradBias, int chunks, uint32_t cols) {
     __shared__ float part[32][33];
     const int tc = threadIdx.x & 31, tr = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + tc;
+    const uint32_t c = (blockIdx.y * gridDim.x + blockIdx.x) * 32u + tc;
     float s = 0.f;
     if (c < cols) {
 #pragma unroll 8
@@ -202,8 +203,9 @@ int backwardWithBias(DropoutParams& p, float* pGradBias) {
                  : tc == 16 ? launchDropoutBias<DT, 16>(p, chunks)
                             : launchDropoutBias<DT, 4>(p, chunks);
     if (rc) return rc;
-    hipLaunchKernelGGL(dropout_bias_sum_kernel, dim3((p.cols + 31) / 32), dim3(1024), 0, stream(), p.partials, pGradBias,
-                       chunks, p.cols);
+    const uint32_t blocks = ((uint32_t)p.cols + 31u) / 32u, width = std::min(blocks, 1u << 16);
+    hipLaunchKernelGGL(dropout_bias_sum_kernel, dim3(width, (blocks + width - 1) / width), dim3(1024), 0, stream(), p.partials,
+                       pGradBias, chunks, (uint32_t)p.cols);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }

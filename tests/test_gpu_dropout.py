@@ -258,3 +258,23 @@ def test_refusals(bad):
     for name, args in (("omHipDropout", (a["x"], None, None, a["out"])), ("omHipDropoutBackward", (a["x"], a["out"], None))):
         with pytest.raises(om.OmHipError, match=name):
             om.call(name, a["dt"], *args, a["rows"], a["cols"], a["p"], a["rng"], 0)
+
+
+@pytest.mark.gpu
+def test_more_columns_than_one_dimension_of_a_grid(hip):
+    """One row of 2^27 + 72 columns: the bias gradient's sums take 32 columns a workgroup of 1024 threads, 2^32 threads and
+    more. Of one row they are the kept values themselves (a factor of 2 is exact)."""
+    cols = 2 ** 27 + 72
+    print(f"case 1x{cols}", flush=True)
+    x = np.resize(O.randn((100003,), 5, 1.0).astype(np.float16), cols)
+    dx, gx, gb = to_dev(hip, x.view(np.uint16)), empty_dev(hip, (cols,), np.uint16), empty_dev(hip, (cols,))
+    hip.HIPBackend.dropoutBackward(dx, gx, gb, 1, cols, 0.5, state(hip, 21, 4), 6, 0)
+    g = gx.numpy().view(np.float16)
+    assert np.all((g == 0) | (g == 2 * x))
+    assert np.array_equal(gb.numpy(), g.astype(np.float32))
+    for first in (0, 2 ** 24, cols // 8 - 9):   # groups of 8 columns
+        for group in range(first, first + 9):
+            words = philox([group, 6, 4, 0], [21, 0])
+            keep = [((words[j // 2] >> (16 * (j % 2))) & 0xFFFF) >= threshold(0.5) for j in range(8)]
+            at = slice(8 * group, 8 * group + 8)
+            assert np.array_equal(g[at], np.where(keep, 2 * x[at], 0).astype(np.float16))
