@@ -375,14 +375,15 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
 
 // The first workgroups: the means of gamma dz and gamma dz xhat of 16 groups, a wave each. The others: dgamma and dbeta
 // of 32 channels, 32 interleaved runs over images and chunks a channel (with 8 runs, the loads' latency took 58 us at
-// 32 x 28 x 28 x 512).
+// 32 x 28 x 28 x 512). Workgroups count through both dimensions of the grid: 2^26 groups are 2^32 threads, and a grid keeps
+// 32 bits of its threads in a dimension. What lies past the last channel finds nothing to do.
 __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p, uint32_t groupBlocks) {
     __shared__ float2 part[1024];
     const int t = threadIdx.x;
     float2 s{0.f, 0.f};
-    const uint32_t groups = (uint32_t)(p.N * p.G);
-    if (blockIdx.x < groupBlocks) {
-        const uint32_t id = blockIdx.x * 16u + (uint32_t)(t >> 6), lane = (uint32_t)t & 63u;
+    const uint32_t groups = (uint32_t)(p.N * p.G), block = blockIdx.y * gridDim.x + blockIdx.x;
+    if (block < groupBlocks) {
+        const uint32_t id = block * 16u + (uint32_t)(t >> 6), lane = (uint32_t)t & 63u;
         if (id >= groups) return;
         const uint32_t image = id / (uint32_t)p.G, g = id - image * (uint32_t)p.G;
         const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNor
         if (lane == 0) p.means[id] = {s.x * f, s.y * f};
         return;
     }
-    const int c = (int)(blockIdx.x - groupBlocks) * 32 + (t & 31);
+    const int c = (int)(block - groupBlocks) * 32 + (t & 31);
     if (c < p.C) {
 #pragma unroll 8
         for (long long e = t >> 5; e < (long long)p.N * p.chunks; e += 32) {
@@ -529,7 +530,8 @@ int launchBackward(const GroupNormParams& p) {
         hipLaunchKernelGGL((group_norm_sums_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     if (groupBlocks + channelBlocks > 0) {
-        hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(groupBlocks + channelBlocks), dim3(1024), 0, stream(), p,
+        const int blocks = groupBlocks + channelBlocks, width = std::min(blocks, 1 << 16);
+        hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(width, (blocks + width - 1) / width), dim3(1024), 0, stream(), p,
                            (uint32_t)groupBlocks);
         OMHIP_CHECK_LAUNCH();
     }

@@ -381,3 +381,40 @@ def test_infinity_is_no_constant(hip, size):
     bad[0, [3, 5]] = True
     assert np.array_equal(np.isnan(inv), bad)
     assert np.array_equal(np.isnan(y), np.broadcast_to(bad[:, None], y.shape))
+
+
+@pytest.mark.gpu
+def test_more_groups_than_one_dimension_of_a_grid(hip):
+    """65535 images of 1025 groups: 2^26 pairs and more, 16 of them a workgroup of 1024 threads in the backward's join.
+    Images repeat after 61, so 61 of them are the reference."""
+    N, P, C, G, dt = 65535, 1, 4100, 1025, 0
+    some, per = 61, C // G
+    print(f"case {N}x{P}x{C}/{G}", flush=True)
+    x, g = (store(O.randn((some, C), k, 1.0), dt) for k in (1, 2))
+    every = np.arange(N) % some
+    dx, dg = to_dev(hip, x[every]), to_dev(hip, g[every])
+    y, gx = empty_dev(hip, (N, C), np.uint16), empty_dev(hip, (N, C), np.uint16)
+    mean, inv = empty_dev(hip, (N, G)), empty_dev(hip, (N, G))
+    gamma = O.randn((C,), 3, 0.3) + np.float32(1)
+    dgamma, ggamma, gbeta = to_dev(hip, gamma), empty_dev(hip, (C,)), empty_dev(hip, (C,))
+    hip.HIPBackend.groupNormNhwc(dx, dgamma, None, y, mean, inv, N, P, C, G, EPS, 0, dt)
+    hip.HIPBackend.groupNormNhwcBackward(dg, dx, None, mean, inv, dgamma, None, gx, ggamma, gbeta, N, P, C, G, 0, dt)
+    got = gx.numpy()
+    assert np.array_equal(got, got[every])
+    v = value(x, dt).astype(np.float64).reshape(some, G, per)
+    mu = v.mean(2, keepdims=True)
+    s = 1 / np.sqrt(((v - mu) ** 2).mean(2, keepdims=True) + EPS)
+    xhat = (v - mu) * s
+    w = value(g, dt).astype(np.float64).reshape(some, G, per)
+    d = w * gamma.reshape(G, per)
+    avg = lambda t: t.mean(2, keepdims=True)  # noqa: E731
+    want = s * (d - avg(d) - xhat * avg(d * xhat))
+    # the saved mean and inv are off by (n + 4) u spread and (2 n + 8) u; 64 u of the terms covers four values a group
+    size = s * (np.abs(d) + avg(np.abs(d)) + (1 + np.abs(xhat)) * (1 + s * np.abs(v).max(2, keepdims=True)) * avg(np.abs(d) * (1 + np.abs(xhat))))
+    off = np.abs(value(got[:some], dt).reshape(want.shape) - want)
+    assert np.all(off <= 1.01 * (64 * U * size + HALF_STEP[dt] * np.abs(want)) + TINY[dt])
+    times = np.bincount(every, minlength=some)[:, None]
+    for name, out, t in (("gamma", ggamma, w * xhat), ("beta", gbeta, w)):
+        t, most = t.reshape(some, C), (np.abs(w) * (1 + np.abs(xhat)) * (1 + s * np.abs(v).max(2, keepdims=True))).reshape(some, C)
+        # 32 runs of at most N / 32 additions, then 5
+        assert np.all(np.abs(out.numpy() - (t * times).sum(0)) <= 1.01 * (N // 32 + 70) * U * (most * times).sum(0)), name
