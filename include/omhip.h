@@ -500,7 +500,8 @@ int omHipMultiHeadAttentionHalf(int nDtype, const uint16_t* pX, const uint16_t* 
  * of 128 queries or keys, masked by bCausal or not.
  * P is rounded to nDtype before P V. nHeadDim a multiple of 8 up to 128, nHeads a multiple of
  * nKVHeads; pointers 16-byte aligned, strides multiples of 8 elements, row strides below 2^23.
- * Every element of pOut and pLse is written; nSeqK 0 is a sequence without keys. */
+ * Every element of pOut and pLse is written; nSeqK 0 is a sequence without keys. At most 2^24 - 1
+ * blocks of 128 queries over all images and heads. */
 int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
                                    long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
                                    const int* pKeyLens, int bCausal, uint16_t* pOut, float* pLse, int nBatch, int nSeqQ,
@@ -515,7 +516,8 @@ int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_
  * by powers of two so that small ones keep their bits), sums are in fp32 in a fixed order:
  * repeated calls agree bit for bit. Row statistics use the library's per-stream workspace.
  * Inputs and gradients must not overlap, nor two images' gradients: an image stride that the
- * forward pass takes for inputs shared by images (0) is refused here. */
+ * forward pass takes for inputs shared by images (0) is refused here. At most 2^23 - 1 blocks of
+ * 128 keys over all images and key heads, besides the forward pass's limit. */
 int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
                                long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
                                const int* pKeyLens, int bCausal, const uint16_t* pOut, const float* pLse,

@@ -891,7 +891,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 // What both directions ask of their sizes; 0, 1 (nothing to do) or -1.
 int checkSizes(const char* name, int nDtype, long long nLdQ, long long nStrideQ, long long nLdKV, long long nStrideKV,
-               int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale) {
+               int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale, bool backward) {
     if (nDtype != 0 && nDtype != 1) return fail("%s: dtype must be 0 (fp16) or 1 (bf16)", name);
     if (nBatch < 0 || nSeqQ < 0 || nSeqK < 0) return fail("%s: negative size", name);
     if (nHeads < 1 || nKVHeads < 1 || nHeads % nKVHeads != 0)
@@ -906,8 +906,15 @@ int checkSizes(const char* name, int nDtype, long long nLdQ, long long nStrideQ,
     if (nStrideQ < 0 || nStrideKV < 0) return fail("%s: negative stride", name);
     // grid and row counters
     if (nSeqQ > (1 << 30) || nSeqK > (1 << 30)) return fail("%s: a sequence exceeds 2^30 tokens", name);
-    if ((long long)nBatch * nHeads * ((std::max(nSeqQ, nSeqK) + 63LL) / 64) > 0x3fffffffLL)
+    const long long heads = (long long)nBatch * nHeads;   // below 2^51 (row strides); at most 2^24 tiles each
+    if (heads > 0x3fffffffLL || heads * ((std::max(nSeqQ, nSeqK) + 63LL) / 64) > 0x3fffffffLL)
         return fail("%s: too many (image, head, token) triples", name);
+    // a launch takes 2^32 - 1 threads in a dimension, and silently drops the bits above: 256 threads for a block of
+    // queries, 512 for one of keys (shared walks, which multiply them, are for grids of a few per CU)
+    if (heads * ((nSeqQ + kBlockQ - 1LL) / kBlockQ) * 256 > 0xffffffffLL)
+        return fail("%s: too many (image, head, block of %d queries) triples", name, kBlockQ);
+    if (backward && (long long)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1LL) / kBlockQ) * 512 > 0xffffffffLL)
+        return fail("%s: too many (image, key head, block of %d keys) triples", name, kBlockQ);
     return nBatch == 0 ? 1 : 0;
 }
 
@@ -926,7 +933,7 @@ int omHipAttentionTrainForwardHalf(int nDtype, const uint16_t* pQ, const uint16_
     const char* name = "omHipAttentionTrainForwardHalf";
     clearError();
     const int rc = checkSizes(name, nDtype, nLdQ, nStrideQ, nLdKV, nStrideKV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
-                              nHeadDim, fScale);
+                              nHeadDim, fScale, false);
     if (rc < 0) return -1;
     if (rc || nSeqQ == 0) return 0;
     if (!pQ || !pOut || !pLse || (nSeqK > 0 && (!pK || !pV))) return fail("%s: null pointer", name);
@@ -960,7 +967,7 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
     const char* name = "omHipAttentionBackwardHalf";
     clearError();
     const int rc = checkSizes(name, nDtype, nLdQ, nStrideQ, nLdKV, nStrideKV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
-                              nHeadDim, fScale);
+                              nHeadDim, fScale, true);
     if (rc < 0) return -1;
     if (rc || (nSeqQ == 0 && nSeqK == 0)) return 0;
     if ((nSeqQ > 0 && (!pQ || !pOut || !pLse || !pGradOut || !pGradQ)) || (nSeqK > 0 && (!pK || !pV || !pGradK || !pGradV)))

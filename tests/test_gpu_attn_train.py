@@ -472,3 +472,34 @@ def test_misaligned_lengths_are_refused(place):
     for name, n in (("omHipAttentionTrainForwardHalf", 2), ("omHipAttentionBackwardHalf", 6)):
         with pytest.raises(om.OmHipError, match="aligned"):
             om.call(name, *args, *[4096] * n, 1, 10, 10, 2, 1, 64, 0.125)
+
+
+# One launch takes 2^32 - 1 threads: 256 for each block of 128 queries of a head, 512 for each block of 128 keys of a key
+# head in the backward pass. The query pointer is null, so a size that is let through is refused for that.
+def sizes(batch, seq_q, seq_k, heads, kv):
+    return dict(batch=batch, seq_q=seq_q, seq_k=seq_k, heads=heads, kv=kv, ldq=64 * heads, ldkv=64 * kv, q=None)
+
+
+def refuse_both(a, forward, backward):
+    import omnimatchdeeplearningtool_amd as om
+    a = {**GOOD, **a}
+    p = a["ptr"]
+    front = [a["dtype"], a["q"], p, p, a["ldq"], a["sq"], a["ldkv"], a["skv"], None, None, 0]
+    back = [a["batch"], a["seq_q"], a["seq_k"], a["heads"], a["kv"], a["dim"], a["scale"]]
+    for name, middle, why in (("omHipAttentionTrainForwardHalf", [p, p], forward), ("omHipAttentionBackwardHalf", [p] * 6, backward)):
+        with pytest.raises(om.OmHipError, match=f"{name}.*{why}"):
+            om.call(name, *front, *middle, *back)
+
+
+@pytest.mark.parametrize("a,forward,backward", [
+    (sizes(2 ** 20, 128, 100, 16, 1), "too many", "too many"),           # 2^24 blocks of queries
+    (sizes(2 ** 19, 129, 100, 16, 1), "too many", "too many"),
+    (sizes(2 ** 20 - 1, 128, 100, 16, 1), "null", "null"),
+    (sizes(2 ** 19, 50, 50, 16, 16), "null", "too many"),                # 2^23 blocks of keys
+    (sizes(2 ** 18, 50, 129, 16, 16), "null", "too many"),
+    (sizes(2 ** 19 - 1, 50, 50, 16, 16), "null", "null"),
+    (sizes(2 ** 30, 2 ** 30, 8, 2 ** 16, 1), "too many", "too many"),    # 2^70 triples: not a 64-bit number
+    (sizes(2 ** 30, 8, 2 ** 30, 2 ** 16, 1), "too many", "too many"),
+], ids=str)
+def test_more_blocks_than_a_launch_takes(a, forward, backward):
+    refuse_both(a, forward, backward)
