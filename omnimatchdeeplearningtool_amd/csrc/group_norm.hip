@@ -103,9 +103,10 @@ __device__ __forceinline__ void forRows(const W& w, F&& f) {
 template <bool EVEN>
 struct Channels {
     float mean[8], inv[8], gamma[8], beta[8];
-    // m, v: the image's groups' means and inverse deviations
-    __device__ __forceinline__ void load(const GroupNormParams& p, int c, int n, const float* m, const float* v) {
-        const int g0 = (int)p.byPer.div((uint32_t)c), g1 = (int)p.byPer.div((uint32_t)(c + n - 1));   // the first and the last channel's group
+    // m, v: means and inverse deviations of the image's groups from `first` on
+    __device__ __forceinline__ void load(const GroupNormParams& p, int c, int n, const float* m, const float* v, int first = 0) {
+        // the first and the last channel's group
+        const int g0 = (int)p.byPer.div((uint32_t)c) - first, g1 = (int)p.byPer.div((uint32_t)(c + n - 1)) - first;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             gamma[i] = 1.f;
@@ -122,7 +123,7 @@ struct Channels {
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int g = i < n ? (int)p.byPer.div((uint32_t)(c + i)) : g0;
+                const int g = i < n ? (int)p.byPer.div((uint32_t)(c + i)) - first : g0;
                 mean[i] = m[g];
                 inv[i] = v[g];
             }
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(256) void group_norm_small_kernel(GroupNormParams p
     __syncthreads();
     if (w.n <= 0) return;
     Channels<EVEN> ch;
-    ch.load(p, w.c, w.n, mean - g0, inv - g0);
+    ch.load(p, w.c, w.n, mean, inv, g0);
     applyRows<DT, TC, ACT, EVEN>(p, w, ch);
 }
 
@@ -426,15 +427,15 @@ __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNor
     }
 }
 
-// dx of the workgroup's rows; means: those of the image's groups
+// dx of the workgroup's rows; means: those of the image's groups from `first` on
 template <int DT, int TC, int ACT, bool EVEN>
-__device__ __forceinline__ void gradientRows(const GroupNormParams& p, const Place<TC>& w, const float2* means) {
+__device__ __forceinline__ void gradientRows(const GroupNormParams& p, const Place<TC>& w, const float2* means, int first = 0) {
     using W = Place<TC>;
     Channels<EVEN> ch;
     ch.load(p, w.c, w.n, p.mean + (long long)w.image * p.G, p.inv + (long long)w.image * p.G);
     float2 m[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = means[p.byPer.div((uint32_t)(i < w.n ? w.c + i : w.c))];
+    for (int i = 0; i < 8; ++i) m[i] = means[(int)p.byPer.div((uint32_t)(i < w.n ? w.c + i : w.c)) - first];
     forStores(p.stream, [&](auto streamTag) {
         forRows<W>(w, [&](auto rowsTag, int r) {
             constexpr int ROWS = decltype(rowsTag)::value;
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256) void group_norm_small_backward_kernel(GroupNor
         if (lane == 0) means[g] = {s.x * f, s.y * f};
     }
     __syncthreads();
-    if (w.n > 0) gradientRows<DT, TC, ACT, EVEN>(p, w, means - g0);
+    if (w.n > 0) gradientRows<DT, TC, ACT, EVEN>(p, w, means, g0);
 }
 
 // ---------------------------------------------------------------- launches
