@@ -14,6 +14,8 @@ import numpy as np
 import pytest
 
 import oracle as O
+import test_gpu_attn_train as attention
+import test_gpu_group_norm as group_norm
 from conftest import empty_dev, to_dev
 from test_gpu_attn_train import bits, value
 from test_gpu_dropout import factor, mask, state
@@ -145,3 +147,63 @@ def test_training_step_as_a_graph(hip):
         assert np.array_equal(again, block.results()["y"]) and not np.array_equal(again, want["y"])
     finally:
         g.destroy()
+
+
+# ---------------------------------------------------------------- each call from what the step left before it
+class Left:
+    """A buffer that the step left, in another shape."""
+
+    def __init__(self, buf, shape):
+        self.a = buf.numpy().reshape(shape)
+
+    def numpy(self):
+        return self.a
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
+def test_each_call_of_the_step(hip, bf16):
+    """Every call's results from the tensors that the step itself left as its inputs, element by element: only the call's own
+    roundings remain. uh half a step of the type, u = 2^-24; a product of k terms in fp32 is off by (k + 3) u of its terms'
+    magnitudes, its bias among them, and by uh of itself where it is rounded to the type. Attention and group norm are held
+    to the bounds of their own tests."""
+    uh, u, tiny = 2.0 ** -8 if bf16 else 2.0 ** -11, 2.0 ** -24, 0.0 if bf16 else 2.0 ** -25
+    block = Block(hip, bf16)
+    block.step()
+    d, dt = block.d, block.dt
+    halves = {k: value(d[k].numpy(), bf16).astype(np.float64) for k in ("n", "qkv", "ctx", "proj", "y", "gproj", "gctx", "gqkv", "gn")}
+    x, dy, wqkv, wout = (t.astype(np.float64) for t in (block.x, block.dy, block.wqkv, block.wout))
+
+    def close(name, got, want, size, terms, half=True):
+        off, lim = np.abs(got - want), 1.01 * ((terms + 3) * u * size + (uh * np.abs(want) if half else 0.0)) + (tiny if half else 0.0)
+        assert np.all(off <= lim), (name, float((off / lim).max()))
+
+    def product(name, a, b, bias=0.0, half=True, got=None):
+        got = halves[name] if got is None else got
+        close(name, got, a @ b + bias, np.abs(a) @ np.abs(b) + np.abs(bias), a.shape[1], half)
+
+    product("qkv", halves["n"], wqkv, block.bqkv)
+    product("proj", halves["ctx"], wout)
+    product("gctx", halves["gproj"], wout.T)
+    product("gn", halves["gqkv"], wqkv.T)
+    product("gwout", halves["ctx"].T, halves["gproj"], half=False, got=d["gwout"].numpy())
+    product("gwqkv", halves["n"].T, halves["gqkv"], half=False, got=d["gwqkv"].numpy())
+    close("gbqkv", d["gbqkv"].numpy(), halves["gqkv"].sum(0), np.abs(halves["gqkv"]).sum(0), T, half=False)
+    keep = mask(T, C, P, SEED, STEP, STREAM) * factor(P)
+    kept = (halves["proj"] + block.bout) * keep
+    close("y", halves["y"], x + kept, np.abs(x) + np.abs(kept) + np.abs(halves["proj"] * keep), 1)
+    close("gproj", halves["gproj"], dy * keep, np.abs(dy * keep), 0)
+    close("gbout", d["gbout"].numpy(), (dy * keep).sum(0), np.abs(dy * keep).sum(0), T, half=False)
+
+    attn = object.__new__(attention.Case)   # check() takes what the calls were given and left
+    attn.bf16, attn.causal, attn.qlens, attn.klens, attn.packed, attn.widths = bf16, False, None, None, True, [3 * C]
+    attn.dims, attn.scale, attn.first = (B, S, S, H, H, D), float(np.float32(D ** -0.5)), [0, C, 2 * C]
+    attn.store, attn.grad = [value(d["qkv"].numpy(), bf16).reshape(B, S, 3 * C)], value(d["gctx"].numpy(), bf16).reshape(B, S, H, D)
+    attn.dout, attn.dlse, attn.dgrads = Left(d["ctx"], (B, S, H, D)), d["lse"], [Left(d["gqkv"], (B, S, 3 * C))]
+    attn.check()
+    norm = object.__new__(group_norm.Case)
+    norm.dt, norm.a, norm.dims, norm.shift = dt, 0, (B, S, C, G), 0
+    norm.x, norm.g = bits(block.x, bf16).reshape(B, S, C), d["gn"].numpy().reshape(B, S, C)
+    norm.gamma, norm.beta = block.gamma, block.beta
+    norm.y, norm.gx, norm.mean, norm.inv = Left(d["n"], -1), Left(d["gx"], -1), d["mean"], d["inv"]
+    norm.ggamma, norm.gbeta = d["ggamma"], d["gbeta"]
+    norm.check()
