@@ -278,3 +278,32 @@ def test_more_columns_than_one_dimension_of_a_grid(hip):
             keep = [((words[j // 2] >> (16 * (j % 2))) & 0xFFFF) >= threshold(0.5) for j in range(8)]
             at = slice(8 * group, 8 * group + 8)
             assert np.array_equal(g[at], np.where(keep, 2 * x[at], 0).astype(np.float16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [0, 1], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("cols", [1024, 1021], ids=str)
+def test_large_output_in_half_precision(hip, cols, dt):
+    """Over 24 MB of 16-bit values, which leave with streaming stores: kept and doubled (exact) or dropped, with the host's
+    mask at both ends, forward and backward, with and without a bias gradient."""
+    rows = 12401
+    print(f"case {rows}x{cols} dtype {dt}", flush=True)
+    x = store(O.randn((rows, cols), 6, 1.0), dt)
+    v = value(x, dt)
+    dx, rng = to_dev(hip, x), state(hip, 12, 34)
+    out, gx, alone = (empty_dev(hip, x.shape, x.dtype) for _ in range(3))
+    gb = empty_dev(hip, (cols,))
+    hip.HIPBackend.dropout(dx, None, None, out, rows, cols, 0.5, rng, 2, dt)
+    hip.HIPBackend.dropoutBackward(dx, gx, gb, rows, cols, 0.5, rng, 2, dt)
+    hip.HIPBackend.dropoutBackward(dx, alone, None, rows, cols, 0.5, rng, 2, dt)
+    y = value(out.numpy(), dt)
+    assert np.all((y == 0) | (y == 2 * v))
+    assert np.array_equal(gx.numpy(), out.numpy()) and np.array_equal(alone.numpy(), out.numpy())
+    assert np.array_equal(y[:20] != 0, mask(20, cols, 0.5, 12, 34, 2) & (v[:20] != 0))
+    last, per_row = rows - 1, -(-cols // 8)
+    for c in range(per_row):
+        words = philox([last * per_row + c, 2, 34, 0], [12, 0])
+        keep = np.array([((words[j // 2] >> (16 * (j % 2))) & 0xFFFF) >= threshold(0.5) for j in range(8)])[:cols - 8 * c]
+        at = slice(8 * c, 8 * c + 8)
+        assert np.array_equal(y[last, at] != 0, keep & (v[last, at] != 0))
+    assert np.all(np.abs(gb.numpy() - y.sum(0, dtype=np.float64)) <= 1.01 * (rows + 2) * U * np.abs(y).sum(0, dtype=np.float64))

@@ -418,3 +418,12 @@ def test_more_groups_than_one_dimension_of_a_grid(hip):
         t, most = t.reshape(some, C), (np.abs(w) * (1 + np.abs(xhat)) * (1 + s * np.abs(v).max(2, keepdims=True))).reshape(some, C)
         # 32 runs of at most N / 32 additions, then 5
         assert np.all(np.abs(out.numpy() - (t * times).sum(0)) <= 1.01 * (N // 32 + 70) * U * (most * times).sum(0)), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [0, 1], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("a,C", [(1, 128), (2, 125), (1, 125)], ids=str)
+def test_large_output_in_half_precision(hip, a, C, dt):
+    """Over 24 MB of 16-bit values: streaming stores, whole groups of 8 channels and not, ReLU's saved output among the
+    inputs."""
+    run(hip, 2, 51000, C, 1, dt=dt, a=a)
