@@ -220,25 +220,66 @@ __global__ __launch_bounds__(256) void group_norm_moments_kernel(GroupNormParams
     leavePart(p, w, part);
 }
 
-// One wave per (image, group).
-__global__ __launch_bounds__(64) void group_norm_join_kernel(GroupNormParams p) {
-    const int g = blockIdx.x, image = blockIdx.y, lane = threadIdx.x;
+// (mean, inv) of an (image, group). Its entries are shared by as many waves as leave a lane eight of them, 16 at most, and
+// a lane loads eight before it joins them: all but the last chunk have the same count of rows, which makes the joins' factors
+// constants, so that no join waits for a division. (A wave a group, entry after entry, took longer than everything else where
+// groups are few and wide: 12000 pixels x 2048 channels in one group, forward, bf16: 1235 us, now 73; 16384 x 256 in one: 593,
+// now 35.5; the sums of 32 groups of 8 channels in 16 chunks take the same time either way.)
+__global__ __launch_bounds__(1024) void group_norm_join_kernel(GroupNormParams p) {
+    __shared__ Moments part[16];
+    const int g = blockIdx.x, image = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
-    const uint32_t n = (uint32_t)p.chunks * (uint32_t)p.per;
+    const uint32_t n = (uint32_t)p.chunks * (uint32_t)p.per, threads = blockDim.x;
     Moments t{0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (uint32_t e = lane; e < n; e += 64) {
-        const uint32_t chunk = p.byPer.div(e), c = e - chunk * (uint32_t)p.per;
-        const float2 v = from[(long long)chunk * p.C + c];
-        t = join(t, {(float)chunkRows(p, (int)chunk), v.x, v.y});
-    }
+    for (uint32_t first = threadIdx.x; first < n; first += 8u * threads) {
+        const int m = (int)min(8u, (n - first + threads - 1u) / threads);   // entries first, first + threads, ...
+        float2 v[8];
+        uint32_t chunk[8];
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-        t = join(t, {__shfl_down(t.n, s, 64), __shfl_down(t.mean, s, 64), __shfl_down(t.m2, s, 64)});
-    if (lane == 0) {
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t e = i < m ? first + (uint32_t)i * threads : first;
+            chunk[i] = p.byPer.div(e);
+            v[i] = from[(long long)chunk[i] * p.C + (e - chunk[i] * (uint32_t)p.per)];
+        }
+        const float rows = (float)chunkRows(p, (int)chunk[0]);
+        if (chunk[0] + 1u < (uint32_t)p.chunks && p.byPer.div(first + (uint32_t)(m - 1) * threads) + 1u == (uint32_t)p.chunks) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)   // the last chunk is among them
+                if (i < m) t = join(t, {(float)chunkRows(p, (int)chunk[i]), v[i].x, v[i].y});
+        } else {
+            Moments u{rows * (float)m, v[0].x, v[0].y};
+#pragma unroll
+            for (int i = 1; i < 8; ++i)
+                if (i < m) {
+                    const float d = v[i].x - u.mean;
+                    u.mean = __builtin_fmaf(d, 1.f / (float)(i + 1), u.mean);
+                    u.m2 += v[i].y + d * (rows * ((float)i / (float)(i + 1))) * d;
+                }
+            t = join(t, u);
+        }
+    }
+    auto joinLanes = [&] {
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1)
+            t = join(t, {__shfl_down(t.n, s, 64), __shfl_down(t.mean, s, 64), __shfl_down(t.m2, s, 64)});
+    };
+    joinLanes();
+    if (waves > 1) {
+        if (lane == 0) part[wave] = t;
+        __syncthreads();
+        if (wave > 0) return;
+        t = lane < waves ? part[lane] : Moments{0.f, 0.f, 0.f};
+        joinLanes();
+    }
+    if (threadIdx.x == 0) {
         p.mean[(long long)image * p.G + g] = t.mean;
         p.inv[(long long)image * p.G + g] = 1.f / sqrtf(t.m2 / t.n + p.eps);
     }
+}
+
+// Waves that share a group's entries, `each` entries a lane.
+int joinWaves(const GroupNormParams& p, int each) {
+    return (int)std::clamp<long long>((long long)p.chunks * p.per / (64 * each), 1, 16);
 }
 
 // y of the workgroup's rows
@@ -374,36 +415,47 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
     leavePart(p, w, part);
 }
 
-// The first workgroups: the means of gamma dz and gamma dz xhat of 16 groups, a wave each. The others: dgamma and dbeta
-// of 32 channels, 32 interleaved runs over images and chunks a channel (with 8 runs, the loads' latency took 58 us at
-// 32 x 28 x 28 x 512). Workgroups count through both dimensions of the grid: 2^26 groups are 2^32 threads, and a grid keeps
+// The first workgroups: the means of gamma dz and gamma dz xhat of 16 >> share groups, 1 << share waves each
+// (12000 x 2048 in one group, bf16: 472 us with a wave a group, now 146). The others: dgamma and dbeta of 32 channels, 32 interleaved runs over images and chunks a channel (with 8 runs, the loads' latency took 58 us
+// at 32 x 28 x 28 x 512). Workgroups count through both dimensions of the grid: 2^26 groups are 2^32 threads, and a grid keeps
 // 32 bits of its threads in a dimension. What lies past the last channel finds nothing to do.
-__global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p, uint32_t groupBlocks) {
+template <bool SHARED>
+__global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p, uint32_t groupBlocks, uint32_t shareBits) {
+    const uint32_t share = SHARED ? shareBits : 0u;
     __shared__ float2 part[1024];
     const int t = threadIdx.x;
     float2 s{0.f, 0.f};
     const uint32_t groups = (uint32_t)(p.N * p.G), block = blockIdx.y * gridDim.x + blockIdx.x;
     if (block < groupBlocks) {
-        const uint32_t id = block * 16u + (uint32_t)(t >> 6), lane = (uint32_t)t & 63u;
-        if (id >= groups) return;
-        const uint32_t image = id / (uint32_t)p.G, g = id - image * (uint32_t)p.G;
-        const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
-        const uint32_t n = (uint32_t)p.chunks * (uint32_t)p.per;
+        const uint32_t wave = (uint32_t)t >> 6, id = (block * 16u + wave) >> share, threads = 64u << share;
+        if (id < groups) {
+            const uint32_t image = id / (uint32_t)p.G, g = id - image * (uint32_t)p.G;
+            const float2* from = p.partial + (long long)image * p.chunks * p.C + (long long)g * p.per;
+            const uint32_t n = (uint32_t)p.chunks * (uint32_t)p.per;
 #pragma unroll 4
-        for (uint32_t e = lane; e < n; e += 64) {
-            const uint32_t chunk = p.byPer.div(e), k = e - chunk * (uint32_t)p.per;
-            const float2 v = from[(long long)chunk * p.C + k];
-            const float gamma = p.gamma ? p.gamma[g * p.per + k] : 1.f;
-            s.x = __builtin_fmaf(gamma, v.x, s.x);
-            s.y = __builtin_fmaf(gamma, v.y, s.y);
+            for (uint32_t e = (uint32_t)t & (threads - 1u); e < n; e += threads) {
+                const uint32_t chunk = p.byPer.div(e), k = e - chunk * (uint32_t)p.per;
+                const float2 v = from[(long long)chunk * p.C + k];
+                const float gamma = p.gamma ? p.gamma[g * p.per + k] : 1.f;
+                s.x = __builtin_fmaf(gamma, v.x, s.x);
+                s.y = __builtin_fmaf(gamma, v.y, s.y);
+            }
         }
 #pragma unroll
         for (int d = 32; d > 0; d /= 2) {
             s.x += __shfl_down(s.x, d, 64);
             s.y += __shfl_down(s.y, d, 64);
         }
+        if (share > 0) {
+            if ((t & 63) == 0) part[wave] = s;
+            __syncthreads();
+            for (uint32_t i = 1; i < 1u << share && wave + i < 16u; ++i) {   // whole for a group's first wave, the only one that counts
+                s.x += part[wave + i].x;
+                s.y += part[wave + i].y;
+            }
+        }
         const float f = 1.f / ((float)p.P * (float)p.per);
-        if (lane == 0) p.means[id] = {s.x * f, s.y * f};
+        if (((uint32_t)t & (threads - 1u)) == 0 && id < groups) p.means[id] = {s.x * f, s.y * f};
         return;
     }
     const int c = (int)(block - groupBlocks) * 32 + (t & 31);
@@ -513,7 +565,7 @@ int launchForward(const GroupNormParams& p) {
     }
     hipLaunchKernelGGL((group_norm_moments_kernel<DT, TC, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
-    hipLaunchKernelGGL(group_norm_join_kernel, dim3(p.G, p.N), dim3(64), 0, stream(), p);
+    hipLaunchKernelGGL(group_norm_join_kernel, dim3(p.G, p.N), dim3(64 * joinWaves(p, 8)), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
     hipLaunchKernelGGL((group_norm_apply_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
     OMHIP_CHECK_LAUNCH();
@@ -523,7 +575,9 @@ int launchForward(const GroupNormParams& p) {
 template <int DT, int TC, int ACT, bool EVEN>
 int launchBackward(const GroupNormParams& p) {
     const dim3 grid((p.C + p.width - 1) / p.width, p.chunks, p.N);
-    const int groupBlocks = p.small ? 0 : (p.N * p.G + 15) / 16;
+    int share = 0;   // 16 entries a lane (8: 16384 x 64 in 8 groups 14.4 us, a wave a group 13.4)
+    while (2 << share <= joinWaves(p, 16)) ++share;
+    const int groupBlocks = p.small ? 0 : (int)((((long long)p.N * p.G << share) + 15) / 16);
     const int channelBlocks = (p.gradGamma || p.gradBeta) && !(p.small && p.N == 1) ? (p.C + 31) / 32 : 0;
     if (p.small)
         hipLaunchKernelGGL((group_norm_small_backward_kernel<DT, TC, ACT, EVEN>), grid, dim3(256), 0, stream(), p);
@@ -532,8 +586,8 @@ int launchBackward(const GroupNormParams& p) {
     OMHIP_CHECK_LAUNCH();
     if (groupBlocks + channelBlocks > 0) {
         const int blocks = groupBlocks + channelBlocks, width = std::min(blocks, 1 << 16);
-        hipLaunchKernelGGL(group_norm_join_backward_kernel, dim3(width, (blocks + width - 1) / width), dim3(1024), 0, stream(), p,
-                           (uint32_t)groupBlocks);
+        hipLaunchKernelGGL(share ? group_norm_join_backward_kernel<true> : group_norm_join_backward_kernel<false>, dim3(width, (blocks + width - 1) / width), dim3(1024), 0, stream(), p,
+                           (uint32_t)groupBlocks, (uint32_t)share);
         OMHIP_CHECK_LAUNCH();
     }
     if (p.small) return 0;

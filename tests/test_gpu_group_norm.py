@@ -303,7 +303,8 @@ def far_case(hip, size, dt, spread):
     return c
 
 
-FAR = [(3, 20, 64, 8), (1, 20, 60, 4), (2, 300, 12, 4), (1, 400, 64, 1)]   # one launch, one launch of one image, three launches
+FAR = [(3, 20, 64, 8), (1, 20, 60, 4), (2, 300, 12, 4), (1, 400, 64, 1),   # one launch, one launch of one image, three launches
+       (1, 650, 1000, 1)]                                                      # several waves join a group
 
 
 @pytest.mark.gpu
@@ -427,3 +428,12 @@ def test_large_output_in_half_precision(hip, a, C, dt):
     """Over 24 MB of 16-bit values: streaming stores, whole groups of 8 channels and not, ReLU's saved output among the
     inputs."""
     run(hip, 2, 51000, C, 1, dt=dt, a=a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [1, 2], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", [(1, 5000, 256, 1), (1, 701, 2040, 1), (2, 900, 1000, 2), (1, 3001, 1030, 10), (3, 257, 1536, 3)], ids=str)
+def test_few_wide_groups(hip, size, dt):
+    """Groups whose partial sums several waves join: last chunks of fewer rows, widths that are no multiple of 8."""
+    run(hip, *size, dt=dt, a=sum(size) % 3, seed=sum(size))
+    run(hip, *size, dt=dt, mean=50.0, affine=False, seed=sum(size) + 1)
