@@ -498,7 +498,8 @@ int omHipMultiHeadAttentionHalf(int nDtype, const uint16_t* pX, const uint16_t* 
  * whose scores are all -inf get O = 0 and lse = -inf. What lies past a length is not read, so
  * it may hold anything; a NaN or infinity within the lengths may reach every row of its block
  * of 128 queries or keys, masked by bCausal or not.
- * P is rounded to nDtype before P V. nHeadDim a multiple of 8 up to 128, nHeads a multiple of
+ * P is rounded to nDtype before P V; pLse uses the hardware's fp32 exponential and logarithm (a few
+ * 2^-24 of the scores' and its own size). nHeadDim a multiple of 8 up to 128, nHeads a multiple of
  * nKVHeads; pointers 16-byte aligned, strides multiples of 8 elements, row strides below 2^23.
  * Every element of pOut and pLse is written; nSeqK 0 is a sequence without keys. At most 2^24 - 1
  * blocks of 128 queries over all images and heads. */
@@ -540,7 +541,8 @@ int omHipDropout(int nDtype, const void* pX, const float* pBias, const void* pRe
                  float fProb, const uint64_t* pRng, int nStream);
 /* NEW: the gradient of omHipDropout with the same fProb, state and nStream: pGradX = keep ?
  * pGradOut * s : 0 in nDtype (the residual's gradient is pGradOut itself) and, where it is not
- * NULL, pGradBias [nCols] fp32 = the sums of the unrounded pGradX over the rows, in a fixed order.
+ * NULL, pGradBias [nCols] fp32 = the sums of the unrounded pGradX over the rows, added in fp32 in a
+ * fixed order.
  * pGradX may be pGradOut. */
 int omHipDropoutBackward(int nDtype, const void* pGradOut, void* pGradX, float* pGradBias, int nRows, int nCols, float fProb,
                          const uint64_t* pRng, int nStream);
@@ -551,7 +553,8 @@ int omHipDropoutBackward(int nDtype, const void* pGradOut, void* pGradX, float* 
 /* NEW: pY = act((x - mean) / sqrt(var + fEps) * pGamma + pBeta) on x [nBatch, nPixels, nChannels]
  * (tokens), mean and biased variance over the pixels and the nChannels / nGroups channels of a
  * group. nDtype 0 binary16, 1 bfloat16, 2 fp32 (pX, pY); statistics and pGamma, pBeta [nChannels]
- * (NULL: 1, 0) fp32. nAct 0 none, 1 ReLU, 2 SiLU (z / (1 + exp(-z))). pMean and pInvStd [nBatch,
+ * (NULL: 1, 0) fp32. nAct 0 none, 1 ReLU, 2 SiLU (z / (1 + exp(-z)), from the hardware's fp32
+ * exponential and reciprocal: off by about (|z| + 4) 2^-24 of itself). pMean and pInvStd [nBatch,
  * nGroups] (may be NULL) receive mean and 1 / sqrt(var + fEps) for the backward pass. Statistics
  * hold for means far above the spread, up to the largest fp32; the sum of a group's squared
  * differences from its mean has to stay within fp32. They are added in a fixed order. pY may be

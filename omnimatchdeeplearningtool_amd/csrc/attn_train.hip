@@ -109,11 +109,11 @@ __device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc
 //    2^6 (at most 2^14); bf16 needs none.
 //  * the next tile's K and V land in the other pair of buffers meanwhile.
 // 32 x 32 x 16 MFMAs with 32 queries a wave: an LDS fragment feeds 32 columns, half of what 16 x 16 tiles would read.
-// Measured: 2 images x 4096 tokens, 16 query heads on 4 of 128, causal, bf16: 140 us (0.98 PFLOP/s of the visible pairs;
-// a large library product reaches 1.27 here), matrix cores busy 56 % of CU cycles at 1.96 GHz, no bank conflicts: bound by
-// the two waves of a SIMD that share its issue between MFMAs (1024 cycles a tile) and exponentials (1050). ViT-B/16 b64
-// (197 tokens, 768 heads of 64, fp16): 21.7 us, 3.6 TB/s over its compulsory bytes; four tiles a walk, so its start
-// and end (copies in, results out) are half of it.
+// Measured: 2 images x 4096 tokens, 16 query heads on 4 of 128, causal, bf16: 141-160 us by card (0.86-0.98 PFLOP/s of the
+// visible pairs; a large library product reaches 1.27 here), matrix cores busy 56 % of CU cycles at 1.94 GHz, no bank
+// conflicts: bound by the two waves of a SIMD that share its issue between MFMAs (1024 cycles a tile) and exponentials (1050).
+// ViT-B/16 b64 (197 tokens, 768 heads of 64, fp16): 23.6-25.5 us, 3.1-3.3 TB/s over its compulsory bytes; four tiles a walk,
+// so its start and end (copies in, results out), which nothing overlaps, are half of it.
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainParams p) {
     using T = AtTile<KD>;
@@ -263,6 +263,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AttnTrainPar
     sum = atSumHalves(sum);
     const bool empty = !(query < nQ) || sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
+    // the hardware's logarithm: a few 2^-24 of log2(sum), as the sum itself
     const float lse = empty ? -INFINITY : m * (c * kAtLn2) + (__logf(sum) - kShift * kAtLn2);
     const long long row = ((long long)b * p.Sq + query) * p.H + head;
     const long long stat = ((long long)b * p.H + head) * p.Sq + query;
@@ -351,7 +352,7 @@ struct DsScale {
 // without a key) get shift = -inf, which makes their probabilities 0.
 // dQ and dK / dV are two kernels that each compute S and dP, 7 products where one pass would need 5: sums of a row's dQ
 // over workgroups would have to be added atomically, in an order that changes, or written whole for every block of keys.
-// Measured (sizes as for the forward pass): 212 us (0.97 PFLOP/s), matrix cores busy 53 %; ViT-B/16 b64 36 us.
+// Measured (sizes as for the forward pass): 211-242 us by card (0.85-0.98 PFLOP/s), matrix cores busy 54 %; ViT-B/16 b64 37.
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p) {
     using T = AtTile<KD>;
@@ -394,7 +395,9 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AttnTrainParams p
     };
     // Q and dO of the wave's queries, and delta. Head dimensions up to 64: by whole rows, Q through its part of the second
     // pair of buffers, which tile 1 is copied to after the first barrier, dO through rows of its own; larger ones straight
-    // into fragments (LDS for dO would leave one workgroup a CU, and the chunks of dO and O for delta spill).
+    // into fragments, 32 rows for 16 bytes an instruction: rows of dO's own would leave one workgroup a CU, and a head
+    // dimension of 128 is at 256 registers and 12-20 bytes of scratch without the chunks of dO and O for delta. (dO through
+    // the first pair of buffers, free until the first tile is fetched, has not been measured.)
     constexpr bool kStaged = KD <= 2;
     __shared__ __attribute__((aligned(256))) uint16_t gStage[kStaged ? kBlockQ * T::RS : 8];
     __shared__ float rowDelta[kWaves][32];
@@ -567,8 +570,8 @@ __global__ __launch_bounds__(256) void attn_train_dq_join_kernel(AttnTrainParams
 //  * the second, one tile behind, computes dP = dO V^T, dS from that P, and dK^T += Q^T dS.
 // One wave doing both needs 128 + 64 registers for its sums and K, V fragments at a head dimension of 128, so only one
 // fits a SIMD and every LDS read and exponential of it is waited out: 465-489 us at 2 x 4096 x 16 heads on 4 of 128,
-// causal, against 296-319 us (0.93 PFLOP/s, matrix cores busy 48 %) for two waves that fill each other's gaps. ViT-B/16
-// b64: 40 us. Q and dO tiles are in three buffers: the next one's copy, the first waves' and the second waves'.
+// causal, against 289-319 us (0.86-0.95 PFLOP/s, matrix cores busy 51 %) for two waves that fill each other's gaps. ViT-B/16
+// b64: 41 us. Q and dO tiles are in three buffers: the next one's copy, the first waves' and the second waves'.
 // Where the blocks of keys are few for the card, `parts` workgroups take a share of a block's walk each and leave fp32
 // sums, which attn_train_dkv_join_kernel adds in order.
 constexpr int kTileQ = 32;

@@ -131,6 +131,8 @@ struct Channels {
     }
 };
 
+// The hardware's exponential and reciprocal: off by about (|z| + 4) 2^-24 of itself (the exponent's rounding); 0 may stand for
+// it below z = -87, where it is less than 2^-125.
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 template <int ACT>
