@@ -417,14 +417,16 @@ __global__ __launch_bounds__(256) void group_norm_sums_kernel(GroupNormParams p)
     leavePart(p, w, part);
 }
 
-// The first workgroups: the means of gamma dz and gamma dz xhat of 16 >> share groups, 1 << share waves each
-// (12000 x 2048 in one group, bf16: 472 us with a wave a group, now 146). The others: dgamma and dbeta of 32 channels, 32 interleaved runs over images and chunks a channel (with 8 runs, the loads' latency took 58 us
-// at 32 x 28 x 28 x 512). Workgroups count through both dimensions of the grid: 2^26 groups are 2^32 threads, and a grid keeps
-// 32 bits of its threads in a dimension. What lies past the last channel finds nothing to do.
+// The first workgroups: the means of gamma dz and gamma dz xhat of 16 >> share groups, 1 << share waves each (12000 x 2048 in
+// one group, bf16: 472 us with a wave a group, now 146; SHARED: share is not 0, a choice at run time alone cost 8 x 1024 x 320
+// in 32 groups 1 us of 17.4). The others: dgamma and dbeta of 32 channels, 32 interleaved runs over images and chunks a channel
+// (with 8 runs, the loads' latency took 58 us at 32 x 28 x 28 x 512). Workgroups count through both dimensions of the grid: 2^26
+// groups are 2^32 threads, and a grid keeps 32 bits of its threads in a dimension. What lies past the last channel finds
+// nothing to do.
 template <bool SHARED>
 __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNormParams p, uint32_t groupBlocks, uint32_t shareBits) {
-    const uint32_t share = SHARED ? shareBits : 0u;
     __shared__ float2 part[1024];
+    const uint32_t share = SHARED ? shareBits : 0u;
     const int t = threadIdx.x;
     float2 s{0.f, 0.f};
     const uint32_t groups = (uint32_t)(p.N * p.G), block = blockIdx.y * gridDim.x + blockIdx.x;
@@ -448,10 +450,10 @@ __global__ __launch_bounds__(1024) void group_norm_join_backward_kernel(GroupNor
             s.x += __shfl_down(s.x, d, 64);
             s.y += __shfl_down(s.y, d, 64);
         }
-        if (share > 0) {
+        if constexpr (SHARED) {
             if ((t & 63) == 0) part[wave] = s;
             __syncthreads();
-            for (uint32_t i = 1; i < 1u << share && wave + i < 16u; ++i) {   // whole for a group's first wave, the only one that counts
+            for (uint32_t i = 1; i < 1u << share && wave + i < 16u; ++i) {   // all of them for a group's first wave, which leaves the sum
                 s.x += part[wave + i].x;
                 s.y += part[wave + i].y;
             }
@@ -588,8 +590,9 @@ int launchBackward(const GroupNormParams& p) {
     OMHIP_CHECK_LAUNCH();
     if (groupBlocks + channelBlocks > 0) {
         const int blocks = groupBlocks + channelBlocks, width = std::min(blocks, 1 << 16);
-        hipLaunchKernelGGL(share ? group_norm_join_backward_kernel<true> : group_norm_join_backward_kernel<false>, dim3(width, (blocks + width - 1) / width), dim3(1024), 0, stream(), p,
-                           (uint32_t)groupBlocks, (uint32_t)share);
+        hipLaunchKernelGGL(share ? group_norm_join_backward_kernel<true> : group_norm_join_backward_kernel<false>,
+                           dim3(width, (blocks + width - 1) / width), dim3(1024), 0, stream(), p, (uint32_t)groupBlocks,
+                           (uint32_t)share);
         OMHIP_CHECK_LAUNCH();
     }
     if (p.small) return 0;
