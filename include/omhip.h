@@ -525,6 +525,88 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
                                const uint16_t* pGradOut, uint16_t* pGradQ, uint16_t* pGradK, uint16_t* pGradV, int nBatch,
                                int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale);
 
+/* ===== where an attention block's tokens are (NEW; the reference's MultiHeadAttention, vit.ixx:150-239, adds
+ * positions to its input once): norm and rotation of queries and keys, attention with a learned
+ * bias by relative position, attention in a window. Strides, lengths, types and masked values are
+ * as for omHipAttentionTrainForwardHalf where nothing else is said ===== */
+
+/* NEW: pOutQ and pOutK = rotate(x / sqrt(mean(x^2) + fEps) * weight) of each head of pQ and pK in
+ * one pass, in fp32, rounded once. nDtype 0 binary16, 1 bfloat16, 2 fp32. Token t of image b has
+ * its query heads at pQ + b * nStrideQ + t * nLdQ, nHeads of nHeadDim values, and its key heads at
+ * pK likewise, nKVHeads of them (either number may be 0, its pointers are not read then). The
+ * outputs have strides of their own; pOutQ may be pQ and pOutK pK with the same strides.
+ * pWeightQ, pWeightK [nHeadDim] fp32 (NULL: 1).
+ * Rotation: of the first nRotary values of a head, pairs (i, i + nRotary / 2), or (2 i, 2 i + 1) if
+ * bInterleaved, become (a c - b s, b c + a s) with c, s = row `position` of pCos, pSin [nTable,
+ * nRotary / 2] fp32. The position is pPositions[b * nSeq + t] (int32 on the device; NULL: t); one
+ * outside 0 .. nTable - 1, such as -1 for a class token, leaves the token unrotated.
+ * nHeadDim a multiple of 8 up to 256, nRotary a multiple of 8 up to nHeadDim (0: the norm alone);
+ * data 16-byte aligned, strides multiples of 8 elements; at most 2^31 - 1 heads of tokens. The
+ * sum of a head's squares has to stay within fp32. */
+int omHipQkNormRotary(int nDtype, const void* pQ, const void* pK, long long nLdQ, long long nStrideQ, long long nLdK,
+                      long long nStrideK, const float* pWeightQ, const float* pWeightK, const float* pCos, const float* pSin,
+                      const int* pPositions, void* pOutQ, void* pOutK, long long nLdOutQ, long long nStrideOutQ,
+                      long long nLdOutK, long long nStrideOutK, int nBatch, int nSeq, int nHeads, int nKVHeads, int nHeadDim,
+                      int nRotary, int nTable, float fEps, int bInterleaved);
+/* NEW: the gradients of omHipQkNormRotary from its inputs pQ and pK: with g the output's gradient
+ * turned back and xhat = x inv, dx = inv (g w - xhat mean(g w xhat)) into pGradQ and pGradK, laid
+ * out as pQ and pK are, and pGradWeightQ, pGradWeightK [nHeadDim] fp32 (each may be NULL) = the
+ * sums of g xhat over all tokens and heads, in a fixed order. pGradQ may be pGradOutQ and pGradK
+ * pGradOutK where their strides agree. */
+int omHipQkNormRotaryBackward(int nDtype, const void* pGradOutQ, const void* pGradOutK, long long nLdGradQ,
+                              long long nStrideGradQ, long long nLdGradK, long long nStrideGradK, const void* pQ, const void* pK,
+                              long long nLdQ, long long nStrideQ, long long nLdK, long long nStrideK, const float* pWeightQ,
+                              const float* pWeightK, const float* pCos, const float* pSin, const int* pPositions, void* pGradQ,
+                              void* pGradK, float* pGradWeightQ, float* pGradWeightK, int nBatch, int nSeq, int nHeads,
+                              int nKVHeads, int nHeadDim, int nRotary, int nTable, float fEps, int bInterleaved);
+
+/* NEW: omHipAttentionTrainForwardHalf with a learned bias added to the scores: S = fScale Q K^T +
+ * pTable[bucket][head], bucket = pBuckets[query's position - key's position + nZero]. pTable
+ * [nBuckets, nHeads] fp32; pBuckets [nOffsets] int32, the bucket of each difference from -nZero on;
+ * differences past its ends take the first's or the last's. A bucket outside 0 .. nBuckets - 1 adds
+ * nothing; a bias at or below -1e30 hides the key.
+ * Positions: pQueryPos [nSeqQ] and pKeyPos [nSeqK] int32 (any values, shared by the images), as y
+ * (2 width - 1) + x for patches, whose differences tell both distances; or both NULL: in an image
+ * of nQ queries and nK keys (its lengths) query i stands at i + nK - nQ, key j at j. bCausal: j <=
+ * i + nK - nQ. 1 to 4096 offsets, 1 to 16384 buckets, nZero from -2^30 on, at most 2^29 tokens a
+ * sequence. */
+int omHipAttentionBiasForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                  long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                  const int* pKeyLens, int bCausal, const float* pTable, const int* pBuckets,
+                                  const int* pQueryPos, const int* pKeyPos, int nBuckets, int nOffsets, int nZero, uint16_t* pOut,
+                                  float* pLse, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim,
+                                  float fScale);
+/* NEW: the gradients of omHipAttentionBiasForwardHalf at the same arguments: pGradQ, pGradK and
+ * pGradV as omHipAttentionBackwardHalf's, and pGradTable [nBuckets, nHeads] fp32 = the sums of the
+ * unrounded dS = P (dO V^T - delta) over the pairs of each bucket and all images, in fp32 and in an
+ * order that repeats (0 where no pair is in the bucket). delta comes from pOut as it was rounded. */
+int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                   long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                   const int* pKeyLens, int bCausal, const float* pTable, const int* pBuckets,
+                                   const int* pQueryPos, const int* pKeyPos, int nBuckets, int nOffsets, int nZero,
+                                   const uint16_t* pOut, const float* pLse, const uint16_t* pGradOut, uint16_t* pGradQ,
+                                   uint16_t* pGradK, uint16_t* pGradV, float* pGradTable, int nBatch, int nSeqQ, int nSeqK,
+                                   int nHeads, int nKVHeads, int nHeadDim, float fScale);
+
+/* NEW: omHipAttentionTrainForwardHalf in a sliding window: in an image of nQ queries and nK keys
+ * (its lengths) query i stands at p = i + nK - nQ and sees key j where |p - j| < nWindow or j <
+ * nFirst, and j <= p if bCausal. So a single query (nSeqQ 1) with pKeyLens is a sequence's next
+ * token against its cache. Work goes with the keys in sight, not with nSeqK. nWindow at least 1,
+ * nFirst at least 0, at most 2^29 tokens a sequence. A NaN or infinity within the lengths may reach
+ * the rows that see its tile of 64 keys, masked for them or not. */
+int omHipAttentionWindowForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                    long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                    const int* pKeyLens, int bCausal, int nWindow, int nFirst, uint16_t* pOut, float* pLse,
+                                    int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale);
+/* NEW: the gradients of omHipAttentionWindowForwardHalf at the same arguments, as
+ * omHipAttentionBackwardHalf's; keys that no query sees get zeros. */
+int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                     long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                     const int* pKeyLens, int bCausal, int nWindow, int nFirst, const uint16_t* pOut,
+                                     const float* pLse, const uint16_t* pGradOut, uint16_t* pGradQ, uint16_t* pGradK,
+                                     uint16_t* pGradV, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim,
+                                     float fScale);
+
 /* ===== dropout (omCudaDropout, cuda_kernels.cu:2266-2337, keeps a float mask; here the mask is a
  * function of the generator's state and is never stored) ===== */
 

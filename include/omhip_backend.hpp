@@ -283,6 +283,79 @@ public:
                                          nSeqK, nHeads, nKVHeads, nHeadDim, fScale),
               "attentionBackwardHalf");
     }
+    // Norm of every query and key head, weight and rotation by the row of pCos, pSin at the token's position (nullable: its
+    // number), and its gradients from the inputs; nDtype 0 fp16, 1 bf16, 2 fp32
+    static void qkNormRotary(int nDtype, const void* pQ, const void* pK, long long nLdQ, long long nStrideQ, long long nLdK,
+                             long long nStrideK, const float* pWeightQ, const float* pWeightK, const float* pCos,
+                             const float* pSin, const int* pPositions, void* pOutQ, void* pOutK, long long nLdOutQ,
+                             long long nStrideOutQ, long long nLdOutK, long long nStrideOutK, int nBatch, int nSeq, int nHeads,
+                             int nKVHeads, int nHeadDim, int nRotary, int nTable, float fEps, bool bInterleaved) {
+        check(omHipQkNormRotary(nDtype, pQ, pK, nLdQ, nStrideQ, nLdK, nStrideK, pWeightQ, pWeightK, pCos, pSin, pPositions, pOutQ,
+                                pOutK, nLdOutQ, nStrideOutQ, nLdOutK, nStrideOutK, nBatch, nSeq, nHeads, nKVHeads, nHeadDim,
+                                nRotary, nTable, fEps, bInterleaved ? 1 : 0),
+              "qkNormRotary");
+    }
+    static void qkNormRotaryBackward(int nDtype, const void* pGradOutQ, const void* pGradOutK, long long nLdGradQ,
+                                     long long nStrideGradQ, long long nLdGradK, long long nStrideGradK, const void* pQ,
+                                     const void* pK, long long nLdQ, long long nStrideQ, long long nLdK, long long nStrideK,
+                                     const float* pWeightQ, const float* pWeightK, const float* pCos, const float* pSin,
+                                     const int* pPositions, void* pGradQ, void* pGradK, float* pGradWeightQ,
+                                     float* pGradWeightK, int nBatch, int nSeq, int nHeads, int nKVHeads, int nHeadDim,
+                                     int nRotary, int nTable, float fEps, bool bInterleaved) {
+        check(omHipQkNormRotaryBackward(nDtype, pGradOutQ, pGradOutK, nLdGradQ, nStrideGradQ, nLdGradK, nStrideGradK, pQ, pK, nLdQ,
+                                        nStrideQ, nLdK, nStrideK, pWeightQ, pWeightK, pCos, pSin, pPositions, pGradQ, pGradK,
+                                        pGradWeightQ, pGradWeightK, nBatch, nSeq, nHeads, nKVHeads, nHeadDim, nRotary, nTable,
+                                        fEps, bInterleaved ? 1 : 0),
+              "qkNormRotaryBackward");
+    }
+    // attentionTrainForwardHalf with a learned bias, pTable[pBuckets[query's position - key's + nZero]][head], added to the
+    // scores (positions nullable), and its gradients
+    static void attentionBiasForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                         long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                         const int* pKeyLens, bool bCausal, const float* pTable, const int* pBuckets,
+                                         const int* pQueryPos, const int* pKeyPos, int nBuckets, int nOffsets, int nZero,
+                                         uint16_t* pOut, float* pLse, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads,
+                                         int nHeadDim, float fScale) {
+        check(omHipAttentionBiasForwardHalf(nDtype, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens,
+                                            bCausal ? 1 : 0, pTable, pBuckets, pQueryPos, pKeyPos, nBuckets, nOffsets, nZero,
+                                            pOut, pLse, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale),
+              "attentionBiasForwardHalf");
+    }
+    static void attentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                          long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                          const int* pKeyLens, bool bCausal, const float* pTable, const int* pBuckets,
+                                          const int* pQueryPos, const int* pKeyPos, int nBuckets, int nOffsets, int nZero,
+                                          const uint16_t* pOut, const float* pLse, const uint16_t* pGradOut, uint16_t* pGradQ,
+                                          uint16_t* pGradK, uint16_t* pGradV, float* pGradTable, int nBatch, int nSeqQ,
+                                          int nSeqK, int nHeads, int nKVHeads, int nHeadDim, float fScale) {
+        check(omHipAttentionBiasBackwardHalf(nDtype, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens,
+                                             bCausal ? 1 : 0, pTable, pBuckets, pQueryPos, pKeyPos, nBuckets, nOffsets, nZero,
+                                             pOut, pLse, pGradOut, pGradQ, pGradK, pGradV, pGradTable, nBatch, nSeqQ, nSeqK,
+                                             nHeads, nKVHeads, nHeadDim, fScale),
+              "attentionBiasBackwardHalf");
+    }
+    // attentionTrainForwardHalf over the keys less than nWindow from a query's position and the first nFirst, and its gradients
+    static void attentionWindowForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                           long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                           const int* pKeyLens, bool bCausal, int nWindow, int nFirst, uint16_t* pOut,
+                                           float* pLse, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim,
+                                           float fScale) {
+        check(omHipAttentionWindowForwardHalf(nDtype, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens,
+                                              bCausal ? 1 : 0, nWindow, nFirst, pOut, pLse, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                                              nHeadDim, fScale),
+              "attentionWindowForwardHalf");
+    }
+    static void attentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV,
+                                            long long nLdQ, long long nStrideQ, long long nLdKV, long long nStrideKV,
+                                            const int* pQueryLens, const int* pKeyLens, bool bCausal, int nWindow, int nFirst,
+                                            const uint16_t* pOut, const float* pLse, const uint16_t* pGradOut, uint16_t* pGradQ,
+                                            uint16_t* pGradK, uint16_t* pGradV, int nBatch, int nSeqQ, int nSeqK, int nHeads,
+                                            int nKVHeads, int nHeadDim, float fScale) {
+        check(omHipAttentionWindowBackwardHalf(nDtype, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens,
+                                               bCausal ? 1 : 0, nWindow, nFirst, pOut, pLse, pGradOut, pGradQ, pGradK, pGradV,
+                                               nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale),
+              "attentionWindowBackwardHalf");
+    }
     // Dropout with a mask that is a function of the generator's state (pRng, device: seed, step), nStream and the place:
     // keep ? (x + bias) * s : 0, + residual (both nullable); nDtype 0 fp16, 1 bf16, 2 fp32
     static void dropout(int nDtype, const void* pX, const float* pBias, const void* pResidual, void* pOut, int nRows,

@@ -131,6 +131,12 @@ _SIGS = {
     "omHipMultiHeadAttentionHalf": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i],
     "omHipAttentionTrainForwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i, _vp, _vp] + [_i] * 6 + [_fl],
     "omHipAttentionBackwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i] + [_vp] * 6 + [_i] * 6 + [_fl],
+    "omHipQkNormRotary": [_i] + [_vp] * 2 + [_ll] * 4 + [_vp] * 7 + [_ll] * 4 + [_i] * 7 + [_fl, _i],
+    "omHipQkNormRotaryBackward": [_i] + ([_vp] * 2 + [_ll] * 4) * 2 + [_vp] * 9 + [_i] * 7 + [_fl, _i],
+    "omHipAttentionBiasForwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i] + [_vp] * 4 + [_i] * 3 + [_vp] * 2 + [_i] * 6 + [_fl],
+    "omHipAttentionBiasBackwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp, _i] + [_vp] * 4 + [_i] * 3 + [_vp] * 7 + [_i] * 6 + [_fl],
+    "omHipAttentionWindowForwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp] + [_i] * 3 + [_vp] * 2 + [_i] * 6 + [_fl],
+    "omHipAttentionWindowBackwardHalf": [_i] + [_vp] * 3 + [_ll] * 4 + [_vp, _vp] + [_i] * 3 + [_vp] * 6 + [_i] * 6 + [_fl],
     "omHipDropout": [_i, _vp, _vp, _vp, _vp, _i, _i, _fl, _vp, _i],
     "omHipDropoutBackward": [_i, _vp, _vp, _vp, _i, _i, _fl, _vp, _i],
     "omHipGroupNormNhwc": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _fl, _i],
@@ -577,6 +583,66 @@ class HIPBackend:
         call("omHipAttentionBackwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV,
              nStrideKV, _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, _ptr(pOut), _ptr(pLse), _ptr(pGradOut),
              _ptr(pGradQ), _ptr(pGradK), _ptr(pGradV), nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
+
+    @staticmethod
+    def qkNormRotary(pQ, pK, nLdQ, nStrideQ, nLdK, nStrideK, pWeightQ, pWeightK, pCos, pSin, pPositions, pOutQ, pOutK, nLdOutQ,
+                     nStrideOutQ, nLdOutK, nStrideOutK, nBatch, nSeq, nHeads, nKVHeads, nHeadDim, nRotary, nTable, fEps,
+                     bInterleaved=False, nDtype: int = 2) -> None:
+        """rotate(x / sqrt(mean(x^2) + eps) * weight) of every query and key head; pCos and pSin [nTable, nRotary / 2] by
+        position (int32 [nBatch, nSeq] on the device; None: the token's number). Weights may be None."""
+        call("omHipQkNormRotary", nDtype, _ptr(pQ), _ptr(pK), nLdQ, nStrideQ, nLdK, nStrideK, _ptr(pWeightQ), _ptr(pWeightK),
+             _ptr(pCos), _ptr(pSin), _ptr(pPositions), _ptr(pOutQ), _ptr(pOutK), nLdOutQ, nStrideOutQ, nLdOutK, nStrideOutK,
+             nBatch, nSeq, nHeads, nKVHeads, nHeadDim, nRotary, nTable, fEps, 1 if bInterleaved else 0)
+
+    @staticmethod
+    def qkNormRotaryBackward(pGradOutQ, pGradOutK, nLdGradQ, nStrideGradQ, nLdGradK, nStrideGradK, pQ, pK, nLdQ, nStrideQ,
+                             nLdK, nStrideK, pWeightQ, pWeightK, pCos, pSin, pPositions, pGradQ, pGradK, pGradWeightQ,
+                             pGradWeightK, nBatch, nSeq, nHeads, nKVHeads, nHeadDim, nRotary, nTable, fEps, bInterleaved=False,
+                             nDtype: int = 2) -> None:
+        """qkNormRotary's gradients from its inputs, laid out as they are; the weights' (fp32) may be None."""
+        call("omHipQkNormRotaryBackward", nDtype, _ptr(pGradOutQ), _ptr(pGradOutK), nLdGradQ, nStrideGradQ, nLdGradK,
+             nStrideGradK, _ptr(pQ), _ptr(pK), nLdQ, nStrideQ, nLdK, nStrideK, _ptr(pWeightQ), _ptr(pWeightK), _ptr(pCos),
+             _ptr(pSin), _ptr(pPositions), _ptr(pGradQ), _ptr(pGradK), _ptr(pGradWeightQ), _ptr(pGradWeightK), nBatch, nSeq,
+             nHeads, nKVHeads, nHeadDim, nRotary, nTable, fEps, 1 if bInterleaved else 0)
+
+    @staticmethod
+    def attentionBiasForwardHalf(pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, pTable, pBuckets,
+                                 pQueryPos, pKeyPos, nBuckets, nOffsets, nZero, pOut, pLse, nBatch, nSeqQ, nSeqK, nHeads,
+                                 nKVHeads, nHeadDim, fScale, bf16: bool = False) -> None:
+        """attentionTrainForwardHalf with pTable[pBuckets[query's position - key's + nZero]][head] added to the scores;
+        positions (int32 on the device) may both be None."""
+        call("omHipAttentionBiasForwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV, nStrideKV,
+             _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, _ptr(pTable), _ptr(pBuckets), _ptr(pQueryPos),
+             _ptr(pKeyPos), nBuckets, nOffsets, nZero, _ptr(pOut), _ptr(pLse), nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim,
+             fScale)
+
+    @staticmethod
+    def attentionBiasBackwardHalf(pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, pTable, pBuckets,
+                                  pQueryPos, pKeyPos, nBuckets, nOffsets, nZero, pOut, pLse, pGradOut, pGradQ, pGradK, pGradV,
+                                  pGradTable, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale, bf16: bool = False) -> None:
+        """dQ, dK, dV and the table's gradient (fp32) of attentionBiasForwardHalf at the same arguments."""
+        call("omHipAttentionBiasBackwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV, nStrideKV,
+             _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, _ptr(pTable), _ptr(pBuckets), _ptr(pQueryPos),
+             _ptr(pKeyPos), nBuckets, nOffsets, nZero, _ptr(pOut), _ptr(pLse), _ptr(pGradOut), _ptr(pGradQ), _ptr(pGradK),
+             _ptr(pGradV), _ptr(pGradTable), nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
+
+    @staticmethod
+    def attentionWindowForwardHalf(pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, nWindow, nFirst,
+                                   pOut, pLse, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale,
+                                   bf16: bool = False) -> None:
+        """attentionTrainForwardHalf over the keys less than nWindow from a query's position, and the first nFirst."""
+        call("omHipAttentionWindowForwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV, nStrideKV,
+             _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, nWindow, nFirst, _ptr(pOut), _ptr(pLse), nBatch, nSeqQ,
+             nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
+
+    @staticmethod
+    def attentionWindowBackwardHalf(pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, nWindow, nFirst,
+                                    pOut, pLse, pGradOut, pGradQ, pGradK, pGradV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                                    nHeadDim, fScale, bf16: bool = False) -> None:
+        """dQ, dK, dV of attentionWindowForwardHalf at the same arguments."""
+        call("omHipAttentionWindowBackwardHalf", 1 if bf16 else 0, _ptr(pQ), _ptr(pK), _ptr(pV), nLdQ, nStrideQ, nLdKV,
+             nStrideKV, _ptr(pQueryLens), _ptr(pKeyLens), 1 if bCausal else 0, nWindow, nFirst, _ptr(pOut), _ptr(pLse),
+             _ptr(pGradOut), _ptr(pGradQ), _ptr(pGradK), _ptr(pGradV), nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale)
 
     @staticmethod
     def dropout(pX, pBias, pResidual, pOut, nRows, nCols, fProb, pRng, nStream, nDtype: int = 2) -> None:

@@ -1,0 +1,162 @@
+// attn_bias.hip — attention with a learned bias by relative position, forward
+// and backward: the entries of the bias view (attn_train_kernels.hpp holds the
+// attention kernels), and the sums of the table's gradient.
+//
+// S = scale Q K^T + bias, bias_ij = table[bucketOf[pos_i - pos_j + zero]][head]:
+// a table of learned biases, and a map from the difference of two positions to
+// its rows. One map serves sequences (position i; buckets that grow with the
+// distance) and grids of patches (position y (2 width - 1) + x, whose differences
+// tell both distances). dtable is the sum of dS over the pairs of a bucket:
+//  * the dQ kernel, which has dS in registers, adds each to its wave's sums by
+//    offset in LDS, and leaves its workgroup's;
+//  * attn_bias_offsets_kernel adds those of a head, attn_bias_table_kernel the
+//    offsets of each bucket. All in fp32 and in an order that repeats.
+#include "attn_train_kernels.hpp"
+#include "../../include/omhip.h"
+
+#include <climits>
+
+namespace omhip {
+
+namespace {
+
+constexpr int kMaxBuckets = 16384;   // attn_bias_table_kernel's sums take 64 KB of LDS
+constexpr int kMaxSeq = 1 << 29;     // positions stay below 2^31
+
+// offsetSums[head][o] = sum over the head's `units` rows of bins, a quarter a wave.
+__global__ __launch_bounds__(256) void attn_bias_offsets_kernel(AttnBiasParams p, int units) {
+    __shared__ float part[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int o = (int)blockIdx.x * 64 + lane, head = (int)blockIdx.y;
+    const int first = (int)((long long)units * wave / 4), last = (int)((long long)units * (wave + 1) / 4);
+    float s = 0.f;
+    if (o < p.nOffsets) {
+        const float* from = p.bins + (long long)head * units * p.nOffsets + o;
+#pragma unroll 8
+        for (int u = first; u < last; ++u) s += from[(long long)u * p.nOffsets];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && o < p.nOffsets)
+        p.offsetSums[(long long)head * p.nOffsets + o] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+}
+
+// gradTable[bucket][head] = sum of the offsets in the bucket, added by one wave.
+__global__ __launch_bounds__(256) void attn_bias_table_kernel(AttnBiasParams p, int empty) {
+    extern __shared__ float biases[];   // [nBuckets]
+    const int head = (int)blockIdx.x;
+    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) biases[b] = 0.f;
+    __syncthreads();
+    if (threadIdx.x < 64 && !empty)
+        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 64) {
+            const int b = p.bucketOf[o];
+            if ((uint32_t)b < (uint32_t)p.nBuckets) atAdd(biases + b, p.offsetSums[(long long)head * p.nOffsets + o]);
+        }
+    __syncthreads();
+    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) p.gradTable[(long long)b * p.H + head] = biases[b];
+}
+
+int tableGradient(const AttnBiasParams& p, int units) {
+    if (units > 0) {
+        hipLaunchKernelGGL(attn_bias_offsets_kernel, dim3((p.nOffsets + 63) / 64, p.H), dim3(256), 0, stream(), p, units);
+        OMHIP_CHECK_LAUNCH();
+    }
+    hipLaunchKernelGGL(attn_bias_table_kernel, dim3(p.H), dim3(256), (size_t)p.nBuckets * sizeof(float), stream(), p, units == 0);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+// What a bias asks of its arguments; 0 or -1.
+int biasArguments(AttnBiasParams& p, const char* name, const float* pTable, const int* pBuckets, const int* pQueryPos,
+                  const int* pKeyPos, int nBuckets, int nOffsets, int nZero, int nSeqQ, int nSeqK, int nHeads) {
+    if (nSeqQ > kMaxSeq || nSeqK > kMaxSeq) return fail("%s: a sequence exceeds 2^29 tokens", name);
+    if (nBuckets < 1 || nBuckets > kMaxBuckets) return fail("%s: %d buckets (supported: 1 to %d)", name, nBuckets, kMaxBuckets);
+    if (nOffsets < 1 || nOffsets > kMaxOffsets) return fail("%s: %d offsets (supported: 1 to %d)", name, nOffsets, kMaxOffsets);
+    if (nZero < -(1 << 30)) return fail("%s: the map's zero is below -2^30", name);   // its ends' differences fit 32 bits
+    if (nHeads > 65535) return fail("%s: more than 65535 heads", name);
+    if (!pTable || !pBuckets) return fail("%s: null pointer", name);
+    if (!pQueryPos != !pKeyPos && nSeqQ > 0 && nSeqK > 0) return fail("%s: positions of queries and keys go together", name);
+    if (!aligned4(pTable) || !aligned4(pBuckets) || !aligned4(pQueryPos) || !aligned4(pKeyPos))
+        return fail("%s: a pointer is not aligned to its elements", name);
+    p.table = pTable; p.bucketOf = pBuckets;
+    p.qPos = pQueryPos; p.kPos = pKeyPos;
+    p.nBuckets = nBuckets; p.nOffsets = nOffsets; p.zero = nZero;
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace omhip
+
+using namespace omhip;
+
+extern "C" {
+
+int omHipAttentionBiasForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                  long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                  const int* pKeyLens, int bCausal, const float* pTable, const int* pBuckets,
+                                  const int* pQueryPos, const int* pKeyPos, int nBuckets, int nOffsets, int nZero, uint16_t* pOut,
+                                  float* pLse, int nBatch, int nSeqQ, int nSeqK, int nHeads, int nKVHeads, int nHeadDim,
+                                  float fScale) {
+    const char* name = "omHipAttentionBiasForwardHalf";
+    clearError();
+    const int rc = checkSizes(name, nDtype, nLdQ, nStrideQ, nLdKV, nStrideKV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                              nHeadDim, fScale, false);
+    AttnBiasParams p{};
+    if (rc < 0 ||
+        biasArguments(p, name, pTable, pBuckets, pQueryPos, pKeyPos, nBuckets, nOffsets, nZero, nSeqQ, nSeqK, nHeads))
+        return -1;
+    if (rc || nSeqQ == 0) return 0;
+    if (forwardArguments(p, name, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, pOut, pLse, nBatch,
+                         nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale) ||
+        forwardParts(p, (nSeqK + kTileKeys - 1) / kTileKeys))
+        return -1;
+    return nDtype == 1 ? forward<true, kAtBias>(p) : forward<false, kAtBias>(p);
+}
+
+int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
+                                   long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
+                                   const int* pKeyLens, int bCausal, const float* pTable, const int* pBuckets,
+                                   const int* pQueryPos, const int* pKeyPos, int nBuckets, int nOffsets, int nZero,
+                                   const uint16_t* pOut, const float* pLse, const uint16_t* pGradOut, uint16_t* pGradQ,
+                                   uint16_t* pGradK, uint16_t* pGradV, float* pGradTable, int nBatch, int nSeqQ, int nSeqK,
+                                   int nHeads, int nKVHeads, int nHeadDim, float fScale) {
+    const char* name = "omHipAttentionBiasBackwardHalf";
+    clearError();
+    const int rc = checkSizes(name, nDtype, nLdQ, nStrideQ, nLdKV, nStrideKV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads,
+                              nHeadDim, fScale, true);
+    AttnBiasParams p{};
+    if (rc < 0 ||
+        biasArguments(p, name, pTable, pBuckets, pQueryPos, pKeyPos, nBuckets, nOffsets, nZero, nSeqQ, nSeqK, nHeads))
+        return -1;
+    if (!pGradTable) return fail("%s: null pointer", name);
+    if (!aligned4(pGradTable)) return fail("%s: a pointer is not aligned to its elements", name);
+    p.gradTable = pGradTable;
+    p.H = nHeads;
+    if (rc || (nSeqQ == 0 && nSeqK == 0)) return tableGradient(p, 0);
+    if (backwardArguments(p, name, pQ, pK, pV, nLdQ, nStrideQ, nLdKV, nStrideKV, pQueryLens, pKeyLens, bCausal, pOut, pLse,
+                          pGradOut, pGradQ, pGradK, pGradV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale))
+        return -1;
+    const long long blocksQ = (nSeqQ + kBlockQ - 1) / kBlockQ, blocksK = (nSeqK + kBlockQ - 1) / kBlockQ;
+    const int tiles = (nSeqK + kTileKeys - 1) / kTileKeys;
+    p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), nHeadDim <= 64 ? 4 : 2);
+    // A workgroup of dQ keeps its sums over the images that it takes: so many groups of images that the grid has eight
+    // workgroups a CU.
+    const int parts = walkParts((long long)nBatch * nHeads * blocksQ, tiles, 2);
+    const long long each = std::max(1LL, nHeads * blocksQ * parts);   // workgroups of a group
+    p.imageGroups = (int)std::clamp<long long>(8LL * cuCount() / each, 1, nBatch);
+    const long long units = nSeqQ > 0 ? p.imageGroups * blocksQ * parts : 0;
+    if (units > INT_MAX) return fail("%s: too many blocks of queries", name);
+    const size_t tableFloats = (size_t)nHeads * nOffsets;
+    float* more = nullptr;
+    if (backwardParts(p, tiles, p.parts > 1 ? (size_t)nBatch * nKVHeads * blocksK * p.parts * kBlockQ * nHeadDim : 0,
+                      nSeqQ > 0 ? tableFloats * (2 + (size_t)units) : 0, &more))
+        return -1;
+    p.tables = more;
+    p.offsetSums = more + tableFloats;
+    p.bins = p.offsetSums + tableFloats;
+    if (nDtype == 1 ? backward<true, kAtBias>(p) : backward<false, kAtBias>(p)) return -1;
+    return tableGradient(p, (int)units);
+}
+
+}  // extern "C"

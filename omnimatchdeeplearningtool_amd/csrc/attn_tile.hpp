@@ -34,6 +34,7 @@ typedef __bf16 at_bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t at_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t at_u32x2 __attribute__((ext_vector_type(2)));
 typedef short at_i16x4 __attribute__((ext_vector_type(4)));
+typedef int at_i32x4 __attribute__((ext_vector_type(4)));
 typedef float at_f32x4 __attribute__((ext_vector_type(4)));
 typedef float at_f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* AtLdsPtr;
