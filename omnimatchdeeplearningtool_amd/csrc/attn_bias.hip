@@ -10,7 +10,7 @@
 //  * the dQ kernel, which has dS in registers, adds each to its wave's sums by
 //    offset in LDS, and leaves its workgroup's;
 //  * attn_bias_offsets_kernel adds those of a head, attn_bias_table_kernel the
-//    offsets of each bucket. All in fp32 and in an order that repeats.
+//    offsets of each bucket. All in an order that repeats.
 #include "attn_train_kernels.hpp"
 #include "../../include/omhip.h"
 
@@ -20,48 +20,65 @@ namespace omhip {
 
 namespace {
 
-constexpr int kMaxBuckets = 16384;   // attn_bias_table_kernel's sums take 64 KB of LDS
+constexpr int kMaxBuckets = 16384;   // attn_bias_table_kernel's sums take 128 KB of LDS
 constexpr int kMaxSeq = 1 << 29;     // positions stay below 2^31
 
-// offsetSums[head][o] = sum over the head's `units` rows of bins, a quarter a wave.
-__global__ __launch_bounds__(256) void attn_bias_offsets_kernel(AttnBiasParams p, int units) {
-    __shared__ float part[4][64];
+// offsetSums[head][o] = sum over the head's `units` rows of bins, a sixteenth a wave.
+__global__ __launch_bounds__(1024) void attn_bias_offsets_kernel(AttnBiasParams p, int units) {
+    __shared__ double part[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int o = (int)blockIdx.x * 64 + lane, head = (int)blockIdx.y;
-    const int first = (int)((long long)units * wave / 4), last = (int)((long long)units * (wave + 1) / 4);
-    float s = 0.f;
+    const int first = (int)((long long)units * wave / 16), last = (int)((long long)units * (wave + 1) / 16);
+    double s = 0.;
     if (o < p.nOffsets) {
         const float* from = p.bins + (long long)head * units * p.nOffsets + o;
 #pragma unroll 8
-        for (int u = first; u < last; ++u) s += from[(long long)u * p.nOffsets];
+        for (int u = first; u < last; ++u) s += (double)from[(long long)u * p.nOffsets];
     }
     part[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && o < p.nOffsets)
-        p.offsetSums[(long long)head * p.nOffsets + o] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    if (wave == 0 && o < p.nOffsets) {
+        s = 0.;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s += part[k][lane];
+        p.offsetSums[(long long)head * p.nOffsets + o] = (float)s;
+    }
 }
 
-// gradTable[bucket][head] = sum of the offsets in the bucket, added by one wave.
+// gradTable[bucket][head] = sum of the offsets in the bucket, added by one wave, a few loads ahead.
 __global__ __launch_bounds__(256) void attn_bias_table_kernel(AttnBiasParams p, int empty) {
-    extern __shared__ float biases[];   // [nBuckets]
+    extern __shared__ double bucketSums[];   // [nBuckets]
     const int head = (int)blockIdx.x;
-    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) biases[b] = 0.f;
+    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) bucketSums[b] = 0.;
     __syncthreads();
-    if (threadIdx.x < 64 && !empty)
-        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 64) {
-            const int b = p.bucketOf[o];
-            if ((uint32_t)b < (uint32_t)p.nBuckets) atAdd(biases + b, p.offsetSums[(long long)head * p.nOffsets + o]);
+    if (threadIdx.x < 64 && !empty) {
+        const float* from = p.offsetSums + (long long)head * p.nOffsets;
+        constexpr int N = 8;
+        for (int o0 = (int)threadIdx.x; o0 < p.nOffsets; o0 += 64 * N) {
+            int b[N];
+            float v[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int o = min(o0 + 64 * k, p.nOffsets - 1);
+                b[k] = o0 + 64 * k < p.nOffsets ? p.bucketOf[o] : -1;
+                v[k] = from[o];
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if ((uint32_t)b[k] < (uint32_t)p.nBuckets) atAdd(bucketSums + b[k], (double)v[k]);
         }
+    }
     __syncthreads();
-    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) p.gradTable[(long long)b * p.H + head] = biases[b];
+    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) p.gradTable[(long long)b * p.H + head] = (float)bucketSums[b];
 }
 
 int tableGradient(const AttnBiasParams& p, int units) {
     if (units > 0) {
-        hipLaunchKernelGGL(attn_bias_offsets_kernel, dim3((p.nOffsets + 63) / 64, p.H), dim3(256), 0, stream(), p, units);
+        hipLaunchKernelGGL(attn_bias_offsets_kernel, dim3((p.nOffsets + 63) / 64, p.H), dim3(1024), 0, stream(), p, units);
         OMHIP_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(attn_bias_table_kernel, dim3(p.H), dim3(256), (size_t)p.nBuckets * sizeof(float), stream(), p, units == 0);
+    OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE(attn_bias_table_kernel, kMaxBuckets * sizeof(double)));
+    hipLaunchKernelGGL(attn_bias_table_kernel, dim3(p.H), dim3(256), (size_t)p.nBuckets * sizeof(double), stream(), p, units == 0);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }

@@ -160,6 +160,84 @@ __device__ __forceinline__ int atOffset(const AttnBiasParams& p, int a, int b) {
     return min(max(__builtin_elementwise_sub_sat(a, b), -p.zero), p.nOffsets - 1 - p.zero) + p.zero;
 }
 
+// The least and the largest of a wave's values.
+__device__ __forceinline__ void atRange(int v, int& least, int& most) {
+    int lo = v, hi = v;
+#define OMHIP_AT_STEP(ctrl)                                                            \
+    lo = min(lo, __builtin_amdgcn_update_dpp(lo, lo, ctrl, 0xf, 0xf, false));          \
+    hi = max(hi, __builtin_amdgcn_update_dpp(hi, hi, ctrl, 0xf, 0xf, false));
+    OMHIP_AT_STEP(0x111) OMHIP_AT_STEP(0x112) OMHIP_AT_STEP(0x114) OMHIP_AT_STEP(0x118)   // row_shr: lane 15 of each row of 16
+    OMHIP_AT_STEP(0x142) OMHIP_AT_STEP(0x143)                                             // row_bcast 15, 31: lane 63
+#undef OMHIP_AT_STEP
+    least = __builtin_amdgcn_readlane(lo, 63);
+    most = __builtin_amdgcn_readlane(hi, 63);
+}
+
+// Where the offsets of a block of pairs lie: all in the map, all at one end of it (one bias for all), or anywhere.
+enum AtOffsets { kAtInside, kAtLow, kAtHigh, kAtMixed };
+__device__ __forceinline__ AtOffsets atOffsets(const AttnBiasParams& p, int qLeast, int qMost, int kLeast, int kMost) {
+    const int least = __builtin_elementwise_sub_sat(qLeast, kMost), most = __builtin_elementwise_sub_sat(qMost, kLeast);
+    const int first = -p.zero, last = p.nOffsets - 1 - p.zero;
+    if (most <= first) return kAtLow;
+    if (least >= last) return kAtHigh;
+    return least >= first && most <= last ? kAtInside : kAtMixed;
+}
+
+// f(i, offset) of 4 N pairs, i = 0 .. 4 N - 1: positions of queries and keys are sign * (own - theirs[8 (i / 4) + i % 4]) apart.
+// `inside` knows that the offsets are in the map.
+template <int N, int SIGN, bool INSIDE, class F>
+__device__ __forceinline__ void atForOffsets(const AttnBiasParams& p, int own, const int* theirs, F&& f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const at_i32x4 pos = *reinterpret_cast<const at_i32x4*>(theirs + 8 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int q = SIGN > 0 ? own : pos[e], k = SIGN > 0 ? pos[e] : own;
+            f(4 * j + e, INSIDE ? q - k + p.zero : atOffset(p, q, k));
+        }
+    }
+}
+// x[i] = f(x[i], bias) of the same pairs.
+template <int N, int SIGN, class F>
+__device__ __forceinline__ void atAddBiases(const AttnBiasParams& p, AtOffsets kind, const float* biases, int own, const int* theirs,
+                                            F&& f) {
+    if (kind == kAtInside) {
+        atForOffsets<N, SIGN, true>(p, own, theirs, [&](int i, int o) { f(i, biases[o]); });
+    } else if (kind == kAtMixed) {
+        atForOffsets<N, SIGN, false>(p, own, theirs, [&](int i, int o) { f(i, biases[o]); });
+    } else {
+        const float b = biases[kind == kAtLow ? 0 : p.nOffsets - 1];
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) f(i, b);
+    }
+}
+
+// A wave's sums of dS by offset in LDS: [nOffsets], then a lane's own of the map's two ends, [64] each. They are of type T:
+// an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes, no two on one address), so floats are for maps
+// that leave no room for doubles. Lanes on one address are served one after another, hence the ends' own sums. A wave's
+// instructions are done in order, and lanes on one address in an order of the hardware's that repeats.
+template <class T>
+__device__ __forceinline__ void atAdd(T* at, T v) {
+    __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+template <class T, int N>
+__device__ __forceinline__ void atAddSums(const AttnBiasParams& p, AtOffsets kind, T* sums, int lane, int own, const int* theirs,
+                                          const at_f32x16& v) {
+    T* ends = sums + p.nOffsets + lane;
+    if (kind == kAtInside) {
+        atForOffsets<N, 1, true>(p, own, theirs, [&](int i, int o) { atAdd(sums + o, (T)v[i]); });
+    } else if (kind == kAtMixed) {
+        atForOffsets<N, 1, false>(p, own, theirs, [&](int i, int o) {
+            atAdd(o <= 0 ? ends : o >= p.nOffsets - 1 ? ends + 64 : sums + o, (T)v[i]);
+        });
+    } else {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) s += v[i];
+        atAdd(ends + (kind == kAtLow ? 0 : 64), (T)s);
+    }
+}
+
 // Stores a wave's 32 rows of a transposed result (the lane's column is row l; its registers hold head dimensions 32 dt +
 // 8 (r / 4) + 4 h + r % 4) times f, or zeros, as halves. Rows are turned around in `stage`, 32 rows of the wave's own in
 // LDS, and leave as whole chunks of 16 bytes, 64 / CH rows an instruction: stored from the registers, every instruction
@@ -201,14 +279,22 @@ __device__ __forceinline__ void storeColumnF32(float* row, const at_f32x16 (&acc
         }
 }
 
-// Adds to a wave's own sums in LDS: its instructions in order, lanes on one address in an order of the hardware's that repeats.
-__device__ __forceinline__ void atAdd(float* at, float v) {
-    __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+// Positions of `count` tokens from `first` on into LDS, by one wave; they are there after the next wait and barrier. Past
+// `tokens` they are 0. Without positions token t stands at t + off.
+__device__ __forceinline__ void atCopyPositions(const int* positions, int first, int count, int tokens, int off, int lane, int* to) {
+    if (!positions) {
+        if (lane < count) to[lane] = first + lane + off;
+    } else if (lane < count) {
+        const uint32_t bytes = (uint32_t)max(0, min(count, tokens - first)) * 4u;
+        atCopy4(atView(positions + first, bytes), reinterpret_cast<float*>(to), (uint32_t)lane * 4u);
+    }
 }
-
-// Positions of a tile's keys into LDS, by the first wave; they are there after the next barrier.
-__device__ __forceinline__ void atKeyPositions(const AttnBiasParams& p, int key0, int nK, int wave, int lane, int* to) {
-    if (wave == 0) to[lane] = !p.kPos ? key0 + lane : key0 + lane < nK ? p.kPos[key0 + lane] : 0;
+// The position of a lane's own token, of a wave's 32 from `first` on, and their range; past `tokens` the last one's.
+__device__ __forceinline__ int atOwnPosition(const int* positions, int token, int tokens, int off, int& least, int& most) {
+    const int t = min(token, tokens - 1);
+    const int v = !positions ? token + off : t >= 0 ? positions[t] : 0;
+    atRange(v, least, most);
+    return v;
 }
 
 // ---------------------------------------------------------------- forward
@@ -274,7 +360,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     copy.init(wave, lane, ld2, p.D);
     auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int buffer) {
         const int key0 = walk.tile<VIEW>(t) * kTileKeys;
-        if constexpr (VIEW == kAtBias) atKeyPositions(p, key0, nK, wave, lane, keyAt[buffer]);
+        if constexpr (VIEW == kAtBias)
+            if (wave == 0) atCopyPositions(p.kPos, key0, kTileKeys, nK, 0, lane, keyAt[buffer]);
         const long long at = (long long)key0 * p.ldkv;
         copy.run(kBase + at, nK - key0, ld2, p.D, kd, wave);
         copy.run(vBase + at, nK - key0, ld2, p.D, vd, wave);
@@ -284,10 +371,10 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     uint16_t* stage = (wave < 2 ? k1 : v1) + (wave & 1) * 32 * T::RS;
     T::start(p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D, nQ - q0, p.ldq, p.D, stage, lane);
     if (nt > tBegin) fetch(tBegin, k0, v0, 0);
-    int position = 0;   // the lane's query's
+    int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
     if constexpr (VIEW == kAtBias) {
         for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256) biases[o] = atBias(p, head, o);
-        position = !p.qPos ? query + off : query < nQ ? p.qPos[query] : 0;
+        position = atOwnPosition(p.qPos, query, nQ, off, qLeast, qMost);
     }
     __builtin_amdgcn_s_waitcnt(0);
     at_u32x4 qf[T::NS];
@@ -316,15 +403,13 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
         }
         atPipeline<2 * T::NS, 1, 4>();
         if constexpr (VIEW == kAtBias) {
+            int kLeast, kMost;
+            atRange(kp[lane], kLeast, kMost);
+            const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const at_i32x4 pos = *reinterpret_cast<const at_i32x4*>(kp + 32 * kb + 8 * j + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[kb][4 * j + e] = __builtin_fmaf(s[kb][4 * j + e], scaled, biases[atOffset(p, position, pos[e])]);
-                }
+                atAddBiases<4, 1>(p, kind, biases, position, kp + 32 * kb + 4 * h,
+                                  [&](int i, float b) { s[kb][i] = __builtin_fmaf(s[kb][i], scaled, b); });
         }
         if (reach.edge(key0)) {
             const AtSeen seen = reach.seen(query, key0, h);
@@ -491,7 +576,7 @@ struct DsScale {
 // dQ and dK / dV are two kernels that each compute S and dP, 7 products where one pass would need 5: sums of a row's dQ
 // over workgroups would have to be added atomically, in an order that changes, or written whole for every block of keys.
 // Measured (sizes as for the forward pass): 211-242 us by card (0.85-0.98 PFLOP/s), matrix cores busy 54 %; ViT-B/16 b64 37.
-template <bool BF16, int KD, int VIEW>
+template <bool BF16, int KD, int VIEW, class Sum>
 __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p) {
     using T = AtTile<KD>;
     __shared__ __attribute__((aligned(256))) uint16_t k0[kTileKeys * T::RS];
@@ -499,7 +584,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(16))) int keyAt[2][VIEW == kAtBias ? kTileKeys : 4];   // positions
-    extern __shared__ float biases[];   // [nOffsets], then each wave's sums of dS by offset
+    extern __shared__ float biases[];   // [nOffsets] rounded to 64, then each wave's sums of dS
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, qb;
@@ -510,15 +595,15 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     const int kvHead = head / (p.H / p.Hkv);
     const int q0 = (int)qb * kBlockQ + wave * 32;
     const int query = q0 + l;
-    float* sums = nullptr;
+    Sum* sums = nullptr;
     if constexpr (VIEW == kAtBias) {
-        sums = biases + (wave + 1) * p.nOffsets;
+        sums = reinterpret_cast<Sum*>(biases + (p.nOffsets + 63) / 64 * 64) + wave * (p.nOffsets + 128);
         for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256) {
             const float v = atBias(p, head, o);
             biases[o] = v;
             if (group == 0 && qb == 0 && part == 0) p.tables[(long long)head * p.nOffsets + o] = v;
         }
-        for (int o = lane; o < p.nOffsets; o += 64) sums[o] = 0.f;
+        for (int o = lane; o < p.nOffsets + 128; o += 64) sums[o] = 0;
     }
     int bEnd = group + 1, bStep = 1;
     if constexpr (VIEW == kAtBias) bEnd = p.B, bStep = p.imageGroups;
@@ -545,7 +630,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     copy.init(wave, lane, ld2, p.D);
     auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int buffer) {
         const int key0 = walk.tile<VIEW>(t) * kTileKeys;
-        if constexpr (VIEW == kAtBias) atKeyPositions(p, key0, nK, wave, lane, keyAt[buffer]);
+        if constexpr (VIEW == kAtBias)
+            if (wave == 0) atCopyPositions(p.kPos, key0, kTileKeys, nK, 0, lane, keyAt[buffer]);
         const long long o = (long long)key0 * p.ldkv;
         copy.run(kBase + o, nK - key0, ld2, p.D, kd, wave);
         copy.run(vBase + o, nK - key0, ld2, p.D, vd, wave);
@@ -623,9 +709,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         to[0] = shift + kRaise<BF16>;
         to[32] = delta;
     }
-    int position = 0;   // the lane's query's
-    if constexpr (VIEW == kAtBias)
-        position = !p.qPos ? query + off : query < nQ ? p.qPos[query] : 0;
+    int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
+    if constexpr (VIEW == kAtBias) position = atOwnPosition(p.qPos, query, nQ, off, qLeast, qMost);
     at_f32x16 dq[KD];
 #pragma unroll
     for (int t = 0; t < KD; ++t)
@@ -636,6 +721,12 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     auto tile = [&](auto edgeTag, int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
         constexpr bool EDGE = decltype(edgeTag)::value;   // some query does not see some of the keys
         const AtSeen seen = reach.seen(query, key0, h);
+        AtOffsets kind = kAtInside;
+        if constexpr (VIEW == kAtBias) {
+            int kLeast, kMost;
+            atRange(kp[lane], kLeast, kMost);
+            kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             if (EDGE && kb == 1 && key0 + 32 >= reach.end) break;   // the wave's queries see none of these
@@ -648,23 +739,18 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
                 dp = atMfma<BF16>(at.natural(vd, 32 * kb, st), gf[st], dp);
             }
             atPipeline<2 * T::NS, 1, 4>();
+            if constexpr (VIEW == kAtBias)
+                atAddBiases<4, 1>(p, kind, biases, position, kp + 32 * kb + 4 * h,
+                                  [&](int i, float b) { s[i] = __builtin_fmaf(s[i], c, b); });
             float most = 0.f;
-            at_i32x4 pos{};
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float x = __builtin_fmaf(s[r], c, shift);
-                int o = 0;
-                if constexpr (VIEW == kAtBias) {
-                    if (r % 4 == 0) pos = *reinterpret_cast<const at_i32x4*>(kp + 32 * kb + 2 * r + 4 * h);
-                    o = atOffset(p, position, pos[r % 4]);
-                    x += biases[o];
-                }
-                float e = __builtin_amdgcn_exp2f(x);
+                float e = __builtin_amdgcn_exp2f(VIEW == kAtBias ? s[r] + shift : __builtin_fmaf(s[r], c, shift));
                 if (EDGE && seen.hidden<VIEW>(32 * kb + 8 * (r / 4) + r % 4)) e = 0.f;
                 s[r] = e * (dp[r] - delta);
-                if constexpr (VIEW == kAtBias) atAdd(sums + o, s[r]);
                 if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
             }
+            if constexpr (VIEW == kAtBias) atAddSums<Sum, 4>(p, kind, sums, lane, position, kp + 32 * kb + 4 * h, s);
             if constexpr (!BF16) {
                 scale.update(atMaxHalves(most), dq);
 #pragma unroll
@@ -713,11 +799,23 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     if constexpr (VIEW == kAtBias) __syncthreads();   // the buffers and statistics are the next image's
     }
     if constexpr (VIEW == kAtBias) {
-        float* to = p.bins + ((((long long)head * p.imageGroups + group) * p.blocks + qb) * p.keyParts + part) * p.nOffsets;
-        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256) {
-            const float* from = biases + o;
-            to[o] = (from[p.nOffsets] + from[2 * p.nOffsets]) + (from[3 * p.nOffsets] + from[4 * p.nOffsets]);
+        // the ends' lanes, then the waves, in order
+        Sum low = sums[p.nOffsets + lane], high = sums[p.nOffsets + 64 + lane];
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) {
+            low += __shfl_xor(low, m, 64);
+            high += __shfl_xor(high, m, 64);
         }
+        if (lane == 0) {
+            sums[0] += low;
+            sums[p.nOffsets - 1] += high;
+        }
+        __syncthreads();
+        float* to = p.bins + ((((long long)head * p.imageGroups + group) * p.blocks + qb) * p.keyParts + part) * p.nOffsets;
+        const Sum* first = sums - wave * (p.nOffsets + 128);
+        const int each = p.nOffsets + 128;
+        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256)
+            to[o] = (float)((first[o] + first[o + each]) + (first[o + 2 * each] + first[o + 3 * each]));
     }
 }
 
@@ -830,8 +928,7 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     auto fetch = [&](uint16_t* qd, uint16_t* gd, float* sd, int* qp) {   // the next tile of the walk
         const long long first = (long long)fetchT * kTileQ;
         if constexpr (VIEW == kAtBias) {
-            const int query = (int)first + lane;
-            if (wave == 6 && lane < kTileQ) qp[lane] = !p.qPos ? query + off : query < nQ ? p.qPos[query] : 0;
+            if (wave == 6) atCopyPositions(p.qPos, (int)first, kTileQ, nQ, off, lane, qp);
             if (fresh) {
                 const __amdgpu_buffer_rsrc_t from = atView(p.tables + (long long)fetchHead * p.nOffsets, (uint32_t)p.nOffsets * 4u);
                 const int rounded = (p.nOffsets + 63) / 64 * 64;
@@ -860,9 +957,8 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     DsScale<BF16, KD> scale;
 
-    int position = 0;   // the lane's key's
-    if constexpr (VIEW == kAtBias)
-        position = !p.kPos ? key : key < nK ? p.kPos[key] : 0;
+    int position = 0, kLeast = 0, kMost = 0;   // the lane's key's, the wave's
+    if constexpr (VIEW == kAtBias && !SECOND) position = atOwnPosition(p.kPos, key, nK, 0, kLeast, kMost);
     if (n > 0) fetch(lds.q[0], lds.g[0], lds.stats[0], lds.queryAt[0]);
     __builtin_amdgcn_s_waitcnt(0);
     at_u32x4 own[T::NS];   // K, or V
@@ -877,17 +973,18 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         for (int st = 0; st < T::NS; ++st) s = atMfma<BF16>(at.natural(nat, 0, st), own[st], s);
         atPipeline<T::NS, 1, T::NS < 4 ? T::NS : 4>();
         if constexpr (!SECOND) {
+            if constexpr (VIEW == kAtBias) {
+                int qLeast, qMost;
+                atRange(qp[l], qLeast, qMost);
+                atAddBiases<4, -1>(p, atOffsets(p, qLeast, qMost, kLeast, kMost), biases, position, qp + 4 * h,
+                                   [&](int i, float b) { s[i] = __builtin_fmaf(s[i], c, b); });
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const at_f32x4 shift = *reinterpret_cast<const at_f32x4*>(sd + 8 * j + 4 * h);
-                at_i32x4 pos{};
-                if constexpr (VIEW == kAtBias) pos = *reinterpret_cast<const at_i32x4*>(qp + 8 * j + 4 * h);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = __builtin_fmaf(s[4 * j + e], c, shift[e]);
-                    if constexpr (VIEW == kAtBias) x += biases[atOffset(p, pos[e], position)];
-                    s[4 * j + e] = __builtin_amdgcn_exp2f(x);
-                }
+                for (int e = 0; e < 4; ++e)
+                    s[4 * j + e] = __builtin_amdgcn_exp2f(VIEW == kAtBias ? s[4 * j + e] + shift[e] : __builtin_fmaf(s[4 * j + e], c, shift[e]));
             }
             if constexpr (VIEW == kAtWindow) {
                 // rows that see the lane's key: from firstSeen on and below endSeen, a first key's with no end
@@ -1068,12 +1165,14 @@ __global__ __launch_bounds__(256) void attn_train_dkv_join_kernel(AtParams<VIEW>
 }
 
 // ---------------------------------------------------------------- launches
-constexpr int kMaxOffsets = 4096;   // of a bias: a wave's sums of dQ's workgroup take 16 KB of LDS
+// Of a bias: with the tiles of a head dimension of 128 (66 KB) a dQ workgroup has room for four waves' sums in doubles of
+// 2560 offsets, in floats of 4096.
+constexpr int kMaxOffsets = 4096, kMaxWide = 2560;
 
-// Dynamic LDS of a kernel, a bias's tables and sums.
+size_t biasLds(const AttnBiasParams& p, int tables) { return (size_t)((p.nOffsets + 63) / 64 * 64) * sizeof(float) * tables; }
 template <int VIEW>
 size_t dynamicLds(const AtParams<VIEW>& p, int tables) {
-    if constexpr (VIEW == kAtBias) return (size_t)((p.nOffsets + 63) / 64 * 64) * sizeof(float) * tables;
+    if constexpr (VIEW == kAtBias) return biasLds(p, tables);
     return 0;
 }
 #define OMHIP_AT_LDS(kernel, view, tables) \
@@ -1095,16 +1194,35 @@ int launchForward(AtParams<VIEW>& p) {
     return 0;
 }
 
+template <bool BF16, int KD, int VIEW, class Sum>
+int launchDq(const AtParams<VIEW>& p) {
+    size_t lds = 0;
+    if constexpr (VIEW == kAtBias) {
+        constexpr int most = sizeof(Sum) == 8 ? kMaxWide : kMaxOffsets;
+        lds = biasLds(p, 1) + 4 * (size_t)(p.nOffsets + 128) * sizeof(Sum);
+        OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE((attn_train_dq_kernel<BF16, KD, VIEW, Sum>),
+                                                   most * sizeof(float) + 4 * (most + 128) * sizeof(Sum)));
+    }
+    hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD, VIEW, Sum>), dim3(p.heads * p.blocks * p.keyParts), dim3(256), lds, stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
 template <bool BF16, int KD, int VIEW>
 int launchBackward(AtParams<VIEW>& p) {
     if (p.Sq > 0) {
         p.heads = (uint32_t)(p.B * p.H);
         if constexpr (VIEW == kAtBias) p.heads = (uint32_t)(p.imageGroups * p.H);
         p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
-        OMHIP_AT_LDS((attn_train_dq_kernel<BF16, KD, VIEW>), VIEW, 5);
-        hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD, VIEW>), dim3(p.heads * p.blocks * p.keyParts), dim3(256),
-                           dynamicLds<VIEW>(p, 5), stream(), p);
-        OMHIP_CHECK_LAUNCH();
+        if constexpr (VIEW == kAtBias) {
+            if (p.nOffsets <= kMaxWide) {
+                if (launchDq<BF16, KD, VIEW, double>(p)) return -1;
+            } else if (launchDq<BF16, KD, VIEW, float>(p)) {
+                return -1;
+            }
+        } else if (launchDq<BF16, KD, VIEW, float>(p)) {
+            return -1;
+        }
         if (p.keyParts > 1) {
             const long long n = (long long)p.B * p.Sq * p.H * (p.D / 8);
             hipLaunchKernelGGL((attn_train_dq_join_kernel<BF16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream(), p);
