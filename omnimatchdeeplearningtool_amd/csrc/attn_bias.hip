@@ -164,14 +164,14 @@ int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_
     p.imageGroups = (int)std::clamp<long long>(8LL * cuCount() / each, 1, nBatch);
     const long long units = nSeqQ > 0 ? p.imageGroups * blocksQ * parts : 0;
     if (units > INT_MAX) return fail("%s: too many blocks of queries", name);
-    const size_t tableFloats = (size_t)nHeads * nOffsets;
+    const size_t sumFloats = (size_t)nHeads * nOffsets, tableFloats = (size_t)nHeads * (nOffsets + 2 * kMapEnd);
     float* more = nullptr;
     if (backwardParts(p, tiles, p.parts > 1 ? (size_t)nBatch * nKVHeads * blocksK * p.parts * kBlockQ * nHeadDim : 0,
-                      nSeqQ > 0 ? tableFloats * (2 + (size_t)units) : 0, &more))
+                      nSeqQ > 0 ? tableFloats + sumFloats * (1 + (size_t)units) : 0, &more))
         return -1;
     p.tables = more;
     p.offsetSums = more + tableFloats;
-    p.bins = p.offsetSums + tableFloats;
+    p.bins = p.offsetSums + sumFloats;
     if (nDtype == 1 ? backward<true, kAtBias>(p) : backward<false, kAtBias>(p)) return -1;
     return tableGradient(p, (int)units);
 }

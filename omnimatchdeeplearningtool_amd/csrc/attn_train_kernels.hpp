@@ -78,7 +78,7 @@ struct AttnBiasParams : AttnTrainParams {
     const int *qPos, *kPos;    // [Sq], [Sk]; null: as above, and j
     int nBuckets, nOffsets, zero;
     int imageGroups;           // dQ: workgroups that share a head's block of queries over the images
-    float* tables;             // [H, nOffsets] biases by offset times log2 e, which dQ leaves for dK, dV
+    float* tables;             // [H, nOffsets + 2 kMapEnd] biases by offset times log2 e, which dQ leaves for dK, dV
     float* bins;               // [H, imageGroups * blocks * keyParts, nOffsets] sums of dS by offset
     float* offsetSums;         // [H, nOffsets]
     float* gradTable;          // [nBuckets, H]
@@ -134,7 +134,7 @@ struct AtReach {
 
 // Biases by offset in LDS, times log2 e; -inf where the table hides the key, 0 where the offset has no bucket.
 __device__ __forceinline__ float atBias(const AttnBiasParams& p, int head, int offset) {
-    const int b = p.bucketOf[offset];
+    const int b = p.bucketOf[min(max(offset, 0), p.nOffsets - 1)];
     const float v = (uint32_t)b < (uint32_t)p.nBuckets ? p.table[(long long)b * p.H + head] : 0.f;
     return v <= kNoBias ? -INFINITY : v * kAtLog2e;
 }
@@ -154,12 +154,6 @@ __device__ __forceinline__ void atWindow(const AttnWindowParams& p, int first, i
     r.window = p.window;
     r.first = p.first;
 }
-// The offset of a query's position a and a key's b, whatever they are: a difference past 32 bits is past the map too, whose
-// ends are at -zero and nOffsets - 1 - zero.
-__device__ __forceinline__ int atOffset(const AttnBiasParams& p, int a, int b) {
-    return min(max(__builtin_elementwise_sub_sat(a, b), -p.zero), p.nOffsets - 1 - p.zero) + p.zero;
-}
-
 // The least and the largest of a wave's values.
 __device__ __forceinline__ void atRange(int v, int& least, int& most) {
     int lo = v, hi = v;
@@ -173,68 +167,64 @@ __device__ __forceinline__ void atRange(int v, int& least, int& most) {
     most = __builtin_amdgcn_readlane(hi, 63);
 }
 
-// Where the offsets of a block of pairs lie: all in the map, all at one end of it (one bias for all), or anywhere.
-enum AtOffsets { kAtInside, kAtLow, kAtHigh, kAtMixed };
-__device__ __forceinline__ AtOffsets atOffsets(const AttnBiasParams& p, int qLeast, int qMost, int kLeast, int kMost) {
-    const int least = __builtin_elementwise_sub_sat(qLeast, kMost), most = __builtin_elementwise_sub_sat(qMost, kLeast);
-    const int first = -p.zero, last = p.nOffsets - 1 - p.zero;
-    if (most <= first) return kAtLow;
-    if (least >= last) return kAtHigh;
-    return least >= first && most <= last ? kAtInside : kAtMixed;
+// Arrays by offset in LDS have 64 entries more at either end, one of a lane each at least, for differences past the map:
+// lanes that add to one address are served one after another. A lane's entry is its offset taken into -64 + lane .. nOffsets +
+// lane, which leaves what is inside the map where it is, and the rest in the ends' entries.
+constexpr int kMapEnd = 64;
+__device__ __forceinline__ int atEntry(const AttnBiasParams& p, int q, int k, int lane) {
+    const int d = __builtin_elementwise_sub_sat(q, k);   // a difference past 32 bits is past the map too
+    int e;   // min(max(d, low), high): the compiler does not know that low is below high
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(e) : "v"(d), "v"(lane - kMapEnd - p.zero), "v"(p.nOffsets + lane - p.zero));
+    return e + p.zero;
 }
 
-// f(i, offset) of 4 N pairs, i = 0 .. 4 N - 1: positions of queries and keys are sign * (own - theirs[8 (i / 4) + i % 4]) apart.
-// `inside` knows that the offsets are in the map.
-template <int N, int SIGN, bool INSIDE, class F>
-__device__ __forceinline__ void atForOffsets(const AttnBiasParams& p, int own, const int* theirs, F&& f) {
+// Where the offsets of a block of pairs lie: all past one end of the map (one bias for all), or anywhere.
+enum AtOffsets { kAtLow, kAtHigh, kAtMap };
+__device__ __forceinline__ AtOffsets atOffsets(const AttnBiasParams& p, int qLeast, int qMost, int kLeast, int kMost) {
+    if (__builtin_elementwise_sub_sat(qMost, kLeast) <= -p.zero) return kAtLow;
+    return __builtin_elementwise_sub_sat(qLeast, kMost) >= p.nOffsets - 1 - p.zero ? kAtHigh : kAtMap;
+}
+
+// f(i, entry) of 16 pairs: the lane's own token, and the other side's 8 (i / 4) + i % 4 of `theirs`.
+template <bool QUERY, class F>
+__device__ __forceinline__ void atForEntries(const AttnBiasParams& p, int own, const int* theirs, int lane, F&& f) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
+    for (int j = 0; j < 4; ++j) {
         const at_i32x4 pos = *reinterpret_cast<const at_i32x4*>(theirs + 8 * j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int q = SIGN > 0 ? own : pos[e], k = SIGN > 0 ? pos[e] : own;
-            f(4 * j + e, INSIDE ? q - k + p.zero : atOffset(p, q, k));
-        }
+        for (int e = 0; e < 4; ++e) f(4 * j + e, atEntry(p, QUERY ? own : pos[e], QUERY ? pos[e] : own, lane));
     }
 }
-// x[i] = f(x[i], bias) of the same pairs.
-template <int N, int SIGN, class F>
+// x = x f + bias of the same pairs.
+template <bool QUERY>
 __device__ __forceinline__ void atAddBiases(const AttnBiasParams& p, AtOffsets kind, const float* biases, int own, const int* theirs,
-                                            F&& f) {
-    if (kind == kAtInside) {
-        atForOffsets<N, SIGN, true>(p, own, theirs, [&](int i, int o) { f(i, biases[o]); });
-    } else if (kind == kAtMixed) {
-        atForOffsets<N, SIGN, false>(p, own, theirs, [&](int i, int o) { f(i, biases[o]); });
+                                            int lane, float f, at_f32x16& x) {
+    if (kind == kAtMap) {
+        atForEntries<QUERY>(p, own, theirs, lane, [&](int i, int o) { x[i] = __builtin_fmaf(x[i], f, biases[o]); });
     } else {
         const float b = biases[kind == kAtLow ? 0 : p.nOffsets - 1];
 #pragma unroll
-        for (int i = 0; i < 4 * N; ++i) f(i, b);
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(x[i], f, b);
     }
 }
 
-// A wave's sums of dS by offset in LDS: [nOffsets], then a lane's own of the map's two ends, [64] each. They are of type T:
-// an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes, no two on one address), so floats are for maps
-// that leave no room for doubles. Lanes on one address are served one after another, hence the ends' own sums. A wave's
-// instructions are done in order, and lanes on one address in an order of the hardware's that repeats.
+// A wave's sums of dS by offset. They are of type T: an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes,
+// no two on one address), so floats are for maps that leave no room for doubles. A wave's instructions are done in order, and
+// lanes on one address in an order of the hardware's that repeats.
 template <class T>
 __device__ __forceinline__ void atAdd(T* at, T v) {
     __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
-template <class T, int N>
-__device__ __forceinline__ void atAddSums(const AttnBiasParams& p, AtOffsets kind, T* sums, int lane, int own, const int* theirs,
+template <class T>
+__device__ __forceinline__ void atAddSums(const AttnBiasParams& p, AtOffsets kind, T* sums, int own, const int* theirs, int lane,
                                           const at_f32x16& v) {
-    T* ends = sums + p.nOffsets + lane;
-    if (kind == kAtInside) {
-        atForOffsets<N, 1, true>(p, own, theirs, [&](int i, int o) { atAdd(sums + o, (T)v[i]); });
-    } else if (kind == kAtMixed) {
-        atForOffsets<N, 1, false>(p, own, theirs, [&](int i, int o) {
-            atAdd(o <= 0 ? ends : o >= p.nOffsets - 1 ? ends + 64 : sums + o, (T)v[i]);
-        });
+    if (kind == kAtMap) {
+        atForEntries<true>(p, own, theirs, lane, [&](int i, int o) { atAdd(sums + o, (T)v[i]); });
     } else {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4 * N; ++i) s += v[i];
-        atAdd(ends + (kind == kAtLow ? 0 : 64), (T)s);
+        for (int i = 0; i < 16; ++i) s += v[i];
+        atAdd(sums + (kind == kAtLow ? lane - kMapEnd : p.nOffsets + lane), (T)s);
     }
 }
 
@@ -323,7 +313,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(16))) int keyAt[2][VIEW == kAtBias ? kTileKeys : 4];   // positions
-    extern __shared__ float biases[];   // [nOffsets]
+    extern __shared__ float biasesLds[];   // [nOffsets] and the ends
+    const float* biases = biasesLds + kMapEnd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = lane & 31, h = lane >> 5;
     uint32_t bh, qb;
@@ -373,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     if (nt > tBegin) fetch(tBegin, k0, v0, 0);
     int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
     if constexpr (VIEW == kAtBias) {
-        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256) biases[o] = atBias(p, head, o);
+        for (int i = (int)threadIdx.x; i < p.nOffsets + 2 * kMapEnd; i += 256) biasesLds[i] = atBias(p, head, i - kMapEnd);
         position = atOwnPosition(p.qPos, query, nQ, off, qLeast, qMost);
     }
     __builtin_amdgcn_s_waitcnt(0);
@@ -407,9 +398,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
             atRange(kp[lane], kLeast, kMost);
             const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                atAddBiases<4, 1>(p, kind, biases, position, kp + 32 * kb + 4 * h,
-                                  [&](int i, float b) { s[kb][i] = __builtin_fmaf(s[kb][i], scaled, b); });
+            for (int kb = 0; kb < 2; ++kb) atAddBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, scaled, s[kb]);
         }
         if (reach.edge(key0)) {
             const AtSeen seen = reach.seen(query, key0, h);
@@ -584,9 +573,9 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(16))) int keyAt[2][VIEW == kAtBias ? kTileKeys : 4];   // positions
-    extern __shared__ float biases[];   // [nOffsets] rounded to 64, then each wave's sums of dS
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l = lane & 31, h = lane >> 5;
+    extern __shared__ float biasesLds[];   // [nOffsets] and the ends, rounded to 64, then each wave's sums of dS
+    const float* biases = biasesLds + kMapEnd;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t bh, qb;
     atPlace(blockIdx.x, p.heads, p.blocks * p.keyParts, p.causal, bh, qb);
     const int part = (int)(qb % (uint32_t)p.keyParts);
@@ -594,20 +583,24 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     const int group = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);   // group: the image, or of images
     const int kvHead = head / (p.H / p.Hkv);
     const int q0 = (int)qb * kBlockQ + wave * 32;
-    const int query = q0 + l;
     Sum* sums = nullptr;
     if constexpr (VIEW == kAtBias) {
-        sums = reinterpret_cast<Sum*>(biases + (p.nOffsets + 63) / 64 * 64) + wave * (p.nOffsets + 128);
-        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256) {
-            const float v = atBias(p, head, o);
-            biases[o] = v;
-            if (group == 0 && qb == 0 && part == 0) p.tables[(long long)head * p.nOffsets + o] = v;
+        const int each = p.nOffsets + 2 * kMapEnd;
+        Sum* all = reinterpret_cast<Sum*>(biasesLds + (each + 63) / 64 * 64);
+        for (int i = (int)threadIdx.x; i < each; i += 256) {
+            const float v = atBias(p, head, i - kMapEnd);
+            biasesLds[i] = v;
+            if (group == 0 && qb == 0 && part == 0) p.tables[(long long)head * each + i] = v;
         }
-        for (int o = lane; o < p.nOffsets + 128; o += 64) sums[o] = 0;
+        for (int i = (int)threadIdx.x; i < 4 * each; i += 256) all[i] = 0;   // added to after the first barrier
+        sums = all + wave * each + kMapEnd;
     }
     int bEnd = group + 1, bStep = 1;
     if constexpr (VIEW == kAtBias) bEnd = p.B, bStep = p.imageGroups;
     for (int b = group; b < bEnd; b += bStep) {
+    int lane = threadIdx.x & 63;
+    if constexpr (VIEW == kAtBias) asm volatile("" : "+v"(lane));   // else the lane's addresses are kept in 60 registers over the loop
+    const int l = lane & 31, h = lane >> 5, query = q0 + l;
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
     const int off = VIEW == kAtPlain ? p.Sk - p.Sq : nK - nQ;
     const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
@@ -721,7 +714,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     auto tile = [&](auto edgeTag, int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
         constexpr bool EDGE = decltype(edgeTag)::value;   // some query does not see some of the keys
         const AtSeen seen = reach.seen(query, key0, h);
-        AtOffsets kind = kAtInside;
+        AtOffsets kind = kAtMap;
         if constexpr (VIEW == kAtBias) {
             int kLeast, kMost;
             atRange(kp[lane], kLeast, kMost);
@@ -740,8 +733,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
             }
             atPipeline<2 * T::NS, 1, 4>();
             if constexpr (VIEW == kAtBias)
-                atAddBiases<4, 1>(p, kind, biases, position, kp + 32 * kb + 4 * h,
-                                  [&](int i, float b) { s[i] = __builtin_fmaf(s[i], c, b); });
+                atAddBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, c, s);
             float most = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -750,7 +742,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
                 s[r] = e * (dp[r] - delta);
                 if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
             }
-            if constexpr (VIEW == kAtBias) atAddSums<Sum, 4>(p, kind, sums, lane, position, kp + 32 * kb + 4 * h, s);
+            if constexpr (VIEW == kAtBias) atAddSums(p, kind, sums, position, kp + 32 * kb + 4 * h, lane, s);
             if constexpr (!BF16) {
                 scale.update(atMaxHalves(most), dq);
 #pragma unroll
@@ -799,8 +791,9 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     if constexpr (VIEW == kAtBias) __syncthreads();   // the buffers and statistics are the next image's
     }
     if constexpr (VIEW == kAtBias) {
-        // the ends' lanes, then the waves, in order
-        Sum low = sums[p.nOffsets + lane], high = sums[p.nOffsets + 64 + lane];
+        // the ends' entries, then the waves, in order
+        const int lane = threadIdx.x & 63;
+        Sum low = sums[lane - kMapEnd], high = sums[p.nOffsets + lane];
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) {
             low += __shfl_xor(low, m, 64);
@@ -812,8 +805,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         }
         __syncthreads();
         float* to = p.bins + ((((long long)head * p.imageGroups + group) * p.blocks + qb) * p.keyParts + part) * p.nOffsets;
-        const Sum* first = sums - wave * (p.nOffsets + 128);
-        const int each = p.nOffsets + 128;
+        const int each = p.nOffsets + 2 * kMapEnd;
+        const Sum* first = sums - wave * each;
         for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256)
             to[o] = (float)((first[o] + first[o + each]) + (first[o + 2 * each] + first[o + 3 * each]));
     }
@@ -930,10 +923,10 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         if constexpr (VIEW == kAtBias) {
             if (wave == 6) atCopyPositions(p.qPos, (int)first, kTileQ, nQ, off, lane, qp);
             if (fresh) {
-                const __amdgpu_buffer_rsrc_t from = atView(p.tables + (long long)fetchHead * p.nOffsets, (uint32_t)p.nOffsets * 4u);
-                const int rounded = (p.nOffsets + 63) / 64 * 64;
-                for (int o = wave * 64; o < p.nOffsets; o += 512)
-                    atCopy4(from, lds.biases + ((fetchHead - kvHead * group) & 1) * rounded + o, (uint32_t)(o + lane) * 4u);
+                const int each = p.nOffsets + 2 * kMapEnd, rounded = (each + 63) / 64 * 64;
+                const __amdgpu_buffer_rsrc_t from = atView(p.tables + (long long)fetchHead * each, (uint32_t)each * 4u);
+                for (int i = wave * 64; i < each; i += 512)
+                    atCopy4(from, lds.biases + ((fetchHead - kvHead * group) & 1) * rounded + i, (uint32_t)(i + lane) * 4u);
             }
             fresh = false;
         }
@@ -976,8 +969,7 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
             if constexpr (VIEW == kAtBias) {
                 int qLeast, qMost;
                 atRange(qp[l], qLeast, qMost);
-                atAddBiases<4, -1>(p, atOffsets(p, qLeast, qMost, kLeast, kMost), biases, position, qp + 4 * h,
-                                   [&](int i, float b) { s[i] = __builtin_fmaf(s[i], c, b); });
+                atAddBiases<false>(p, atOffsets(p, qLeast, qMost, kLeast, kMost), biases, position, qp + 4 * h, lane, c, s);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1043,9 +1035,9 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     // queries see none of the wave's keys (the first few of a causal walk) has weights 0; leaving it out would cost
     // every trip copies of the sums.
     int t = per > 0 ? t0 + begin % per : 0;   // the wave's next tile
-    const float* biases = lds.biases;
+    const float* biases = lds.biases + kMapEnd;   // of the tile's head
     if constexpr (VIEW == kAtBias && !SECOND)
-        if (per > 0 && (begin / per & 1)) biases += (p.nOffsets + 63) / 64 * 64;
+        if (per > 0 && (begin / per & 1)) biases += (p.nOffsets + 2 * kMapEnd + 63) / 64 * 64;
     auto meet = [&](int i, auto bufTag) {
         constexpr int NEXT = (decltype(bufTag)::value + 1) % 3;
         __builtin_amdgcn_s_waitcnt(0);
@@ -1063,8 +1055,8 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         if (++t == t1) {
             t = t0;
             if constexpr (VIEW == kAtBias && !SECOND) {
-                const int rounded = (p.nOffsets + 63) / 64 * 64;
-                biases = biases == lds.biases ? lds.biases + rounded : lds.biases;
+                const int rounded = (p.nOffsets + 2 * kMapEnd + 63) / 64 * 64;
+                biases = lds.biases + kMapEnd + (biases == lds.biases + kMapEnd ? rounded : 0);
             }
         }
     };
@@ -1121,7 +1113,7 @@ __global__ __launch_bounds__(512, 2) void attn_train_dkv_kernel(AtParams<VIEW> p
     __shared__ __attribute__((aligned(256))) float s2[2 * kTileQ];
     __shared__ __attribute__((aligned(16))) float weights[2 * 4 * kTileQ * 32];   // behind the tiles: their offsets fit a read's 16 bits
     __shared__ __attribute__((aligned(16))) int queryAt[3][VIEW == kAtBias ? kTileQ : 4];
-    extern __shared__ float biases[];   // rounded to 64, twice where a key head has several query heads
+    extern __shared__ float biases[];   // [nOffsets] and the ends, rounded to 64, twice where a key head has several query heads
     const DkvBuffers lds{{q0, q1, q2}, {g0, g1, g2}, {s0, s1, s2}, weights, {queryAt[0], queryAt[1], queryAt[2]}, biases};
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (wave < 4)
@@ -1169,14 +1161,16 @@ __global__ __launch_bounds__(256) void attn_train_dkv_join_kernel(AtParams<VIEW>
 // 2560 offsets, in floats of 4096.
 constexpr int kMaxOffsets = 4096, kMaxWide = 2560;
 
-size_t biasLds(const AttnBiasParams& p, int tables) { return (size_t)((p.nOffsets + 63) / 64 * 64) * sizeof(float) * tables; }
+size_t biasLds(const AttnBiasParams& p, int tables) {
+    return (size_t)((p.nOffsets + 2 * kMapEnd + 63) / 64 * 64) * sizeof(float) * tables;
+}
 template <int VIEW>
 size_t dynamicLds(const AtParams<VIEW>& p, int tables) {
     if constexpr (VIEW == kAtBias) return biasLds(p, tables);
     return 0;
 }
 #define OMHIP_AT_LDS(kernel, view, tables) \
-    if constexpr (view == kAtBias) OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE(kernel, kMaxOffsets * 4 * tables))
+    if constexpr (view == kAtBias) OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE(kernel, (kMaxOffsets + 2 * kMapEnd) * 4 * tables))
 
 template <bool BF16, int KD, int VIEW>
 int launchForward(AtParams<VIEW>& p) {
@@ -1199,9 +1193,9 @@ int launchDq(const AtParams<VIEW>& p) {
     size_t lds = 0;
     if constexpr (VIEW == kAtBias) {
         constexpr int most = sizeof(Sum) == 8 ? kMaxWide : kMaxOffsets;
-        lds = biasLds(p, 1) + 4 * (size_t)(p.nOffsets + 128) * sizeof(Sum);
+        lds = biasLds(p, 1) + 4 * (size_t)(p.nOffsets + 2 * kMapEnd) * sizeof(Sum);
         OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE((attn_train_dq_kernel<BF16, KD, VIEW, Sum>),
-                                                   most * sizeof(float) + 4 * (most + 128) * sizeof(Sum)));
+                                                   (most + 2 * kMapEnd) * (sizeof(float) + 4 * sizeof(Sum))));
     }
     hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD, VIEW, Sum>), dim3(p.heads * p.blocks * p.keyParts), dim3(256), lds, stream(), p);
     OMHIP_CHECK_LAUNCH();
