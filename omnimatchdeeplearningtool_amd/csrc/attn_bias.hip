@@ -67,6 +67,7 @@ __global__ __launch_bounds__(256) void attn_bias_table_kernel(AttnBiasParams p, 
             for (int k = 0; k < N; ++k)
                 if ((uint32_t)b[k] < (uint32_t)p.nBuckets) atAdd(bucketSums + b[k], (double)v[k]);
         }
+        __builtin_amdgcn_s_waitcnt(0);
     }
     __syncthreads();
     for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) p.gradTable[(long long)b * p.H + head] = (float)bucketSums[b];

@@ -185,49 +185,54 @@ __device__ __forceinline__ AtOffsets atOffsets(const AttnBiasParams& p, int qLea
     return __builtin_elementwise_sub_sat(qLeast, kMost) >= p.nOffsets - 1 - p.zero ? kAtHigh : kAtMap;
 }
 
-// f(i, entry) of 16 pairs: the lane's own token, and the other side's 8 (i / 4) + i % 4 of `theirs`.
-template <bool QUERY, class F>
+// f(i, entry) of 4 N pairs: the lane's own token, and the other side's 8 (i / 4) + i % 4 of `theirs`.
+template <bool QUERY, int N = 4, class F>
 __device__ __forceinline__ void atForEntries(const AttnBiasParams& p, int own, const int* theirs, int lane, F&& f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < N; ++j) {
         const at_i32x4 pos = *reinterpret_cast<const at_i32x4*>(theirs + 8 * j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) f(4 * j + e, atEntry(p, QUERY ? own : pos[e], QUERY ? pos[e] : own, lane));
     }
 }
-// x = x f + bias of the same pairs.
-template <bool QUERY>
-__device__ __forceinline__ void atAddBiases(const AttnBiasParams& p, AtOffsets kind, const float* biases, int own, const int* theirs,
-                                            int lane, float f, at_f32x16& x) {
+// f(i, bias) of 16 pairs.
+template <bool QUERY, class F>
+__device__ __forceinline__ void atForBiases(const AttnBiasParams& p, AtOffsets kind, const float* biases, int own, const int* theirs,
+                                            int lane, F&& f) {
     if (kind == kAtMap) {
-        atForEntries<QUERY>(p, own, theirs, lane, [&](int i, int o) { x[i] = __builtin_fmaf(x[i], f, biases[o]); });
+        atForEntries<QUERY>(p, own, theirs, lane, [&](int i, int o) { f(i, biases[o]); });
     } else {
-        const float b = biases[kind == kAtLow ? 0 : p.nOffsets - 1];
+        const float one = biases[kind == kAtLow ? 0 : p.nOffsets - 1];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(x[i], f, b);
+        for (int i = 0; i < 16; ++i) f(i, one);
     }
 }
 
 // A wave's sums of dS by offset. They are of type T: an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes,
 // no two on one address), so floats are for maps that leave no room for doubles. A wave's instructions are done in order, and
 // lanes on one address in an order of the hardware's that repeats.
-template <class T>
-__device__ __forceinline__ void atAdd(T* at, T v) {
-    __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+// Written out: before an atomic of its own the compiler waits for every copy into LDS under way. The wave waits for its adds
+// (__builtin_amdgcn_s_waitcnt) before the barrier behind which they are read.
+__device__ __forceinline__ uint32_t atLdsAddress(const void* at) {
+    return (uint32_t)reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)at);
 }
-template <class T>
-__device__ __forceinline__ void atAddSums(const AttnBiasParams& p, AtOffsets kind, T* sums, int own, const int* theirs, int lane,
-                                          const at_f32x16& v) {
-    if (kind == kAtMap) {
-        atForEntries<true>(p, own, theirs, lane, [&](int i, int o) { atAdd(sums + o, (T)v[i]); });
-    } else {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s += v[i];
-        atAdd(sums + (kind == kAtLow ? lane - kMapEnd : p.nOffsets + lane), (T)s);
-    }
-}
+__device__ __forceinline__ void atAdd(double* at, double v) { asm volatile("ds_add_f64 %0, %1" : : "v"(atLdsAddress(at)), "v"(v)); }
+__device__ __forceinline__ void atAdd(float* at, float v) { asm volatile("ds_add_f32 %0, %1" : : "v"(atLdsAddress(at)), "v"(v)); }
 
+// Values from LDS, waited for here: for arrays that the compiler cannot tell from those which copies are under way to.
+__device__ __forceinline__ float atReadOne(const float* at) {
+    float v;
+    asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(atLdsAddress(at)));
+    return v;
+}
+__device__ __forceinline__ void atReadEight(const uint32_t (&from)[8], float (&v)[8]) {
+    asm volatile("ds_read_b32 %0, %8\n\tds_read_b32 %1, %9\n\tds_read_b32 %2, %10\n\tds_read_b32 %3, %11\n\t"
+                 "ds_read_b32 %4, %12\n\tds_read_b32 %5, %13\n\tds_read_b32 %6, %14\n\tds_read_b32 %7, %15\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                 : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "v"(from[4]), "v"(from[5]), "v"(from[6]),
+                   "v"(from[7]));
+}
 // Stores a wave's 32 rows of a transposed result (the lane's column is row l; its registers hold head dimensions 32 dt +
 // 8 (r / 4) + 4 h + r % 4) times f, or zeros, as halves. Rows are turned around in `stage`, 32 rows of the wave's own in
 // LDS, and leave as whole chunks of 16 bytes, 64 / CH rows an instruction: stored from the registers, every instruction
@@ -279,10 +284,11 @@ __device__ __forceinline__ void atCopyPositions(const int* positions, int first,
         atCopy4(atView(positions + first, bytes), reinterpret_cast<float*>(to), (uint32_t)lane * 4u);
     }
 }
-// The position of a lane's own token, of a wave's 32 from `first` on, and their range; past `tokens` the last one's.
+// The position of a lane's own token and the range of the wave's; past `tokens` they go on from the last one's (on one place,
+// their lanes' adds of nothing to one sum would be served one after another).
 __device__ __forceinline__ int atOwnPosition(const int* positions, int token, int tokens, int off, int& least, int& most) {
     const int t = min(token, tokens - 1);
-    const int v = !positions ? token + off : t >= 0 ? positions[t] : 0;
+    const int v = !positions ? token + off : t >= 0 ? __builtin_elementwise_add_sat(positions[t], token - t) : 0;
     atRange(v, least, most);
     return v;
 }
@@ -312,7 +318,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     __shared__ __attribute__((aligned(256))) uint16_t v0[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
-    __shared__ __attribute__((aligned(16))) int keyAt[2][VIEW == kAtBias ? kTileKeys : 4];   // positions
+    __shared__ __attribute__((aligned(16))) int at0[VIEW == kAtBias ? kTileKeys : 4];   // positions of the keys
+    __shared__ __attribute__((aligned(16))) int at1[VIEW == kAtBias ? kTileKeys : 4];
     extern __shared__ float biasesLds[];   // [nOffsets] and the ends
     const float* biases = biasesLds + kMapEnd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -349,10 +356,10 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     typename T::template Copy<kTileKeys, kWaves> copy;
     const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
     copy.init(wave, lane, ld2, p.D);
-    auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int buffer) {
+    auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int* kp) {
         const int key0 = walk.tile<VIEW>(t) * kTileKeys;
         if constexpr (VIEW == kAtBias)
-            if (wave == 0) atCopyPositions(p.kPos, key0, kTileKeys, nK, 0, lane, keyAt[buffer]);
+            if (wave == 0) atCopyPositions(p.kPos, key0, kTileKeys, nK, 0, lane, kp);
         const long long at = (long long)key0 * p.ldkv;
         copy.run(kBase + at, nK - key0, ld2, p.D, kd, wave);
         copy.run(vBase + at, nK - key0, ld2, p.D, vd, wave);
@@ -361,7 +368,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     // the wave's queries through its part of the second pair of buffers, which tile 1 is copied to after the first barrier
     uint16_t* stage = (wave < 2 ? k1 : v1) + (wave & 1) * 32 * T::RS;
     T::start(p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D, nQ - q0, p.ldq, p.D, stage, lane);
-    if (nt > tBegin) fetch(tBegin, k0, v0, 0);
+    if (nt > tBegin) fetch(tBegin, k0, v0, at0);
     int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
     if constexpr (VIEW == kAtBias) {
         for (int i = (int)threadIdx.x; i < p.nOffsets + 2 * kMapEnd; i += 256) biasesLds[i] = atBias(p, head, i - kMapEnd);
@@ -384,7 +391,15 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     const float margin = fminf(8.f / c, FLT_MAX);
 
     auto tile = [&](int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
-        at_f32x16 s[2];
+        at_f32x16 s[2], bias[2];
+        if constexpr (VIEW == kAtBias) {   // under way while the scores are computed
+            int kLeast, kMost;
+            atRange(kp[lane], kLeast, kMost);
+            const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                atForBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, [&](int i, float b) { bias[kb][i] = b; });
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
@@ -394,11 +409,10 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
         }
         atPipeline<2 * T::NS, 1, 4>();
         if constexpr (VIEW == kAtBias) {
-            int kLeast, kMost;
-            atRange(kp[lane], kLeast, kMost);
-            const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) atAddBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, scaled, s[kb]);
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], scaled, bias[kb][r]);
         }
         if (reach.edge(key0)) {
             const AtSeen seen = reach.seen(query, key0, h);
@@ -458,19 +472,19 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     // Copies of tile t + 1 start once every wave is done with tile t - 1, whose buffers they fill, and are waited for at
     // the top of the next trip. Whole pairs of trips, then what is left: a way out of the middle would cost every trip
     // copies of the sums.
-    auto trip = [&](int t, int buffer, const uint16_t* kd, const uint16_t* vd, uint16_t* kNext, uint16_t* vNext) {
+    auto trip = [&](int t, const uint16_t* kd, const uint16_t* vd, const int* kp, uint16_t* kNext, uint16_t* vNext, int* kpNext) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (t + 1 < nt) fetch(t + 1, kNext, vNext, buffer ^ 1);
+        if (t + 1 < nt) fetch(t + 1, kNext, vNext, kpNext);
         const int key0 = walk.tile<VIEW>(t) * kTileKeys;
-        if (reach.tile(key0)) tile(key0, kd, vd, keyAt[buffer]);
+        if (reach.tile(key0)) tile(key0, kd, vd, kp);
     };
     int t = tBegin;
     for (; t + 1 < nt; t += 2) {
-        trip(t, 0, k0, v0, k1, v1);
-        trip(t + 1, 1, k1, v1, k0, v0);
+        trip(t, k0, v0, at0, k1, v1, at1);
+        trip(t + 1, k1, v1, at1, k0, v0, at0);
     }
-    if (t < nt) trip(t, 0, k0, v0, k1, v1);
+    if (t < nt) trip(t, k0, v0, at0, k1, v1, at1);
 
     sum = atSumHalves(sum);
     const bool empty = !(query < nQ) || sum == 0.f;
@@ -572,9 +586,9 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     __shared__ __attribute__((aligned(256))) uint16_t v0[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v1[kTileKeys * T::RS];
-    __shared__ __attribute__((aligned(16))) int keyAt[2][VIEW == kAtBias ? kTileKeys : 4];   // positions
+    __shared__ __attribute__((aligned(16))) int at0[VIEW == kAtBias ? kTileKeys : 4];   // positions of the keys
+    __shared__ __attribute__((aligned(16))) int at1[VIEW == kAtBias ? kTileKeys : 4];
     extern __shared__ float biasesLds[];   // [nOffsets] and the ends, rounded to 64, then each wave's sums of dS
-    const float* biases = biasesLds + kMapEnd;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t bh, qb;
     atPlace(blockIdx.x, p.heads, p.blocks * p.keyParts, p.causal, bh, qb);
@@ -595,200 +609,229 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         for (int i = (int)threadIdx.x; i < 4 * each; i += 256) all[i] = 0;   // added to after the first barrier
         sums = all + wave * each + kMapEnd;
     }
-    int bEnd = group + 1, bStep = 1;
-    if constexpr (VIEW == kAtBias) bEnd = p.B, bStep = p.imageGroups;
-    for (int b = group; b < bEnd; b += bStep) {
-    int lane = threadIdx.x & 63;
-    if constexpr (VIEW == kAtBias) asm volatile("" : "+v"(lane));   // else the lane's addresses are kept in 60 registers over the loop
-    const int l = lane & 31, h = lane >> 5, query = q0 + l;
-    const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
-    const int off = VIEW == kAtPlain ? p.Sk - p.Sq : nK - nQ;
-    const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
-    const uint16_t* vBase = p.v + (long long)b * p.skv + (long long)kvHead * p.D;
+    // One image. The arrays in dynamic LDS apart from the others (restrict): the compiler would wait for the copies under way
+    // before it touches them.
+    auto image = [&](int b, const float* __restrict__ biases, Sum* __restrict__ sums) __attribute__((always_inline)) {
+        int lane = threadIdx.x & 63;
+        if constexpr (VIEW == kAtBias) asm volatile("" : "+v"(lane));   // else the lane's addresses are kept in 60 registers over the loop
+        const int l = lane & 31, h = lane >> 5, query = q0 + l;
+        const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
+        const int off = VIEW == kAtPlain ? p.Sk - p.Sq : nK - nQ;
+        const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
+        const uint16_t* vBase = p.v + (long long)b * p.skv + (long long)kvHead * p.D;
 
-    const int blockLast = min((int)qb * kBlockQ + kBlockQ, nQ) - 1;
-    int kEnd = blockLast >= (int)qb * kBlockQ ? nK : 0;
-    if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
-    int waveEnd = q0 < nQ ? kEnd : 0;
-    if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
-    AtReach<VIEW> reach{nK, q0, off, waveEnd, 0, 0, 0, 0, p.causal != 0};
-    AtWalk walk{kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0, 0, 0};
-    if constexpr (VIEW == kAtWindow) atWindow(p, (int)qb * kBlockQ, blockLast, kEnd, reach, walk);
-    const int tBegin = (int)((long long)walk.n * part / p.keyParts), nt = (int)((long long)walk.n * (part + 1) / p.keyParts);
+        const int blockLast = min((int)qb * kBlockQ + kBlockQ, nQ) - 1;
+        int kEnd = blockLast >= (int)qb * kBlockQ ? nK : 0;
+        if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
+        int waveEnd = q0 < nQ ? kEnd : 0;
+        if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
+        AtReach<VIEW> reach{nK, q0, off, waveEnd, 0, 0, 0, 0, p.causal != 0};
+        AtWalk walk{kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0, 0, 0};
+        if constexpr (VIEW == kAtWindow) atWindow(p, (int)qb * kBlockQ, blockLast, kEnd, reach, walk);
+        const int tBegin = (int)((long long)walk.n * part / p.keyParts), nt = (int)((long long)walk.n * (part + 1) / p.keyParts);
 
-    const float c = p.scale * kAtLog2e;
-    const typename T::Lane at(lane);
-    typename T::template Copy<kTileKeys, kWaves> copy;
-    const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
-    copy.init(wave, lane, ld2, p.D);
-    auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int buffer) {
-        const int key0 = walk.tile<VIEW>(t) * kTileKeys;
-        if constexpr (VIEW == kAtBias)
-            if (wave == 0) atCopyPositions(p.kPos, key0, kTileKeys, nK, 0, lane, keyAt[buffer]);
-        const long long o = (long long)key0 * p.ldkv;
-        copy.run(kBase + o, nK - key0, ld2, p.D, kd, wave);
-        copy.run(vBase + o, nK - key0, ld2, p.D, vd, wave);
-    };
-    // Q and dO of the wave's queries, and delta. Head dimensions up to 64: by whole rows, Q through its part of the second
-    // pair of buffers, which tile 1 is copied to after the first barrier, dO through rows of its own; larger ones straight
-    // into fragments, 32 rows for 16 bytes an instruction: rows of dO's own would leave one workgroup a CU, and a head
-    // dimension of 128 is at 256 registers and 12-20 bytes of scratch without the chunks of dO and O for delta. (dO through
-    // the first pair of buffers, free until the first tile is fetched, has not been measured.)
-    constexpr bool kStaged = KD <= 2;
-    __shared__ __attribute__((aligned(256))) uint16_t gStage[kStaged ? kBlockQ * T::RS : 8];
-    __shared__ float rowDelta[kWaves][32];
-    const uint16_t* qRows = p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D;
-    const uint16_t* gRows = p.gradOut + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
-    const uint16_t* oRows = p.out + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
-    const long long ldo = (long long)p.H * p.D;
-    const long long image = (long long)b * p.H + head;
-    const float lse = query < nQ ? p.lse[image * p.Sq + query] : -INFINITY;
-    auto dot = [&](const at_u32x4& x, const at_u32x4& y, float d) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x0, x1, y0, y1;
-            atUnpack2<BF16>(x[e], x0, x1);
-            atUnpack2<BF16>(y[e], y0, y1);
-            d = __builtin_fmaf(x0, y0, d);
-            d = __builtin_fmaf(x1, y1, d);
-        }
-        return d;
-    };
-    at_u32x4 qf[T::NS], gf[T::NS];
-    float delta = 0.f;
-    if constexpr (kStaged) {
-        uint16_t *qStage = (wave < 2 ? k1 : v1) + (wave & 1) * 32 * T::RS, *dStage = gStage + wave * 32 * T::RS;
-        T::start(qRows, nQ - q0, p.ldq, p.D, qStage, lane);
-        T::start(gRows, nQ - q0, ldo, p.D, dStage, lane);
-        if (nt > tBegin) fetch(tBegin, k0, v0, 0);
-        constexpr int N = T::CH / 2;   // instructions of 64 / CH rows, a whole chunk a lane
-        at_u32x4 g[N], o[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int row = (i * 64 + lane) / T::CH, d = (i * 64 + lane) % T::CH * 8;
-            const bool in = q0 + row < nQ && d < p.D;
-            g[i] = in ? *reinterpret_cast<const at_u32x4*>(gRows + row * ldo + d) : at_u32x4{0u, 0u, 0u, 0u};
-            o[i] = in ? *reinterpret_cast<const at_u32x4*>(oRows + row * ldo + d) : at_u32x4{0u, 0u, 0u, 0u};
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float d = dot(g[i], o[i], 0.f);
-#pragma unroll
-            for (int s = T::CH / 2; s > 0; s >>= 1) d += __shfl_xor(d, s, 64);
-            if (lane % T::CH == 0) rowDelta[wave][(i * 64 + lane) / T::CH] = d;
-        }
-        __builtin_amdgcn_wave_barrier();   // the wave's own LDS operations complete in order
-        delta = rowDelta[wave][l];
-        __builtin_amdgcn_s_waitcnt(0);
-        T::take(at, qStage, qf);
-        T::take(at, dStage, gf);
-    } else {
-        if (nt > tBegin) fetch(tBegin, k0, v0, 0);
-#pragma unroll
-        for (int s = 0; s < T::NS; ++s) {
-            qf[s] = T::direct(qRows + l * p.ldq, query < nQ, s, h, p.D);
-            gf[s] = T::direct(gRows + l * ldo, query < nQ, s, h, p.D);
-            delta = dot(gf[s], T::direct(oRows + l * ldo, query < nQ, s, h, p.D), delta);
-        }
-        delta = atSumHalves(delta);
-    }
-    float shift = -INFINITY;
-    if (lse == -INFINITY)
-        delta = 0.f;
-    else
-        shift = -lse * kAtLog2e;
-    if (h == 0 && part == 0 && query < p.SqP) {
-        float* to = p.stats + 2 * (image * p.SqP + q0) + l;
-        to[0] = shift + kRaise<BF16>;
-        to[32] = delta;
-    }
-    int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
-    if constexpr (VIEW == kAtBias) position = atOwnPosition(p.qPos, query, nQ, off, qLeast, qMost);
-    at_f32x16 dq[KD];
-#pragma unroll
-    for (int t = 0; t < KD; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
-    DsScale<BF16, KD> scale;
-
-    auto tile = [&](auto edgeTag, int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
-        constexpr bool EDGE = decltype(edgeTag)::value;   // some query does not see some of the keys
-        const AtSeen seen = reach.seen(query, key0, h);
-        AtOffsets kind = kAtMap;
-        if constexpr (VIEW == kAtBias) {
-            int kLeast, kMost;
-            atRange(kp[lane], kLeast, kMost);
-            kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            if (EDGE && kb == 1 && key0 + 32 >= reach.end) break;   // the wave's queries see none of these
-            at_f32x16 s, dp;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
-#pragma unroll
-            for (int st = 0; st < T::NS; ++st) {
-                s = atMfma<BF16>(at.natural(kd, 32 * kb, st), qf[st], s);
-                dp = atMfma<BF16>(at.natural(vd, 32 * kb, st), gf[st], dp);
-            }
-            atPipeline<2 * T::NS, 1, 4>();
+        const float c = p.scale * kAtLog2e;
+        const typename T::Lane at(lane);
+        typename T::template Copy<kTileKeys, kWaves> copy;
+        const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
+        copy.init(wave, lane, ld2, p.D);
+        auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int* kp) {
+            const int key0 = walk.tile<VIEW>(t) * kTileKeys;
             if constexpr (VIEW == kAtBias)
-                atAddBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, c, s);
-            float most = 0.f;
+                if (wave == 0) atCopyPositions(p.kPos, key0, kTileKeys, nK, 0, lane, kp);
+            const long long o = (long long)key0 * p.ldkv;
+            copy.run(kBase + o, nK - key0, ld2, p.D, kd, wave);
+            copy.run(vBase + o, nK - key0, ld2, p.D, vd, wave);
+        };
+        // Q and dO of the wave's queries, and delta. Head dimensions up to 64: by whole rows, Q through its part of the second
+        // pair of buffers, which tile 1 is copied to after the first barrier, dO through rows of its own; larger ones straight
+        // into fragments, 32 rows for 16 bytes an instruction: rows of dO's own would leave one workgroup a CU, and a head
+        // dimension of 128 is at 256 registers and 12-20 bytes of scratch without the chunks of dO and O for delta. (dO through
+        // the first pair of buffers, free until the first tile is fetched, has not been measured.)
+        constexpr bool kStaged = KD <= 2;
+        __shared__ __attribute__((aligned(256))) uint16_t gStage[kStaged ? kBlockQ * T::RS : 8];
+        __shared__ float rowDelta[kWaves][32];
+        const uint16_t* qRows = p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D;
+        const uint16_t* gRows = p.gradOut + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
+        const uint16_t* oRows = p.out + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
+        const long long ldo = (long long)p.H * p.D;
+        const long long image = (long long)b * p.H + head;
+        const float lse = query < nQ ? p.lse[image * p.Sq + query] : -INFINITY;
+        auto dot = [&](const at_u32x4& x, const at_u32x4& y, float d) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float e = __builtin_amdgcn_exp2f(VIEW == kAtBias ? s[r] + shift : __builtin_fmaf(s[r], c, shift));
-                if (EDGE && seen.hidden<VIEW>(32 * kb + 8 * (r / 4) + r % 4)) e = 0.f;
-                s[r] = e * (dp[r] - delta);
-                if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
+            for (int e = 0; e < 4; ++e) {
+                float x0, x1, y0, y1;
+                atUnpack2<BF16>(x[e], x0, x1);
+                atUnpack2<BF16>(y[e], y0, y1);
+                d = __builtin_fmaf(x0, y0, d);
+                d = __builtin_fmaf(x1, y1, d);
             }
-            if constexpr (VIEW == kAtBias) atAddSums(p, kind, sums, position, kp + 32 * kb + 4 * h, lane, s);
-            if constexpr (!BF16) {
-                scale.update(atMaxHalves(most), dq);
+            return d;
+        };
+        at_u32x4 qf[T::NS], gf[T::NS];
+        float delta = 0.f;
+        if constexpr (kStaged) {
+            uint16_t *qStage = (wave < 2 ? k1 : v1) + (wave & 1) * 32 * T::RS, *dStage = gStage + wave * 32 * T::RS;
+            T::start(qRows, nQ - q0, p.ldq, p.D, qStage, lane);
+            T::start(gRows, nQ - q0, ldo, p.D, dStage, lane);
+            if (nt > tBegin) fetch(tBegin, k0, v0, at0);
+            constexpr int N = T::CH / 2;   // instructions of 64 / CH rows, a whole chunk a lane
+            at_u32x4 g[N], o[N];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= scale.f;
+            for (int i = 0; i < N; ++i) {
+                const int row = (i * 64 + lane) / T::CH, d = (i * 64 + lane) % T::CH * 8;
+                const bool in = q0 + row < nQ && d < p.D;
+                g[i] = in ? *reinterpret_cast<const at_u32x4*>(gRows + row * ldo + d) : at_u32x4{0u, 0u, 0u, 0u};
+                o[i] = in ? *reinterpret_cast<const at_u32x4*>(oRows + row * ldo + d) : at_u32x4{0u, 0u, 0u, 0u};
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const at_u32x4 df = atPack8<BF16>(s, u);
+            for (int i = 0; i < N; ++i) {
+                float d = dot(g[i], o[i], 0.f);
 #pragma unroll
-                for (int dt = 0; dt < KD; ++dt) dq[dt] = atMfma<BF16>(at.transposed(kd, 32 * kb + 16 * u, dt), df, dq[dt]);
+                for (int s = T::CH / 2; s > 0; s >>= 1) d += __shfl_xor(d, s, 64);
+                if (lane % T::CH == 0) rowDelta[wave][(i * 64 + lane) / T::CH] = d;
             }
-            atPipeline<2 * KD, 2, KD < 3 ? KD : 3>();
+            __builtin_amdgcn_wave_barrier();   // the wave's own LDS operations complete in order
+            delta = rowDelta[wave][l];
+            __builtin_amdgcn_s_waitcnt(0);
+            T::take(at, qStage, qf);
+            T::take(at, dStage, gf);
+        } else {
+            if (nt > tBegin) fetch(tBegin, k0, v0, at0);
+#pragma unroll
+            for (int s = 0; s < T::NS; ++s) {
+                qf[s] = T::direct(qRows + l * p.ldq, query < nQ, s, h, p.D);
+                gf[s] = T::direct(gRows + l * ldo, query < nQ, s, h, p.D);
+                delta = dot(gf[s], T::direct(oRows + l * ldo, query < nQ, s, h, p.D), delta);
+            }
+            delta = atSumHalves(delta);
+        }
+        float shift = -INFINITY;
+        if (lse == -INFINITY)
+            delta = 0.f;
+        else
+            shift = -lse * kAtLog2e;
+        if (h == 0 && part == 0 && query < p.SqP) {
+            float* to = p.stats + 2 * (image * p.SqP + q0) + l;
+            to[0] = shift + kRaise<BF16>;
+            to[32] = delta;
+        }
+        int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
+        if constexpr (VIEW == kAtBias) position = atOwnPosition(p.qPos, query, nQ, off, qLeast, qMost);
+        at_f32x16 dq[KD];
+#pragma unroll
+        for (int t = 0; t < KD; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
+        DsScale<BF16, KD> scale;
+
+        auto tile = [&](auto edgeTag, int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
+            constexpr bool EDGE = decltype(edgeTag)::value;   // some query does not see some of the keys
+            const AtSeen seen = reach.seen(query, key0, h);
+            AtOffsets kind = kAtMap;
+            if constexpr (VIEW == kAtBias) {
+                int kLeast, kMost;
+                atRange(kp[lane], kLeast, kMost);
+                kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                if (EDGE && kb == 1 && key0 + 32 >= reach.end) break;   // the wave's queries see none of these
+                at_f32x16 s, dp, bias;
+                if constexpr (VIEW == kAtBias)   // under way while the scores are computed
+                    atForBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, [&](int i, float b) { bias[i] = b; });
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+                for (int st = 0; st < T::NS; ++st) {
+                    s = atMfma<BF16>(at.natural(kd, 32 * kb, st), qf[st], s);
+                    dp = atMfma<BF16>(at.natural(vd, 32 * kb, st), gf[st], dp);
+                }
+                atPipeline<2 * T::NS, 1, 4>();
+                float most = 0.f;
+                auto weigh = [&](int r) {
+                    float e = __builtin_amdgcn_exp2f(VIEW == kAtBias ? __builtin_fmaf(s[r], c, bias[r]) + shift : __builtin_fmaf(s[r], c, shift));
+                    if (EDGE && seen.hidden<VIEW>(32 * kb + 8 * (r / 4) + r % 4)) e = 0.f;
+                    s[r] = e * (dp[r] - delta);
+                    if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
+                };
+                if (VIEW == kAtBias && kind == kAtMap) {
+                    if constexpr (VIEW == kAtBias)
+                        atForEntries<true>(p, position, kp + 32 * kb + 4 * h, lane, [&](int i, int o) {
+                            weigh(i);
+                            atAdd(sums + o, (Sum)s[i]);
+                        });
+                    // an add between the others' arithmetic: many at once would fill the wave's counter of LDS operations
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        atValu<EDGE ? 12 : 10>();
+                        atTrans<1>();
+                        atLdsAdds<1>();
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) weigh(r);
+                    if constexpr (VIEW == kAtBias) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sum += s[r];
+                        atAdd(sums + (kind == kAtLow ? lane - kMapEnd : p.nOffsets + lane), (Sum)sum);
+                    }
+                }
+                if constexpr (!BF16) {
+                    scale.update(atMaxHalves(most), dq);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] *= scale.f;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const at_u32x4 df = atPack8<BF16>(s, u);
+#pragma unroll
+                    for (int dt = 0; dt < KD; ++dt) dq[dt] = atMfma<BF16>(at.transposed(kd, 32 * kb + 16 * u, dt), df, dq[dt]);
+                }
+                atPipeline<2 * KD, 2, KD < 3 ? KD : 3>();
+            }
+        };
+        auto step = [&](int t, const uint16_t* kd, const uint16_t* vd, const int* kp) {
+            const int key0 = walk.tile<VIEW>(t) * kTileKeys;
+            if (!reach.tile(key0)) return;
+            if (reach.edge(key0))
+                tile(std::true_type{}, key0, kd, vd, kp);
+            else
+                tile(std::false_type{}, key0, kd, vd, kp);
+        };
+        auto trip = [&](int t, const uint16_t* kd, const uint16_t* vd, const int* kp, uint16_t* kNext, uint16_t* vNext, int* kpNext) {   // as in the forward pass
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (t + 1 < nt) fetch(t + 1, kNext, vNext, kpNext);
+            step(t, kd, vd, kp);
+        };
+        int t = tBegin;
+        for (; t + 1 < nt; t += 2) {
+            trip(t, k0, v0, at0, k1, v1, at1);
+            trip(t + 1, k1, v1, at1, k0, v0, at0);
+        }
+        if (t < nt) trip(t, k0, v0, at0, k1, v1, at1);
+        const float f = p.scale * scale.undo();
+        const bool none = shift == -INFINITY;
+        if (p.keyParts > 1) {
+            if (query < p.Sq)
+                storeColumnF32<KD>(p.rowPart + ((((long long)b * p.Sq + query) * p.H + head) * p.keyParts + part) * p.D, dq, f, h,
+                                   p.D, none);
+        } else {
+            __syncthreads();   // every wave is done with the tiles
+            storeRows<BF16, KD>(p.dq + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D, p.ldq, p.Sq - q0, dq, f,
+                                none, (wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RS, lane, p.D);
         }
     };
-    auto step = [&](int t, const uint16_t* kd, const uint16_t* vd, const int* kp) {
-        const int key0 = walk.tile<VIEW>(t) * kTileKeys;
-        if (!reach.tile(key0)) return;
-        if (reach.edge(key0))
-            tile(std::true_type{}, key0, kd, vd, kp);
-        else
-            tile(std::false_type{}, key0, kd, vd, kp);
-    };
-    auto trip = [&](int t, int buffer, const uint16_t* kd, const uint16_t* vd, uint16_t* kNext, uint16_t* vNext) {   // as in the forward pass
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1, kNext, vNext, buffer ^ 1);
-        step(t, kd, vd, keyAt[buffer]);
-    };
-    int t = tBegin;
-    for (; t + 1 < nt; t += 2) {
-        trip(t, 0, k0, v0, k1, v1);
-        trip(t + 1, 1, k1, v1, k0, v0);
-    }
-    if (t < nt) trip(t, 0, k0, v0, k1, v1);
-    const float f = p.scale * scale.undo();
-    const bool none = shift == -INFINITY;
-    if (p.keyParts > 1) {
-        if (query < p.Sq)
-            storeColumnF32<KD>(p.rowPart + ((((long long)b * p.Sq + query) * p.H + head) * p.keyParts + part) * p.D, dq, f, h,
-                               p.D, none);
+    if constexpr (VIEW == kAtBias) {
+        for (int b = group; b < p.B; b += p.imageGroups) {
+            image(b, biasesLds + kMapEnd, sums);
+            __builtin_amdgcn_s_waitcnt(0);   // the wave's adds
+            __syncthreads();                 // the buffers and statistics are the next image's
+        }
     } else {
-        __syncthreads();   // every wave is done with the tiles
-        storeRows<BF16, KD>(p.dq + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D, p.ldq, p.Sq - q0, dq, f,
-                            none, (wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RS, lane, p.D);
-    }
-    if constexpr (VIEW == kAtBias) __syncthreads();   // the buffers and statistics are the next image's
+        image(group, nullptr, nullptr);
     }
     if constexpr (VIEW == kAtBias) {
         // the ends' entries, then the waves, in order
@@ -850,9 +893,8 @@ constexpr int kTileQ = 32;
 // the others and lets reads of them go ahead of it.
 struct DkvBuffers {
     uint16_t *q[3], *g[3];
-    float* stats[3];     // shift, delta
+    float* stats[3];     // shift, delta, of a bias the positions
     float* weights;      // P by tile parity and pair
-    int* queryAt[3];     // positions
     float* biases;       // by offset, of a key head's first, third ... query head and of its second ...
 };
 
@@ -918,10 +960,11 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     copyG.init(wave, lane, ldg2, p.D);
     int fetchHead = per > 0 ? kvHead * group + begin / per : 0, fetchT = per > 0 ? t0 + begin % per : 0;
     bool fresh = true;   // the next tile is the first of its head, or of the walk
-    auto fetch = [&](uint16_t* qd, uint16_t* gd, float* sd, int* qp) {   // the next tile of the walk
+    auto fetch = [&](uint16_t* qd, uint16_t* gd, float* sd) {   // the next tile of the walk
         const long long first = (long long)fetchT * kTileQ;
         if constexpr (VIEW == kAtBias) {
-            if (wave == 6) atCopyPositions(p.qPos, (int)first, kTileQ, nQ, off, lane, qp);
+            if (wave == 6)
+                atCopyPositions(p.qPos, (int)first, kTileQ, nQ, off, lane, reinterpret_cast<int*>(sd + 2 * kTileQ));
             if (fresh) {
                 const int each = p.nOffsets + 2 * kMapEnd, rounded = (each + 63) / 64 * 64;
                 const __amdgpu_buffer_rsrc_t from = atView(p.tables + (long long)fetchHead * each, (uint32_t)each * 4u);
@@ -952,13 +995,13 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
 
     int position = 0, kLeast = 0, kMost = 0;   // the lane's key's, the wave's
     if constexpr (VIEW == kAtBias && !SECOND) position = atOwnPosition(p.kPos, key, nK, 0, kLeast, kMost);
-    if (n > 0) fetch(lds.q[0], lds.g[0], lds.stats[0], lds.queryAt[0]);
+    if (n > 0) fetch(lds.q[0], lds.g[0], lds.stats[0]);
     __builtin_amdgcn_s_waitcnt(0);
     at_u32x4 own[T::NS];   // K, or V
     T::take(at, stage, own);
 
     // nat: the tile whose product with the wave's own fragments makes S or dP; tr: the one that the sums take
-    auto work = [&](int first, const uint16_t* nat, const uint16_t* tr, const float* sd, float* wd, const int* qp, const float* biases) {
+    auto work = [&](int first, const uint16_t* nat, const uint16_t* tr, const float* sd, float* wd, const float* biases) {
         at_f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
@@ -967,9 +1010,26 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         atPipeline<T::NS, 1, T::NS < 4 ? T::NS : 4>();
         if constexpr (!SECOND) {
             if constexpr (VIEW == kAtBias) {
+                const int* qp = reinterpret_cast<const int*>(sd + 2 * kTileQ);
                 int qLeast, qMost;
                 atRange(qp[l], qLeast, qMost);
-                atAddBiases<false>(p, atOffsets(p, qLeast, qMost, kLeast, kMost), biases, position, qp + 4 * h, lane, c, s);
+                const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
+                if (kind == kAtMap) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t from[8];
+                        float b[8];
+                        atForEntries<false, 2>(p, position, qp + 16 * u + 4 * h, lane,
+                                               [&](int i, int o) { from[i] = atLdsAddress(biases + o); });
+                        atReadEight(from, b);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s[8 * u + i] = __builtin_fmaf(s[8 * u + i], c, b[i]);
+                    }
+                } else {
+                    const float b = atReadOne(biases + (kind == kAtLow ? 0 : p.nOffsets - 1));
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, b);
+                }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1042,16 +1102,16 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         constexpr int NEXT = (decltype(bufTag)::value + 1) % 3;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (i + 1 < n) fetch(lds.q[NEXT], lds.g[NEXT], lds.stats[NEXT], lds.queryAt[NEXT]);
+        if (i + 1 < n) fetch(lds.q[NEXT], lds.g[NEXT], lds.stats[NEXT]);
     };
     auto trip = [&](int i, auto bufTag) {
         constexpr int BUF = decltype(bufTag)::value, MINE = SECOND ? (BUF + 2) % 3 : BUF;
         meet(i, bufTag);
         float* wd = lds.weights + (((SECOND ? ~i : i) & 1) * 4 + pair) * (kTileQ * 32);
         if constexpr (SECOND)
-            work(t * kTileQ, lds.g[MINE], lds.q[MINE], lds.stats[MINE], wd, nullptr, nullptr);
+            work(t * kTileQ, lds.g[MINE], lds.q[MINE], lds.stats[MINE], wd, nullptr);
         else
-            work(t * kTileQ, lds.q[MINE], lds.g[MINE], lds.stats[MINE], wd, lds.queryAt[MINE], biases);
+            work(t * kTileQ, lds.q[MINE], lds.g[MINE], lds.stats[MINE], wd, biases);
         if (++t == t1) {
             t = t0;
             if constexpr (VIEW == kAtBias && !SECOND) {
@@ -1108,13 +1168,13 @@ __global__ __launch_bounds__(512, 2) void attn_train_dkv_kernel(AtParams<VIEW> p
     __shared__ __attribute__((aligned(256))) uint16_t g0[N];
     __shared__ __attribute__((aligned(256))) uint16_t g1[N];
     __shared__ __attribute__((aligned(256))) uint16_t g2[N];
-    __shared__ __attribute__((aligned(256))) float s0[2 * kTileQ];
-    __shared__ __attribute__((aligned(256))) float s1[2 * kTileQ];
-    __shared__ __attribute__((aligned(256))) float s2[2 * kTileQ];
+    __shared__ __attribute__((aligned(256))) float s0[(VIEW == kAtBias ? 3 : 2) * kTileQ];
+    __shared__ __attribute__((aligned(256))) float s1[(VIEW == kAtBias ? 3 : 2) * kTileQ];
+    __shared__ __attribute__((aligned(256))) float s2[(VIEW == kAtBias ? 3 : 2) * kTileQ];
     __shared__ __attribute__((aligned(16))) float weights[2 * 4 * kTileQ * 32];   // behind the tiles: their offsets fit a read's 16 bits
-    __shared__ __attribute__((aligned(16))) int queryAt[3][VIEW == kAtBias ? kTileQ : 4];
-    extern __shared__ float biases[];   // [nOffsets] and the ends, rounded to 64, twice where a key head has several query heads
-    const DkvBuffers lds{{q0, q1, q2}, {g0, g1, g2}, {s0, s1, s2}, weights, {queryAt[0], queryAt[1], queryAt[2]}, biases};
+    // [nOffsets] and the ends, rounded to 64, twice where a key head has several query heads
+    extern __shared__ float biases[];
+    const DkvBuffers lds{{q0, q1, q2}, {g0, g1, g2}, {s0, s1, s2}, weights, biases};
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (wave < 4)
         dkvWalk<BF16, KD, VIEW, false>(p, lds, wave, lane);
