@@ -158,6 +158,7 @@ int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_
     const long long blocksQ = (nSeqQ + kBlockQ - 1) / kBlockQ, blocksK = (nSeqK + kBlockQ - 1) / kBlockQ;
     const int tiles = (nSeqK + kTileKeys - 1) / kTileKeys;
     p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), nHeadDim <= 64 ? 4 : 2);
+    p.partRows = (nSeqK + kBlockQ - 1) / kBlockQ * kBlockQ;
     // A workgroup of dQ keeps its sums over the images that it takes: so many groups of images that the grid has eight
     // workgroups a CU.
     const int parts = walkParts((long long)nBatch * nHeads * blocksQ, tiles, 2);

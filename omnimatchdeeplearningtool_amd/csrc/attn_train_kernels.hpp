@@ -52,7 +52,8 @@ struct AttnTrainParams {
     int keyParts;                   // forward, dQ: of a block of queries
     float *rowPart, *lsePart;       // [B, Sq, H, keyParts, D] contexts or dQ, [B, H, Sq, keyParts] log-sum-exps
     int parts;                      // dK, dV: of a block of keys
-    float *dkPart, *dvPart;         // [B, Hkv, parts, blocks * kBlockQ, D]
+    float *dkPart, *dvPart;         // [B, Hkv, parts, partRows, D], in those workgroups' order
+    int partRows;                   // blocks * kBlockQ; of a window with one part, the first keys
     uint32_t heads, blocks;         // grid: heads x blocks workgroups
 };
 
@@ -66,8 +67,10 @@ enum AtView {
 
 struct AttnWindowParams : AttnTrainParams {
     int window, first;         // key j where |position - j| < window or j < first
-    int sinkBlocks, sinkParts; // dK, dV: blocks of keys with a first one, which every query after them sees, and their parts
-    int partUnits;             // workgroups of a key head that leave fp32 sums: of dkPart and dvPart [B, Hkv, partUnits, kBlockQ, D]
+    // dK, dV of the first keys: blocks that walk over all queries (where they are many), or else
+    // sinkParts workgroups for each 32 of them that take the queries which the blocks' walks leave out
+    int sinkBlocks, sinkParts;
+    float *sinkDk, *sinkDv;    // [B, Hkv, sinkParts, first keys rounded to 32, D]
 };
 
 constexpr float kNoBias = -1e30f;   // a bias at or below hides the key
@@ -898,23 +901,21 @@ struct DkvBuffers {
     float* biases;       // by offset, of a key head's first, third ... query head and of its second ...
 };
 
-// The walk of a block of keys: its number, the share of it, and how many share it.
-struct DkvPlace {
-    int block, part, parts;
+// Tiles t0 .. t1 - 1 of an image's queries that see a key of a block.
+struct DkvTiles {
+    int t0, t1;
 };
 template <int VIEW>
-__device__ __forceinline__ DkvPlace dkvPlace(const AtParams<VIEW>& p, int unit) {
+__device__ __forceinline__ DkvTiles dkvTiles(const AtParams<VIEW>& p, int block, int nQ, int nK, int off) {
+    const int first = block * kBlockQ;
+    DkvTiles t{p.causal ? max(0, first - off) / kTileQ : 0, first < nK ? (nQ + kTileQ - 1) / kTileQ : 0};
     if constexpr (VIEW == kAtWindow) {
-        const int sinks = p.sinkBlocks * p.sinkParts;
-        if (unit < sinks) return {unit / p.sinkParts, unit % p.sinkParts, p.sinkParts};
-        return {p.sinkBlocks + (unit - sinks) / p.parts, (unit - sinks) % p.parts, p.parts};
+        if (block >= p.sinkBlocks) {
+            if (!p.causal) t.t0 = max(0, first - off - p.window + 1) / kTileQ;
+            t.t1 = min(t.t1, (max(0, first + kBlockQ - 1 - off + p.window) + kTileQ - 1) / kTileQ);
+        }
     }
-    return {unit / p.parts, unit % p.parts, p.parts};
-}
-template <int VIEW>
-__host__ __device__ __forceinline__ uint32_t dkvUnits(const AtParams<VIEW>& p) {
-    if constexpr (VIEW == kAtWindow) return (uint32_t)p.sinkBlocks * p.sinkParts + (p.blocks - p.sinkBlocks) * p.parts;
-    return p.blocks * p.parts;
+    return t;
 }
 
 // A wave's work in attn_train_dkv_kernel.
@@ -923,27 +924,22 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     using T = AtTile<KD>;
     constexpr float kLower = BF16 ? 1.f : 1.f / 32768.f;   // takes kRaise out
     const int l = lane & 31, h = lane >> 5, pair = wave & 3;
-    uint32_t bh, unit;
-    atPlace(blockIdx.x, p.heads, dkvUnits<VIEW>(p), p.causal || VIEW == kAtWindow, bh, unit);   // the first keys' walks are longest
-    const auto [block, part, parts] = dkvPlace<VIEW>(p, (int)unit);
+    uint32_t bh, block;
+    // causal, or first keys with longer walks: the first keys' walks are longest
+    atPlace(blockIdx.x, p.heads, p.blocks * p.parts, p.causal || VIEW == kAtWindow, bh, block);
+    const int part = (int)(block % (uint32_t)p.parts);
+    block /= (uint32_t)p.parts;
     const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv);
     const int group = p.H / p.Hkv;
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
     const int off = VIEW == kAtPlain ? p.Sk - p.Sq : nK - nQ;
-    const int key0 = block * kBlockQ + pair * 32;
+    const int key0 = (int)block * kBlockQ + pair * 32;
     const int key = key0 + l;
 
     // query tiles that see a key of the workgroup: t0 .. t1 of each head of the group; this part's share of them
-    int t0 = p.causal ? max(0, block * kBlockQ - off) / kTileQ : 0;
-    int t1 = block * kBlockQ < nK ? (nQ + kTileQ - 1) / kTileQ : 0;
-    if constexpr (VIEW == kAtWindow) {
-        if (block >= p.sinkBlocks) {   // first keys are seen by every query after them, the others from their window only
-            if (!p.causal) t0 = max(0, block * kBlockQ - off - p.window + 1) / kTileQ;
-            t1 = min(t1, (max(0, block * kBlockQ + kBlockQ - 1 - off + p.window) + kTileQ - 1) / kTileQ);
-        }
-    }
+    const auto [t0, t1] = dkvTiles<VIEW>(p, (int)block, nQ, nK, off);
     const int per = max(0, t1 - t0), total = per * group;
-    const int begin = (int)((long long)total * part / parts), n = (int)((long long)total * (part + 1) / parts) - begin;
+    const int begin = (int)((long long)total * part / p.parts), n = (int)((long long)total * (part + 1) / p.parts) - begin;
 
     const typename T::Lane at(lane);
     // K or V of the wave's keys through LDS that nothing is copied to, and no weights go to, before the first barrier
@@ -1149,11 +1145,13 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
         if constexpr (!SECOND) __syncthreads();   // the second waves' last trip begins; nothing is copied any more
     }
     const float f = SECOND ? p.scale * kLower * scale.undo() : kLower;
-    if (parts > 1) {
-        long long row = ((long long)bh * p.parts + part) * ((long long)p.blocks * kBlockQ) + key;
-        if constexpr (VIEW == kAtWindow) row = ((long long)bh * p.partUnits + unit) * kBlockQ + pair * 32 + l;
+    bool part32 = p.parts > 1;   // fp32 sums for attn_train_dkv_join_kernel
+    if constexpr (VIEW == kAtWindow) part32 = part32 || key < p.partRows;
+    if (part32) {
+        const long long row = ((long long)bh * p.parts + part) * p.partRows + key;
         storeColumnF32<KD>((SECOND ? p.dkPart : p.dvPart) + row * p.D, acc, f, h, p.D, false);
-    } else {
+    }
+    if (p.parts == 1) {
         __syncthreads();   // every wave is done with the tiles and the weights
         storeRows<BF16, KD>((SECOND ? p.dk : p.dv) + first, p.ldkv, p.Sk - key0, acc, f, key >= nK, stage, lane, p.D);
     }
@@ -1182,7 +1180,7 @@ __global__ __launch_bounds__(512, 2) void attn_train_dkv_kernel(AtParams<VIEW> p
         dkvWalk<BF16, KD, VIEW, true>(p, lds, wave, lane);
 }
 
-// The parts' sums of dK (blockIdx.y 0) or dV (1), eight values of a key a thread. A window: of the keys in blocks with parts.
+// The parts' sums of dK (blockIdx.y 0) or dV (1), eight values of a key a thread, of the first `keys`.
 template <bool BF16, int VIEW>
 __global__ __launch_bounds__(256) void attn_train_dkv_join_kernel(AtParams<VIEW> p, int keys) {
     const int chunks = p.D / 8;
@@ -1193,27 +1191,168 @@ __global__ __launch_bounds__(256) void attn_train_dkv_join_kernel(AtParams<VIEW>
     const int kvHead = (int)(bkh % p.Hkv);
     const int key = (int)(bkh / p.Hkv % keys), b = (int)(bkh / p.Hkv / keys);
     const long long bh = (long long)b * p.Hkv + kvHead;
-    int parts = p.parts;
-    long long rows = (long long)p.blocks * kBlockQ, row = bh * parts * rows + key;   // between parts; the first one
-    if constexpr (VIEW == kAtWindow) {
-        const int block = key / kBlockQ, after = block - p.sinkBlocks;
-        const int unit = after < 0 ? block * p.sinkParts : p.sinkBlocks * p.sinkParts + after * p.parts;
-        if (after < 0) parts = p.sinkParts;
-        if (parts == 1) return;   // the block's only walk has left its results
-        rows = kBlockQ;
-        row = (bh * p.partUnits + unit) * kBlockQ + key % kBlockQ;
-    }
-    const float* from = (blockIdx.y ? p.dvPart : p.dkPart) + row * p.D + c * 8;
     at_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int part = 0; part < parts; ++part)
+    auto add = [&](const float* from, long long rows, int parts) {
+        from += (bh * parts * rows + key) * p.D + c * 8;
+#pragma unroll 4
+        for (int part = 0; part < parts; ++part)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            s[e] += *reinterpret_cast<const at_f32x4*>(from + (long long)part * rows * p.D + 4 * e);
+            for (int e = 0; e < 2; ++e)
+                s[e] += *reinterpret_cast<const at_f32x4*>(from + (long long)part * rows * p.D + 4 * e);
+    };
+    add(blockIdx.y ? p.dvPart : p.dkPart, p.partRows, p.parts);
+    if constexpr (VIEW == kAtWindow)
+        if (p.sinkParts > 0 && key < p.first) add(blockIdx.y ? p.sinkDv : p.sinkDk, (p.first + 31) / 32 * 32, p.sinkParts);
     at_u32x4 v = {atPack2<BF16>(s[0][0], s[0][1]), atPack2<BF16>(s[0][2], s[0][3]), atPack2<BF16>(s[1][0], s[1][1]),
                   atPack2<BF16>(s[1][2], s[1][3])};
     if (key >= atLength(p.kLens, b, p.Sk)) v = at_u32x4{0u, 0u, 0u, 0u};
     uint16_t* to = (blockIdx.y ? p.dv : p.dk) + (long long)b * p.skv + (long long)key * p.ldkv + (long long)kvHead * p.D;
     *reinterpret_cast<at_u32x4*>(to + c * 8) = v;
+}
+
+// ---------------------------------------------------------------- backward: dK and dV of a window's first keys
+// Every query after a first key sees it, the other keys of its block only those in their windows: the block's walk leaves out
+// the far queries' tiles, which these workgroups take for 32 keys at a time. A wave has tiles of its own: S = Q K^T, dP = dO
+// V^T, dV^T += dO^T P, dK^T += Q^T dS, with K, V and both sums in its registers; the next tile's Q and dO land in the wave's
+// other buffers meanwhile. The waves' sums are added in order and left in fp32, a part a workgroup, for the join.
+// Walks of whole blocks over all queries kept three of four waves at work that no key asked for: 2 x 4096 x 16 heads on 4 of
+// 128, window 512, 4 first keys: dK, dV and join @SINKS@.
+template <bool BF16, int KD>
+__global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_window_sinks_kernel(AttnWindowParams p) {
+    using T = AtTile<KD>;
+    constexpr float kLower = BF16 ? 1.f : 1.f / 32768.f;   // takes kRaise out
+    constexpr int N = kTileQ * T::RS;
+    __shared__ __attribute__((aligned(256))) uint16_t q0[4 * N];
+    __shared__ __attribute__((aligned(256))) uint16_t g0[4 * N];
+    __shared__ __attribute__((aligned(256))) uint16_t q1[4 * N];
+    __shared__ __attribute__((aligned(256))) uint16_t g1[4 * N];
+    __shared__ __attribute__((aligned(256))) float s0[4 * 2 * kTileQ];
+    __shared__ __attribute__((aligned(256))) float s1[4 * 2 * kTileQ];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = lane & 31, h = lane >> 5;
+    const int groups = (p.first + 31) / 32, part = (int)(blockIdx.x % (uint32_t)p.sinkParts);
+    const int keyGroup = (int)(blockIdx.x / (uint32_t)p.sinkParts) % groups;
+    const uint32_t bh = blockIdx.x / (uint32_t)(p.sinkParts * groups);
+    const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv);
+    const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk), off = nK - nQ;
+    const int key0 = keyGroup * 32;
+    const bool sees = key0 + l < min(p.first, nK);
+
+    // the far tiles of each head: before t0 (not causal) and from t1 on
+    const auto [t0, t1] = dkvTiles<kAtWindow>(p, key0 / kBlockQ, nQ, nK, off);
+    const int end = max(t0, t1), before = p.causal ? 0 : t0, per = key0 < nK ? before + max(0, (nQ + kTileQ - 1) / kTileQ - end) : 0;
+    const int total = per * (p.H / p.Hkv);
+
+    const typename T::Lane at(lane);
+    typename T::template Copy<kTileQ, 1> copyQ, copyG;
+    const uint32_t ldq2 = (uint32_t)p.ldq * 2u, ldg2 = (uint32_t)(p.H * p.D) * 2u;
+    copyQ.init(0, lane, ldq2, p.D);
+    copyG.init(0, lane, ldg2, p.D);
+    auto fetch = [&](int i, uint16_t* qd, uint16_t* gd, float* sd) {
+        const int head = kvHead * (p.H / p.Hkv) + i / per, x = i % per, t = x < before ? x : x - before + end;
+        const long long first = (long long)t * kTileQ;
+        copyQ.run(p.q + (long long)b * p.sq + first * p.ldq + (long long)head * p.D, nQ - (int)first, ldq2, p.D, qd + wave * N, 0);
+        copyG.run(p.gradOut + (((long long)b * p.Sq + first) * p.H + head) * p.D, nQ - (int)first, ldg2, p.D, gd + wave * N, 0);
+        atCopy4(atView(p.stats + 2 * (((long long)b * p.H + head) * p.SqP + first), 2 * kTileQ * 4), sd + wave * 2 * kTileQ, lane * 4);
+    };
+    const long long firstKey = (long long)b * p.skv + (long long)key0 * p.ldkv + (long long)kvHead * p.D;
+    T::start(p.k + firstKey, nK - key0, p.ldkv, p.D, q1 + wave * N, lane);
+    T::start(p.v + firstKey, nK - key0, p.ldkv, p.D, g1 + wave * N, lane);
+    const int step = 4 * p.sinkParts;
+    int i = part * 4 + wave;
+    if (i < total) fetch(i, q0, g0, s0);
+    __builtin_amdgcn_s_waitcnt(0);
+    at_u32x4 kf[T::NS], vf[T::NS];
+    T::take(at, q1 + wave * N, kf);
+    T::take(at, g1 + wave * N, vf);
+    __builtin_amdgcn_s_waitcnt(0);   // read before the next copies land there
+
+    const float c = p.scale * kAtLog2e;
+    at_f32x16 dk[KD], dv[KD];
+#pragma unroll
+    for (int t = 0; t < KD; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
+    DsScale<BF16, KD> scale;
+    auto tile = [&](const uint16_t* qt, const uint16_t* gt, const float* sd) {
+        at_f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+        for (int st = 0; st < T::NS; ++st) {
+            s = atMfma<BF16>(at.natural(qt, 0, st), kf[st], s);
+            dp = atMfma<BF16>(at.natural(gt, 0, st), vf[st], dp);
+        }
+        atPipeline<2 * T::NS, 1, 4>();
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const at_f32x4 shift = *reinterpret_cast<const at_f32x4*>(sd + 8 * j + 4 * h);
+            const at_f32x4 delta = *reinterpret_cast<const at_f32x4*>(sd + kTileQ + 8 * j + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * j + e;
+                s[r] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, shift[e])) : 0.f;
+                dp[r] = s[r] * (dp[r] - delta[e]);
+                if constexpr (!BF16) most = fmaxf(most, fabsf(dp[r]));
+            }
+        }
+        if constexpr (!BF16) {
+            scale.update(atMaxHalves(most), dk);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] *= scale.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const at_u32x4 pf = atPack8<BF16>(s, u), df = atPack8<BF16>(dp, u);
+#pragma unroll
+            for (int dt = 0; dt < KD; ++dt) {
+                dv[dt] = atMfma<BF16>(at.transposed(gt, 16 * u, dt), pf, dv[dt]);
+                dk[dt] = atMfma<BF16>(at.transposed(qt, 16 * u, dt), df, dk[dt]);
+            }
+        }
+        atPipeline<4 * KD, 2, KD < 3 ? KD : 3>();
+    };
+    auto trip = [&](int i, const uint16_t* qt, const uint16_t* gt, const float* st, uint16_t* qNext, uint16_t* gNext, float* sNext) {
+        if (i + step < total) fetch(i + step, qNext, gNext, sNext);
+        tile(qt + wave * N, gt + wave * N, st + wave * 2 * kTileQ);
+        __builtin_amdgcn_s_waitcnt(0);   // the next tile is here, this one read
+    };
+    for (; i + step < total; i += 2 * step) {
+        trip(i, q0, g0, s0, q1, g1, s1);
+        trip(i + step, q1, g1, s1, q0, g0, s0);
+    }
+    if (i < total) trip(i, q0, g0, s0, q1, g1, s1);
+
+    // the waves' sums, in order, then the rows that are first keys
+    const float fk = p.scale * kLower * scale.undo();
+    constexpr int R = T::RS + 4;   // floats a row: the lanes' rows in different banks
+    float *sumK = reinterpret_cast<float*>(q0), *sumV = reinterpret_cast<float*>(g0);   // [32, R]
+    for (int w = 0; w < 4; ++w) {
+        __syncthreads();
+        if (wave != w || key0 + l >= p.first) continue;
+#pragma unroll
+        for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int o = l * R + 32 * dt + 2 * r + 4 * h;
+                at_f32x4 x = {dk[dt][r] * fk, dk[dt][r + 1] * fk, dk[dt][r + 2] * fk, dk[dt][r + 3] * fk};
+                at_f32x4 y = {dv[dt][r] * kLower, dv[dt][r + 1] * kLower, dv[dt][r + 2] * kLower, dv[dt][r + 3] * kLower};
+                if (w > 0) {
+                    x += *reinterpret_cast<const at_f32x4*>(sumK + o);
+                    y += *reinterpret_cast<const at_f32x4*>(sumV + o);
+                }
+                *reinterpret_cast<at_f32x4*>(sumK + o) = x;
+                *reinterpret_cast<at_f32x4*>(sumV + o) = y;
+            }
+    }
+    __syncthreads();
+    const long long to = (((long long)bh * p.sinkParts + part) * groups * 32 + key0) * p.D;
+    for (int x = (int)threadIdx.x; x < min(32, p.first - key0) * (p.D / 4); x += 256) {
+        const int row = x / (p.D / 4), d = x % (p.D / 4) * 4;
+        *reinterpret_cast<at_f32x4*>(p.sinkDk + to + (long long)row * p.D + d) = *reinterpret_cast<const at_f32x4*>(sumK + row * R + d);
+        *reinterpret_cast<at_f32x4*>(p.sinkDv + to + (long long)row * p.D + d) = *reinterpret_cast<const at_f32x4*>(sumV + row * R + d);
+    }
 }
 
 // ---------------------------------------------------------------- launches
@@ -1288,12 +1427,18 @@ int launchBackward(AtParams<VIEW>& p) {
         p.blocks = (uint32_t)((p.Sk + kBlockQ - 1) / kBlockQ);
         const int tables = p.H > p.Hkv ? 2 : 1;
         OMHIP_AT_LDS((attn_train_dkv_kernel<BF16, KD, VIEW>), VIEW, 2);
-        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD, VIEW>), dim3(p.heads * dkvUnits<VIEW>(p)), dim3(512),
+        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD, VIEW>), dim3(p.heads * p.blocks * p.parts), dim3(512),
                            dynamicLds<VIEW>(p, tables), stream(), p);
         OMHIP_CHECK_LAUNCH();
-        int keys = p.parts > 1 ? p.Sk : 0;   // the first ones, in blocks with parts
-        if constexpr (VIEW == kAtWindow)
-            if (p.parts == 1 && p.sinkParts > 1) keys = (int)std::min<long long>(p.Sk, (long long)p.sinkBlocks * kBlockQ);
+        int keys = p.parts > 1 ? p.Sk : 0;   // with fp32 sums
+        if constexpr (VIEW == kAtWindow) {
+            if (p.sinkParts > 0) {
+                hipLaunchKernelGGL((attn_window_sinks_kernel<BF16, KD>), dim3(p.heads * ((p.first + 31) / 32) * p.sinkParts),
+                                   dim3(256), 0, stream(), p);
+                OMHIP_CHECK_LAUNCH();
+            }
+            if (p.parts == 1) keys = p.partRows;
+        }
         if (keys > 0) {
             const long long n = (long long)p.B * keys * p.Hkv * (p.D / 8);
             hipLaunchKernelGGL((attn_train_dkv_join_kernel<BF16, VIEW>), dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0,

@@ -24,6 +24,22 @@ int checkWindow(const char* name, int nSeqQ, int nSeqK, int nWindow, int nFirst)
     return 0;
 }
 
+constexpr int kMaxSinks = 256;     // first keys that get workgroups of their own
+
+// Workgroups that share a block's walk of `tiles` 64-row tiles, all blocks' walks alike: those with which the last one ends
+// first where `resident` a CU run at once. A walk's start and end are as long as four tiles, the join of parts as eight.
+int evenParts(long long blocks, int tiles, int resident) {
+    const long long room = (long long)resident * cuCount();
+    int best = 1;
+    long long least = 0;
+    for (int parts = 1; parts <= std::min(16, std::max(1, tiles / 4)); ++parts) {
+        const long long rounds = (blocks * parts + room - 1) / room;
+        const long long time = rounds * ((tiles + parts - 1) / parts + 4) + (parts > 1 ? 8 : 0);
+        if (parts == 1 || time < least) best = parts, least = time;
+    }
+    return best;
+}
+
 // Tiles of 64 rows that a block of 128 sees through a window, of `most`.
 int windowTiles(int window, int causal, int most) {
     return (int)std::min<long long>(most, ((long long)window * (causal ? 1 : 2) + kBlockQ) / kTileKeys + 1);
@@ -76,25 +92,29 @@ int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint1
         return -1;
     p.window = std::min(nWindow, std::max(nSeqQ, nSeqK));
     p.first = std::min(nFirst, nSeqK);
-    const int group = nHeads / nKVHeads, perCu = nHeadDim <= 64 ? 4 : 2;
+    const int group = nHeads / nKVHeads, resident = nHeadDim <= 64 ? 2 : 1;
     const int allQ = p.SqP / kTileKeys, allK = (nSeqK + kTileKeys - 1) / kTileKeys;
     const long long blocks = (nSeqK + kBlockQ - 1) / kBlockQ, heads = (long long)nBatch * nKVHeads;
-    const int walk = windowTiles(p.window, p.causal, allQ) * group;   // of a block of keys
-    p.parts = walkParts(heads * blocks, walk, perCu);
-    // The first keys' blocks walk over every query after them: as many parts as make those as long as the others' walks,
-    // and no more than fill the card.
-    p.sinkBlocks = (p.first + kBlockQ - 1) / kBlockQ;
-    p.sinkParts = p.parts;
-    if (p.sinkBlocks > 0) {
-        const long long equal = (long long)allQ * group / std::max(4, walk / p.parts);
-        const long long most = 8LL * cuCount() / (heads * p.sinkBlocks);
-        p.sinkParts = (int)std::clamp<long long>(std::min(equal, most), p.parts, std::max(p.parts, 64));
+    const int walk = windowTiles(p.window, p.causal, allQ);   // of a block of keys, for each query head
+    p.parts = evenParts(heads * blocks, walk * group, resident);
+    // The first keys: by workgroups of their own, unless they are so many that their blocks may as well walk over everything,
+    // or the window is as wide as the sequences.
+    if (p.first > kMaxSinks) {
+        p.sinkBlocks = (p.first + kBlockQ - 1) / kBlockQ;
+        p.parts = walkParts(heads * blocks, allQ * group, 2 * resident);
+    } else if (p.first > 0 && p.window < std::max(nSeqQ, nSeqK)) {
+        const long long groups = heads * ((p.first + 31) / 32);
+        p.sinkParts = (int)std::clamp<long long>(std::min<long long>((long long)resident * cuCount() / groups,
+                                                                     ((long long)std::max(1, allQ - walk) * group + 3) / 4), 1, 64);
     }
-    const long long units = (long long)p.sinkBlocks * p.sinkParts + (blocks - p.sinkBlocks) * p.parts;
-    p.partUnits = (int)(p.parts > 1 ? units : p.sinkParts > 1 ? (long long)p.sinkBlocks * p.sinkParts : 0);
+    p.partRows = p.parts > 1 ? (int)blocks * kBlockQ : p.sinkParts > 0 ? p.first : 0;
+    const size_t sinks = (size_t)heads * p.sinkParts * ((p.first + 31) / 32 * 32) * nHeadDim;
+    float* more = nullptr;
     if (backwardParts(p, std::min(allK, windowTiles(p.window, p.causal, allK) + (p.first + kTileKeys - 1) / kTileKeys),
-                      (size_t)heads * p.partUnits * kBlockQ * nHeadDim, 0, nullptr))
+                      (size_t)heads * p.parts * p.partRows * nHeadDim, 2 * sinks, &more))
         return -1;
+    p.sinkDk = more;
+    p.sinkDv = more + sinks;
     return nDtype == 1 ? backward<true, kAtWindow>(p) : backward<false, kAtWindow>(p);
 }
 

@@ -220,17 +220,17 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(QkNormParams p) {
     }
 }
 
-// gradWeight of a side (blockIdx.y): the workgroups' sums of 32 columns, eight runs of workgroups added in order.
-__global__ __launch_bounds__(256) void qk_norm_join_kernel(QkNormParams p) {
-    __shared__ float part[8][32];
+// gradWeight of a side (blockIdx.y): the workgroups' sums of 32 columns, 32 runs of workgroups added in order.
+__global__ __launch_bounds__(1024) void qk_norm_join_kernel(QkNormParams p) {
+    __shared__ float part[32][32];
     const QkSide& side = p.side[blockIdx.y];
     if (!side.gradWeight) return;
     const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + lane;
     const uint32_t before = blockIdx.y ? p.side[0].blocks : 0u;
-    const uint32_t first = (uint32_t)((uint64_t)side.blocks * run / 8), last = (uint32_t)((uint64_t)side.blocks * (run + 1) / 8);
+    const uint32_t first = (uint32_t)((uint64_t)side.blocks * run / 32), last = (uint32_t)((uint64_t)side.blocks * (run + 1) / 32);
     float s = 0.f;
     if (c < p.D) {
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t k = first; k < last; ++k) s += p.partials[(long long)(before + k) * p.D + c];
     }
     part[run][lane] = s;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void qk_norm_join_kernel(QkNormParams p) {
     if (run == 0 && c < p.D) {
         s = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += part[k][lane];
+        for (int k = 0; k < 32; ++k) s += part[k][lane];
         side.gradWeight[c] = s;
     }
 }
@@ -255,7 +255,7 @@ int launch(const QkNormParams& p, bool backward) {
         OMHIP_CHECK_LAUNCH();
     }
     if (backward && (p.side[0].gradWeight || p.side[1].gradWeight)) {
-        hipLaunchKernelGGL(qk_norm_join_kernel, dim3((unsigned)((p.D + 31) / 32), 2), dim3(256), 0, stream(), p);
+        hipLaunchKernelGGL(qk_norm_join_kernel, dim3((unsigned)((p.D + 31) / 32), 2), dim3(1024), 0, stream(), p);
         OMHIP_CHECK_LAUNCH();
     }
     return 0;

@@ -131,14 +131,15 @@ def test_scales(hip, scale):
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True], ids=["both", "causal"])
 def test_a_window_over_everything_is_plain_attention(hip, causal):
-    """Bit for bit, where both walk alike."""
+    """Bit for bit where both walk alike (context, log-sum-exp, dQ); dK and dV may be shared by other numbers of workgroups."""
     for dims in ((2, 200, 200, 4, 2, 64), (1, 130, 130, 2, 2, 128)):
         c, p = Window(hip, *dims, window=10 ** 9, causal=causal, seed=4), Case(hip, *dims, causal=causal, seed=4)
         for x in (c, p):
             x.forward()
             x.backward()
-        for a, b in zip(c.results(), p.results()):
+        for a, b in zip(c.results()[:3], p.results()[:3]):
             assert np.array_equal(a, b)
+        c.check()
 
 
 @pytest.mark.gpu
