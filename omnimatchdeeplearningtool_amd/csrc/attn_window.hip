@@ -8,6 +8,7 @@
 // blocks of keys over the queries whose windows reach them, the first keys'
 // over all, by several workgroups.
 #include "attn_train_kernels.hpp"
+#include "buffer_io.hpp"
 #include "../../include/omhip.h"
 
 namespace omhip {
@@ -16,6 +17,229 @@ namespace {
 
 constexpr int kMaxSeq = 1 << 29;   // positions, and sums of one and a window, stay below 2^31
 
+// ---------------------------------------------------------------- few queries: a sequence's next tokens
+constexpr int kTokenKeys = 32, kMaxTokenParts = 64;
+
+struct TokenParams : AttnWindowParams {
+    int rows;             // queries of a key head, Sq * H / Hkv, at most 32
+    int parts;            // workgroups of a key head
+    float* partial;       // [B * Hkv, parts, rows, D + 4]: contexts, then their log-sum-exp
+    unsigned* arrivals;   // [B * Hkv], zero at rest
+};
+
+// The queries of all heads that read a key head are the 32 columns of one MFMA operand, so its keys are read once. A wave
+// takes 32 keys in sight at a time, S^T = K Q^T, running softmax, O^T += V^T P^T as in the forward kernel; nothing is shared
+// between waves before their contexts are joined in LDS, and the workgroups' by the last one to arrive, with accesses coherent
+// past the XCDs' L2s (partials have landed before the counter goes up). Bound by latency: the keys in sight of a cache are a
+// few 100 KB, which enough workgroups read at once. Measured: 16 caches of up to 8192 tokens, 16 heads on 4 of 128, window
+// 1024, 4 first keys: 12.6 us (the forward kernel and its join 27.5); one of 4096, 8 heads of 64, window 256: 7.6 (10.0).
+template <bool BF16, int KD>
+__global__ __launch_bounds__(256, 2) void attn_window_token_kernel(TokenParams p) {
+    using T = AtTile<KD>;
+    constexpr float kShift = BF16 ? 0.f : 6.f;   // as in the forward kernel
+    constexpr int N = kTokenKeys * T::RS, CHUNKS = T::RS / 4;
+    __shared__ __attribute__((aligned(256))) uint16_t tiles[4 * 2 * N];   // a wave's K and V, then its contexts [32, RS] in fp32
+    __shared__ float tops[4][32], totals[4][32];
+    __shared__ int last;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = lane & 31, h = lane >> 5;
+    const int part = (int)(blockIdx.x % (uint32_t)p.parts);
+    const uint32_t bh = blockIdx.x / (uint32_t)p.parts;
+    const int b = (int)(bh / (uint32_t)p.Hkv), kvHead = (int)(bh % (uint32_t)p.Hkv), group = p.H / p.Hkv;
+    const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk), off = nK - nQ;
+    const int token = l / group, head = kvHead * group + l % group;
+    const bool some = l < p.rows && token < nQ;
+
+    // tiles in sight: of the first keys, then of the window from the first query's on
+    const int sinkTiles = (min(p.first, nK) + kTokenKeys - 1) / kTokenKeys;
+    const int t0 = max(0, off - p.window + 1) / kTokenKeys, t1 = nQ > 0 ? (nK + kTokenKeys - 1) / kTokenKeys : 0;
+    const AtWalk walk = sinkTiles >= t0 ? AtWalk{t1, 0, 0} : AtWalk{max(0, sinkTiles + t1 - t0), sinkTiles, t0 - sinkTiles};
+    const int end = (int)((long long)walk.n * (part + 1) / p.parts);
+    int i = (int)((long long)walk.n * part / p.parts) + wave;
+
+    uint16_t *kt = tiles + wave * 2 * N, *vt = kt + N;
+    const long long kv = (long long)b * p.skv + (long long)kvHead * p.D;
+    auto fetch = [&](int key0) {
+        T::start(p.k + kv + (long long)key0 * p.ldkv, nK - key0, p.ldkv, p.D, kt, lane);
+        T::start(p.v + kv + (long long)key0 * p.ldkv, nK - key0, p.ldkv, p.D, vt, lane);
+    };
+    if (i < end) fetch(walk.tile<kAtWindow>(i) * kTokenKeys);
+    const float c = fmaxf(fabsf(p.scale * kAtLog2e), FLT_MIN);
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    const uint16_t* row = p.q + (long long)b * p.sq + (long long)token * p.ldq + (long long)head * p.D;
+    at_u32x4 qf[T::NS];
+#pragma unroll
+    for (int s = 0; s < T::NS; ++s) {
+        qf[s] = T::direct(row, some, s, h, p.D);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
+    }
+    const typename T::Lane at(lane);
+    const AtReach<kAtWindow> reach{nK, 0, off, 0, 0, 0, p.window, p.first, p.causal != 0};
+    at_f32x16 o[KD];
+#pragma unroll
+    for (int t = 0; t < KD; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+    float m = -INFINITY, sum = 0.f;
+    for (; i < end; i += 4) {
+        const int key0 = walk.tile<kAtWindow>(i) * kTokenKeys;
+        __builtin_amdgcn_s_waitcnt(0);
+        at_f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int st = 0; st < T::NS; ++st) s = atMfma<BF16>(at.natural(kt, 0, st), qf[st], s);
+        const AtSeen seen = reach.seen(token, key0, h);
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (!some || seen.hidden<kAtWindow>(8 * (r / 4) + r % 4)) s[r] = -INFINITY;
+            top = fmaxf(top, s[r]);
+        }
+        top = atMaxHalves(top);
+        const float next = fmaxf(m, top);
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
+        const float base = next == -INFINITY ? 0.f : kShift - next * c;
+        sum *= alpha;
+        m = next;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, base));
+            sum += s[r];
+        }
+#pragma unroll
+        for (int dt = 0; dt < KD; ++dt) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) o[dt] = atMfma<BF16>(at.transposed(vt, 16 * u, dt), atPack8<BF16>(s, u), o[dt]);
+        }
+        __builtin_amdgcn_s_waitcnt(0);   // the tile is read
+        if (i + 4 < end) fetch(walk.tile<kAtWindow>(i + 4) * kTokenKeys);
+    }
+    sum = atSumHalves(sum);
+    if (h == 0) {
+        tops[wave][l] = m;
+        totals[wave][l] = sum;
+    }
+    float* own = reinterpret_cast<float*>(kt);   // chunk c of 4 values of column l in slot c ^ l: a read or write hits all banks
+#pragma unroll
+    for (int dt = 0; dt < KD; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<at_f32x4*>(own + l * T::RS + ((8 * dt + r / 2 + h) ^ (l & (CHUNKS - 1))) * 4) =
+                at_f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
+    __syncthreads();
+
+    const int chunks = p.D / 4, work = p.rows * chunks;
+    auto result = [&](int column, int chunk, const at_f32x4& v, float lse) {   // a column's context and log-sum-exp
+        const int i = column / group, j = kvHead * group + column % group;
+        uint16_t* to = p.out + (((long long)b * p.Sq + i) * p.H + j) * p.D + chunk * 4;
+        *reinterpret_cast<at_u32x2*>(to) = at_u32x2{atPack2<BF16>(v[0], v[1]), atPack2<BF16>(v[2], v[3])};
+        if (chunk == 0) p.lse[((long long)b * p.H + j) * p.Sq + i] = lse;
+    };
+    const int pitch = p.D + 4;
+    const uint32_t partBytes = (uint32_t)(p.rows * pitch) * 4u;
+    const __amdgpu_buffer_rsrc_t partials = bufferRsrc(p.partial + (long long)bh * p.parts * p.rows * pitch, p.parts > 1 ? partBytes * p.parts : 0u);
+    for (int x = (int)threadIdx.x; x < work; x += 256) {
+        const int column = x / chunks, chunk = x % chunks;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w][column]);
+        float total = 0.f;
+        at_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = tops[w][column] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((tops[w][column] - top) * c);
+            total += f * totals[w][column];
+            v += f * *reinterpret_cast<const at_f32x4*>(reinterpret_cast<const float*>(tiles + w * 2 * N) + column * T::RS +
+                                                        (chunk ^ (column & (CHUNKS - 1))) * 4);
+        }
+        const bool empty = total == 0.f;
+        v *= empty ? 0.f : 1.f / total;
+        const float lse = empty ? -INFINITY : top * (c * kAtLn2) + (__logf(total) - kShift * kAtLn2);
+        if (p.parts == 1) {
+            result(column, chunk, v, lse);
+        } else {
+            const uint32_t to = (uint32_t)((part * p.rows + column) * pitch + chunk * 4) * 4u;
+            bufStore4Agent(partials, to, 0, v);
+            if (chunk == 0) bufStore1Agent(partials, to + (uint32_t)p.D * 4u, 0, lse);
+        }
+    }
+    if (p.parts == 1) return;
+    __builtin_amdgcn_s_waitcnt(0);   // this wave's partials have landed
+    __syncthreads();                 // every wave's have
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(p.arrivals + bh, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(p.parts - 1);
+    __syncthreads();
+    if (!last) return;
+    for (int x = (int)threadIdx.x; x < work; x += 256) {   // as attn_train_join_kernel, eight parts' loads at a time
+        const int column = x / chunks, chunk = x % chunks;
+        float top = -INFINITY, total = 0.f;
+        at_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int first = 0; first < p.parts; first += 8) {
+            float lse[8], most = top;
+            f32x4 part8[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {   // past the last part: out of range, no access
+                const uint32_t from = (uint32_t)(((first + k) * p.rows + column) * pitch) * 4u;
+                part8[k] = bufLoad4Agent(partials, first + k < p.parts ? from + (uint32_t)chunk * 16u : kOOB, 0);
+                lse[k] = bufLoad1Agent(partials, first + k < p.parts ? from + (uint32_t)p.D * 4u : kOOB, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (first + k >= p.parts) lse[k] = -INFINITY;
+                most = fmaxf(most, lse[k]);
+            }
+            const float from0 = most == -INFINITY ? 0.f : most, alpha = top == -INFINITY ? 0.f : __expf(top - from0);
+            total *= alpha;
+            v *= alpha;
+            top = most;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float w = __expf(lse[k] - from0);
+                total += w;
+                v += w * part8[k];
+            }
+        }
+        const bool empty = total == 0.f;
+        v *= empty ? 0.f : 1.f / total;
+        result(column, chunk, v, empty ? -INFINITY : (top == -INFINITY ? 0.f : top) + __logf(total));
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(p.arrivals + bh, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+}
+
+template <bool BF16>
+int launchToken(const TokenParams& p) {
+    const dim3 grid((uint32_t)(p.B * p.Hkv) * (uint32_t)p.parts);
+    switch ((p.D + 31) / 32) {
+        case 1: hipLaunchKernelGGL((attn_window_token_kernel<BF16, 1>), grid, dim3(256), 0, stream(), p); break;
+        case 2: hipLaunchKernelGGL((attn_window_token_kernel<BF16, 2>), grid, dim3(256), 0, stream(), p); break;
+        case 3: hipLaunchKernelGGL((attn_window_token_kernel<BF16, 3>), grid, dim3(256), 0, stream(), p); break;
+        default: hipLaunchKernelGGL((attn_window_token_kernel<BF16, 4>), grid, dim3(256), 0, stream(), p); break;
+    }
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+// Queries of few tokens: workgroups share a key head's keys in sight, 32 a wave, as far as they all run at once.
+int tokens(const AttnWindowParams& p, int nDtype) {
+    TokenParams t{};
+    static_cast<AttnWindowParams&>(t) = p;
+    t.rows = p.Sq * (p.H / p.Hkv);
+    const long long heads = (long long)p.B * p.Hkv, resident = (long long)(p.D <= 64 ? 4 : 2) * cuCount();
+    const long long seen = std::min<long long>(p.Sk, (long long)p.window + p.Sq + p.first) / kTokenKeys + 2;   // tiles
+    t.parts = (int)std::clamp<long long>(std::min((seen + 3) / 4, (resident + heads - 1) / heads), 1, kMaxTokenParts);
+    if (t.parts > 1) {
+        t.partial = static_cast<float*>(workspace((size_t)heads * t.parts * t.rows * (p.D + 4) * sizeof(float), kWsOperand));
+        t.arrivals = static_cast<unsigned*>(workspace((size_t)heads * sizeof(unsigned), kWsCounters));
+        if (!t.partial || !t.arrivals) return -1;   // workspace() recorded the cause
+    }
+    return nDtype == 1 ? launchToken<true>(t) : launchToken<false>(t);
+}
+
+// ---------------------------------------------------------------- sizes
 // Sizes past checkSizes: what a window adds; 0 or -1.
 int checkWindow(const char* name, int nSeqQ, int nSeqK, int nWindow, int nFirst) {
     if (nSeqQ > kMaxSeq || nSeqK > kMaxSeq) return fail("%s: a sequence exceeds 2^29 tokens", name);
@@ -69,6 +293,7 @@ int omHipAttentionWindowForwardHalf(int nDtype, const uint16_t* pQ, const uint16
         return -1;
     p.window = std::min(nWindow, std::max(nSeqQ, nSeqK));
     p.first = std::min(nFirst, nSeqK);
+    if ((long long)nSeqQ * (nHeads / nKVHeads) <= 32) return tokens(p, nDtype);
     const int all = (nSeqK + kTileKeys - 1) / kTileKeys;
     if (forwardParts(p, std::min(all, windowTiles(p.window, p.causal, all) + (p.first + kTileKeys - 1) / kTileKeys))) return -1;
     return nDtype == 1 ? forward<true, kAtWindow>(p) : forward<false, kAtWindow>(p);
