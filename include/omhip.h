@@ -568,7 +568,7 @@ int omHipQkNormRotaryBackward(int nDtype, const void* pGradOutQ, const void* pGr
  * Positions: pQueryPos [nSeqQ] and pKeyPos [nSeqK] int32 (any values, shared by the images), as y
  * (2 width - 1) + x for patches, whose differences tell both distances; or both NULL: in an image
  * of nQ queries and nK keys (its lengths) query i stands at i + nK - nQ, key j at j. bCausal: j <=
- * i + nK - nQ. 1 to 4096 offsets, 1 to 16384 buckets, nZero from -2^30 on, at most 2^29 tokens a
+ * i + nK - nQ. 1 to 4096 offsets, 1 to 16384 buckets, nZero within +-2^30, at most 2^29 tokens a
  * sequence. */
 int omHipAttentionBiasForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
                                   long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,

@@ -90,7 +90,7 @@ int biasArguments(AttnBiasParams& p, const char* name, const float* pTable, cons
     if (nSeqQ > kMaxSeq || nSeqK > kMaxSeq) return fail("%s: a sequence exceeds 2^29 tokens", name);
     if (nBuckets < 1 || nBuckets > kMaxBuckets) return fail("%s: %d buckets (supported: 1 to %d)", name, nBuckets, kMaxBuckets);
     if (nOffsets < 1 || nOffsets > kMaxOffsets) return fail("%s: %d offsets (supported: 1 to %d)", name, nOffsets, kMaxOffsets);
-    if (nZero < -(1 << 30)) return fail("%s: the map's zero is below -2^30", name);   // its ends' differences fit 32 bits
+    if (nZero < -(1 << 30) || nZero > 1 << 30) return fail("%s: the map's zero is past +-2^30", name);   // its ends' differences fit 32 bits
     if (nHeads > 65535) return fail("%s: more than 65535 heads", name);
     if (!pTable || !pBuckets) return fail("%s: null pointer", name);
     if (!pQueryPos != !pKeyPos && nSeqQ > 0 && nSeqK > 0) return fail("%s: positions of queries and keys go together", name);

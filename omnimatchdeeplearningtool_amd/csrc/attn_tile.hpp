@@ -106,8 +106,6 @@ __device__ __forceinline__ void atReads() { if constexpr (N > 0) __builtin_amdgc
 template <int N>
 __device__ __forceinline__ void atValu() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
 template <int N>
-__device__ __forceinline__ void atLdsAdds() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x200, N, 0); }   // and writes
-template <int N>
 __device__ __forceinline__ void atTrans() { if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x400, N, 0); }
 // N MFMAs that take `reads` LDS reads, READS a MFMA: `ahead` of them first, then one MFMA and READS reads in turn.
 template <int N, int READS, int AHEAD>

@@ -198,19 +198,6 @@ __device__ __forceinline__ void atForEntries(const AttnBiasParams& p, int own, c
         for (int e = 0; e < 4; ++e) f(4 * j + e, atEntry(p, QUERY ? own : pos[e], QUERY ? pos[e] : own, lane));
     }
 }
-// f(i, bias) of 16 pairs.
-template <bool QUERY, class F>
-__device__ __forceinline__ void atForBiases(const AttnBiasParams& p, AtOffsets kind, const float* biases, int own, const int* theirs,
-                                            int lane, F&& f) {
-    if (kind == kAtMap) {
-        atForEntries<QUERY>(p, own, theirs, lane, [&](int i, int o) { f(i, biases[o]); });
-    } else {
-        const float one = biases[kind == kAtLow ? 0 : p.nOffsets - 1];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f(i, one);
-    }
-}
-
 // A wave's sums of dS by offset. They are of type T: an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes,
 // no two on one address), so floats are for maps that leave no room for doubles. A wave's instructions are done in order, and
 // lanes on one address in an order of the hardware's that repeats.
@@ -394,15 +381,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     const float margin = fminf(8.f / c, FLT_MAX);
 
     auto tile = [&](int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
-        at_f32x16 s[2], bias[2];
-        if constexpr (VIEW == kAtBias) {   // under way while the scores are computed
-            int kLeast, kMost;
-            atRange(kp[lane], kLeast, kMost);
-            const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                atForBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, [&](int i, float b) { bias[kb][i] = b; });
-        }
+        at_f32x16 s[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
@@ -412,10 +391,21 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
         }
         atPipeline<2 * T::NS, 1, 4>();
         if constexpr (VIEW == kAtBias) {
+            int kLeast, kMost;
+            atRange(kp[lane], kLeast, kMost);
+            const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
+            if (kind == kAtMap) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < 2; ++kb)
+                    atForEntries<true>(p, position, kp + 32 * kb + 4 * h, lane,
+                                       [&](int i, int o) { s[kb][i] = __builtin_fmaf(s[kb][i], scaled, biases[o]); });
+            } else {
+                const float one = biases[kind == kAtLow ? 0 : p.nOffsets - 1];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], scaled, bias[kb][r]);
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], scaled, one);
+            }
         }
         if (reach.edge(key0)) {
             const AtSeen seen = reach.seen(query, key0, h);
@@ -728,21 +718,20 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
             for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
         DsScale<BF16, KD> scale;
 
-        auto tile = [&](auto edgeTag, int key0, const uint16_t* kd, const uint16_t* vd, const int* kp) {
+        auto tile = [&](auto edgeTag, auto mapTag, int key0, const uint16_t* kd, const uint16_t* vd, const int* kp, float one, Sum* end) {
             constexpr bool EDGE = decltype(edgeTag)::value;   // some query does not see some of the keys
+            constexpr bool MAP = VIEW == kAtBias && decltype(mapTag)::value;   // biases by pair, else one for the tile
             const AtSeen seen = reach.seen(query, key0, h);
-            AtOffsets kind = kAtMap;
-            if constexpr (VIEW == kAtBias) {
-                int kLeast, kMost;
-                atRange(kp[lane], kLeast, kMost);
-                kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
-            }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 if (EDGE && kb == 1 && key0 + 32 >= reach.end) break;   // the wave's queries see none of these
                 at_f32x16 s, dp, bias;
-                if constexpr (VIEW == kAtBias)   // under way while the scores are computed
-                    atForBiases<true>(p, kind, biases, position, kp + 32 * kb + 4 * h, lane, [&](int i, float b) { bias[i] = b; });
+                // biases are under way while the scores are computed; larger heads have no registers for them until then
+                constexpr bool kAhead = MAP && KD <= 2;
+                if constexpr (kAhead) {
+                    atForEntries<true>(p, position, kp + 32 * kb + 4 * h, lane, [&](int i, int o) { bias[i] = biases[o]; });
+                    __builtin_amdgcn_sched_barrier(0);   // the order below is for the fragments' reads
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
@@ -752,33 +741,27 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
                 }
                 atPipeline<2 * T::NS, 1, 4>();
                 float most = 0.f;
-                auto weigh = [&](int r) {
-                    float e = __builtin_amdgcn_exp2f(VIEW == kAtBias ? __builtin_fmaf(s[r], c, bias[r]) + shift : __builtin_fmaf(s[r], c, shift));
+                auto weigh = [&](int r, float b) {
+                    float x = __builtin_fmaf(s[r], c, shift);
+                    if constexpr (VIEW == kAtBias) x = __builtin_fmaf(s[r], c, b) + shift;
+                    float e = __builtin_amdgcn_exp2f(x);
                     if (EDGE && seen.hidden<VIEW>(32 * kb + 8 * (r / 4) + r % 4)) e = 0.f;
                     s[r] = e * (dp[r] - delta);
                     if constexpr (!BF16) most = fmaxf(most, fabsf(s[r]));
                 };
-                if (VIEW == kAtBias && kind == kAtMap) {
-                    if constexpr (VIEW == kAtBias)
-                        atForEntries<true>(p, position, kp + 32 * kb + 4 * h, lane, [&](int i, int o) {
-                            weigh(i);
-                            atAdd(sums + o, (Sum)s[i]);
-                        });
-                    // an add between the others' arithmetic: many at once would fill the wave's counter of LDS operations
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        atValu<EDGE ? 12 : 10>();
-                        atTrans<1>();
-                        atLdsAdds<1>();
-                    }
+                if constexpr (MAP) {
+                    atForEntries<true>(p, position, kp + 32 * kb + 4 * h, lane, [&](int i, int o) {
+                        weigh(i, kAhead ? bias[i] : biases[o]);
+                        atAdd(sums + o, (Sum)s[i]);
+                    });
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) weigh(r);
+                    for (int r = 0; r < 16; ++r) weigh(r, one);
                     if constexpr (VIEW == kAtBias) {
                         float sum = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) sum += s[r];
-                        atAdd(sums + (kind == kAtLow ? lane - kMapEnd : p.nOffsets + lane), (Sum)sum);
+                        atAdd(end, (Sum)sum);
                     }
                 }
                 if constexpr (!BF16) {
@@ -798,10 +781,18 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         auto step = [&](int t, const uint16_t* kd, const uint16_t* vd, const int* kp) {
             const int key0 = walk.tile<VIEW>(t) * kTileKeys;
             if (!reach.tile(key0)) return;
-            if (reach.edge(key0))
-                tile(std::true_type{}, key0, kd, vd, kp);
+            if constexpr (VIEW == kAtBias) {
+                int kLeast, kMost;
+                atRange(kp[lane], kLeast, kMost);
+                const AtOffsets kind = atOffsets(p, qLeast, qMost, kLeast, kMost);
+                if (kind != kAtMap && !reach.edge(key0))
+                    return tile(std::false_type{}, std::false_type{}, key0, kd, vd, kp, biases[kind == kAtLow ? 0 : p.nOffsets - 1],
+                                sums + (kind == kAtLow ? lane - kMapEnd : p.nOffsets + lane));
+            }
+            if (reach.edge(key0))   // of a bias by pair, at the map's ends too
+                tile(std::true_type{}, std::true_type{}, key0, kd, vd, kp, 0.f, nullptr);
             else
-                tile(std::false_type{}, key0, kd, vd, kp);
+                tile(std::false_type{}, std::true_type{}, key0, kd, vd, kp, 0.f, nullptr);
         };
         auto trip = [&](int t, const uint16_t* kd, const uint16_t* vd, const int* kp, uint16_t* kNext, uint16_t* vNext, int* kpNext) {   // as in the forward pass
             __builtin_amdgcn_s_waitcnt(0);

@@ -218,7 +218,7 @@ def test_positions_of_any_value(hip):
     run(hip, 1, 80, 70, 2, 2, 32, seed=1, buckets=np.arange(9), zero=4, where=where)
     run(hip, 1, 80, 70, 2, 2, 32, seed=2, buckets=np.arange(9), zero=4, where=(np.full(80, 7), np.full(70, 9)))
     run(hip, 1, 80, 70, 2, 2, 32, seed=3, buckets=np.arange(200), zero=-50, where=(np.arange(80) * 3, np.arange(70)))
-    run(hip, 1, 80, 70, 2, 2, 32, seed=4, buckets=np.arange(9), zero=top)
+    run(hip, 1, 80, 70, 2, 2, 32, seed=4, buckets=np.arange(9), zero=2 ** 30)
     run(hip, 1, 80, 70, 2, 2, 32, seed=5, buckets=np.arange(9), zero=-2 ** 30)
 
 
@@ -356,7 +356,7 @@ GOOD = dict(dtype=0, ldq=128, sq=1280, ldkv=64, skv=640, batch=1, seq_q=10, seq_
             ptr=4096, q=4096, lens=None, table=4096, buckets=4096, qpos=None, kpos=None, n=5, offsets=9, zero=4)
 BAD = [dict(table=None), dict(buckets=None), dict(table=4098), dict(buckets=4097), dict(qpos=4096), dict(kpos=4096),
        dict(qpos=4098, kpos=4096), dict(qpos=4096, kpos=4098), dict(n=0), dict(n=-1), dict(n=16385), dict(offsets=0),
-       dict(offsets=4097), dict(zero=-2 ** 30 - 1), dict(zero=-2 ** 31), dict(seq_q=2 ** 29 + 1), dict(seq_k=2 ** 29 + 1), dict(dtype=2), dict(batch=-1), dict(heads=3, kv=2),
+       dict(offsets=4097), dict(zero=-2 ** 30 - 1), dict(zero=-2 ** 31), dict(zero=2 ** 30 + 1), dict(zero=2 ** 31 - 1), dict(seq_q=2 ** 29 + 1), dict(seq_k=2 ** 29 + 1), dict(dtype=2), dict(batch=-1), dict(heads=3, kv=2),
        dict(dim=12), dict(dim=136), dict(scale=float("inf")), dict(ldq=120), dict(ldkv=56), dict(sq=1284), dict(q=None),
        dict(q=4098), dict(ptr=None), dict(ptr=4104), dict(lens=4098), dict(heads=65536, kv=1, ldq=65536 * 64)]
 
