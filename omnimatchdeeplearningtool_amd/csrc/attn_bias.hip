@@ -9,9 +9,10 @@
 // tell both distances). dtable is the sum of dS over the pairs of a bucket:
 //  * the dQ kernel, which has dS in registers, adds each to its wave's sums by
 //    offset in LDS, and leaves its workgroup's;
-//  * attn_bias_offsets_kernel adds those of a head, attn_bias_table_kernel the
-//    offsets of each bucket. All in an order that repeats.
+//  * attn_bias_table_kernel adds those of a head, then the offsets of each
+//    bucket. All in an order that repeats.
 #include "attn_train_kernels.hpp"
+#include "buffer_io.hpp"
 #include "../../include/omhip.h"
 
 #include <climits>
@@ -23,45 +24,51 @@ namespace {
 constexpr int kMaxBuckets = 16384;   // attn_bias_table_kernel's sums take 128 KB of LDS
 constexpr int kMaxSeq = 1 << 29;     // positions stay below 2^31
 
-// offsetSums[head][o] = sum over the head's `units` rows of bins, a sixteenth a wave.
-__global__ __launch_bounds__(1024) void attn_bias_offsets_kernel(AttnBiasParams p, int units) {
+// A workgroup adds 64 offsets' sums of a head over its `units` rows of bins, a sixteenth a wave, into offsetSums; the head's
+// last one to arrive adds the offsets of each bucket, by one wave, into gradTable. What passes between workgroups is written and
+// read coherently past the XCDs' L2s and has landed before the counter goes up. Two launches measured 9.6 us where this one
+// measures 7.2 (12 heads, 128 units, 731 offsets). units 0: no pair, and so zeros.
+__global__ __launch_bounds__(1024) void attn_bias_table_kernel(AttnBiasParams p, int units) {
     __shared__ double part[16][64];
+    __shared__ int last;
+    extern __shared__ double bucketSums[];   // [nBuckets]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int o = (int)blockIdx.x * 64 + lane, head = (int)blockIdx.y;
-    const int first = (int)((long long)units * wave / 16), last = (int)((long long)units * (wave + 1) / 16);
-    double s = 0.;
-    if (o < p.nOffsets) {
-        const float* from = p.bins + (long long)head * units * p.nOffsets + o;
+    const __amdgpu_buffer_rsrc_t sums = bufferRsrc(p.offsetSums + (long long)head * p.nOffsets, units > 0 ? (uint32_t)p.nOffsets * 4u : 0u);
+    if (units > 0) {
+        const int first = (int)((long long)units * wave / 16), end = (int)((long long)units * (wave + 1) / 16);
+        double s = 0.;
+        if (o < p.nOffsets) {
+            const float* from = p.bins + (long long)head * units * p.nOffsets + o;
 #pragma unroll 8
-        for (int u = first; u < last; ++u) s += (double)from[(long long)u * p.nOffsets];
-    }
-    part[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && o < p.nOffsets) {
-        s = 0.;
+            for (int u = first; u < end; ++u) s += (double)from[(long long)u * p.nOffsets];
+        }
+        part[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0) {
+            s = 0.;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) s += part[k][lane];
-        p.offsetSums[(long long)head * p.nOffsets + o] = (float)s;
+            for (int k = 0; k < 16; ++k) s += part[k][lane];
+            bufStore1Agent(sums, (uint32_t)o * 4u, 0, (float)s);   // past the last offset: out of range, not written
+            __builtin_amdgcn_s_waitcnt(0);                         // the sums have landed
+            if (lane == 0)
+                last = __hip_atomic_fetch_add(p.arrivals + head, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        }
+        __syncthreads();
+        if (!last) return;
     }
-}
-
-// gradTable[bucket][head] = sum of the offsets in the bucket, added by one wave, a few loads ahead.
-__global__ __launch_bounds__(256) void attn_bias_table_kernel(AttnBiasParams p, int empty) {
-    extern __shared__ double bucketSums[];   // [nBuckets]
-    const int head = (int)blockIdx.x;
-    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) bucketSums[b] = 0.;
+    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 1024) bucketSums[b] = 0.;
     __syncthreads();
-    if (threadIdx.x < 64 && !empty) {
-        const float* from = p.offsetSums + (long long)head * p.nOffsets;
-        constexpr int N = 8;
-        for (int o0 = (int)threadIdx.x; o0 < p.nOffsets; o0 += 64 * N) {
+    if (wave == 0 && units > 0) {
+        constexpr int N = 8;   // loads under way
+        for (int o0 = lane; o0 < p.nOffsets; o0 += 64 * N) {
             int b[N];
             float v[N];
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const int o = min(o0 + 64 * k, p.nOffsets - 1);
-                b[k] = o0 + 64 * k < p.nOffsets ? p.bucketOf[o] : -1;
-                v[k] = from[o];
+                const int i = o0 + 64 * k;
+                b[k] = i < p.nOffsets ? p.bucketOf[i] : -1;
+                v[k] = bufLoad1Agent(sums, (uint32_t)i * 4u, 0);
             }
 #pragma unroll
             for (int k = 0; k < N; ++k)
@@ -70,16 +77,18 @@ __global__ __launch_bounds__(256) void attn_bias_table_kernel(AttnBiasParams p, 
         __builtin_amdgcn_s_waitcnt(0);
     }
     __syncthreads();
-    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 256) p.gradTable[(long long)b * p.H + head] = (float)bucketSums[b];
+    for (int b = (int)threadIdx.x; b < p.nBuckets; b += 1024) p.gradTable[(long long)b * p.H + head] = (float)bucketSums[b];
+    if (threadIdx.x == 0 && units > 0) __hip_atomic_store(p.arrivals + head, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
 }
 
-int tableGradient(const AttnBiasParams& p, int units) {
+int tableGradient(AttnBiasParams& p, int units) {
     if (units > 0) {
-        hipLaunchKernelGGL(attn_bias_offsets_kernel, dim3((p.nOffsets + 63) / 64, p.H), dim3(1024), 0, stream(), p, units);
-        OMHIP_CHECK_LAUNCH();
+        p.arrivals = static_cast<unsigned*>(workspace((size_t)p.H * sizeof(unsigned), kWsCounters));
+        if (!p.arrivals) return -1;   // workspace() recorded the cause
     }
     OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE(attn_bias_table_kernel, kMaxBuckets * sizeof(double)));
-    hipLaunchKernelGGL(attn_bias_table_kernel, dim3(p.H), dim3(256), (size_t)p.nBuckets * sizeof(double), stream(), p, units == 0);
+    hipLaunchKernelGGL(attn_bias_table_kernel, dim3(units > 0 ? (p.nOffsets + 63) / 64 : 1, p.H), dim3(1024),
+                       (size_t)p.nBuckets * sizeof(double), stream(), p, units);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }
@@ -157,7 +166,8 @@ int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_
         return -1;
     const long long blocksQ = (nSeqQ + kBlockQ - 1) / kBlockQ, blocksK = (nSeqK + kBlockQ - 1) / kBlockQ;
     const int tiles = (nSeqK + kTileKeys - 1) / kTileKeys;
-    p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), nHeadDim <= 64 ? 4 : 2);
+    // two workgroups a CU: 2 x 2048 tokens, 8 heads of 64, causal: dK, dV and join 49.6 us (four 55.1, one 60.6)
+    p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), 2);
     p.partRows = (nSeqK + kBlockQ - 1) / kBlockQ * kBlockQ;
     // A workgroup of dQ keeps its sums over the images that it takes: so many groups of images that the grid has eight
     // workgroups a CU.

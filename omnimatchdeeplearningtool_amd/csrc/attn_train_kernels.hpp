@@ -84,6 +84,7 @@ struct AttnBiasParams : AttnTrainParams {
     float* tables;             // [H, nOffsets + 2 kMapEnd] biases by offset times log2 e, which dQ leaves for dK, dV
     float* bins;               // [H, imageGroups * blocks * keyParts, nOffsets] sums of dS by offset
     float* offsetSums;         // [H, nOffsets]
+    unsigned* arrivals;        // [H], zero at rest
     float* gradTable;          // [nBuckets, H]
 };
 
