@@ -30,7 +30,7 @@ namespace omhip {
 
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;         // of a workgroup that holds queries; pairs of waves of one that holds keys
 constexpr int kTileKeys = 64;    // keys per LDS tile
 constexpr int kBlockQ = 32 * kWaves;
 
@@ -301,9 +301,10 @@ __device__ __forceinline__ int atOwnPosition(const int* positions, int token, in
 // conflicts: bound by the two waves of a SIMD that share its issue between MFMAs (1024 cycles a tile) and exponentials (1050).
 // ViT-B/16 b64 (197 tokens, 768 heads of 64, fp16): 23.6-25.5 us, 3.1-3.3 TB/s over its compulsory bytes; four tiles a walk,
 // so its start and end (copies in, results out), which nothing overlaps, are half of it.
-template <bool BF16, int KD, int VIEW>
-__global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIEW> p) {
+template <bool BF16, int KD, int VIEW, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_train_forward_kernel(AtParams<VIEW> p) {
     using T = AtTile<KD>;
+    constexpr int BLOCK = 32 * W;   // queries of the workgroup
     constexpr float kShift = BF16 ? 0.f : 6.f;
     __shared__ __attribute__((aligned(256))) uint16_t k0[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v0[kTileKeys * T::RS];
@@ -323,20 +324,20 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     const int kvHead = head / (p.H / p.Hkv);
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
     const int off = VIEW == kAtPlain ? p.Sk - p.Sq : nK - nQ;
-    const int q0 = (int)qb * kBlockQ + wave * 32;   // the wave's first query
+    const int q0 = (int)qb * BLOCK + wave * 32;   // the wave's first query
     const int query = q0 + l;
     const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
     const uint16_t* vBase = p.v + (long long)b * p.skv + (long long)kvHead * p.D;
 
     // keys seen by the workgroup's and by the wave's queries
-    const int blockLast = min((int)qb * kBlockQ + kBlockQ, nQ) - 1;
-    int kEnd = blockLast >= (int)qb * kBlockQ ? nK : 0;
+    const int blockLast = min((int)qb * BLOCK + BLOCK, nQ) - 1;
+    int kEnd = blockLast >= (int)qb * BLOCK ? nK : 0;
     if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
     int waveEnd = q0 < nQ ? kEnd : 0;
     if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
     AtReach<VIEW> reach{nK, q0, off, waveEnd, 0, 0, 0, 0, p.causal != 0};
     AtWalk walk{kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0, 0, 0};
-    if constexpr (VIEW == kAtWindow) atWindow(p, (int)qb * kBlockQ, blockLast, kEnd, reach, walk);
+    if constexpr (VIEW == kAtWindow) atWindow(p, (int)qb * BLOCK, blockLast, kEnd, reach, walk);
     const int tBegin = (int)((long long)walk.n * part / p.keyParts), nt = (int)((long long)walk.n * (part + 1) / p.keyParts);
 
     // of a score; with a bias, scores are scaled before it is added and c is 1
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     const float c = VIEW == kAtBias ? 1.f : fmaxf(fabsf(scaled), FLT_MIN);
     const uint32_t flip = VIEW != kAtBias && p.scale < 0.f ? 0x80008000u : 0u;
     const typename T::Lane at(lane);
-    typename T::template Copy<kTileKeys, kWaves> copy;
+    typename T::template Copy<kTileKeys, W> copy;
     const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
     copy.init(wave, lane, ld2, p.D);
     auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int* kp) {
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void attn_train_forward_kernel(AtParams<VIE
     if (nt > tBegin) fetch(tBegin, k0, v0, at0);
     int position = 0, qLeast = 0, qMost = 0;   // the lane's query's, the wave's
     if constexpr (VIEW == kAtBias) {
-        for (int i = (int)threadIdx.x; i < p.nOffsets + 2 * kMapEnd; i += 256) biasesLds[i] = atBias(p, head, i - kMapEnd);
+        for (int i = (int)threadIdx.x; i < p.nOffsets + 2 * kMapEnd; i += 64 * W) biasesLds[i] = atBias(p, head, i - kMapEnd);
         position = atOwnPosition(p.qPos, query, nQ, off, qLeast, qMost);
     }
     __builtin_amdgcn_s_waitcnt(0);
@@ -573,9 +574,10 @@ struct DsScale {
 // dQ and dK / dV are two kernels that each compute S and dP, 7 products where one pass would need 5: sums of a row's dQ
 // over workgroups would have to be added atomically, in an order that changes, or written whole for every block of keys.
 // Measured (sizes as for the forward pass): 211-242 us by card (0.85-0.98 PFLOP/s), matrix cores busy 54 %; ViT-B/16 b64 37.
-template <bool BF16, int KD, int VIEW, class Sum>
-__global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p) {
+template <bool BF16, int KD, int VIEW, class Sum, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_train_dq_kernel(AtParams<VIEW> p) {
     using T = AtTile<KD>;
+    constexpr int BLOCK = 32 * W;   // queries of the workgroup
     __shared__ __attribute__((aligned(256))) uint16_t k0[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t v0[kTileKeys * T::RS];
     __shared__ __attribute__((aligned(256))) uint16_t k1[kTileKeys * T::RS];
@@ -590,17 +592,17 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
     qb = p.blocks - 1 - qb / (uint32_t)p.keyParts;   // causal: the longest walks first
     const int group = (int)(bh / (uint32_t)p.H), head = (int)(bh % (uint32_t)p.H);   // group: the image, or of images
     const int kvHead = head / (p.H / p.Hkv);
-    const int q0 = (int)qb * kBlockQ + wave * 32;
+    const int q0 = (int)qb * BLOCK + wave * 32;
     Sum* sums = nullptr;
     if constexpr (VIEW == kAtBias) {
         const int each = p.nOffsets + 2 * kMapEnd;
         Sum* all = reinterpret_cast<Sum*>(biasesLds + (each + 63) / 64 * 64);
-        for (int i = (int)threadIdx.x; i < each; i += 256) {
+        for (int i = (int)threadIdx.x; i < each; i += 64 * W) {
             const float v = atBias(p, head, i - kMapEnd);
             biasesLds[i] = v;
             if (group == 0 && qb == 0 && part == 0) p.tables[(long long)head * each + i] = v;
         }
-        for (int i = (int)threadIdx.x; i < 4 * each; i += 256) all[i] = 0;   // added to after the first barrier
+        for (int i = (int)threadIdx.x; i < W * each; i += 64 * W) all[i] = 0;   // added to after the first barrier
         sums = all + wave * each + kMapEnd;
     }
     // One image. The arrays in dynamic LDS apart from the others (restrict): the compiler would wait for the copies under way
@@ -614,19 +616,19 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         const uint16_t* kBase = p.k + (long long)b * p.skv + (long long)kvHead * p.D;
         const uint16_t* vBase = p.v + (long long)b * p.skv + (long long)kvHead * p.D;
 
-        const int blockLast = min((int)qb * kBlockQ + kBlockQ, nQ) - 1;
-        int kEnd = blockLast >= (int)qb * kBlockQ ? nK : 0;
+        const int blockLast = min((int)qb * BLOCK + BLOCK, nQ) - 1;
+        int kEnd = blockLast >= (int)qb * BLOCK ? nK : 0;
         if (p.causal) kEnd = min(kEnd, blockLast + off + 1);
         int waveEnd = q0 < nQ ? kEnd : 0;
         if (p.causal) waveEnd = min(waveEnd, q0 + 32 + off);
         AtReach<VIEW> reach{nK, q0, off, waveEnd, 0, 0, 0, 0, p.causal != 0};
         AtWalk walk{kEnd > 0 ? (kEnd + kTileKeys - 1) / kTileKeys : 0, 0, 0};
-        if constexpr (VIEW == kAtWindow) atWindow(p, (int)qb * kBlockQ, blockLast, kEnd, reach, walk);
+        if constexpr (VIEW == kAtWindow) atWindow(p, (int)qb * BLOCK, blockLast, kEnd, reach, walk);
         const int tBegin = (int)((long long)walk.n * part / p.keyParts), nt = (int)((long long)walk.n * (part + 1) / p.keyParts);
 
         const float c = p.scale * kAtLog2e;
         const typename T::Lane at(lane);
-        typename T::template Copy<kTileKeys, kWaves> copy;
+        typename T::template Copy<kTileKeys, W> copy;
         const uint32_t ld2 = (uint32_t)p.ldkv * 2u;
         copy.init(wave, lane, ld2, p.D);
         auto fetch = [&](int t, uint16_t* kd, uint16_t* vd, int* kp) {
@@ -643,8 +645,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         // dimension of 128 is at 256 registers and 12-20 bytes of scratch without the chunks of dO and O for delta. (dO through
         // the first pair of buffers, free until the first tile is fetched, has not been measured.)
         constexpr bool kStaged = KD <= 2;
-        __shared__ __attribute__((aligned(256))) uint16_t gStage[kStaged ? kBlockQ * T::RS : 8];
-        __shared__ float rowDelta[kWaves][32];
+        __shared__ __attribute__((aligned(256))) uint16_t gStage[kStaged ? BLOCK * T::RS : 8];
+        __shared__ float rowDelta[W][32];
         const uint16_t* qRows = p.q + (long long)b * p.sq + (long long)q0 * p.ldq + (long long)head * p.D;
         const uint16_t* gRows = p.gradOut + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
         const uint16_t* oRows = p.out + (((long long)b * p.Sq + q0) * p.H + head) * p.D;
@@ -845,8 +847,8 @@ __global__ __launch_bounds__(256, 2) void attn_train_dq_kernel(AtParams<VIEW> p)
         float* to = p.bins + ((((long long)head * p.imageGroups + group) * p.blocks + qb) * p.keyParts + part) * p.nOffsets;
         const int each = p.nOffsets + 2 * kMapEnd;
         const Sum* first = sums - wave * each;
-        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 256)
-            to[o] = (float)((first[o] + first[o + each]) + (first[o + 2 * each] + first[o + 3 * each]));
+        for (int o = (int)threadIdx.x; o < p.nOffsets; o += 64 * W)
+            to[o] = (float)(W == 2 ? first[o] + first[o + each] : (first[o] + first[o + each]) + (first[o + 2 * each] + first[o + 3 * each]));
     }
 }
 
@@ -897,25 +899,25 @@ struct DkvBuffers {
 struct DkvTiles {
     int t0, t1;
 };
-template <int VIEW>
+template <int VIEW, int BLOCK = kBlockQ>
 __device__ __forceinline__ DkvTiles dkvTiles(const AtParams<VIEW>& p, int block, int nQ, int nK, int off) {
-    const int first = block * kBlockQ;
+    const int first = block * BLOCK;
     DkvTiles t{p.causal ? max(0, first - off) / kTileQ : 0, first < nK ? (nQ + kTileQ - 1) / kTileQ : 0};
     if constexpr (VIEW == kAtWindow) {
         if (block >= p.sinkBlocks) {
             if (!p.causal) t.t0 = max(0, first - off - p.window + 1) / kTileQ;
-            t.t1 = min(t.t1, (max(0, first + kBlockQ - 1 - off + p.window) + kTileQ - 1) / kTileQ);
+            t.t1 = min(t.t1, (max(0, first + BLOCK - 1 - off + p.window) + kTileQ - 1) / kTileQ);
         }
     }
     return t;
 }
 
 // A wave's work in attn_train_dkv_kernel.
-template <bool BF16, int KD, int VIEW, bool SECOND>
+template <bool BF16, int KD, int VIEW, int PAIRS, bool SECOND>
 __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffers& lds, int wave, int lane) {
     using T = AtTile<KD>;
     constexpr float kLower = BF16 ? 1.f : 1.f / 32768.f;   // takes kRaise out
-    const int l = lane & 31, h = lane >> 5, pair = wave & 3;
+    const int l = lane & 31, h = lane >> 5, pair = wave % PAIRS;
     uint32_t bh, block;
     // causal, or first keys with longer walks: the first keys' walks are longest
     atPlace(blockIdx.x, p.heads, p.blocks * p.parts, p.causal || VIEW == kAtWindow, bh, block);
@@ -925,11 +927,11 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     const int group = p.H / p.Hkv;
     const int nQ = atLength(p.qLens, b, p.Sq), nK = atLength(p.kLens, b, p.Sk);
     const int off = VIEW == kAtPlain ? p.Sk - p.Sq : nK - nQ;
-    const int key0 = (int)block * kBlockQ + pair * 32;
+    const int key0 = (int)block * 32 * PAIRS + pair * 32;
     const int key = key0 + l;
 
     // query tiles that see a key of the workgroup: t0 .. t1 of each head of the group; this part's share of them
-    const auto [t0, t1] = dkvTiles<VIEW>(p, (int)block, nQ, nK, off);
+    const auto [t0, t1] = dkvTiles<VIEW, 32 * PAIRS>(p, (int)block, nQ, nK, off);
     const int per = max(0, t1 - t0), total = per * group;
     const int begin = (int)((long long)total * part / p.parts), n = (int)((long long)total * (part + 1) / p.parts) - begin;
 
@@ -941,7 +943,7 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     const long long first = (long long)b * p.skv + (long long)key0 * p.ldkv + (long long)kvHead * p.D;
     T::start((SECOND ? p.v : p.k) + first, nK - key0, p.ldkv, p.D, stage, lane);
     const float c = p.scale * kAtLog2e;
-    constexpr int kCopyWaves = T::CH * kTileQ / 64 < 8 ? T::CH * kTileQ / 64 : 8;   // a head dimension of 32 has 2 instructions
+    constexpr int kCopyWaves = T::CH * kTileQ / 64 < 2 * PAIRS ? T::CH * kTileQ / 64 : 2 * PAIRS;   // a head dimension of 32 has 2 instructions
     typename T::template Copy<kTileQ, kCopyWaves> copyQ, copyG;
     const uint32_t ldq2 = (uint32_t)p.ldq * 2u, ldg2 = (uint32_t)(p.H * p.D) * 2u;
     copyQ.init(wave, lane, ldq2, p.D);
@@ -951,12 +953,12 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     auto fetch = [&](uint16_t* qd, uint16_t* gd, float* sd) {   // the next tile of the walk
         const long long first = (long long)fetchT * kTileQ;
         if constexpr (VIEW == kAtBias) {
-            if (wave == 6)
+            if (wave == 2 * PAIRS - 2)
                 atCopyPositions(p.qPos, (int)first, kTileQ, nQ, off, lane, reinterpret_cast<int*>(sd + 2 * kTileQ));
             if (fresh) {
                 const int each = p.nOffsets + 2 * kMapEnd, rounded = (each + 63) / 64 * 64;
                 const __amdgpu_buffer_rsrc_t from = atView(p.tables + (long long)fetchHead * each, (uint32_t)each * 4u);
-                for (int i = wave * 64; i < each; i += 512)
+                for (int i = wave * 64; i < each; i += 128 * PAIRS)
                     atCopy4(from, lds.biases + ((fetchHead - kvHead * group) & 1) * rounded + i, (uint32_t)(i + lane) * 4u);
             }
             fresh = false;
@@ -966,7 +968,7 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
             copyQ.run(p.q + (long long)b * p.sq + first * p.ldq + (long long)fetchHead * p.D, rows, ldq2, p.D, qd, wave);
             copyG.run(p.gradOut + (((long long)b * p.Sq + first) * p.H + fetchHead) * p.D, rows, ldg2, p.D, gd, wave);
         }
-        if (wave == 7)   // rows past the query length hold -inf and 0
+        if (wave == 2 * PAIRS - 1)   // rows past the query length hold -inf and 0
             atCopy4(atView(p.stats + 2 * (((long long)b * p.H + fetchHead) * p.SqP + first), 2 * kTileQ * 4), sd, lane * 4);
         if (++fetchT == t1) {
             fetchT = t0;
@@ -1095,7 +1097,7 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     auto trip = [&](int i, auto bufTag) {
         constexpr int BUF = decltype(bufTag)::value, MINE = SECOND ? (BUF + 2) % 3 : BUF;
         meet(i, bufTag);
-        float* wd = lds.weights + (((SECOND ? ~i : i) & 1) * 4 + pair) * (kTileQ * 32);
+        float* wd = lds.weights + (((SECOND ? ~i : i) & 1) * PAIRS + pair) * (kTileQ * 32);
         if constexpr (SECOND)
             work(t * kTileQ, lds.g[MINE], lds.q[MINE], lds.stats[MINE], wd, nullptr);
         else
@@ -1149,8 +1151,8 @@ __device__ __forceinline__ void dkvWalk(const AtParams<VIEW>& p, const DkvBuffer
     }
 }
 
-template <bool BF16, int KD, int VIEW>
-__global__ __launch_bounds__(512, 2) void attn_train_dkv_kernel(AtParams<VIEW> p) {
+template <bool BF16, int KD, int VIEW, int PAIRS>
+__global__ __launch_bounds__(128 * PAIRS, 2) void attn_train_dkv_kernel(AtParams<VIEW> p) {
     constexpr int N = kTileQ * AtTile<KD>::RS;
     __shared__ __attribute__((aligned(256))) uint16_t q0[N];
     __shared__ __attribute__((aligned(256))) uint16_t q1[N];
@@ -1161,15 +1163,15 @@ __global__ __launch_bounds__(512, 2) void attn_train_dkv_kernel(AtParams<VIEW> p
     __shared__ __attribute__((aligned(256))) float s0[(VIEW == kAtBias ? 3 : 2) * kTileQ];
     __shared__ __attribute__((aligned(256))) float s1[(VIEW == kAtBias ? 3 : 2) * kTileQ];
     __shared__ __attribute__((aligned(256))) float s2[(VIEW == kAtBias ? 3 : 2) * kTileQ];
-    __shared__ __attribute__((aligned(16))) float weights[2 * 4 * kTileQ * 32];   // behind the tiles: their offsets fit a read's 16 bits
+    __shared__ __attribute__((aligned(16))) float weights[2 * PAIRS * kTileQ * 32];   // behind the tiles: their offsets fit a read's 16 bits
     // [nOffsets] and the ends, rounded to 64, twice where a key head has several query heads
     extern __shared__ float biases[];
     const DkvBuffers lds{{q0, q1, q2}, {g0, g1, g2}, {s0, s1, s2}, weights, biases};
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (wave < 4)
-        dkvWalk<BF16, KD, VIEW, false>(p, lds, wave, lane);
+    if (wave < PAIRS)
+        dkvWalk<BF16, KD, VIEW, PAIRS, false>(p, lds, wave, lane);
     else
-        dkvWalk<BF16, KD, VIEW, true>(p, lds, wave, lane);
+        dkvWalk<BF16, KD, VIEW, PAIRS, true>(p, lds, wave, lane);
 }
 
 // The parts' sums of dK (blockIdx.y 0) or dV (1), eight values of a key a thread, of the first `keys`.
@@ -1364,14 +1366,31 @@ size_t dynamicLds(const AtParams<VIEW>& p, int tables) {
 #define OMHIP_AT_LDS(kernel, view, tables) \
     if constexpr (view == kAtBias) OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE(kernel, (kMaxOffsets + 2 * kMapEnd) * 4 * tables))
 
+// Workgroups of a bias for sequences of up to 64 tokens and head dimensions of up to 64 (windows of an image) have half as many
+// waves: of four, two would hold no token. 1024 windows of 7 x 7, 4 heads of 32: backward
+// 75 us, with four waves 100.
+template <int KD, int VIEW>
+constexpr bool kShort = VIEW == kAtBias && KD <= 2;
+
+template <bool BF16, int KD, int VIEW, int W>
+int launchForwardKernel(const AtParams<VIEW>& p) {
+    OMHIP_AT_LDS((attn_train_forward_kernel<BF16, KD, VIEW, W>), VIEW, 1);
+    hipLaunchKernelGGL((attn_train_forward_kernel<BF16, KD, VIEW, W>), dim3(p.heads * p.blocks * p.keyParts), dim3(64 * W),
+                       dynamicLds<VIEW>(p, 1), stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
 template <bool BF16, int KD, int VIEW>
 int launchForward(AtParams<VIEW>& p) {
     p.heads = (uint32_t)(p.B * p.H);
     p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
-    OMHIP_AT_LDS((attn_train_forward_kernel<BF16, KD, VIEW>), VIEW, 1);
-    hipLaunchKernelGGL((attn_train_forward_kernel<BF16, KD, VIEW>), dim3(p.heads * p.blocks * p.keyParts), dim3(256),
-                       dynamicLds<VIEW>(p, 1), stream(), p);
-    OMHIP_CHECK_LAUNCH();
+    if constexpr (kShort<KD, VIEW>) {
+        if (p.Sq <= kBlockQ / 2 ? launchForwardKernel<BF16, KD, VIEW, kWaves / 2>(p) : launchForwardKernel<BF16, KD, VIEW, kWaves>(p))
+            return -1;
+    } else if (launchForwardKernel<BF16, KD, VIEW, kWaves>(p)) {
+        return -1;
+    }
     if (p.keyParts > 1) {
         const long long n = (long long)p.B * p.Sq * p.H * (p.D / 8);
         hipLaunchKernelGGL((attn_train_join_kernel<BF16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream(), p);
@@ -1380,16 +1399,33 @@ int launchForward(AtParams<VIEW>& p) {
     return 0;
 }
 
-template <bool BF16, int KD, int VIEW, class Sum>
-int launchDq(const AtParams<VIEW>& p) {
+template <bool BF16, int KD, int VIEW, class Sum, int W>
+int launchDqKernel(const AtParams<VIEW>& p) {
     size_t lds = 0;
     if constexpr (VIEW == kAtBias) {
         constexpr int most = sizeof(Sum) == 8 ? kMaxWide : kMaxOffsets;
-        lds = biasLds(p, 1) + 4 * (size_t)(p.nOffsets + 2 * kMapEnd) * sizeof(Sum);
-        OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE((attn_train_dq_kernel<BF16, KD, VIEW, Sum>),
-                                                   (most + 2 * kMapEnd) * (sizeof(float) + 4 * sizeof(Sum))));
+        lds = biasLds(p, 1) + W * (size_t)(p.nOffsets + 2 * kMapEnd) * sizeof(Sum);
+        OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE((attn_train_dq_kernel<BF16, KD, VIEW, Sum, W>),
+                                                   (most + 2 * kMapEnd) * (sizeof(float) + W * sizeof(Sum))));
     }
-    hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD, VIEW, Sum>), dim3(p.heads * p.blocks * p.keyParts), dim3(256), lds, stream(), p);
+    hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD, VIEW, Sum, W>), dim3(p.heads * p.blocks * p.keyParts), dim3(64 * W), lds,
+                       stream(), p);
+    OMHIP_CHECK_LAUNCH();
+    return 0;
+}
+
+template <bool BF16, int KD, int VIEW, class Sum>
+int launchDq(const AtParams<VIEW>& p) {
+    if constexpr (kShort<KD, VIEW>)
+        if (p.Sq <= kBlockQ / 2) return launchDqKernel<BF16, KD, VIEW, Sum, kWaves / 2>(p);
+    return launchDqKernel<BF16, KD, VIEW, Sum, kWaves>(p);
+}
+
+template <bool BF16, int KD, int VIEW, int PAIRS>
+int launchDkvKernel(const AtParams<VIEW>& p) {
+    OMHIP_AT_LDS((attn_train_dkv_kernel<BF16, KD, VIEW, PAIRS>), VIEW, 2);
+    hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD, VIEW, PAIRS>), dim3(p.heads * p.blocks * p.parts), dim3(128 * PAIRS),
+                       dynamicLds<VIEW>(p, p.H > p.Hkv ? 2 : 1), stream(), p);
     OMHIP_CHECK_LAUNCH();
     return 0;
 }
@@ -1418,11 +1454,12 @@ int launchBackward(AtParams<VIEW>& p) {
     if (p.Sk > 0) {
         p.heads = (uint32_t)(p.B * p.Hkv);
         p.blocks = (uint32_t)((p.Sk + kBlockQ - 1) / kBlockQ);
-        const int tables = p.H > p.Hkv ? 2 : 1;
-        OMHIP_AT_LDS((attn_train_dkv_kernel<BF16, KD, VIEW>), VIEW, 2);
-        hipLaunchKernelGGL((attn_train_dkv_kernel<BF16, KD, VIEW>), dim3(p.heads * p.blocks * p.parts), dim3(512),
-                           dynamicLds<VIEW>(p, tables), stream(), p);
-        OMHIP_CHECK_LAUNCH();
+        if constexpr (kShort<KD, VIEW>) {
+            if (p.Sk <= kBlockQ / 2 ? launchDkvKernel<BF16, KD, VIEW, kWaves / 2>(p) : launchDkvKernel<BF16, KD, VIEW, kWaves>(p))
+                return -1;
+        } else if (launchDkvKernel<BF16, KD, VIEW, kWaves>(p)) {
+            return -1;
+        }
         int keys = p.parts > 1 ? p.Sk : 0;   // with fp32 sums
         if constexpr (VIEW == kAtWindow) {
             if (p.sinkParts > 0) {
