@@ -12,7 +12,6 @@
 //  * attn_bias_table_kernel adds those of a head, then the offsets of each
 //    bucket. All in an order that repeats.
 #include "attn_train_kernels.hpp"
-#include "buffer_io.hpp"
 #include "../../include/omhip.h"
 
 #include <climits>

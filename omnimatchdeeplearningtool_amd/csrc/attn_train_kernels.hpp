@@ -19,6 +19,7 @@
 #pragma once
 
 #include "attn_tile.hpp"
+#include "buffer_io.hpp"
 #include "omhip_internal.hpp"
 
 #include <algorithm>
@@ -71,6 +72,7 @@ struct AttnWindowParams : AttnTrainParams {
     // sinkParts workgroups for each 32 of them that take the queries which the blocks' walks leave out
     int sinkBlocks, sinkParts;
     float *sinkDk, *sinkDv;    // [B, Hkv, sinkParts, first keys rounded to 32, D]
+    unsigned* arrivals;        // [B * Hkv * (first + 31) / 32], zero at rest; null where the join adds the sinks' parts
 };
 
 constexpr float kNoBias = -1e30f;   // a bias at or below hides the key
@@ -1208,10 +1210,12 @@ __global__ __launch_bounds__(256) void attn_train_dkv_join_kernel(AtParams<VIEW>
 // Every query after a first key sees it, the other keys of its block only those in their windows: the block's walk leaves out
 // the far queries' tiles, which these workgroups take for 32 keys at a time. A wave has tiles of its own: S = Q K^T, dP = dO
 // V^T, dV^T += dO^T P, dK^T += Q^T dS, with K, V and both sums in its registers; the next tile's Q and dO land in the wave's
-// other buffers meanwhile. The waves' sums are added in order and left in fp32, a part a workgroup, for the join.
+// other buffers meanwhile. The waves' sums are added in order and left in fp32, a part a workgroup; where the blocks' walks are
+// not shared, the last workgroup of 32 keys to arrive adds them and the block's own sum and writes dK and dV (parts are
+// written and read coherently past the XCDs' L2s and have landed before the counter goes up), else the join does.
 // Walks of whole blocks over all queries kept three of four waves at work that no key asked for: 2 x 4096 x 16 heads on 4 of
-// 128, window 512, 4 first keys: dK, dV and joins 165 us, with these workgroups 127 (98 + 18 + 7; a wave's 3 or 4 tiles are as
-// long as its start and end).
+// 128, window 512, 4 first keys: dK, dV and join 165 us, with these workgroups 120 (99 + 21; a wave's 3 or 4 tiles are as long as
+// its start and end).
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_window_sinks_kernel(AttnWindowParams p) {
     using T = AtTile<KD>;
@@ -1342,12 +1346,50 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_window_sinks_kernel
             }
     }
     __syncthreads();
-    const long long to = (((long long)bh * p.sinkParts + part) * groups * 32 + key0) * p.D;
-    for (int x = (int)threadIdx.x; x < min(32, p.first - key0) * (p.D / 4); x += 256) {
-        const int row = x / (p.D / 4), d = x % (p.D / 4) * 4;
-        *reinterpret_cast<at_f32x4*>(p.sinkDk + to + (long long)row * p.D + d) = *reinterpret_cast<const at_f32x4*>(sumK + row * R + d);
-        *reinterpret_cast<at_f32x4*>(p.sinkDv + to + (long long)row * p.D + d) = *reinterpret_cast<const at_f32x4*>(sumV + row * R + d);
+    const int rows = min(32, p.first - key0), quads = p.D / 4;
+    const long long own = (long long)bh * p.sinkParts * groups * 32 * p.D;   // the key head's parts
+    const uint32_t pitch = (uint32_t)(groups * 32 * p.D) * 4u, bytes = pitch * (uint32_t)p.sinkParts;
+    const __amdgpu_buffer_rsrc_t partK = bufferRsrc(p.sinkDk + own, bytes), partV = bufferRsrc(p.sinkDv + own, bytes);
+    for (int x = (int)threadIdx.x; x < rows * quads; x += 256) {
+        const int row = x / quads, d = x % quads * 4;
+        const uint32_t to = (uint32_t)part * pitch + (uint32_t)((key0 + row) * p.D + d) * 4u;
+        bufStore4Agent(partK, to, 0, *reinterpret_cast<const at_f32x4*>(sumK + row * R + d));
+        bufStore4Agent(partV, to, 0, *reinterpret_cast<const at_f32x4*>(sumV + row * R + d));
     }
+    if (!p.arrivals) return;
+    __shared__ int last;
+    __builtin_amdgcn_s_waitcnt(0);   // this wave's parts have landed
+    __syncthreads();                 // every wave's have
+    unsigned* arrival = p.arrivals + bh * (uint32_t)groups + keyGroup;
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(arrival, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(p.sinkParts - 1);
+    __syncthreads();
+    if (!last) return;
+    for (int x = (int)threadIdx.x; x < rows * quads; x += 256) {
+        const int row = x / quads, d = x % quads * 4;
+        const uint32_t from = (uint32_t)((key0 + row) * p.D + d) * 4u;
+        const long long block = ((long long)bh * p.partRows + key0 + row) * p.D + d;   // the block's walk, of the launch before
+        at_f32x4 k = *reinterpret_cast<const at_f32x4*>(p.dkPart + block), v = *reinterpret_cast<const at_f32x4*>(p.dvPart + block);
+        for (int first = 0; first < p.sinkParts; first += 8) {
+            f32x4 a[8], c8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {   // past the last part: out of range, zeros
+                const uint32_t at8 = first + i < p.sinkParts ? from + (uint32_t)(first + i) * pitch : kOOB;
+                a[i] = bufLoad4Agent(partK, at8, 0);
+                c8[i] = bufLoad4Agent(partV, at8, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                k += a[i];
+                v += c8[i];
+            }
+        }
+        if (key0 + row >= nK) k = v = at_f32x4{0.f, 0.f, 0.f, 0.f};
+        const long long to = firstKey + (long long)row * p.ldkv + d;
+        *reinterpret_cast<at_u32x2*>(p.dk + to) = at_u32x2{atPack2<BF16>(k[0], k[1]), atPack2<BF16>(k[2], k[3])};
+        *reinterpret_cast<at_u32x2*>(p.dv + to) = at_u32x2{atPack2<BF16>(v[0], v[1]), atPack2<BF16>(v[2], v[3])};
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(arrival, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
 }
 
 // ---------------------------------------------------------------- launches
@@ -1467,7 +1509,6 @@ int launchBackward(AtParams<VIEW>& p) {
                                    dim3(256), 0, stream(), p);
                 OMHIP_CHECK_LAUNCH();
             }
-            if (p.parts == 1) keys = p.partRows;
         }
         if (keys > 0) {
             const long long n = (long long)p.B * keys * p.Hkv * (p.D / 8);

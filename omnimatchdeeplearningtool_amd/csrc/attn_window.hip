@@ -8,7 +8,6 @@
 // blocks of keys over the queries whose windows reach them, the first keys'
 // over all, by several workgroups.
 #include "attn_train_kernels.hpp"
-#include "buffer_io.hpp"
 #include "../../include/omhip.h"
 
 namespace omhip {
@@ -323,11 +322,11 @@ int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint1
     const int walk = windowTiles(p.window, p.causal, allQ);   // of a block of keys, for each query head
     p.parts = evenParts(heads * blocks, walk * group, resident);
     // The first keys: by workgroups of their own, unless they are so many that their blocks may as well walk over everything,
-    // or the window is as wide as the sequences.
+    // the window is as wide as the sequences, or there are no queries (and no workspace).
     if (p.first > kMaxSinks) {
         p.sinkBlocks = (p.first + kBlockQ - 1) / kBlockQ;
         p.parts = walkParts(heads * blocks, allQ * group, 2 * resident);
-    } else if (p.first > 0 && p.window < std::max(nSeqQ, nSeqK)) {
+    } else if (p.first > 0 && nSeqQ > 0 && p.window < std::max(nSeqQ, nSeqK)) {
         const long long groups = heads * ((p.first + 31) / 32);
         p.sinkParts = (int)std::clamp<long long>(std::min<long long>((long long)resident * cuCount() / groups,
                                                                      ((long long)std::max(1, allQ - walk) * group + 3) / 4), 1, 64);
@@ -338,6 +337,10 @@ int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint1
     if (backwardParts(p, std::min(allK, windowTiles(p.window, p.causal, allK) + (p.first + kTileKeys - 1) / kTileKeys),
                       (size_t)heads * p.parts * p.partRows * nHeadDim, 2 * sinks, &more))
         return -1;
+    if (p.sinkParts > 0 && p.parts == 1) {
+        p.arrivals = static_cast<unsigned*>(workspace((size_t)heads * ((p.first + 31) / 32) * sizeof(unsigned), kWsCounters));
+        if (!p.arrivals) return -1;   // workspace() recorded the cause
+    }
     p.sinkDk = more;
     p.sinkDv = more + sinks;
     return nDtype == 1 ? backward<true, kAtWindow>(p) : backward<false, kAtWindow>(p);

@@ -92,6 +92,16 @@ def test_walks_shared_by_workgroups(hip, Sq, Sk, H, Hkv, D, window, first, causa
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True], ids=["both", "causal"])
+@pytest.mark.parametrize("first", [1, 32, 33, 129, 256, 257, 300])
+def test_first_keys_of_far_queries(hip, first, causal):
+    """Queries far past their windows, by workgroups for 32 first keys up to 256 of them and by whole walks beyond; images
+    without queries or keys, and with fewer keys than first ones."""
+    run(hip, 4, 500, 500, 2, 1, 64, window=10, first=first, causal=causal, qlens=[500, 0, 500, 300], klens=[500, 500, 0, 20],
+        bf16=first % 2 == 0, seed=first)
+
+
+@pytest.mark.gpu
 def test_what_lies_past_a_length_is_not_read(hip):
     for bf16 in (False, True):
         c = Window(hip, 2, 100, 140, 2, 2, 64, bf16=bf16, qlens=[37, 100], klens=[70, 129], window=30, first=2, seed=5)
@@ -275,6 +285,12 @@ def test_empty_sequences(hip):
     H.attentionWindowBackwardHalf(None, q, q, 64, 0, 64, 320, None, None, False, *w, None, None, None, None, dk, dv, 2, 0, 5, 1, 1, 64,
                                   1.0)
     assert np.all(dk.numpy() == 0) and np.all(dv.numpy() == 0)
+    for window, first in ((2, 1), (2, 3), (1, 0), (2, 400)):   # first keys whose queries would be out of their window
+        for g in (dk, dv):
+            g.upload(np.full(640, 0x1234, np.uint16))
+        H.attentionWindowBackwardHalf(None, q, q, 64, 0, 64, 320, None, None, first == 1, window, first, None, None, None, None, dk, dv, 2,
+                                      0, 5, 1, 1, 64, 1.0)
+        assert np.all(dk.numpy() == 0) and np.all(dv.numpy() == 0)
     H.attentionWindowBackwardHalf(*[None] * 3, 64, 0, 64, 0, None, None, False, *w, *[None] * 6, 0, 5, 5, 1, 1, 64, 1.0)
 
 
