@@ -306,6 +306,9 @@ int run(const char* name, int nDtype, const QkArray (&x)[2], const QkArray (&g)[
             if (a->ld >= (1LL << 40) || a->stride >= (1LL << 60) / std::max(1, nBatch)) return fail("%s: a stride is too large", name);
         }
         if (!rowsApart(nBatch, nSeq, out[k].ld, out[k].stride, width)) return fail("%s: rows of the results would overlap", name);
+        for (const QkArray* a : {&x[k], &g[k]})   // a row is written once it is read, so in place means row for row
+            if (tokens > 0 && a->p == out[k].p && (a->ld != out[k].ld || a->stride != out[k].stride) && (a == &x[k] || backward))
+                return fail("%s: results in place of an input with other strides", name);
     }
     const int w = nHeadDim % 16 == 0 && nRotary % 16 == 0 ? 8 : 4;
     QkNormParams p{};

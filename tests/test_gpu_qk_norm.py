@@ -358,3 +358,11 @@ def test_overlapping_results_are_refused():
             call(om, {**GOOD, "strideo": bad}, False)
         with pytest.raises(om.OmHipError, match="overlap"):
             call(om, {**GOOD, "stride": bad}, True)
+
+
+def test_results_in_place_with_other_strides_are_refused():
+    import omnimatchdeeplearningtool_amd as om
+    with pytest.raises(om.OmHipError, match="in place"):
+        call(om, {**GOOD, "ldo": 136, "strideo": 1360}, False)
+    with pytest.raises(om.OmHipError, match="in place"):
+        call(om, {**GOOD, "x": 8192, "ldo": 136, "strideo": 1360}, True)
