@@ -89,11 +89,12 @@ __global__ __launch_bounds__(256, 2) void attn_window_token_kernel(TokenParams p
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
         for (int st = 0; st < T::NS; ++st) s = atMfma<BF16>(at.natural(kt, 0, st), qf[st], s);
-        const AtSeen seen = reach.seen(token, key0, h);
+        AtSeen seen = reach.seen(token, key0, h);
+        if (!some) seen.bits[0] = 0u;
         float top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            if (!some || seen.hidden<kAtWindow>(8 * (r / 4) + r % 4)) s[r] = -INFINITY;
+            s[r] = seen.pick<kAtWindow>(8 * (r / 4) + r % 4, s[r], -INFINITY);
             top = fmaxf(top, s[r]);
         }
         top = atMaxHalves(top);
