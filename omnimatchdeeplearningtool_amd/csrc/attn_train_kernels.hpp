@@ -192,8 +192,7 @@ __device__ __forceinline__ int atEntry(const AttnBiasParams& p, int q, int k, in
 
 // A head's biases by offset and the ends', times log2 e, into `to` by a workgroup: -inf where the table hides the key, 0 where the
 // offset has no bucket. Four entries of a thread are under way at once: one by one, every entry would wait for its bucket and
-// then for its bias (ViT-B/16 b64, 14 x 14 grid: forward
-// 35.9 -> 34.6 us).
+// then for its bias (ViT-B/16 b64, 14 x 14 grid: forward 35.9 -> 34.6 us).
 template <int THREADS, class F>
 __device__ __forceinline__ void atFillBiases(const AttnBiasParams& p, int head, F&& to) {
     constexpr int N = 4;
@@ -230,6 +229,7 @@ __device__ __forceinline__ void atForEntries(const AttnBiasParams& p, int own, c
         for (int e = 0; e < 4; ++e) f(4 * j + e, atEntry(p, QUERY ? own : pos[e], QUERY ? pos[e] : own, lane));
     }
 }
+
 // A wave's sums of dS by offset. They are of type T: an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes,
 // no two on one address), so floats are for maps that leave no room for doubles. A wave's instructions are done in order, and
 // lanes on one address in an order of the hardware's that repeats.
@@ -255,6 +255,7 @@ __device__ __forceinline__ void atReadEight(const uint32_t (&from)[8], float (&v
                  : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "v"(from[4]), "v"(from[5]), "v"(from[6]),
                    "v"(from[7]));
 }
+
 // Stores a wave's 32 rows of a transposed result (the lane's column is row l; its registers hold head dimensions 32 dt +
 // 8 (r / 4) + 4 h + r % 4) times f, or zeros, as halves. Rows are turned around in `stage`, 32 rows of the wave's own in
 // LDS, and leave as whole chunks of 16 bytes, 64 / CH rows an instruction: stored from the registers, every instruction

@@ -31,7 +31,7 @@ struct TokenParams : AttnWindowParams {
 // between waves before their contexts are joined in LDS, and the workgroups' by the last one to arrive, with accesses coherent
 // past the XCDs' L2s (partials have landed before the counter goes up). Bound by latency: the keys in sight of a cache are a
 // few 100 KB, which enough workgroups read at once. Measured: 16 caches of up to 8192 tokens, 16 heads on 4 of 128, window
-// 1024, 4 first keys: 12.6 us (the forward kernel and its join 27.5); one of 4096, 8 heads of 64, window 256: 7.6 (10.0).
+// 1024, 4 first keys: 12 us (the forward kernel and its join 27.5); one of 4096, 8 heads of 64, window 256: 7.2 (10.0).
 template <bool BF16, int KD>
 __global__ __launch_bounds__(256, 2) void attn_window_token_kernel(TokenParams p) {
     using T = AtTile<KD>;

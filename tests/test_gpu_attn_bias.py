@@ -223,6 +223,17 @@ def test_positions_of_any_value(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("offsets", [2560, 2561])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_maps_around_the_sums_in_doubles(hip, D, offsets):
+    """Sums by offset are doubles up to 2560 offsets, where they fill a CU's LDS beside the tiles of 128, and floats beyond;
+    sequences of up to 64 tokens have half the waves."""
+    for S in (60, 200):
+        at = np.arange(S) * 9
+        run(hip, 2, S, S, 2, 2, D, seed=7, bf16=S == 60, buckets=np.arange(offsets) // 3, zero=offsets // 2, where=(at, at))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
 def test_the_largest_map(hip, D):
     """4096 offsets, the last ones used, in 16384 buckets; key heads shared by two."""
