@@ -322,13 +322,14 @@ int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint1
     const long long blocks = (nSeqK + kBlockQ - 1) / kBlockQ, heads = (long long)nBatch * nKVHeads;
     const int walk = windowTiles(p.window, p.causal, allQ);   // of a block of keys, for each query head
     p.parts = evenParts(heads * blocks, walk * group, resident);
-    // The first keys: by workgroups of their own, unless they are so many that their blocks may as well walk over everything,
-    // the window is as wide as the sequences, or there are no queries (and no workspace).
-    if (p.first > kMaxSinks) {
+    // The first keys: by workgroups of their own, unless they are so many that their blocks may as well walk over everything
+    // (or more than a launch's 2^32 - 1 threads take), the window is as wide as the sequences, or there are no queries (and no
+    // workspace).
+    const long long groups = heads * ((p.first + 31) / 32);
+    if (p.first > kMaxSinks || groups * 256 > 0xffffffffLL) {
         p.sinkBlocks = (p.first + kBlockQ - 1) / kBlockQ;
         p.parts = walkParts(heads * blocks, allQ * group, 2 * resident);
     } else if (p.first > 0 && nSeqQ > 0 && p.window < std::max(nSeqQ, nSeqK)) {
-        const long long groups = heads * ((p.first + 31) / 32);
         p.sinkParts = (int)std::clamp<long long>(std::min<long long>((long long)resident * cuCount() / groups,
                                                                      ((long long)std::max(1, allQ - walk) * group + 3) / 4), 1, 64);
     }

@@ -266,6 +266,30 @@ def test_repeats_agree_and_graphs_replay(hip, streams):
 
 
 @pytest.mark.gpu
+def test_more_first_keys_than_a_launch_takes(hip):
+    """2^22 + 1 images of 97 first keys: a workgroup of 256 threads for each 32 of them would be more than 2^32 threads. Scores
+    are 0, so every key has 1/97 of dO (1) for dV; dP is what delta is, and dK 0."""
+    B, Sk, D = 2 ** 22 + 1, 97, 8
+    H = hip.HIPBackend
+    kv, dk, dv = (empty_dev(hip, (B * Sk * D // 2,)) for _ in range(3))    # two halves each
+    q, out, grad, dq = (empty_dev(hip, (B * D // 2,)) for _ in range(4))
+    lse = empty_dev(hip, (B,))
+    pair = lambda x: float(np.full(2, x, np.float16).view(np.float32)[0])
+    for b, n, x in ((kv, B * Sk * D // 2, pair(0.5)), (dk, B * Sk * D // 2, pair(3.)), (dv, B * Sk * D // 2, pair(3.)),
+                    (q, B * D // 2, 0.), (out, B * D // 2, pair(0.5)), (grad, B * D // 2, pair(1.)), (lse, B, float(np.log(97.)))):
+        H.fillValue(b, n, x)
+    H.attentionWindowBackwardHalf(q, kv, kv, D, D, D, Sk * D, None, None, True, 1, Sk, out, lse, grad, dq, dk, dv, B, 1, Sk, 1, 1, D,
+                                  1.0)
+    for image in (0, 1, 2 ** 20, 2 ** 21 + 1, B - 1):
+        got = np.empty((2, Sk, D), np.float16)
+        for g, to in zip((dk, dv), got):
+            hip.call("omHipCopyD2H", to.ctypes.data, g.ptr + image * Sk * D * 2, to.nbytes)
+        assert np.all(got[0] == 0)
+        # P and dV are rounded to halves; P's exponent, between 4 and 16 in fp32, is a few half steps of 2^-21 off
+        assert np.all(np.abs(got[1].astype(np.float64) * 97 - 1) <= 2 * 2. ** -11 + 2. ** -19)
+
+
+@pytest.mark.gpu
 def test_empty_sequences(hip):
     """No keys: zeros and -inf. No queries: zero dK, dV. No images: nothing."""
     H = hip.HIPBackend
