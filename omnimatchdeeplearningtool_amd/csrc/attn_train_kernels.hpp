@@ -1612,7 +1612,7 @@ int checkSizes(const char* name, int nDtype, long long nLdQ, long long nStrideQ,
     if (heads > 0x3fffffffLL || heads * ((std::max(nSeqQ, nSeqK) + 63LL) / 64) > 0x3fffffffLL)
         return fail("%s: too many (image, head, token) triples", name);
     // a launch takes 2^32 - 1 threads in a dimension, and silently drops the bits above: 256 threads for a block of
-    // queries, 512 for one of keys (shared walks, which multiply them, are for grids of a few per CU)
+    // queries, 512 for one of keys (shared walks multiply them: walkParts for grids of a few per CU, evenParts has a bound)
     if (heads * ((nSeqQ + kBlockQ - 1LL) / kBlockQ) * 256 > 0xffffffffLL)
         return fail("%s: too many (image, head, block of %d queries) triples", name, kBlockQ);
     if (backward && (long long)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1LL) / kBlockQ) * 512 > 0xffffffffLL)

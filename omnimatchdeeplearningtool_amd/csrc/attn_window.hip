@@ -7,6 +7,7 @@
 // of queries walk over the tiles of their windows and of the first keys alone;
 // blocks of keys over the queries whose windows reach them, the first keys'
 // over all, by several workgroups.
+#include "attn_share.hpp"
 #include "attn_train_kernels.hpp"
 #include "../../include/omhip.h"
 
@@ -250,20 +251,6 @@ int checkWindow(const char* name, int nSeqQ, int nSeqK, int nWindow, int nFirst)
 
 constexpr int kMaxSinks = 256;     // first keys that get workgroups of their own
 
-// Workgroups that share a block's walk of `tiles` 64-row tiles, all blocks' walks alike: those with which the last one ends
-// first where `resident` a CU run at once. A walk's start and end are as long as four tiles, the join of parts as eight.
-int evenParts(long long blocks, int tiles, int resident) {
-    const long long room = (long long)resident * cuCount();
-    int best = 1;
-    long long least = 0;
-    for (int parts = 1; parts <= std::min(16, std::max(1, tiles / 4)); ++parts) {
-        const long long rounds = (blocks * parts + room - 1) / room;
-        const long long time = rounds * ((tiles + parts - 1) / parts + 4) + (parts > 1 ? 8 : 0);
-        if (parts == 1 || time < least) best = parts, least = time;
-    }
-    return best;
-}
-
 // Tiles of 64 rows that a block of 128 sees through a window, of `most`.
 int windowTiles(int window, int causal, int most) {
     return (int)std::min<long long>(most, ((long long)window * (causal ? 1 : 2) + kBlockQ) / kTileKeys + 1);
@@ -321,7 +308,7 @@ int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint1
     const int allQ = p.SqP / kTileKeys, allK = (nSeqK + kTileKeys - 1) / kTileKeys;
     const long long blocks = (nSeqK + kBlockQ - 1) / kBlockQ, heads = (long long)nBatch * nKVHeads;
     const int walk = windowTiles(p.window, p.causal, allQ);   // of a block of keys, for each query head
-    p.parts = evenParts(heads * blocks, walk * group, resident);
+    p.parts = evenParts(heads * blocks, walk * group, (long long)resident * cuCount());
     // The first keys: by workgroups of their own, unless they are so many that their blocks may as well walk over everything
     // (or more than a launch's 2^32 - 1 threads take), the window is as wide as the sequences, or there are no queries (and no
     // workspace).
