@@ -166,11 +166,11 @@ int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_
     const long long blocksQ = (nSeqQ + kBlockQ - 1) / kBlockQ, blocksK = (nSeqK + kBlockQ - 1) / kBlockQ;
     const int tiles = (nSeqK + kTileKeys - 1) / kTileKeys;
     // two workgroups a CU: 2 x 2048 tokens, 8 heads of 64, causal: dK, dV and join 49.6 us (four 55.1, one 60.6)
-    p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), 2);
+    p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), 2LL * cuCount());
     p.partRows = (nSeqK + kBlockQ - 1) / kBlockQ * kBlockQ;
     // A workgroup of dQ keeps its sums over the images that it takes: so many groups of images that the grid has eight
     // workgroups a CU.
-    const int parts = walkParts((long long)nBatch * nHeads * blocksQ, tiles, 2);
+    const int parts = walkParts((long long)nBatch * nHeads * blocksQ, tiles, 2LL * cuCount());
     const long long each = std::max(1LL, nHeads * blocksQ * parts);   // workgroups of a group
     p.imageGroups = (int)std::clamp<long long>(8LL * cuCount() / each, 1, nBatch);
     const long long units = nSeqQ > 0 ? p.imageGroups * blocksQ * parts : 0;

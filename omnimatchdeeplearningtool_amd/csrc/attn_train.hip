@@ -47,7 +47,7 @@ int omHipAttentionBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* p
                           pGradOut, pGradQ, pGradK, pGradV, nBatch, nSeqQ, nSeqK, nHeads, nKVHeads, nHeadDim, fScale))
         return -1;
     const size_t keyBlocks = (size_t)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1) / kBlockQ);
-    p.parts = walkParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads), nHeadDim <= 64 ? 4 : 2);
+    p.parts = walkParts((long long)keyBlocks, p.SqP / kTileKeys * (nHeads / nKVHeads), (nHeadDim <= 64 ? 4LL : 2LL) * cuCount());
     p.partRows = (nSeqK + kBlockQ - 1) / kBlockQ * kBlockQ;
     if (backwardParts(p, (nSeqK + kTileKeys - 1) / kTileKeys, p.parts > 1 ? keyBlocks * p.parts * kBlockQ * nHeadDim : 0, 0,
                       nullptr))

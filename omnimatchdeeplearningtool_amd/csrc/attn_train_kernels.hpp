@@ -18,6 +18,7 @@
 // and attn_bias.hip hold the entries of one each.
 #pragma once
 
+#include "attn_share.hpp"
 #include "attn_tile.hpp"
 #include "buffer_io.hpp"
 #include "omhip_internal.hpp"
@@ -1570,16 +1571,6 @@ int backward(AtParams<VIEW>& p) {
     }
 }
 
-// Workgroups that share a block's walk of `tiles` 64-row tiles: as many as give every CU `perCu` workgroups and no more
-// (one workgroup past that starts a second round: 1 x 2048 x 5 heads of 128 causal backward 75.3 us, rounded up 89.4), of
-// four tiles at least. Two of them, the long walk of one block and the short one of another, make a causal grid even; dK / dV
-// of head dimensions up to 64 hold two workgroups a CU at once and ask for four. (Parts cost fp32 sums of every row: 2 x
-// 4096 x 16 heads on 4 of 128 backward 499 us with two a CU, 516 with four, about 730 unshared.)
-int walkParts(long long blocks, int tiles, int perCu) {
-    if (blocks == 0 || tiles == 0) return 1;
-    return (int)std::clamp<long long>((long long)perCu * cuCount() / blocks, 1, std::max(1, tiles / 4));
-}
-
 // ---------------------------------------------------------------- checks
 // Whether the images' rows of `width` elements lie apart, image after image or token after token (gradients are written
 // there).
@@ -1612,7 +1603,7 @@ int checkSizes(const char* name, int nDtype, long long nLdQ, long long nStrideQ,
     if (heads > 0x3fffffffLL || heads * ((std::max(nSeqQ, nSeqK) + 63LL) / 64) > 0x3fffffffLL)
         return fail("%s: too many (image, head, token) triples", name);
     // a launch takes 2^32 - 1 threads in a dimension, and silently drops the bits above: 256 threads for a block of
-    // queries, 512 for one of keys (shared walks multiply them: walkParts for grids of a few per CU, evenParts has a bound)
+    // queries, 512 for one of keys (shared walks, which multiply them, are for grids of a few per CU)
     if (heads * ((nSeqQ + kBlockQ - 1LL) / kBlockQ) * 256 > 0xffffffffLL)
         return fail("%s: too many (image, head, block of %d queries) triples", name, kBlockQ);
     if (backward && (long long)nBatch * nKVHeads * ((nSeqK + kBlockQ - 1LL) / kBlockQ) * 512 > 0xffffffffLL)
@@ -1642,7 +1633,7 @@ int forwardArguments(AttnTrainParams& p, const char* name, const uint16_t* pQ, c
 
 // The parts of the forward walks of `tiles` tiles and their workspace; 0 or -1.
 int forwardParts(AttnTrainParams& p, int tiles) {
-    p.keyParts = walkParts((long long)p.B * p.H * ((p.Sq + kBlockQ - 1) / kBlockQ), tiles, 2);
+    p.keyParts = walkParts((long long)p.B * p.H * ((p.Sq + kBlockQ - 1) / kBlockQ), tiles, 2LL * cuCount());
     if (p.keyParts > 1) {
         const size_t rows = (size_t)p.B * p.H * p.Sq * p.keyParts;
         p.rowPart = static_cast<float*>(workspace(rows * (p.D + 1) * sizeof(float), kWsOperand));
@@ -1685,7 +1676,7 @@ int backwardArguments(AttnTrainParams& p, const char* name, const uint16_t* pQ, 
 // each and, where `more` is given, of so many others; 0 or -1.
 int backwardParts(AttnTrainParams& p, int tiles, size_t sums, size_t others, float** more) {
     const size_t rows = (size_t)p.B * p.H * p.SqP;
-    p.keyParts = walkParts((long long)p.B * p.H * ((p.Sq + kBlockQ - 1) / kBlockQ), tiles, 2);
+    p.keyParts = walkParts((long long)p.B * p.H * ((p.Sq + kBlockQ - 1) / kBlockQ), tiles, 2LL * cuCount());
     const size_t rowSums = p.keyParts > 1 ? (size_t)p.B * p.H * p.Sq * p.keyParts * p.D : 0;
     if (rows) {
         p.stats = static_cast<float*>(workspace(((rows + sums) * 2 + rowSums + others) * sizeof(float), kWsOperand));

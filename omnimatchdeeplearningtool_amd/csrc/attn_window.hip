@@ -7,7 +7,6 @@
 // of queries walk over the tiles of their windows and of the first keys alone;
 // blocks of keys over the queries whose windows reach them, the first keys'
 // over all, by several workgroups.
-#include "attn_share.hpp"
 #include "attn_train_kernels.hpp"
 #include "../../include/omhip.h"
 
@@ -304,20 +303,21 @@ int omHipAttentionWindowBackwardHalf(int nDtype, const uint16_t* pQ, const uint1
         return -1;
     p.window = std::min(nWindow, std::max(nSeqQ, nSeqK));
     p.first = std::min(nFirst, nSeqK);
-    const int group = nHeads / nKVHeads, resident = nHeadDim <= 64 ? 2 : 1;
+    const int group = nHeads / nKVHeads;
+    const long long room = (nHeadDim <= 64 ? 2LL : 1LL) * cuCount();   // workgroups of dK and dV that run at once
     const int allQ = p.SqP / kTileKeys, allK = (nSeqK + kTileKeys - 1) / kTileKeys;
     const long long blocks = (nSeqK + kBlockQ - 1) / kBlockQ, heads = (long long)nBatch * nKVHeads;
     const int walk = windowTiles(p.window, p.causal, allQ);   // of a block of keys, for each query head
-    p.parts = evenParts(heads * blocks, walk * group, (long long)resident * cuCount());
+    p.parts = walkParts(heads * blocks, walk * group, room);
     // The first keys: by workgroups of their own, unless they are so many that their blocks may as well walk over everything
     // (or more than a launch's 2^32 - 1 threads take), the window is as wide as the sequences, or there are no queries (and no
     // workspace).
     const long long groups = heads * ((p.first + 31) / 32);
     if (p.first > kMaxSinks || groups * 256 > 0xffffffffLL) {
         p.sinkBlocks = (p.first + kBlockQ - 1) / kBlockQ;
-        p.parts = walkParts(heads * blocks, allQ * group, 2 * resident);
+        p.parts = walkParts(heads * blocks, allQ * group, 2 * room);
     } else if (p.first > 0 && nSeqQ > 0 && p.window < std::max(nSeqQ, nSeqK)) {
-        p.sinkParts = (int)std::clamp<long long>(std::min<long long>((long long)resident * cuCount() / groups,
+        p.sinkParts = (int)std::clamp<long long>(std::min<long long>(room / groups,
                                                                      ((long long)std::max(1, allQ - walk) * group + 3) / 4), 1, 64);
     }
     p.partRows = p.parts > 1 ? (int)blocks * kBlockQ : p.sinkParts > 0 ? p.first : 0;

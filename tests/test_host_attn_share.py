@@ -1,4 +1,4 @@
-"""The choice of how many workgroups share a walk of the windowed attention's backward pass (no GPU needed)."""
+"""The choice of how many workgroups share a walk of the attention kernels for training (no GPU needed)."""
 import os
 import subprocess
 
@@ -6,7 +6,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_shared_walks_fit_a_launch(tmp_path):
-    """No choice starts more threads than a launch takes."""
+    """No choice starts more threads than a launch takes, shares a grid that fills the card, or keeps more sums than that needs."""
     exe = tmp_path / "share"
     subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", os.path.join(ROOT, "tests", "cpp", "test_attn_share.cpp"), "-o", str(exe)],
                    check=True)
