@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_token_kernel(TokenParams p
                                                         (chunk ^ (column & (CHUNKS - 1))) * 4);
         }
         const bool empty = total == 0.f;
-        v *= empty ? 0.f : 1.f / total;
+        v = empty ? at_f32x4{0.f, 0.f, 0.f, 0.f} : v * (1.f / total);   // not by 0: a NaN of V is in the sums of hidden columns too
         const float lse = empty ? -INFINITY : top * (c * kAtLn2) + (__logf(total) - kShift * kAtLn2);
         if (p.parts == 1) {
             result(column, chunk, v, lse);
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_token_kernel(TokenParams p
             }
         }
         const bool empty = total == 0.f;
-        v *= empty ? 0.f : 1.f / total;
+        v = empty ? at_f32x4{0.f, 0.f, 0.f, 0.f} : v * (1.f / total);
         result(column, chunk, v, empty ? -INFINITY : (top == -INFINITY ? 0.f : top) + __logf(total));
     }
     if (threadIdx.x == 0) __hip_atomic_store(p.arrivals + bh, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
