@@ -232,7 +232,7 @@ __device__ __forceinline__ void atForEntries(const AttnBiasParams& p, int own, c
 }
 
 // A wave's sums of dS by offset. They are of type T: an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes,
-// no two on one address), so floats are for maps that leave no room for doubles. A wave's instructions are done in order, and
+// no two on one address), so floats are for maps that leave no room for doubles (mostWide). A wave's instructions are done in order, and
 // lanes on one address in an order of the hardware's that repeats.
 // Written out: before an atomic of its own the compiler waits for every copy into LDS under way. The wave waits for its adds
 // (__builtin_amdgcn_s_waitcnt) before the barrier behind which they are read.
@@ -1424,9 +1424,17 @@ __global__ __launch_bounds__(256, KD <= 2 ? 2 : 1) void attn_window_sinks_kernel
 }
 
 // ---------------------------------------------------------------- launches
-// Of a bias: with the tiles of a head dimension of 128 (66 KB) a dQ workgroup has room for four waves' sums in doubles of
-// 2560 offsets, in floats of 4096.
-constexpr int kMaxOffsets = 4096, kMaxWide = 2560;
+constexpr int kMaxOffsets = 4096;   // of a bias's map
+
+// The longest map whose sums in doubles fit a dQ workgroup's LDS beside its biases (rounded to 64) and static arrays: the tiles
+// and positions of two buffers, dO's rows, delta. Four waves: 3697 offsets at a head dimension of 32, 3015 at 64, 2560 at 128;
+// two waves: any map. Beyond, sums are floats.
+template <int KD, int W>
+constexpr int mostWide() {
+    constexpr int rs = AtTile<KD>::RS, fixed = 4 * kTileKeys * rs * 2 + 2 * kTileKeys * 4 + (KD <= 2 ? 32 * W * rs * 2 : 0) + 32 * W * 4;
+    constexpr int kLds = 160 << 10, kPadding = 256;   // of the static arrays' alignment
+    return std::min(kMaxOffsets, (kLds - fixed - kPadding - 63 * 4) / (4 + 8 * W) - 2 * kMapEnd);
+}
 
 size_t biasLds(const AttnBiasParams& p, int tables) {
     return (size_t)((p.nOffsets + 2 * kMapEnd + 63) / 64 * 64) * sizeof(float) * tables;
@@ -1476,10 +1484,10 @@ template <bool BF16, int KD, int VIEW, class Sum, int W>
 int launchDqKernel(const AtParams<VIEW>& p) {
     size_t lds = 0;
     if constexpr (VIEW == kAtBias) {
-        constexpr int most = sizeof(Sum) == 8 ? kMaxWide : kMaxOffsets;
+        constexpr int most = sizeof(Sum) == 8 ? mostWide<KD, W>() : kMaxOffsets;
         lds = biasLds(p, 1) + W * (size_t)(p.nOffsets + 2 * kMapEnd) * sizeof(Sum);
         OMHIP_CHECK(OMHIP_SET_MAX_DYNAMIC_LDS_ONCE((attn_train_dq_kernel<BF16, KD, VIEW, Sum, W>),
-                                                   (most + 2 * kMapEnd) * (sizeof(float) + W * sizeof(Sum))));
+                                                   (most + 2 * kMapEnd) * (sizeof(float) + W * sizeof(Sum)) + 63 * sizeof(float)));
     }
     hipLaunchKernelGGL((attn_train_dq_kernel<BF16, KD, VIEW, Sum, W>), dim3(p.heads * p.blocks * p.keyParts), dim3(64 * W), lds,
                        stream(), p);
@@ -1487,11 +1495,22 @@ int launchDqKernel(const AtParams<VIEW>& p) {
     return 0;
 }
 
-template <bool BF16, int KD, int VIEW, class Sum>
+template <bool BF16, int KD, int VIEW, int W>
+int launchDqSums(const AtParams<VIEW>& p) {
+    if constexpr (VIEW == kAtBias) {
+        if constexpr (mostWide<KD, W>() < kMaxOffsets)
+            if (p.nOffsets > mostWide<KD, W>()) return launchDqKernel<BF16, KD, VIEW, float, W>(p);
+        return launchDqKernel<BF16, KD, VIEW, double, W>(p);
+    } else {
+        return launchDqKernel<BF16, KD, VIEW, float, W>(p);
+    }
+}
+
+template <bool BF16, int KD, int VIEW>
 int launchDq(const AtParams<VIEW>& p) {
     if constexpr (kShort<KD, VIEW>)
-        if (p.Sq <= kBlockQ / 2) return launchDqKernel<BF16, KD, VIEW, Sum, kWaves / 2>(p);
-    return launchDqKernel<BF16, KD, VIEW, Sum, kWaves>(p);
+        if (p.Sq <= kBlockQ / 2) return launchDqSums<BF16, KD, VIEW, kWaves / 2>(p);
+    return launchDqSums<BF16, KD, VIEW, kWaves>(p);
 }
 
 template <bool BF16, int KD, int VIEW, int PAIRS>
@@ -1509,15 +1528,7 @@ int launchBackward(AtParams<VIEW>& p) {
         p.heads = (uint32_t)(p.B * p.H);
         if constexpr (VIEW == kAtBias) p.heads = (uint32_t)(p.imageGroups * p.H);
         p.blocks = (uint32_t)((p.Sq + kBlockQ - 1) / kBlockQ);
-        if constexpr (VIEW == kAtBias) {
-            if (p.nOffsets <= kMaxWide) {
-                if (launchDq<BF16, KD, VIEW, double>(p)) return -1;
-            } else if (launchDq<BF16, KD, VIEW, float>(p)) {
-                return -1;
-            }
-        } else if (launchDq<BF16, KD, VIEW, float>(p)) {
-            return -1;
-        }
+        if (launchDq<BF16, KD, VIEW>(p)) return -1;
         if (p.keyParts > 1) {
             const long long n = (long long)p.B * p.Sq * p.H * (p.D / 8);
             hipLaunchKernelGGL((attn_train_dq_join_kernel<BF16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream(), p);
