@@ -3,6 +3,8 @@ formulas in float64, element by element (attn_views says how far off a result ma
 import numpy as np
 import pytest
 
+import oracle as O
+from conftest import empty_dev, to_dev
 from test_gpu_attn_train import bits, value
 from test_gpu_attn_window import Window, run
 
@@ -106,6 +108,44 @@ def test_what_lies_past_a_length_is_not_read(hip, D, Sk, window):
         g = bits(c.grad, bf16)
         g[0, 2:] = 0x7fff
         c.dgrad.upload(g)
+        c.forward()
+        c.backward()
+        c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
+def test_new_keys_straight_into_caches(hip, bf16):
+    """Caches of different lengths: a call an image writes its new key's row in place, the same bits as one call into a dense
+    buffer; caches of one length: one call for all, at the cache's stride. No other row is touched, and the step's attention
+    follows the formulas on the cache as it then is."""
+    B, S, H, Hkv, D, dt = 3, 200, 4, 2, 64, 1 if bf16 else 0
+    w, kv = (H + 2 * Hkv) * D, Hkv * D
+    token = to_dev(hip, bits(O.randn((B, w), 5, 1.0), bf16))
+    angle = np.arange(S)[:, None] * 1000.0 ** (-np.arange(D // 2) * 2.0 / D)
+    tables = [None, None, to_dev(hip, np.cos(angle).astype(np.float32)), to_dev(hip, np.sin(angle).astype(np.float32))]
+    norm = hip.HIPBackend.qkNormRotary
+    for lens in ([7, 199, 64], [80, 80, 80]):
+        c = Window(hip, B, 1, S, H, Hkv, D, bf16=bf16, causal=True, window=50, first=4, klens=[n + 1 for n in lens], seed=8)
+        before = c.dev[1].numpy()
+        pos = to_dev(hip, np.array(lens, np.int32))
+        q, rows = empty_dev(hip, (B, H * D), np.uint16), empty_dev(hip, (B, kv), np.uint16)
+        norm(token.ptr, token.ptr + 2 * H * D, w, w, w, w, *tables, pos, q, rows, H * D, H * D, kv, kv, B, 1, H, Hkv, D, D, S, 1e-6, False, dt)
+        mine = c.dev[0]
+        if len(set(lens)) == 1:
+            norm(token.ptr, token.ptr + 2 * H * D, w, w, w, w, *tables, pos, mine, c.dev[1].ptr + 2 * lens[0] * kv, H * D, H * D, kv, S * kv,
+                 B, 1, H, Hkv, D, D, S, 1e-6, False, dt)
+        else:
+            for b, n in enumerate(lens):
+                at = token.ptr + 2 * b * w
+                norm(at, at + 2 * H * D, w, w, w, w, *tables, pos.ptr + 4 * b, mine.ptr + 2 * b * H * D, c.dev[1].ptr + 2 * (b * S + n) * kv,
+                     H * D, H * D, kv, S * kv, 1, 1, H, Hkv, D, D, S, 1e-6, False, dt)
+        after = c.dev[1].numpy()
+        for b, n in enumerate(lens):
+            assert np.array_equal(after[b, n], rows.numpy()[b])
+            after[b, n] = before[b, n]
+        assert np.array_equal(after, before) and np.array_equal(mine.numpy().reshape(B, -1), q.numpy())
+        c.store[0], c.store[1] = value(mine.numpy(), bf16), value(c.dev[1].numpy(), bf16)
         c.forward()
         c.backward()
         c.check()
