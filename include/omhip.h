@@ -578,8 +578,11 @@ int omHipAttentionBiasForwardHalf(int nDtype, const uint16_t* pQ, const uint16_t
                                   float fScale);
 /* NEW: the gradients of omHipAttentionBiasForwardHalf at the same arguments: pGradQ, pGradK and
  * pGradV as omHipAttentionBackwardHalf's, and pGradTable [nBuckets, nHeads] fp32 = the sums of the
- * unrounded dS = P (dO V^T - delta) over the pairs of each bucket and all images, in fp32 and in an
- * order that repeats (0 where no pair is in the bucket). delta comes from pOut as it was rounded. */
+ * unrounded dS = P (dO V^T - delta) over the pairs of each bucket and all images (0 where no pair is
+ * in the bucket), in fp32 or more. Its sums are in a fixed order but for one thing: lanes of a wave that
+ * add to one place in one instruction are served as the hardware chooses. Repeated calls have
+ * agreed bit for bit in every run, but nothing promises it (pGradQ, pGradK and pGradV are in a fixed
+ * order throughout). delta comes from pOut as it was rounded. */
 int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_t* pK, const uint16_t* pV, long long nLdQ,
                                    long long nStrideQ, long long nLdKV, long long nStrideKV, const int* pQueryLens,
                                    const int* pKeyLens, int bCausal, const float* pTable, const int* pBuckets,

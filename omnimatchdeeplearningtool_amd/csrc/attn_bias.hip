@@ -10,7 +10,8 @@
 //  * the dQ kernel, which has dS in registers, adds each to its wave's sums by
 //    offset in LDS, and leaves its workgroup's;
 //  * attn_bias_table_kernel adds those of a head, then the offsets of each
-//    bucket. All in an order that repeats.
+//    bucket. All in a fixed order, but for lanes of a wave that add to one
+//    address at once (attn_train_kernels.hpp).
 #include "attn_train_kernels.hpp"
 #include "../../include/omhip.h"
 

@@ -232,8 +232,9 @@ __device__ __forceinline__ void atForEntries(const AttnBiasParams& p, int own, c
 }
 
 // A wave's sums of dS by offset. They are of type T: an LDS add of doubles takes 9 cycles of a CU, one of floats 177 (64 lanes,
-// no two on one address), so floats are for maps that leave no room for doubles (mostWide). A wave's instructions are done in order, and
-// lanes on one address in an order of the hardware's that repeats.
+// no two on one address), so floats are for maps that leave no room for doubles (mostWide). A wave's instructions are done in order; the
+// lanes of one on the same address are served in an order of the hardware's, which has repeated in every run but which nothing
+// promises.
 // Written out: before an atomic of its own the compiler waits for every copy into LDS under way. The wave waits for its adds
 // (__builtin_amdgcn_s_waitcnt) before the barrier behind which they are read.
 __device__ __forceinline__ uint32_t atLdsAddress(const void* at) {
