@@ -166,11 +166,14 @@ int omHipAttentionBiasBackwardHalf(int nDtype, const uint16_t* pQ, const uint16_
         return -1;
     const long long blocksQ = (nSeqQ + kBlockQ - 1) / kBlockQ, blocksK = (nSeqK + kBlockQ - 1) / kBlockQ;
     const int tiles = (nSeqK + kTileKeys - 1) / kTileKeys;
-    // two workgroups a CU: 2 x 2048 tokens, 8 heads of 64, causal: dK, dV and join 49.6 us (four 55.1, one 60.6)
+    // two workgroups a CU at any head dimension. Whole backward, us, with two (one, three, four): causal 2 x 2048, 8 heads of 32: 74
+    // (89, 73, 75), of 64: 94 (106, 95, 98), of 128: 167 (172, 178, 189); 1 x 4096, 4 of 32: 73 (91, 72, 75). Without a mask walks are
+    // alike and one is enough: 4 x 1024, 8 of 64: 84 (78, 90, 92), 2 x 1000, 8 on 4 of 96: 85 (76, 85, 85).
     p.parts = walkParts((long long)nBatch * nKVHeads * blocksK, p.SqP / kTileKeys * (nHeads / nKVHeads), 2LL * cuCount());
     p.partRows = (nSeqK + kBlockQ - 1) / kBlockQ * kBlockQ;
     // A workgroup of dQ keeps its sums over the images that it takes: so many groups of images that the grid has eight
-    // workgroups a CU.
+    // workgroups a CU. Whole backward, us, with 2, 4, 8 and 16 a CU: 1024 x 49, 4 heads of 32: 85, 70, 72, 75; 2000 x 49, 6 of 64: 329, 316,
+    // 289, 286; 64 x 197, 12 of 64: 120, 125, 120, 120; 64 x 257, 16 of 96: 532, 535, 523, 542.
     const int parts = walkParts((long long)nBatch * nHeads * blocksQ, tiles, 2LL * cuCount());
     const long long each = std::max(1LL, nHeads * blocksQ * parts);   // workgroups of a group
     p.imageGroups = (int)std::clamp<long long>(8LL * cuCount() / each, 1, nBatch);

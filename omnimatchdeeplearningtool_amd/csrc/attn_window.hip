@@ -17,6 +17,8 @@ namespace {
 constexpr int kMaxSeq = 1 << 29;   // positions, and sums of one and a window, stay below 2^31
 
 // ---------------------------------------------------------------- few queries: a sequence's next tokens
+// At most 64 workgroups share a key head's keys, whose parts the last one reads alone. One query, us, with 16, 32, 64 and 128: a cache
+// of 16384, 8 heads of 64: 14, 13, 18, 28; of 65536, 8 on 2 of 128: 42, 27, 22, 26; of 131072, 4 of 64: 64, 37, 30, 35.
 constexpr int kTokenKeys = 32, kMaxTokenParts = 64;
 
 struct TokenParams : AttnWindowParams {
@@ -223,7 +225,8 @@ int launchToken(const TokenParams& p) {
     return 0;
 }
 
-// Queries of few tokens: workgroups share a key head's keys in sight, 32 a wave, as far as they all run at once.
+// Queries of few tokens: workgroups share a key head's keys in sight, 32 a wave, as far as they all run at once (16 caches of up to
+// 8192, 16 heads on 4 of 128, window 1024: 8 a key head 11.9 us, one 15.0; 8 of 8192, 8 of 128, all keys in sight: 44 and 76).
 int tokens(const AttnWindowParams& p, int nDtype) {
     TokenParams t{};
     static_cast<AttnWindowParams&>(t) = p;
@@ -248,7 +251,13 @@ int checkWindow(const char* name, int nSeqQ, int nSeqK, int nWindow, int nFirst)
     return 0;
 }
 
-constexpr int kMaxSinks = 256;     // first keys that get workgroups of their own
+// First keys that get workgroups of their own; more go with their blocks' walks over everything. Backward with workgroups of their
+// own (whole walks), us, of first keys of        32         256         300         512         1024
+//   2 x 4096, 16 heads on 4 of 128, window 512   194 (330)  236 (347)   257 (350)   292 (366)   443 (399)
+//   1 x 8192, 8 of 64, window 256                 55 (137)   69 (142)    76 (144)    88 (149)   118 (164)
+//   4 x 2048, 8 of 64, window 128 both ways       51 (67)    74 (74)     77 (81)     87 (89)    126 (122)
+//   16 x 1024, 4 of 32, window 64                 32 (38)    43 (44)     47 (47)     53 (52)     67 (55)
+constexpr int kMaxSinks = 256;
 
 // Tiles of 64 rows that a block of 128 sees through a window, of `most`.
 int windowTiles(int window, int causal, int most) {
